@@ -15,8 +15,10 @@ from __future__ import annotations
 
 import hashlib
 import os
+import re
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -26,9 +28,9 @@ INCLUDE = ROOT / "include"
 LIB_DIR = PACKAGE / "_lib"
 CORE_LIBRARY = LIB_DIR / "libconvnd_b200.so"
 SHIM_LIBRARY = LIB_DIR / "_C.so"
+OBJECT_DIR = LIB_DIR / "build"
 
 CORE_SOURCES = ["problem.cpp", "capi.cu", "fprop.cu", "tc_conv.cu", "pack.cu", "generic.cu"]
-CORE_HEADERS = ["internal.h", "ptx.cuh", "fprop.cuh", "tc_conv.cuh", "pack.cuh", "generic.cuh"]
 SHIM_SOURCES = ["shim.cpp"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -67,10 +69,37 @@ def _run(command: list[str], verbose: bool) -> None:
         print(result.stdout + result.stderr, file=sys.stderr)
 
 
+def _with_headers(source: Path) -> list[Path]:
+    """The source and every project header it includes, directly or through another."""
+    found, pending = [], [source]
+    while pending:
+        path = pending.pop()
+        if path in found:
+            continue
+        found.append(path)
+        for name in re.findall(r'^\s*#\s*include\s+"([^"]+)"', path.read_text(), re.MULTILINE):
+            pending += [folder / name for folder in (CSRC, INCLUDE) if (folder / name).exists()]
+    return [source] + sorted(found[1:])
+
+
+def _compile_object(name: str, flags: list[str], verbose: bool, force: bool) -> Path:
+    """Compile one source of the core library, unless its object is up to date."""
+    target = OBJECT_DIR / (name + ".o")
+    digest = _digest(_with_headers(CSRC / name), " ".join(flags))
+    if not force and _up_to_date(target, digest):
+        return target
+    temporary = target.with_suffix(".o.tmp")
+    _run([_nvcc(), *flags, "-c", str(CSRC / name), "-o", str(temporary)], verbose)
+    temporary.replace(target)
+    _stamp(target, digest)
+    return target
+
+
 def build_core(verbose: bool = False, force: bool = False) -> Path:
-    """Compile the C-ABI library with nvcc for sm_100a (cross-compiles without a GPU)."""
-    LIB_DIR.mkdir(exist_ok=True)
-    inputs = [CSRC / name for name in CORE_SOURCES + CORE_HEADERS] + [INCLUDE / "convnd_b200.h"]
+    """Compile the C-ABI library with nvcc for sm_100a (cross-compiles without a GPU):
+    one object per source, in parallel, then one link."""
+    OBJECT_DIR.mkdir(parents=True, exist_ok=True)
+    inputs = sorted({path for name in CORE_SOURCES for path in _with_headers(CSRC / name)})
     flags = [
         *ARCH_FLAGS,
         "-O3",
@@ -78,7 +107,6 @@ def build_core(verbose: bool = False, force: bool = False) -> Path:
         "-std=c++17",
         "-Xcompiler",
         "-fPIC,-O2,-fvisibility=hidden",
-        "-shared",
         f"-I{INCLUDE}",
         f"-I{CSRC}",
         "--expt-relaxed-constexpr",
@@ -86,9 +114,11 @@ def build_core(verbose: bool = False, force: bool = False) -> Path:
     digest = _digest(inputs, " ".join(flags))
     if not force and _up_to_date(CORE_LIBRARY, digest):
         return CORE_LIBRARY
-    sources = [str(CSRC / name) for name in CORE_SOURCES]
+    with ThreadPoolExecutor(max_workers=min(len(CORE_SOURCES), os.cpu_count() or 1)) as pool:
+        objects = list(pool.map(
+            lambda name: _compile_object(name, flags, verbose, force), CORE_SOURCES))
     temporary = CORE_LIBRARY.with_suffix(".so.tmp")
-    _run([_nvcc(), *flags, *sources, "-o", str(temporary)], verbose)
+    _run([_nvcc(), *ARCH_FLAGS, "-shared", *map(str, objects), "-o", str(temporary)], verbose)
     temporary.replace(CORE_LIBRARY)
     _stamp(CORE_LIBRARY, digest)
     return CORE_LIBRARY
@@ -100,7 +130,7 @@ def build_shim(verbose: bool = False, force: bool = False) -> Path:
     from torch.utils import cpp_extension
 
     LIB_DIR.mkdir(exist_ok=True)
-    inputs = [CSRC / name for name in SHIM_SOURCES] + [INCLUDE / "convnd_b200.h"]
+    inputs = [path for name in SHIM_SOURCES for path in _with_headers(CSRC / name)]
     includes = [f"-I{path}" for path in cpp_extension.include_paths()]
     cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
