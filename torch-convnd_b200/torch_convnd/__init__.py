@@ -9,6 +9,7 @@ never compiles anything.
 
 from ._geometry import DEFAULT_WORKSPACE_BYTES
 from ._layout import channels_last, is_channels_last
+from ._layers import gated_recurrence, layer_norm, linear
 from ._native import (
     device_status,
     launch_count,
@@ -42,8 +43,11 @@ __all__ = [
     "device_status",
     "ensure_native_definitions",
     "export_onnx",
+    "gated_recurrence",
     "is_channels_last",
     "launch_count",
+    "layer_norm",
+    "linear",
     "load_native",
     "native_unavailable_reason",
     "partial_conv_nd",

@@ -78,6 +78,9 @@ def core() -> ctypes.CDLL:
         library.cnd_collect_kernel_timings.argtypes = [
             ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_float), ctypes.c_int32]
         library.cnd_collect_kernel_timings.restype = ctypes.c_int
+        library.cnd_gated_recurrence_blocks.argtypes = [
+            ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]
+        library.cnd_gated_recurrence_blocks.restype = ctypes.c_int64
         library.cnd_last_error.restype = ctypes.c_char_p
         library.cnd_version.restype = ctypes.c_char_p
         _CORE = library

@@ -49,8 +49,10 @@ CONV_ND_ACT_BACKWARD_SCHEMA = (
 
 def _first_call(name):
     def run(*args):
-        from ._native import load_native
+        from ._native import is_loaded, load_native
 
+        if is_loaded():  # the shim's kernels are registered and none takes these tensors
+            raise RuntimeError(f"torch_convnd::{name} supports strided CPU and CUDA tensors only")
         load_native()
         return getattr(torch.ops.torch_convnd, name).default(*args)
 
@@ -112,6 +114,8 @@ def ensure_native_definitions() -> None:
         library.impl("conv_nd_act_backward", _first_call("conv_nd_act_backward"),
                      "CompositeExplicitAutograd")
         from ._autograd import register_training
+        from ._layers import define
 
         register_training()
+        define(library)
         _LIBRARY = library
