@@ -2,41 +2,26 @@
 //
 //   dz = dy act'(z),  dx = dz W,  dW = dz^T x,  dbias = column sums of dz.
 //
-// The products run on the CUDA cores: 64 x 64 tiles, each of 256 threads 4 x 4 of them,
-// float32 sums (float64 for float64).
+// 16-bit and float32 products run on the tensor cores (product.cu). What they need beside
+// the products is one kernel here, prepare_kernel: it reads a matrix once and writes it as a
+// product's operand, multiplied by the activation's slope on the way (dz), split into three
+// bfloat16 terms (float32), or with rows padded to 16 bytes (sizes that TMA cannot address),
+// and sums its columns (dbias). Operands that TMA can read as they lie are not copied. float64
+// runs on the CUDA cores.
 #include <algorithm>
 
+#include "activation.cuh"
 #include "layers.cuh"
+#include "product.cuh"
 
 namespace cnd {
 namespace layers {
 namespace {
 
-// GELU'(v) = Phi(v) + v phi(v); SiLU'(v) = s (1 + v (1 - s)), s = 1 / (1 + exp(-v)).
-template <typename A>
-__device__ __forceinline__ A activate(A v, int act) {
-  if (act == CND_ACT_GELU) return A(0.5) * v * (A(1) + erf(v * A(0.70710678118654752440)));
-  if (act == CND_ACT_SILU) return v / (A(1) + exp(-v));
-  return v;
-}
-
-template <typename A>
-__device__ __forceinline__ A activation_slope(A v, int act) {
-  if (act == CND_ACT_GELU) {
-    const A cdf = A(0.5) * (A(1) + erf(v * A(0.70710678118654752440)));
-    return cdf + v * exp(A(-0.5) * v * v) * A(0.39894228040143267794);
-  }
-  if (act == CND_ACT_SILU) {
-    const A s = A(1) / (A(1) + exp(-v));
-    return s * (A(1) + v * (A(1) - s));
-  }
-  return A(1);
-}
-
 // d[m][n] = sum_k a(m, k) b(n, k), element (i, k) of an operand at i * row + k * col.
-struct ProductArgs {
-  const void *a, *b, *bias, *residual;
-  void *d, *pre;
+struct DoubleProduct {
+  const double *a, *b, *bias, *residual;
+  double *d, *pre;
   int64_t m, n, k;
   int64_t a_row, a_col, b_row, b_col;
   int act;
@@ -44,33 +29,30 @@ struct ProductArgs {
 
 constexpr int kTile = 64, kDepth = 16;
 
-template <typename T>
-__global__ void __launch_bounds__(256) product_kernel(const ProductArgs p) {
-  using A = typename Wide<T>::type;
-  __shared__ A sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
+// 64 x 64 tiles, 4 x 4 values a thread.
+__global__ void __launch_bounds__(256) double_product_kernel(const DoubleProduct p) {
+  __shared__ double sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const int64_t m0 = static_cast<int64_t>(blockIdx.x) * kTile;
   const int64_t n0 = static_cast<int64_t>(blockIdx.y) * kTile;
-  const T* a = static_cast<const T*>(p.a);
-  const T* b = static_cast<const T*>(p.b);
-  A sum[4][4] = {};
+  double sum[4][4] = {};
   for (int64_t k0 = 0; k0 < p.k; k0 += kDepth) {
     for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
       const int r = p.a_col == 1 ? i / kDepth : i % kTile;
       const int k = p.a_col == 1 ? i % kDepth : i / kTile;
       const bool in = m0 + r < p.m && k0 + k < p.k;
-      sa[k][r] = in ? widen(a[(m0 + r) * p.a_row + (k0 + k) * p.a_col]) : A(0);
+      sa[k][r] = in ? p.a[(m0 + r) * p.a_row + (k0 + k) * p.a_col] : 0.0;
     }
     for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
       const int r = p.b_col == 1 ? i / kDepth : i % kTile;
       const int k = p.b_col == 1 ? i % kDepth : i / kTile;
       const bool in = n0 + r < p.n && k0 + k < p.k;
-      sb[k][r] = in ? widen(b[(n0 + r) * p.b_row + (k0 + k) * p.b_col]) : A(0);
+      sb[k][r] = in ? p.b[(n0 + r) * p.b_row + (k0 + k) * p.b_col] : 0.0;
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kDepth; ++k) {
-      A u[4], v[4];
+      double u[4], v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         u[i] = sa[k][ty * 4 + i];
@@ -90,42 +72,145 @@ __global__ void __launch_bounds__(256) product_kernel(const ProductArgs p) {
     for (int j = 0; j < 4; ++j) {
       const int64_t n = n0 + tx + 16 * j;
       if (n >= p.n) break;
-      A v = sum[i][j];
-      if (p.bias != nullptr) v += widen(static_cast<const T*>(p.bias)[n]);
-      if (p.pre != nullptr) static_cast<T*>(p.pre)[m * p.n + n] = narrow<T>(v);
-      v = activate<A>(v, p.act);
-      if (p.residual != nullptr) v += widen(static_cast<const T*>(p.residual)[m * p.n + n]);
-      static_cast<T*>(p.d)[m * p.n + n] = narrow<T>(v);
+      double v = sum[i][j];
+      if (p.bias != nullptr) v += p.bias[n];
+      if (p.pre != nullptr) p.pre[m * p.n + n] = v;
+      v = activate<true>(v, p.act);
+      if (p.residual != nullptr) v += p.residual[m * p.n + n];
+      p.d[m * p.n + n] = v;
     }
   }
 }
 
+// ---- operands --------------------------------------------------------------------------
+
+struct PrepareArgs {
+  const void* src;  // [rows][width], rows src_stride apart
+  const void* pre;  // [rows][width] dense, or NULL: no activation
+  void* dst;        // NULL: column sums only
+  void* sums;       // [gridDim.y][width] partial column sums, or NULL
+  int64_t rows, width, src_stride, pitch, plane;
+  int act, vectors;
+};
+
+constexpr int kPrepareColumns = 256;  // columns of a block: 32 lanes of 8
+
+// T: source type. A block takes 256 columns and a range of rows, a warp one row of it at a
+// time, a lane 8 consecutive columns: 16-byte loads and stores where rows allow them.
 template <typename T>
-__global__ void __launch_bounds__(256)
-    slope_kernel(const T* dy, const T* pre, T* dz, int64_t count, int act) {
+__global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
   using A = typename Wide<T>::type;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += step) {
-    dz[i] = narrow<T>(widen(dy[i]) * activation_slope<A>(widen(pre[i]), act));
+  constexpr bool kExact = sizeof(T) >= 4;
+  constexpr int kLoad = sizeof(T) == 2 ? 8 : 16 / sizeof(T);
+  __shared__ A part[8][kPrepareColumns];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kPrepareColumns + lane * 8;
+  const int64_t first = a.rows * blockIdx.y / gridDim.y;
+  const int64_t last = a.rows * (blockIdx.y + 1) / gridDim.y;
+  A sum[8] = {};
+  if (col < a.width) {
+#pragma unroll 2
+    for (int64_t row = first + warp; row < last; row += 8) {
+      const T* src = static_cast<const T*>(a.src) + row * a.src_stride + col;
+      const T* pre = static_cast<const T*>(a.pre) + row * a.width + col;
+      T v[8], z[8];
+      if (a.vectors) {
+#pragma unroll
+        for (int i = 0; i < 8; i += kLoad) {
+          *reinterpret_cast<Pack<T, kLoad>*>(v + i) = *reinterpret_cast<const Pack<T, kLoad>*>(src + i);
+          if (a.pre != nullptr) {
+            *reinterpret_cast<Pack<T, kLoad>*>(z + i) =
+                *reinterpret_cast<const Pack<T, kLoad>*>(pre + i);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[i] = col + i < a.width ? src[i] : narrow<T>(A(0));
+          if (a.pre != nullptr) z[i] = col + i < a.width ? pre[i] : narrow<T>(A(0));
+        }
+      }
+      A w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = widen(v[i]);
+      if (a.pre != nullptr) {
+        if (a.act == CND_ACT_GELU) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] *= activation_slope<kExact>(widen(z[i]), CND_ACT_GELU);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] *= activation_slope<kExact>(widen(z[i]), CND_ACT_SILU);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += w[i];
+      if (a.dst == nullptr) continue;
+      if constexpr (sizeof(T) == 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (col + i < a.width) static_cast<T*>(a.dst)[row * a.pitch + col + i] = w[i];
+        }
+      } else if constexpr (sizeof(T) == 4) {
+        // x = x0 + x1 + x2, each the nearest bfloat16 of what is left; an infinity or NaN
+        // is x0 alone
+        Pack<__nv_bfloat16, 8> t[3];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          t[0].v[i] = __float2bfloat16_rn(w[i]);
+          float rest = w[i] - __bfloat162float(t[0].v[i]);
+          if (!isfinite(rest)) {
+            // near the largest float32, x0 would round up to infinity: round it down
+            t[0].v[i] = isfinite(w[i]) ? __float2bfloat16_rz(w[i]) : t[0].v[i];
+            rest = isfinite(w[i]) ? w[i] - __bfloat162float(t[0].v[i]) : 0.0f;
+          }
+          t[1].v[i] = __float2bfloat16_rn(rest);
+          t[2].v[i] = __float2bfloat16_rn(rest - __bfloat162float(t[1].v[i]));
+        }
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.dst) + row * a.pitch + col;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          *reinterpret_cast<Pack<__nv_bfloat16, 8>*>(dst + p * a.plane) = t[p];
+        }
+      } else {
+        Pack<T, 8> t;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t.v[i] = narrow<T>(w[i]);
+        *reinterpret_cast<Pack<T, 8>*>(static_cast<T*>(a.dst) + row * a.pitch + col) = t;
+      }
+    }
   }
+  if (a.sums == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[warp][lane * 8 + i] = sum[i];
+  __syncthreads();
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * kPrepareColumns + threadIdx.x;
+  if (c >= a.width) return;
+  A total = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) total += part[w][threadIdx.x];
+  static_cast<A*>(a.sums)[blockIdx.y * a.width + c] = total;
 }
 
+// Partial column sums [count][width] added in order: a block takes 32 columns, its warps
+// contiguous ranges of the partial rows, and the range sums are added in range order.
 template <typename T>
 __global__ void __launch_bounds__(256)
-    column_sum_kernel(const T* dz, T* dbias, int64_t rows, int64_t width) {
+    column_join_kernel(const void* sums, int count, int64_t width, T* out) {
   using A = typename Wide<T>::type;
   __shared__ A part[8][32];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   A sum = 0;
   if (c < width) {
-    for (int64_t r = rows * warp / 8; r < rows * (warp + 1) / 8; ++r) sum += widen(dz[r * width + c]);
+    const A* p = static_cast<const A*>(sums) + c;
+#pragma unroll 8
+    for (int r = count * warp / 8; r < count * (warp + 1) / 8; ++r) sum += p[r * width];
   }
   part[warp][lane] = sum;
   __syncthreads();
   if (warp != 0 || c >= width) return;
   for (int w = 1; w < 8; ++w) sum += part[w][lane];
-  dbias[c] = narrow<T>(sum);
+  out[c] = narrow<T>(sum);
 }
 
 template <typename F>
@@ -141,12 +226,119 @@ void with_dtype(int dtype, F&& f) {
   }
 }
 
-void launch_product(int dtype, const ProductArgs& p, cudaStream_t stream) {
+int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
+size_t up1024(size_t v) { return (v + 1023) / 1024 * 1024; }
+
+// Row ranges of prepare_kernel's grid: about eight blocks an SM, 32 rows or more each.
+int prepare_ranges(int64_t rows, int64_t width) {
+  const int64_t across = (width + kPrepareColumns - 1) / kPrepareColumns;
+  const int64_t ranges = std::min<int64_t>((rows + 31) / 32, (148 * 8 + across - 1) / across);
+  return static_cast<int>(std::max<int64_t>(1, ranges));
+}
+
+// Bytes of a prepared [rows][width] operand.
+size_t operand_bytes(int dtype, int64_t rows, int64_t width) {
+  return up1024(static_cast<size_t>(rows) * up8(width) * (dtype == CND_F32 ? 6 : 2));
+}
+
+// Writes src (times the slope at pre) as an operand into dst (NULL: column sums only).
+void prepare(int dtype, const void* src, const void* pre, int act, int64_t rows, int64_t width,
+             int64_t stride, void* dst, int64_t pitch, void* sums, cudaStream_t stream) {
+  PrepareArgs a{};
+  a.src = src;
+  a.pre = pre;
+  a.dst = dst;
+  a.sums = sums;
+  a.rows = rows;
+  a.width = width;
+  a.src_stride = stride;
+  a.pitch = pitch;
+  a.plane = rows * pitch;
+  a.act = act;
+  a.vectors = width % 8 == 0 && stride * element_size(dtype) % 16 == 0 && aligned16(src) &&
+              aligned16(pre);
+  const dim3 grid(static_cast<unsigned>((width + kPrepareColumns - 1) / kPrepareColumns),
+                  static_cast<unsigned>(prepare_ranges(rows, width)));
+  with_dtype(dtype, [&](auto zero) {
+    prepare_kernel<decltype(zero)><<<grid, 256, 0, stream>>>(a);
+  });
+  count_launch();
+}
+
+Operand operand_at(const void* data, int64_t rows, int64_t pitch, bool k_major) {
+  return Operand{data, pitch, rows * pitch, k_major};
+}
+
+// What of a 16-bit or float32 problem has to be copied before TMA can read it.
+bool copies_x(const cnd_linear& p) { return p.dtype == CND_F32 || p.x_stride % 8 != 0; }
+bool copies_w(const cnd_linear& p) { return p.dtype == CND_F32 || p.in_features % 8 != 0; }
+bool copies_dz(const cnd_linear& p) {
+  return p.dtype == CND_F32 || p.activation != CND_ACT_NONE || p.out_features % 8 != 0;
+}
+
+// Workspace of a call: byte offsets of its regions.
+struct Layout {
+  size_t dz = 0, x = 0, w = 0, sums = 0, splits = 0, total = 0;
+};
+
+size_t take(size_t* total, size_t bytes) {
+  const size_t at = *total;
+  *total += up1024(bytes);
+  return at;
+}
+
+int parts_of(const cnd_linear& p) { return p.dtype == CND_F32 ? 3 : 1; }
+
+Layout forward_layout(const cnd_linear& p) {
+  Layout l;
+  if (p.dtype == CND_F64) return l;
+  if (copies_x(p)) l.x = take(&l.total, operand_bytes(p.dtype, p.rows, p.in_features));
+  if (copies_w(p)) l.w = take(&l.total, operand_bytes(p.dtype, p.out_features, p.in_features));
+  const ProductPlan plan = plan_product(p.rows, p.out_features, p.in_features, parts_of(p));
+  l.splits = take(&l.total, product_workspace(plan, p.rows, p.out_features));
+  return l;
+}
+
+Layout backward_layout(const cnd_linear& p, const int32_t mask[3]) {
+  Layout l;
+  const bool products = mask[0] || mask[1];
+  if (p.dtype == CND_F64) {
+    if (p.activation != CND_ACT_NONE) {
+      l.dz = take(&l.total, static_cast<size_t>(p.rows) * p.out_features * sizeof(double));
+    }
+  } else {
+    if (products && copies_dz(p)) {
+      l.dz = take(&l.total, operand_bytes(p.dtype, p.rows, p.out_features));
+    }
+    if (mask[1] && copies_x(p)) l.x = take(&l.total, operand_bytes(p.dtype, p.rows, p.in_features));
+    if (mask[0] && copies_w(p)) {
+      l.w = take(&l.total, operand_bytes(p.dtype, p.out_features, p.in_features));
+    }
+  }
+  if (mask[2]) {
+    l.sums = take(&l.total, static_cast<size_t>(prepare_ranges(p.rows, p.out_features)) *
+                                p.out_features * (p.dtype == CND_F64 ? 8 : 4));
+  }
+  if (p.dtype != CND_F64) {
+    size_t splits = 0;
+    if (mask[0]) {
+      splits = product_workspace(plan_product(p.rows, p.in_features, p.out_features, parts_of(p)),
+                                 p.rows, p.in_features);
+    }
+    if (mask[1]) {
+      splits = std::max(splits, product_workspace(plan_product(p.out_features, p.in_features,
+                                                               p.rows, parts_of(p)),
+                                                  p.out_features, p.in_features));
+    }
+    l.splits = take(&l.total, splits);
+  }
+  return l;
+}
+
+void launch_double(const DoubleProduct& p, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>((p.m + kTile - 1) / kTile),
                   static_cast<unsigned>((p.n + kTile - 1) / kTile));
-  with_dtype(dtype, [&](auto zero) {
-    product_kernel<decltype(zero)><<<grid, 256, 0, stream>>>(p);
-  });
+  double_product_kernel<<<grid, 256, 0, stream>>>(p);
   count_launch();
 }
 
@@ -186,8 +378,9 @@ int check_workspace(const char* who, const void* workspace, size_t bytes, size_t
 extern "C" {
 
 size_t cnd_linear_forward_workspace_size(const cnd_linear* problem) {
-  (void)problem;
-  return 0;
+  using namespace cnd::layers;
+  if (check_linear("cnd_linear_forward", problem) != CND_OK || problem->rows == 0) return 0;
+  return forward_layout(*problem).total;
 }
 
 int cnd_linear_forward(const cnd_linear* problem, const void* x, const void* weight,
@@ -202,34 +395,69 @@ int cnd_linear_forward(const cnd_linear* problem, const void* x, const void* wei
   if (x == nullptr || weight == nullptr || y == nullptr) {
     return fail(CND_ERR_INVALID, "cnd_linear_forward: x, weight and y must not be NULL");
   }
-  rc = check_workspace("cnd_linear_forward", workspace, workspace_bytes,
-                       cnd_linear_forward_workspace_size(problem));
+  const cnd_linear& q = *problem;
+  const int64_t rows = q.rows, in = q.in_features, out = q.out_features;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
+  if (q.dtype == CND_F64) {
+    DoubleProduct p{};
+    p.a = static_cast<const double*>(x);
+    p.b = static_cast<const double*>(weight);
+    p.bias = static_cast<const double*>(bias);
+    p.residual = static_cast<const double*>(residual);
+    p.d = static_cast<double*>(y);
+    p.pre = static_cast<double*>(pre);
+    p.m = rows;
+    p.n = out;
+    p.k = in;
+    p.a_row = q.x_stride;
+    p.b_row = in;
+    p.a_col = p.b_col = 1;
+    p.act = q.activation;
+    launch_double(p, stream);
+    return launch_status("cnd_linear_forward");
+  }
+  if (!aligned16(x) || !aligned16(weight)) {
+    return fail(CND_ERR_INVALID, "cnd_linear_forward: x and weight must be 16-byte aligned");
+  }
+  const Layout l = forward_layout(q);
+  rc = check_workspace("cnd_linear_forward", workspace, workspace_bytes, l.total);
   if (rc != CND_OK) return rc;
-  ProductArgs p{};
-  p.a = x;
-  p.b = weight;
-  p.bias = bias;
-  p.residual = residual;
+  char* base = static_cast<char*>(workspace);
+  Product p{};
+  p.a = operand_at(x, rows, q.x_stride, true);
+  p.b = operand_at(weight, out, in, true);
+  if (copies_x(q)) {
+    prepare(q.dtype, x, nullptr, CND_ACT_NONE, rows, in, q.x_stride, base + l.x, up8(in), nullptr,
+            stream);
+    p.a = operand_at(base + l.x, rows, up8(in), true);
+  }
+  if (copies_w(q)) {
+    prepare(q.dtype, weight, nullptr, CND_ACT_NONE, out, in, in, base + l.w, up8(in), nullptr,
+            stream);
+    p.b = operand_at(base + l.w, out, up8(in), true);
+  }
+  p.m = rows;
+  p.n = out;
+  p.k = in;
+  p.parts = parts_of(q);
+  p.bf16 = q.dtype != CND_F16;
+  p.dtype = q.dtype;
   p.d = y;
   p.pre = pre;
-  p.m = problem->rows;
-  p.n = problem->out_features;
-  p.k = problem->in_features;
-  p.a_row = problem->x_stride;
-  p.a_col = 1;
-  p.b_row = problem->in_features;
-  p.b_col = 1;
-  p.act = problem->activation;
-  launch_product(problem->dtype, p, static_cast<cudaStream_t>(stream_handle));
-  return launch_status("cnd_linear_forward");
+  p.bias = bias;
+  p.residual = residual;
+  p.act = q.activation;
+  return launch_product(p, plan_product(rows, out, in, p.parts), base + l.splits, stream);
 }
 
 size_t cnd_linear_backward_workspace_size(const cnd_linear* problem,
                                           const int32_t output_mask[3]) {
-  (void)output_mask;
-  if (problem == nullptr || problem->activation == CND_ACT_NONE) return 0;
-  return static_cast<size_t>(problem->rows) * static_cast<size_t>(problem->out_features) *
-         cnd::layers::element_size(problem->dtype);
+  using namespace cnd::layers;
+  if (check_linear("cnd_linear_backward", problem) != CND_OK || output_mask == nullptr ||
+      problem->rows == 0) {
+    return 0;
+  }
+  return backward_layout(*problem, output_mask).total;
 }
 
 int cnd_linear_backward(const cnd_linear* problem, const void* dy, const void* pre,
@@ -244,69 +472,112 @@ int cnd_linear_backward(const cnd_linear* problem, const void* dy, const void* p
   if (output_mask == nullptr) {
     return fail(CND_ERR_INVALID, "cnd_linear_backward: output_mask must not be NULL");
   }
-  if (!output_mask[0] && !output_mask[1] && !output_mask[2]) return CND_OK;
-  const int64_t rows = problem->rows, in = problem->in_features, out = problem->out_features;
-  const bool act = problem->activation != CND_ACT_NONE;
-  if ((output_mask[1] && dweight == nullptr) || (output_mask[2] && dbias == nullptr) ||
+  const bool want_x = output_mask[0], want_w = output_mask[1], want_b = output_mask[2];
+  if (!want_x && !want_w && !want_b) return CND_OK;
+  const cnd_linear& q = *problem;
+  const int64_t rows = q.rows, in = q.in_features, out = q.out_features;
+  const bool act = q.activation != CND_ACT_NONE;
+  if ((want_w && dweight == nullptr) || (want_b && dbias == nullptr) ||
       (rows > 0 && (dy == nullptr || (act && pre == nullptr) ||
-                    (output_mask[0] && (dx == nullptr || weight == nullptr)) ||
-                    (output_mask[1] && x == nullptr)))) {
+                    (want_x && (dx == nullptr || weight == nullptr)) ||
+                    (want_w && x == nullptr)))) {
     return fail(CND_ERR_INVALID, "cnd_linear_backward: a required buffer is NULL");
   }
-  rc = check_workspace("cnd_linear_backward", workspace, workspace_bytes,
-                       cnd_linear_backward_workspace_size(problem, output_mask));
-  if (rc != CND_OK) return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
-  const void* dz = dy;
-  if (act && rows > 0) {
-    const int64_t count = rows * out;
-    const unsigned grid = static_cast<unsigned>(
-        std::min<int64_t>((count + 255) / 256, static_cast<int64_t>(sm_count()) * 32));
-    with_dtype(problem->dtype, [&](auto zero) {
+  if (rows == 0) {
+    const size_t size = element_size(q.dtype);
+    if (want_w) cudaMemsetAsync(dweight, 0, static_cast<size_t>(out) * in * size, stream);
+    if (want_b) cudaMemsetAsync(dbias, 0, static_cast<size_t>(out) * size, stream);
+    return launch_status("cnd_linear_backward");
+  }
+  if (q.dtype != CND_F64 && (!aligned16(dy) || !aligned16(pre) || (want_w && !aligned16(x)) ||
+                             (want_x && !aligned16(weight)))) {
+    return fail(CND_ERR_INVALID,
+                "cnd_linear_backward: dy, pre, x and weight must be 16-byte aligned");
+  }
+  const Layout l = backward_layout(q, output_mask);
+  rc = check_workspace("cnd_linear_backward", workspace, workspace_bytes, l.total);
+  if (rc != CND_OK) return rc;
+  char* base = static_cast<char*>(workspace);
+  const bool copy = q.dtype == CND_F64 ? act : (want_x || want_w) && copies_dz(q);
+  const int64_t pitch = q.dtype == CND_F64 ? out : up8(out);
+  if (copy || want_b) {
+    prepare(q.dtype, dy, act ? pre : nullptr, q.activation, rows, out, out,
+            copy ? base + l.dz : nullptr, pitch, want_b ? base + l.sums : nullptr, stream);
+  }
+  if (want_b) {
+    with_dtype(q.dtype, [&](auto zero) {
       using T = decltype(zero);
-      slope_kernel<T><<<grid, 256, 0, stream>>>(static_cast<const T*>(dy),
-                                                static_cast<const T*>(pre),
-                                                static_cast<T*>(workspace), count,
-                                                problem->activation);
+      column_join_kernel<T><<<static_cast<unsigned>((out + 31) / 32), 256, 0, stream>>>(
+          base + l.sums, prepare_ranges(rows, out), out, static_cast<T*>(dbias));
     });
     count_launch();
-    dz = workspace;
   }
-  if (output_mask[0] && rows > 0) {
-    ProductArgs p{};
+  if (q.dtype == CND_F64) {
+    DoubleProduct p{};
+    p.a = copy ? reinterpret_cast<const double*>(base + l.dz) : static_cast<const double*>(dy);
+    if (want_x) {
+      p.b = static_cast<const double*>(weight);
+      p.d = static_cast<double*>(dx);
+      p.m = rows;
+      p.n = in;
+      p.k = out;
+      p.a_row = out;
+      p.a_col = 1;
+      p.b_row = 1;
+      p.b_col = in;
+      launch_double(p, stream);
+    }
+    if (want_w) {
+      p.b = static_cast<const double*>(x);
+      p.d = static_cast<double*>(dweight);
+      p.m = out;
+      p.n = in;
+      p.k = rows;
+      p.a_row = 1;
+      p.a_col = out;
+      p.b_row = 1;
+      p.b_col = q.x_stride;
+      launch_double(p, stream);
+    }
+    return launch_status("cnd_linear_backward");
+  }
+  const Operand dz = copy ? operand_at(base + l.dz, rows, pitch, true)
+                          : operand_at(dy, rows, out, true);
+  Product p{};
+  p.parts = parts_of(q);
+  p.bf16 = q.dtype != CND_F16;
+  p.dtype = q.dtype;
+  if (want_x) {
     p.a = dz;
-    p.b = weight;
-    p.d = dx;
+    p.b = operand_at(weight, out, in, false);
+    if (copies_w(q)) {
+      prepare(q.dtype, weight, nullptr, CND_ACT_NONE, out, in, in, base + l.w, up8(in), nullptr,
+              stream);
+      p.b = operand_at(base + l.w, out, up8(in), false);
+    }
     p.m = rows;
     p.n = in;
     p.k = out;
-    p.a_row = out;
-    p.a_col = 1;
-    p.b_row = 1;
-    p.b_col = in;
-    launch_product(problem->dtype, p, stream);
+    p.d = dx;
+    rc = launch_product(p, plan_product(p.m, p.n, p.k, p.parts), base + l.splits, stream);
+    if (rc != CND_OK) return rc;
   }
-  if (output_mask[1]) {
-    ProductArgs p{};
+  if (want_w) {
     p.a = dz;
-    p.b = x;
-    p.d = dweight;
+    p.a.k_major = false;
+    p.b = operand_at(x, rows, q.x_stride, false);
+    if (copies_x(q)) {
+      prepare(q.dtype, x, nullptr, CND_ACT_NONE, rows, in, q.x_stride, base + l.x, up8(in),
+              nullptr, stream);
+      p.b = operand_at(base + l.x, rows, up8(in), false);
+    }
     p.m = out;
     p.n = in;
     p.k = rows;
-    p.a_row = 1;
-    p.a_col = out;
-    p.b_row = 1;
-    p.b_col = problem->x_stride;
-    launch_product(problem->dtype, p, stream);
-  }
-  if (output_mask[2]) {
-    with_dtype(problem->dtype, [&](auto zero) {
-      using T = decltype(zero);
-      column_sum_kernel<T><<<static_cast<unsigned>((out + 31) / 32), 256, 0, stream>>>(
-          static_cast<const T*>(dz), static_cast<T*>(dbias), rows, out);
-    });
-    count_launch();
+    p.d = dweight;
+    rc = launch_product(p, plan_product(p.m, p.n, p.k, p.parts), base + l.splits, stream);
+    if (rc != CND_OK) return rc;
   }
   return launch_status("cnd_linear_backward");
 }

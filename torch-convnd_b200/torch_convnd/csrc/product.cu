@@ -1,0 +1,832 @@
+// Matrix products of the linear layers on tcgen05.
+//
+//   D[m][n] = act(sum_k A(m, k) B(n, k) + bias[n]) + residual[m][n]
+//
+// A persistent kernel: one warp loads 64-deep operand tiles by TMA into a ring of shared
+// memory stages, one warp issues the MMAs into TMEM accumulators, eight warps read them
+// back, apply the epilogue and hand finished 128-byte wide tiles to TMA stores. Two
+// accumulator sets let the epilogue of one tile run under the main loop of the next. Either
+// operand may be K-major or MN-major (dx reads W, dW reads dz and x as they lie in memory).
+//
+// Tiles. A 128 x 256 tile per CTA needs 96 operand bytes per clock and SM to keep the tensor
+// core busy (two 16-bit operands, 384 rows of 64 per 512 cycles), more than an SM's share of
+// L2. A pair of CTAs that multiply one 256 x 256 tile together (cta_group::2: each holds its
+// own 128 rows of A and half of B) needs 64, so large products run on pairs; smaller ones
+// on single CTAs with 128 or 64 columns, so that all SMs have a tile.
+//
+// float32 operands arrive as three bfloat16 terms each (x = x0 + x1 + x2, 24 significant
+// bits); the six products down to 2^-24 are summed. The tensor core truncates each
+// accumulation, an error that grows with the number of steps, so the leading product
+// x0 y0 is collected in TMEM for 256 of k only and then added to float32 registers, while
+// the five small products, 2^-8 of it and less, keep one accumulator for the whole tile.
+//
+// A long k with few tiles is cut into splits, whose float32 partial tiles a second launch
+// adds in order before the epilogue: repeated calls give the same bits.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstdlib>
+
+#include "activation.cuh"
+#include "layers.cuh"
+#include "pair.cuh"
+#include "product.cuh"
+
+namespace cnd {
+namespace layers {
+namespace {
+
+constexpr int kBM = 128, kBK = 64;
+constexpr int kEpilogueWarps = 8, kGroupThreads = 128;
+constexpr int kBlockThreads = 64 + 32 * kEpilogueWarps;
+constexpr uint32_t kUnitBytes = kBM * 128;  // staging tile: 128 rows of 128 bytes
+constexpr uint32_t kSharedLimit = 232448;
+constexpr int kMostStages = 8;
+constexpr int kChunkBlocks = 4;  // k blocks per float32 accumulation (three-term operands)
+constexpr uint32_t kSiteLoad = 0x501, kSiteMma = 0x502, kSiteAccumulator = 0x503,
+                   kSiteEpilogue = 0x504, kSiteDrain = 0x505;
+
+struct Maps {
+  CUtensorMap a, b, out, pre;
+};
+
+struct KernelArgs {
+  int64_t m, n;
+  int tiles_m, tiles_n, splits, k_blocks;
+  int stages, buffers;  // operand stages; staging tiles per epilogue group
+  uint32_t idesc;
+  uint32_t a_step, b_step;  // descriptor units (16 bytes) per 16 of k
+  uint32_t a_lbo, b_lbo;
+  int a_k_major, b_k_major;
+  int act, tma_out, vector_residual;
+  const void* bias;
+  const void* residual;
+  void* d;
+  void* pre;
+  unsigned int* error;
+  uint64_t timeout_ns;
+};
+
+// Tiles in groups of 8 rows of tiles, walked down the rows first, so that the tiles in
+// flight share both operands in L2.
+__device__ __forceinline__ void tile_of(const KernelArgs& a, int index, int* tm, int* tn) {
+  constexpr int kGroup = 8;
+  const int per_group = kGroup * a.tiles_n;
+  const int group = index / per_group;
+  const int first = group * kGroup;
+  const int rows = min(kGroup, a.tiles_m - first);
+  const int inside = index - group * per_group;
+  *tm = first + inside % rows;
+  *tn = inside / rows;
+}
+
+template <int kPair>
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, dev::ErrorWord err,
+                                     uint32_t site, uint64_t timeout_ns) {
+  if constexpr (kPair == 1) {
+    return dev::mbar_wait(bar, parity, err, site, timeout_ns);
+  } else {
+    if (dev::mbar_try_wait_cluster(bar, parity)) return true;
+    const uint64_t start = dev::global_timer_ns();
+    for (uint32_t spin = 0;; ++spin) {
+      if (dev::mbar_try_wait_cluster(bar, parity)) return true;
+      if ((spin & 63u) == 63u && dev::global_timer_ns() - start > timeout_ns) {
+        atomicCAS(err.word, 0u, site);
+        return false;
+      }
+    }
+  }
+}
+
+template <int kPair>
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, dev::ErrorWord err,
+                                          uint32_t site, uint64_t timeout_ns) {
+  return __all_sync(0xffffffffu, wait<kPair>(bar, parity, err, site, timeout_ns)) != 0;
+}
+
+// Writes 32 values of a row (columns half * 32 ... of a unit) into a 128-byte-wide staging
+// tile with the 128-byte TMA swizzle (16-byte chunk c of row r at chunk c ^ (r & 7)).
+template <typename Out>
+__device__ __forceinline__ void stage_row(uint8_t* tile, int row, int half, const float (&v)[32]) {
+  constexpr int kPerChunk = 16 / sizeof(Out);
+  constexpr int kChunks = 32 / kPerChunk;
+  uint8_t* base = tile + row * 128;
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    Pack<Out, kPerChunk> p;
+#pragma unroll
+    for (int i = 0; i < kPerChunk; ++i) p.v[i] = narrow<Out>(v[c * kPerChunk + i]);
+    *reinterpret_cast<Pack<Out, kPerChunk>*>(base + (((half * kChunks + c) ^ (row & 7)) * 16)) = p;
+  }
+}
+
+// Copies a staging tile to rows of a matrix that TMA cannot address, a warp per row.
+template <typename Out>
+__device__ __forceinline__ void copy_unit(const uint8_t* tile, Out* d, int64_t row0, int64_t col0,
+                                          int64_t m, int64_t n, int warp, int lane) {
+  constexpr int kColumns = 128 / sizeof(Out);
+  for (int r = warp; r < kBM; r += 4) {
+    if (row0 + r >= m) break;
+#pragma unroll
+    for (int c = lane; c < kColumns; c += 32) {
+      if (col0 + c < n) {
+        const int byte = c * static_cast<int>(sizeof(Out));
+        d[(row0 + r) * n + col0 + c] =
+            *reinterpret_cast<const Out*>(tile + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
+      }
+    }
+  }
+}
+
+template <typename Out>
+__device__ __forceinline__ void load_residual(const KernelArgs& a, int64_t row, int64_t col,
+                                              float (&r)[32]) {
+  constexpr int kPer = 16 / sizeof(Out);
+  const Out* p = static_cast<const Out*>(a.residual) + row * a.n + col;
+#pragma unroll
+  for (int c = 0; c < 32 / kPer; ++c) {
+    Pack<Out, kPer> q;
+    if (a.vector_residual) {
+      if (row < a.m && col + c * kPer < a.n) {
+        q = *reinterpret_cast<const Pack<Out, kPer>*>(p + c * kPer);
+      } else {
+        q = Pack<Out, kPer>{};
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        q.v[i] = row < a.m && col + c * kPer + i < a.n ? p[c * kPer + i] : narrow<Out>(0.0f);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) r[c * kPer + i] = widen(q.v[i]);
+  }
+}
+
+template <int kPair, int kBN, int kParts, typename Out>
+__global__ void __launch_bounds__(kBlockThreads, 1)
+    product_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ KernelArgs a) {
+  constexpr bool kExact = sizeof(Out) == 4;
+  constexpr int kColsB = kBN / kPair;  // rows of B that this CTA holds
+  constexpr uint32_t kPartA = kBM * 128, kPartB = kColsB * 128;
+  constexpr uint32_t kStageBytes = kParts * (kPartA + kPartB);
+  constexpr int kUnit = 128 / sizeof(Out);      // columns of a staging tile
+  constexpr int kGroupCols = kBN / 2 < kUnit ? kUnit : kBN / 2;  // columns of a group
+  constexpr int kHalves = kGroupCols / 32;
+  constexpr uint32_t kColumns = kParts == 1 ? 2 * kBN : 512;
+
+  extern __shared__ __align__(1024) uint8_t shared[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(shared) + 1023) & ~uintptr_t{1023});
+  uint8_t* staging = smem + a.stages * kStageBytes;
+  float* bias_s = reinterpret_cast<float*>(staging + 2 * a.buffers * kUnitBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(bias_s + kBN);
+  uint64_t* empty = full + kMostStages;
+  uint64_t* acc_full = empty + kMostStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* cross_empty = acc_empty + 2;  // three-term operands: the small products' sets
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cross_empty + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = kPair == 2 ? dev::cluster_rank() : 0;
+  const dev::ErrorWord err{a.error};
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      dev::mbar_init(&full[s], 1);
+      dev::mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      dev::mbar_init(&acc_full[s], 1);
+      dev::mbar_init(&acc_empty[s], kPair * kEpilogueWarps);
+      dev::mbar_init(&cross_empty[s], kPair * kEpilogueWarps);
+    }
+    dev::fence_barrier_init();
+  }
+  if (warp == 0) {
+    __syncwarp();
+    dev::tmem_alloc_pair<kPair>(tmem_slot, kColumns);
+  }
+  dev::tc_fence_before();
+  if constexpr (kPair == 2) {
+    dev::cluster_sync();
+  } else {
+    __syncthreads();
+  }
+  dev::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const int workers = static_cast<int>(gridDim.x) / kPair;
+  const int worker = static_cast<int>(blockIdx.x) / kPair;
+  const int items = a.tiles_m * a.tiles_n * a.splits;
+
+  if (warp == 0) {
+    // ---- TMA loads: one lane ----
+    if (lane == 0) {
+      dev::prefetch_tensormap(&maps.a);
+      dev::prefetch_tensormap(&maps.b);
+      int stage = 0;
+      uint32_t phase = 0, issued = 0;
+      bool ok = true;
+      for (int item = worker; item < items && ok; item += workers) {
+        const int split = item % a.splits;
+        int tm, tn;
+        tile_of(a, item / a.splits, &tm, &tn);
+        const int m0 = (tm * kPair + static_cast<int>(rank)) * kBM;
+        const int n0 = tn * kBN + static_cast<int>(rank) * kColsB;
+        const int first = static_cast<int>(static_cast<int64_t>(a.k_blocks) * split / a.splits);
+        const int last = static_cast<int>(static_cast<int64_t>(a.k_blocks) * (split + 1) / a.splits);
+        for (int kb = first; kb < last; ++kb) {
+          if (!wait<kPair>(&empty[stage], phase ^ 1u, err, kSiteLoad, a.timeout_ns)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) dev::mbar_arrive_expect_tx(&full[stage], kPair * kStageBytes);
+          const uint32_t bar =
+              kPair == 2 ? dev::map_to_rank(&full[stage], 0) : dev::smem_u32(&full[stage]);
+          uint8_t* dst = smem + stage * kStageBytes;
+#pragma unroll
+          for (int p = 0; p < kParts; ++p) {
+            if (a.a_k_major) {
+              dev::tma_load_3d_to<kPair>(dst, &maps.a, bar, kb * kBK, m0, p);
+            } else {
+#pragma unroll
+              for (int i = 0; i < kBM / 64; ++i) {
+                dev::tma_load_3d_to<kPair>(dst + i * (kBK * 128), &maps.a, bar, m0 + 64 * i,
+                                           kb * kBK, p);
+              }
+            }
+            dst += kPartA;
+          }
+#pragma unroll
+          for (int p = 0; p < kParts; ++p) {
+            if (a.b_k_major) {
+              dev::tma_load_3d_to<kPair>(dst, &maps.b, bar, kb * kBK, n0, p);
+            } else {
+#pragma unroll
+              for (int i = 0; i < kColsB / 64; ++i) {
+                dev::tma_load_3d_to<kPair>(dst + i * (kBK * 128), &maps.b, bar, n0 + 64 * i,
+                                           kb * kBK, p);
+              }
+            }
+            dst += kPartB;
+          }
+          ++issued;
+          if (++stage == a.stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok && issued > 0 && rank == 0) {
+        // give loads in flight a bounded time to land before the block may exit
+        const int previous = stage == 0 ? a.stages - 1 : stage - 1;
+        wait<kPair>(&full[previous], stage == 0 ? phase ^ 1u : phase, err, kSiteDrain,
+                    a.timeout_ns / 8 + 1);
+      }
+    }
+  } else if (warp == 1) {
+    // ---- MMAs: the leader CTA's warp, converged; elect.sync issues ----
+    if (rank == 0) {
+      const uint32_t base = dev::warp_uniform(tmem);
+      const uint64_t a_hi = dev::make_smem_desc(0, a.a_lbo, 1024, 2);
+      const uint64_t b_hi = dev::make_smem_desc(0, a.b_lbo, 1024, 2);
+      int stage = 0;
+      uint32_t phase = 0;
+      int set = 0, cross = 0;
+      uint32_t set_phase = 0, cross_phase = 0;
+      bool ok = true;
+      for (int item = worker; item < items && ok; item += workers) {
+        const int split = item % a.splits;
+        const int first = static_cast<int>(static_cast<int64_t>(a.k_blocks) * split / a.splits);
+        const int last = static_cast<int>(static_cast<int64_t>(a.k_blocks) * (split + 1) / a.splits);
+        if constexpr (kParts == 3) {
+          if (!wait_warp<kPair>(&cross_empty[cross], cross_phase ^ 1u, err, kSiteAccumulator,
+                                a.timeout_ns)) {
+            break;
+          }
+        }
+        const uint32_t d_cross = base + 256 + cross * kBN;
+        for (int kb = first; kb < last && ok;) {
+          if (!wait_warp<kPair>(&acc_empty[set], set_phase ^ 1u, err, kSiteAccumulator,
+                                a.timeout_ns)) {
+            ok = false;
+            break;
+          }
+          dev::tc_fence_after();
+          const uint32_t d = base + set * kBN;
+          const int stop = kParts == 3 ? min(kb + kChunkBlocks, last) : last;
+          for (const int begin = kb; kb < stop; ++kb) {
+            if (!wait_warp<kPair>(&full[stage], phase, err, kSiteMma, a.timeout_ns)) {
+              ok = false;
+              break;
+            }
+            dev::tc_fence_after();
+            const uint32_t as = dev::warp_uniform(dev::smem_u32(smem + stage * kStageBytes) >> 4);
+            const uint32_t bs = as + (kParts * kPartA >> 4);
+#pragma unroll
+            for (int ks = 0; ks < kBK / 16; ++ks) {
+              const uint32_t ao = as + ks * a.a_step, bo = bs + ks * a.b_step;
+              if constexpr (kParts == 1) {
+                dev::mma_f16_pair<kPair>(d, a_hi | ao, b_hi | bo, a.idesc, kb > begin || ks > 0);
+              } else {
+                constexpr uint32_t pa = kPartA >> 4, pb = kPartB >> 4;
+                const uint32_t more = kb > first || ks > 0;
+                dev::mma_f16_pair<kPair>(d_cross, a_hi | (ao + 2 * pa), b_hi | bo, a.idesc, more);
+                dev::mma_f16_pair<kPair>(d_cross, a_hi | ao, b_hi | (bo + 2 * pb), a.idesc, 1);
+                dev::mma_f16_pair<kPair>(d_cross, a_hi | (ao + pa), b_hi | (bo + pb), a.idesc, 1);
+                dev::mma_f16_pair<kPair>(d_cross, a_hi | (ao + pa), b_hi | bo, a.idesc, 1);
+                dev::mma_f16_pair<kPair>(d_cross, a_hi | ao, b_hi | (bo + pb), a.idesc, 1);
+                dev::mma_f16_pair<kPair>(d, a_hi | ao, b_hi | bo, a.idesc, kb > begin || ks > 0);
+              }
+            }
+            dev::mma_commit_pair<kPair>(&empty[stage]);
+            if (++stage == a.stages) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+          dev::mma_commit_pair<kPair>(&acc_full[set]);
+          if (++set == 2) {
+            set = 0;
+            set_phase ^= 1u;
+          }
+        }
+        if constexpr (kParts == 3) {
+          if (++cross == 2) {
+            cross = 0;
+            cross_phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else {
+    // ---- epilogue: two groups of four warps, each a half of the tile's columns ----
+    const int group = (warp - 2) >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const int epi = threadIdx.x - 64;
+    const bool leader = (epi & (kGroupThreads - 1)) == 0;
+    const bool works = group * kGroupCols < kBN;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t release = kPair == 2 ? dev::map_to_rank(&acc_empty[0], 0) : 0;
+    const uint32_t release_cross = kPair == 2 ? dev::map_to_rank(&cross_empty[0], 0) : 0;
+    uint8_t* own = staging + group * a.buffers * kUnitBytes;
+    const auto free_set = [&](uint64_t* bars, uint32_t remote, int s) {
+      dev::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (kPair == 2) {
+          dev::mbar_arrive_cluster(remote + 8 * s);
+        } else {
+          dev::mbar_arrive(&bars[s]);
+        }
+      }
+    };
+    int set = 0, cross = 0, buffer = 0;
+    uint32_t set_phase = 0;
+    bool ok = true;
+    for (int item = worker; item < items && ok; item += workers) {
+      const int split = item % a.splits;
+      int tm, tn;
+      tile_of(a, item / a.splits, &tm, &tn);
+      const int64_t row0 = static_cast<int64_t>(tm * kPair + static_cast<int>(rank)) * kBM;
+      const int64_t col0 = static_cast<int64_t>(tn) * kBN + group * kGroupCols;
+      // bias of the tile's columns, after every thread has finished the previous tile's
+      dev::named_barrier(1, 32 * kEpilogueWarps);
+      for (int c = epi; c < kBN; c += 32 * kEpilogueWarps) {
+        const int64_t column = static_cast<int64_t>(tn) * kBN + c;
+        bias_s[c] = a.bias != nullptr && column < a.n
+                        ? widen(static_cast<const Out*>(a.bias)[column])
+                        : 0.0f;
+      }
+      dev::named_barrier(1, 32 * kEpilogueWarps);
+
+      float sums[kParts == 3 ? kHalves : 1][32];
+      if constexpr (kParts == 3) {
+        const int first = static_cast<int>(static_cast<int64_t>(a.k_blocks) * split / a.splits);
+        const int last = static_cast<int>(static_cast<int64_t>(a.k_blocks) * (split + 1) / a.splits);
+        for (int kb = first; kb < last; kb += kChunkBlocks) {
+          if (!wait_warp<kPair>(&acc_full[set], set_phase, err, kSiteEpilogue, a.timeout_ns)) {
+            ok = false;
+            break;
+          }
+          dev::tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h) {
+            uint32_t v[32];
+            dev::tmem_load32(tmem + lanes + set * kBN + group * kGroupCols + h * 32, v);
+            dev::tmem_load_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              sums[h][i] = kb == first ? __uint_as_float(v[i]) : sums[h][i] + __uint_as_float(v[i]);
+            }
+          }
+          free_set(acc_empty, release, set);
+          if (++set == 2) {
+            set = 0;
+            set_phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          uint32_t v[32];
+          dev::tmem_load32(tmem + lanes + 256 + cross * kBN + group * kGroupCols + h * 32, v);
+          dev::tmem_load_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sums[h][i] += __uint_as_float(v[i]);
+        }
+        free_set(cross_empty, release_cross, cross);
+        cross ^= 1;
+      } else {
+        if (!wait_warp<kPair>(&acc_full[set], set_phase, err, kSiteEpilogue, a.timeout_ns)) {
+          ok = false;
+          break;
+        }
+        dev::tc_fence_after();
+      }
+
+      const uint32_t acc = tmem + lanes + set * kBN + group * kGroupCols;
+      uint8_t *tile = own, *pre_tile = own;
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        constexpr int kHalvesPerUnit = kUnit / 32;
+        if (!works) break;
+        if (h % kHalvesPerUnit == 0) {
+          // a free staging tile for this unit (and one for its pre-activation)
+          if (leader) {
+            if (a.buffers == 2 && a.pre == nullptr) {
+              dev::bulk_wait_group_read<1>();
+            } else {
+              dev::bulk_wait_group_read<0>();
+            }
+          }
+          dev::named_barrier(2 + group, kGroupThreads);
+          tile = own + buffer * kUnitBytes;
+          pre_tile = own + (a.buffers - 1) * kUnitBytes;
+          if (a.buffers == 2 && a.pre == nullptr) buffer ^= 1;
+        }
+        float v[32], r[32];
+        if (kParts == 1 && a.residual != nullptr) {
+          load_residual<Out>(a, row0 + row, col0 + h * 32, r);
+        }
+        if constexpr (kParts == 3) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = sums[h][i];
+        } else {
+          uint32_t raw[32];
+          dev::tmem_load32(acc + h * 32, raw);
+          dev::tmem_load_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
+          if (h == kHalves - 1) free_set(acc_empty, release, set);
+        }
+        const float* bias = bias_s + group * kGroupCols + h * 32;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 b4 = *reinterpret_cast<const float4*>(bias + i);
+          v[i] += b4.x;
+          v[i + 1] += b4.y;
+          v[i + 2] += b4.z;
+          v[i + 3] += b4.w;
+        }
+        const int64_t unit_col = col0 + (h / kHalvesPerUnit) * kUnit;
+        const bool unit_done = h % kHalvesPerUnit == kHalvesPerUnit - 1;
+        if (a.pre != nullptr) {
+          stage_row<Out>(pre_tile, row, h % kHalvesPerUnit, v);
+          if (a.buffers == 1) {
+            // one staging tile: the pre-activation leaves before the output is staged (units
+            // of one half only: float32)
+            dev::fence_proxy_async();
+            dev::named_barrier(2 + group, kGroupThreads);
+            if (a.tma_out) {
+              if (leader && unit_col < a.n) {
+                dev::tma_store_2d(&maps.pre, pre_tile, static_cast<int>(unit_col),
+                                  static_cast<int>(row0));
+                dev::bulk_commit_group();
+                dev::bulk_wait_group_read<0>();
+              }
+            } else {
+              copy_unit<Out>(pre_tile, static_cast<Out*>(a.pre), row0, unit_col, a.m, a.n, quarter,
+                             lane);
+            }
+            dev::named_barrier(2 + group, kGroupThreads);
+          }
+        }
+        if (a.act == CND_ACT_GELU) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = activate<kExact>(v[i], CND_ACT_GELU);
+        } else if (a.act == CND_ACT_SILU) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = activate<kExact>(v[i], CND_ACT_SILU);
+        }
+        if (a.residual != nullptr) {
+          if (kParts == 3) load_residual<Out>(a, row0 + row, col0 + h * 32, r);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += r[i];
+        }
+        stage_row<Out>(tile, row, h % kHalvesPerUnit, v);
+        if (unit_done) {
+          dev::fence_proxy_async();
+          dev::named_barrier(2 + group, kGroupThreads);
+          if (a.tma_out) {
+            if (leader && unit_col < a.n) {
+              // partial tiles of a split lie below one another
+              const int y = static_cast<int>(row0) + split * a.tiles_m * kPair * kBM;
+              if (row0 < a.m) {
+                dev::tma_store_2d(&maps.out, tile, static_cast<int>(unit_col), y);
+                if (a.pre != nullptr && a.buffers == 2) {
+                  dev::tma_store_2d(&maps.pre, pre_tile, static_cast<int>(unit_col),
+                                    static_cast<int>(row0));
+                }
+              }
+            }
+            if (leader) dev::bulk_commit_group();
+          } else {
+            copy_unit<Out>(tile, static_cast<Out*>(a.d), row0, unit_col, a.m, a.n, quarter, lane);
+            if (a.pre != nullptr && a.buffers == 2) {
+              copy_unit<Out>(pre_tile, static_cast<Out*>(a.pre), row0, unit_col, a.m, a.n, quarter,
+                             lane);
+            }
+          }
+        }
+      }
+      if constexpr (kParts == 1) {
+        if (!works) free_set(acc_empty, release, set);
+        if (++set == 2) {
+          set = 0;
+          set_phase ^= 1u;
+        }
+      }
+    }
+    if (leader) dev::bulk_wait_group<0>();
+  }
+  dev::tc_fence_before();
+  if constexpr (kPair == 2) {
+    dev::cluster_sync();
+  } else {
+    __syncthreads();
+  }
+  if (warp == 0) {
+    dev::tc_fence_after();
+    __syncwarp();
+    dev::tmem_dealloc_pair<kPair>(tmem, kColumns);
+  }
+}
+
+// Adds the partial tiles of a split product in split order and applies the epilogue.
+template <typename Out>
+__global__ void __launch_bounds__(256)
+    join_kernel(const float* partials, int splits, int64_t split_stride, int64_t pitch, int64_t m,
+                int64_t n, const void* bias, const void* residual, void* d, void* pre, int act) {
+  constexpr bool kExact = sizeof(Out) == 4;
+  const int64_t quads = pitch / 4, count = m * quads;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += step) {
+    const int64_t row = i / quads, col = i % quads * 4;
+    const float* p = partials + row * pitch + col;
+    float4 sum = *reinterpret_cast<const float4*>(p);
+#pragma unroll 4
+    for (int s = 1; s < splits; ++s) {
+      const float4 v = *reinterpret_cast<const float4*>(p + s * split_stride);
+      sum.x += v.x;
+      sum.y += v.y;
+      sum.z += v.z;
+      sum.w += v.w;
+    }
+    const float v4[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t c = col + j;
+      if (c >= n) break;
+      float v = v4[j];
+      if (bias != nullptr) v += widen(static_cast<const Out*>(bias)[c]);
+      if (pre != nullptr) static_cast<Out*>(pre)[row * n + c] = narrow<Out>(v);
+      v = activate<kExact>(v, act);
+      if (residual != nullptr) v += widen(static_cast<const Out*>(residual)[row * n + c]);
+      static_cast<Out*>(d)[row * n + c] = narrow<Out>(v);
+    }
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult status;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &status) !=
+            cudaSuccess ||
+        status != cudaDriverEntryPointSuccess) {
+      fn = nullptr;
+    }
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  }();
+  return encode;
+}
+
+bool encode_operand(CUtensorMap* map, const Operand& o, int64_t rows, int64_t k, int parts,
+                    bool bf16, int box_rows) {
+  const cuuint64_t inner = static_cast<cuuint64_t>(o.k_major ? k : rows);
+  const cuuint64_t outer = static_cast<cuuint64_t>(o.k_major ? rows : k);
+  const cuuint64_t dims[3] = {inner, outer, static_cast<cuuint64_t>(parts)};
+  const int64_t plane = parts > 1 ? o.plane : o.pitch * static_cast<int64_t>(outer);
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(o.pitch) * 2,
+                                 static_cast<cuuint64_t>(plane) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(o.k_major ? box_rows : kBK), 1};
+  const cuuint32_t ones[3] = {1, 1, 1};
+  return encoder()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                   3, const_cast<void*>(o.data), dims, strides, box, ones,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool encode_output(CUtensorMap* map, void* d, int dtype, int64_t rows, int64_t n, int64_t pitch) {
+  const int size = element_size(dtype);
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch) * size};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), kBM};
+  const cuuint32_t ones[2] = {1, 1};
+  const CUtensorMapDataType type = dtype == CND_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == CND_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return encoder()(map, type, 2, d, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+using Kernel = void (*)(Maps, KernelArgs);
+
+template <typename Out>
+Kernel pick(const ProductPlan& plan, int parts) {
+  if constexpr (sizeof(Out) == 4) {
+    if (parts == 3) return product_tc_kernel<1, 128, 3, Out>;
+  }
+  if (plan.pair == 2) return product_tc_kernel<2, 256, 1, Out>;
+  return plan.bn == 128 ? product_tc_kernel<1, 128, 1, Out> : product_tc_kernel<1, 64, 1, Out>;
+}
+
+uint64_t wait_timeout() {
+  static const uint64_t value = [] {
+    const char* env = std::getenv("CND_WAIT_TIMEOUT_MS");
+    const long long parsed = env != nullptr ? std::atoll(env) : 0;
+    return (parsed > 0 ? static_cast<uint64_t>(parsed) : uint64_t{2000}) * 1000000u;
+  }();
+  return value;
+}
+
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+}  // namespace
+
+ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts) {
+  // Times in cycles of one SM: an operand block of 64 by bn columns takes bn * 2 cycles of
+  // the tensor core (six products: 12), an epilogue 10 per column, a launch that joins splits
+  // the time of its traffic.
+  const int64_t sms = 148, blocks = (k + kBK - 1) / kBK;
+  ProductPlan best{1, 64, 1};
+  double best_cost = 0;
+  for (int pair = 2; pair >= 1; --pair) {
+    for (int bn : {256, 128, 64}) {
+      if ((pair == 2) != (bn == 256) || (parts == 3 && bn != 128)) continue;
+      const int64_t tiles = ((m + kBM * pair - 1) / (kBM * pair)) * ((n + bn - 1) / bn);
+      const int64_t slots = sms / pair;
+      for (int64_t splits = 1; splits <= 64; ++splits) {
+        if (splits > 1 && (blocks / splits < 4 || tiles * splits > 2 * slots)) break;
+        const int64_t waves = (tiles * splits + slots - 1) / slots;
+        const double main = static_cast<double>((blocks + splits - 1) / splits) * bn * 2 *
+                            (parts == 3 ? 6 : 1) * (bn == 64 ? 1.5 : 1.0);
+        const double tail = 10.0 * bn + 1500;
+        double cost = waves * std::max(main, tail) + std::min(main, tail) + 1500;
+        if (splits > 1) {
+          cost += 6000 + static_cast<double>(splits + 1) * m * n * 4 / 3000.0;
+        }
+        if (best_cost == 0 || cost < best_cost) {
+          best_cost = cost;
+          best = ProductPlan{pair, bn, static_cast<int>(splits)};
+        }
+      }
+    }
+  }
+  return best;
+}
+
+size_t product_workspace(const ProductPlan& plan, int64_t m, int64_t n) {
+  if (plan.splits <= 1) return 0;
+  return static_cast<size_t>(plan.splits) * round_up(m, kBM * plan.pair) * round_up(n, 4) *
+         sizeof(float);
+}
+
+int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
+                   cudaStream_t stream) {
+  if (encoder() == nullptr) return fail(CND_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const int bm = kBM * plan.pair;
+  const bool split = plan.splits > 1;
+  if (round_up(p.m, bm) * plan.splits > INT32_MAX || p.n > INT32_MAX - 256 ||
+      p.k > INT32_MAX - 64) {
+    return fail(CND_ERR_UNSUPPORTED, "linear: a matrix dimension exceeds 2^31");
+  }
+  KernelArgs a{};
+  a.m = p.m;
+  a.n = p.n;
+  a.tiles_m = static_cast<int>((p.m + bm - 1) / bm);
+  a.tiles_n = static_cast<int>((p.n + plan.bn - 1) / plan.bn);
+  a.splits = plan.splits;
+  a.k_blocks = static_cast<int>((p.k + kBK - 1) / kBK);
+  if (static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits > INT32_MAX) {
+    return fail(CND_ERR_UNSUPPORTED, "linear: too many tiles");
+  }
+  const int out_dtype = split ? static_cast<int>(CND_F32) : p.dtype;
+  a.buffers = p.parts == 3 ? 1 : 2;
+  const uint32_t stage = p.parts * (kBM + plan.bn / plan.pair) * 128;
+  const uint32_t fixed = 1024 + 2 * a.buffers * kUnitBytes + plan.bn * sizeof(float) + 256;
+  a.stages = static_cast<int>(std::min<uint32_t>((kSharedLimit - fixed) / stage, kMostStages));
+  const uint32_t shared = fixed + a.stages * stage;
+  a.idesc = (1u << 4) | ((p.bf16 ? 1u : 0u) << 7) | ((p.bf16 ? 1u : 0u) << 10) |
+            (p.a.k_major ? 0u : 1u << 15) | (p.b.k_major ? 0u : 1u << 16) |
+            (static_cast<uint32_t>(plan.bn) >> 3 << 17) | (static_cast<uint32_t>(bm) >> 4 << 24);
+  a.a_k_major = p.a.k_major;
+  a.b_k_major = p.b.k_major;
+  a.a_step = (p.a.k_major ? 32 : 16 * 128) >> 4;
+  a.b_step = (p.b.k_major ? 32 : 16 * 128) >> 4;
+  a.a_lbo = p.a.k_major ? 16 : kBK * 128;
+  a.b_lbo = p.b.k_major ? 16 : kBK * 128;
+  a.error = device_error_word();
+  a.timeout_ns = wait_timeout();
+  if (a.error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
+  Maps maps{};
+  if (!encode_operand(&maps.a, p.a, p.m, p.k, p.parts, p.bf16, kBM) ||
+      !encode_operand(&maps.b, p.b, p.n, p.k, p.parts, p.bf16, plan.bn / plan.pair)) {
+    return fail(CND_ERR_CUDA, "linear: encoding an operand's tensor map failed");
+  }
+  const int64_t pitch = round_up(p.n, 4);
+  if (split) {
+    // partial tiles below one another, each split's rows rounded up to whole tiles
+    a.tma_out = 1;
+    if (!encode_output(&maps.out, workspace, CND_F32, round_up(p.m, bm) * plan.splits, pitch,
+                       pitch)) {
+      return fail(CND_ERR_CUDA, "linear: encoding the partial sums' tensor map failed");
+    }
+  } else {
+    const int size = element_size(p.dtype);
+    a.bias = p.bias;
+    a.residual = p.residual;
+    a.d = p.d;
+    a.pre = p.pre;
+    a.act = p.act;
+    a.vector_residual = aligned16(p.residual) && p.n * size % 16 == 0;
+    a.tma_out = p.n * size % 16 == 0 && aligned16(p.d) && aligned16(p.pre);
+    if (a.tma_out &&
+        (!encode_output(&maps.out, p.d, p.dtype, p.m, p.n, p.n) ||
+         (p.pre != nullptr && !encode_output(&maps.pre, p.pre, p.dtype, p.m, p.n, p.n)))) {
+      return fail(CND_ERR_CUDA, "linear: encoding an output's tensor map failed");
+    }
+  }
+  const Kernel kernel = out_dtype == CND_F32    ? pick<float>(plan, p.parts)
+                        : out_dtype == CND_BF16 ? pick<__nv_bfloat16>(plan, p.parts)
+                                                : pick<__half>(plan, p.parts);
+  const int items = a.tiles_m * a.tiles_n * a.splits;
+  const int slots = sm_count() / plan.pair;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(std::min(items, slots) * plan.pair));
+  config.blockDim = dim3(kBlockThreads);
+  config.dynamicSmemBytes = shared;
+  config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  if (plan.pair == 2) {
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = 2;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+  }
+  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(kSharedLimit));
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&config, kernel, maps, a);
+  if (e != cudaSuccess) return fail(CND_ERR_CUDA, "linear: %s", cudaGetErrorString(e));
+  count_launch();
+  if (split) {
+    const int64_t quads = p.m * (pitch / 4);
+    const unsigned grid = static_cast<unsigned>(
+        std::min<int64_t>((quads + 255) / 256, static_cast<int64_t>(sm_count()) * 8));
+    const int64_t stride = round_up(p.m, bm) * pitch;
+    const float* partials = static_cast<const float*>(workspace);
+    const auto join = [&](auto* kernel_join) {
+      kernel_join<<<grid, 256, 0, stream>>>(partials, plan.splits, stride, pitch, p.m, p.n, p.bias,
+                                            p.residual, p.d, p.pre, p.act);
+    };
+    if (p.dtype == CND_F32) {
+      join(join_kernel<float>);
+    } else if (p.dtype == CND_BF16) {
+      join(join_kernel<__nv_bfloat16>);
+    } else {
+      join(join_kernel<__half>);
+    }
+    count_launch();
+  }
+  return launch_status("linear");
+}
+
+}  // namespace layers
+}  // namespace cnd

@@ -107,6 +107,11 @@ Rows as_rows(const at::Tensor& t) {
   return {t, stride == 0 ? width : stride};
 }
 
+// A copy where the data does not start on a 16-byte boundary.
+at::Tensor aligned(const at::Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 ? t : t.clone();
+}
+
 int64_t leading(const at::Tensor& t) {
   int64_t rows = 1;
   for (int64_t d = 0; d + 1 < t.dim(); ++d) rows *= t.size(d);
@@ -366,9 +371,9 @@ std::tuple<at::Tensor, at::Tensor> linear_forward(const at::Tensor& input,
                                                   c10::string_view activation, bool train) {
   cnd_linear p = check_linear(input, weight, bias, residual, activation);
   const c10::cuda::CUDAGuard guard(input.device());
-  const Rows x = as_rows(input);
+  const Rows x = as_rows(aligned(input));
   p.x_stride = x.stride;
-  const at::Tensor w = weight.contiguous();
+  const at::Tensor w = aligned(weight.contiguous());
   OptTensor b, r;
   if (given(bias)) b = bias->contiguous();
   if (given(residual)) r = residual->contiguous();
@@ -418,10 +423,10 @@ Grads linear_backward_cuda(const at::Tensor& grad_output, const at::Tensor& pre,
                            c10::string_view activation, Mask output_mask) {
   cnd_linear p = check_linear_backward(grad_output, pre, input, weight, activation);
   const c10::cuda::CUDAGuard guard(input.device());
-  const Rows x = as_rows(input);
+  const Rows x = as_rows(aligned(input));
   p.x_stride = x.stride;
-  const at::Tensor dy = grad_output.contiguous(), w = weight.contiguous();
-  const at::Tensor z = pre.contiguous();
+  const at::Tensor dy = aligned(grad_output.contiguous()), w = aligned(weight.contiguous());
+  const at::Tensor z = aligned(pre.contiguous());
   OptTensor dx, dweight, dbias;
   if (output_mask[0]) dx = at::empty(input.sizes(), input.options());
   if (output_mask[1]) dweight = at::empty(weight.sizes(), weight.options());
