@@ -1,97 +1,844 @@
 // Gated linear recurrence along the middle axis of [outer][steps][inner]:
 //
 //   f_t = sigmoid(g_t),  h_t = f_t h_{t-1} + (1 - f_t) x_t;
-//   G_t = dy_t + f_{t+1} G_{t+1},  dx_t = (1 - f_t) G_t,
-//   dg_t = f_t (1 - f_t) (h_{t-1} - x_t) G_t,  dh_{-1} = f_0 G_0.
+//   q_t = f_t (dy_t + q_{t+1}),  dx_t = (1 - f_t) (dy_t + q_{t+1}),
+//   dg_t = f_t (1 - f_t) (h_{t-1} - x_t) (dy_t + q_{t+1}),  dh_{-1} = q_0.
 //
-// One thread per column walks the steps. The forward keeps the state before each block of
-// kBlockSteps steps, from which the backward recomputes the others in float32, so it reads
-// x, g and dy only and its h carry no rounding to the tensors' type.
+// A run of steps acts on a state as one affine map h -> a h + b, and maps compose:
+// (a1, b1) then (a2, b2) is (a1 a2, a2 b1 + b2). So a thread reduces a few consecutive steps
+// to a map, a block composes its threads' maps in shared memory to find the state each of
+// them starts from, and the thread then walks its steps from that state: x, g and dy are
+// read once and stay in registers between the two walks. The work is bound by memory
+// traffic: 3 elements a step forward, 5 backward.
+//
+// Column layout (inner > 1): the lanes of a warp hold neighbouring columns, the warps of a
+// block follow one another in time. Step layout (inner = 1, steps contiguous): the lanes of a
+// warp hold neighbouring runs of steps of one column and compose their maps by shuffles.
+//
+// A block that has its columns to itself loops over the chunks of the time axis. Where
+// the columns are too few to fill the SMs, every (chunk, column block) is a block of its own
+// and chunks exchange their maps through global memory: blocks take tickets in time order,
+// so whoever a block waits for is already running; each chunk composes the maps of the
+// chunks before it in its group of kGroup, in order, with the state that the last chunk
+// of the group before published. The association is fixed, so repeated calls give the
+// same bits. Waits are bounded and end at once when any wait has expired.
+//
+// The forward keeps the state before each block of 64 steps (256 in step layout), from which
+// the backward recomputes the others in float32: it reads x, g and dy only, and its states
+// carry no rounding to the tensors' type.
 #include <algorithm>
+#include <cstdlib>
 
 #include "layers.cuh"
+#include "ptx.cuh"
 
 namespace cnd {
 namespace layers {
 namespace {
 
-constexpr int kBlockSteps = 16;
-constexpr int kThreads = 128;
+constexpr int kWarps = 8;       // most warps of a block
+constexpr int kGroup = 32;      // chunks that are composed without an intermediate state
+constexpr uint32_t kSiteForward = 0x601, kSiteBackward = 0x602;
+
+// Steps a thread holds: forward and backward in column layout, both in step layout.
+constexpr int kForwardSteps = 16, kBackwardSteps = 8, kAlongSteps = 8;
+constexpr int kStateBlock = kBackwardSteps * kWarps;  // 64
+constexpr int kAlongBlock = 32 * kAlongSteps;         // 256
+
+template <typename A>
+struct Map {
+  A a, b;
+};
+
+// `first`, then `second`.
+template <typename A>
+__device__ __forceinline__ Map<A> then(const Map<A>& first, const Map<A>& second) {
+  return {first.a * second.a, second.a * first.b + second.b};
+}
 
 struct RecurrenceArgs {
   const void *x, *gate, *initial, *dy, *dlast, *states_in;
   void *y, *last, *states, *dx, *dgate, *dinitial;
-  int64_t outer, steps, inner;
+  int64_t outer, steps, inner, columns;
+  int64_t chunks;
+  int column_blocks;
+  // exchange between chunks (shared != 0): maps [chunks][padded], states [groups][padded],
+  // flags [chunks + groups][column_blocks], one ticket counter
+  int shared;
+  void *maps, *bases;
+  unsigned int *flags, *ticket, *error;
+  uint64_t timeout_ns;
 };
 
-// f = sigmoid(g) and 1 - f, each to full relative accuracy (exact 0 and 1 at +-inf).
-template <typename A>
+__device__ __forceinline__ int steps_here(int64_t left, int most) {
+  return left < 0 ? 0 : left < most ? static_cast<int>(left) : most;
+}
+
+// f = sigmoid(g) and 1 - f, each to full relative accuracy (exact 0 and 1 at +-inf). For
+// 16-bit tensors by the fast exponential and reciprocal, good to 2^-20.
+template <typename T, typename A>
 __device__ __forceinline__ void gates(A g, A* f, A* keep) {
-  const A e = exp(-fabs(g));
-  const A r = A(1) / (A(1) + e);
-  *f = g >= A(0) ? r : e * r;
-  *keep = g >= A(0) ? e * r : r;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) recurrence_forward_kernel(const RecurrenceArgs a) {
-  using A = typename Wide<T>::type;
-  const int64_t columns = a.outer * a.inner;
-  const int64_t column = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (column >= columns) return;
-  const int64_t base = column / a.inner * a.steps * a.inner + column % a.inner;
-  const T* x = static_cast<const T*>(a.x) + base;
-  const T* gate = static_cast<const T*>(a.gate) + base;
-  T* y = static_cast<T*>(a.y) + base;
-  A h = a.initial != nullptr ? static_cast<const A*>(a.initial)[column] : A(0);
-  for (int64_t t = 0; t < a.steps; ++t) {
-    if (a.states != nullptr && t % kBlockSteps == 0) {
-      static_cast<A*>(a.states)[t / kBlockSteps * columns + column] = h;
-    }
-    A f, keep;
-    gates<A>(widen(gate[t * a.inner]), &f, &keep);
-    h = f * h + keep * widen(x[t * a.inner]);
-    y[t * a.inner] = narrow<T>(h);
+  A e, r;
+  if constexpr (sizeof(T) == 2) {
+    e = __expf(-fabsf(g));
+    r = __fdividef(1.0f, 1.0f + e);
+  } else {
+    e = exp(-fabs(g));
+    r = A(1) / (A(1) + e);
   }
-  static_cast<A*>(a.last)[column] = h;
+  const A s = e * r;
+  *f = g >= A(0) ? r : s;
+  *keep = g >= A(0) ? s : r;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) recurrence_backward_kernel(const RecurrenceArgs a) {
-  using A = typename Wide<T>::type;
-  const int64_t columns = a.outer * a.inner;
-  const int64_t column = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (column >= columns) return;
-  const int64_t base = column / a.inner * a.steps * a.inner + column % a.inner;
-  const T* x = static_cast<const T*>(a.x) + base;
-  const T* gate = static_cast<const T*>(a.gate) + base;
-  const T* dy = a.dy != nullptr ? static_cast<const T*>(a.dy) + base : nullptr;
-  A flow = a.dlast != nullptr ? static_cast<const A*>(a.dlast)[column] : A(0);
-  for (int64_t block = (a.steps - 1) / kBlockSteps; block >= 0; --block) {
-    const int64_t first = block * kBlockSteps;
-    const int count = static_cast<int>(a.steps - first < kBlockSteps ? a.steps - first : kBlockSteps);
-    A before[kBlockSteps];
-    A h = static_cast<const A*>(a.states_in)[block * columns + column];
-    for (int i = 0; i < count; ++i) {
-      before[i] = h;
-      A f, keep;
-      gates<A>(widen(gate[(first + i) * a.inner]), &f, &keep);
-      h = f * h + keep * widen(x[(first + i) * a.inner]);
-    }
-    for (int i = count - 1; i >= 0; --i) {
-      const int64_t at = (first + i) * a.inner;
-      A f, keep;
-      gates<A>(widen(gate[at]), &f, &keep);
-      const A total = flow + (dy != nullptr ? widen(dy[at]) : A(0));
-      if (a.dx != nullptr) static_cast<T*>(a.dx)[base + at] = narrow<T>(keep * total);
-      if (a.dgate != nullptr) {
-        static_cast<T*>(a.dgate)[base + at] =
-            narrow<T>(f * keep * (before[i] - widen(x[at])) * total);
+__device__ __forceinline__ unsigned int load_acquire(const unsigned int* p) {
+  unsigned int v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void store_release(unsigned int* p, unsigned int v) {
+  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+
+// Waits, a whole warp, until *flag is set. Gives up (error word set) after the timeout, or
+// as soon as another wait has.
+__device__ __forceinline__ void wait_flag(const unsigned int* flag, const RecurrenceArgs& a,
+                                          unsigned int site) {
+  if ((threadIdx.x & 31) == 0 && load_acquire(flag) == 0) {
+    const uint64_t start = dev::global_timer_ns();
+    for (uint32_t spin = 1; load_acquire(flag) == 0; ++spin) {
+      if (spin % 64 == 0) {
+        if (*static_cast<volatile unsigned int*>(a.error) != 0) break;
+        if (dev::global_timer_ns() - start > a.timeout_ns) {
+          atomicCAS(a.error, 0u, site);
+          break;
+        }
       }
-      flow = f * total;
     }
   }
-  if (a.dinitial != nullptr) static_cast<A*>(a.dinitial)[column] = flow;
+  __syncwarp();
+}
+
+// Sets *flag after the warp's earlier stores.
+__device__ __forceinline__ void publish(unsigned int* flag) {
+  __threadfence();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) store_release(flag, 1u);
+}
+
+template <typename A>
+__device__ __forceinline__ Map<A> load_map(const void* maps, int64_t i) {
+  if constexpr (sizeof(A) == 4) {
+    const float2 v = __ldcg(static_cast<const float2*>(maps) + i);
+    return {v.x, v.y};
+  } else {
+    const double2 v = __ldcg(static_cast<const double2*>(maps) + i);
+    return {v.x, v.y};
+  }
+}
+
+// V columns (or one column's run of steps) of a thread, loaded at once where they lie together.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+  return *reinterpret_cast<const Pack<T, V>*>(p);
+}
+
+template <typename A>
+__device__ __forceinline__ Map<A> shuffle_up(const Map<A>& m, int d) {
+  return {__shfl_up_sync(0xffffffffu, m.a, d), __shfl_up_sync(0xffffffffu, m.b, d)};
+}
+template <typename A>
+__device__ __forceinline__ Map<A> shuffle_down(const Map<A>& m, int d) {
+  return {__shfl_down_sync(0xffffffffu, m.a, d), __shfl_down_sync(0xffffffffu, m.b, d)};
+}
+
+// The state at this chunk's start, for column slot `slot` of `slots` of the block, from
+// the chunks before it (order = 0, 1, ... in the direction of the walk). `scratch`:
+// [kWarps][slots] maps. `begin` is the state before the first chunk. Every thread of the
+// block calls it; warp w composes the 4 maps w * 4 ... of the group.
+template <typename A, int kSlots>
+__device__ __forceinline__ void look_back(const RecurrenceArgs& a, int64_t order, int block,
+                                          Map<A>* scratch, unsigned int site) {
+  constexpr int kEach = kGroup / kWarps;
+  constexpr int kPer = kSlots > 32 ? kSlots / 32 : 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t first = order / kGroup * kGroup;
+  const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
+  Map<A> m[kPer];
+#pragma unroll
+  for (int v = 0; v < kPer; ++v) m[v] = {A(1), A(0)};
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int64_t at = first + warp * kEach + i;
+    if (at < order) {
+      wait_flag(a.flags + at * a.column_blocks + block, a, site);
+#pragma unroll
+      for (int v = 0; v < kPer; ++v) {
+        const int slot = kSlots == 1 ? 0 : lane * kPer + v;
+        m[v] = then(m[v], load_map<A>(a.maps, at * padded + static_cast<int64_t>(block) * kSlots + slot));
+      }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < kPer; ++v) {
+    if (kSlots > 1 || lane == 0) scratch[warp * kSlots + (kSlots == 1 ? 0 : lane * kPer + v)] = m[v];
+  }
+  if (first > 0 && warp == 0) {
+    wait_flag(a.flags + (a.chunks + order / kGroup) * a.column_blocks + block, a, site);
+  }
+  __syncthreads();
+}
+
+// State before this chunk: the group's first state through the maps left in `scratch`.
+template <typename A, int kSlots>
+__device__ __forceinline__ A carried(const RecurrenceArgs& a, int64_t order, int block, int slot,
+                                     const Map<A>* scratch, A begin) {
+  const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
+  A h = begin;
+  if (order >= kGroup) {
+    h = __ldcg(static_cast<const A*>(a.bases) + order / kGroup * padded +
+               static_cast<int64_t>(block) * kSlots + slot);
+  }
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const Map<A> m = scratch[w * kSlots + slot];
+    h = m.a * h + m.b;
+  }
+  return h;
+}
+
+// ---- column layout ---------------------------------------------------------------------
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+    columns_forward_kernel(const __grid_constant__ RecurrenceArgs a) {
+  using A = typename Wide<T>::type;
+  constexpr int kSteps = kForwardSteps, kSlots = 32 * V;
+  __shared__ Map<A> maps[kWarps][kSlots];
+  __shared__ Map<A> before[kWarps * kSlots];
+  __shared__ unsigned int taken;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warps = blockDim.x >> 5;
+  int block = blockIdx.x;
+  int64_t chunk = 0, stop = a.chunks;
+  if (a.shared) {
+    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u);
+    __syncthreads();
+    chunk = taken / a.column_blocks;
+    block = static_cast<int>(taken - chunk * a.column_blocks);
+    stop = chunk + 1;
+  }
+  const int64_t column = (static_cast<int64_t>(block) * 32 + lane) * V;
+  const bool live = column < a.columns;
+  const int64_t base = live ? column / a.inner * a.steps * a.inner + column % a.inner : 0;
+  A begin[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    begin[v] = live && a.initial != nullptr ? static_cast<const A*>(a.initial)[column + v] : A(0);
+  }
+  for (; chunk < stop; ++chunk) {
+    const int64_t first = (chunk * warps + warp) * kSteps;
+    const T* x = static_cast<const T*>(a.x) + base + first * a.inner;
+    const T* gate = static_cast<const T*>(a.gate) + base + first * a.inner;
+    const int count = live ? steps_here(a.steps - first, kSteps) : 0;
+    Pack<T, V> px[kSteps], pg[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      if (i < count) {
+        px[i] = load_pack<T, V>(x + i * a.inner);
+        pg[i] = load_pack<T, V>(gate + i * a.inner);
+      }
+    }
+    A f[kSteps][V], b[kSteps][V];
+    Map<A> own[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) own[v] = {A(1), A(0)};
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        f[i][v] = A(1);
+        b[i][v] = A(0);
+        if (i < count) {
+          A keep;
+          gates<T>(widen(pg[i].v[v]), &f[i][v], &keep);
+          b[i][v] = keep * widen(px[i].v[v]);
+        }
+        own[v] = then(own[v], Map<A>{f[i][v], b[i][v]});
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) maps[warp][lane * V + v] = own[v];
+    __syncthreads();
+    Map<A> earlier[V];  // the block's warps before this one
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      earlier[v] = {A(1), A(0)};
+      for (int w = 0; w < warp; ++w) earlier[v] = then(earlier[v], maps[w][lane * V + v]);
+    }
+    A state[V];
+    if (a.shared) {
+      const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
+      const int64_t at = static_cast<int64_t>(block) * kSlots + lane * V;
+      if (warp == warps - 1 && chunk + 1 < a.chunks) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          static_cast<Map<A>*>(a.maps)[chunk * padded + at + v] = then(earlier[v], own[v]);
+        }
+        publish(a.flags + chunk * a.column_blocks + block);
+      }
+      look_back<A, kSlots>(a, chunk, block, before, kSiteForward);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        state[v] = carried<A, kSlots>(a, chunk, block, lane * V + v, before, begin[v]);
+        state[v] = earlier[v].a * state[v] + earlier[v].b;
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) state[v] = earlier[v].a * begin[v] + earlier[v].b;
+      if (chunk + 1 < stop) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          for (int w = warp; w < warps; ++w) {
+            earlier[v] = then(earlier[v], maps[w][lane * V + v]);
+          }
+          begin[v] = earlier[v].a * begin[v] + earlier[v].b;
+        }
+        __syncthreads();
+      }
+    }
+    if (a.states != nullptr && live && first < a.steps && first % kStateBlock == 0) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        static_cast<A*>(a.states)[first / kStateBlock * a.columns + column + v] = state[v];
+      }
+    }
+    T* y = static_cast<T*>(a.y) + base + first * a.inner;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      Pack<T, V> out;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        state[v] = f[i][v] * state[v] + b[i][v];
+        out.v[v] = narrow<T>(state[v]);
+      }
+      if (i < count) *reinterpret_cast<Pack<T, V>*>(y + i * a.inner) = out;
+    }
+    const int64_t end = a.steps > 0 ? a.steps - 1 : 0;
+    if (live && first <= end && end < first + kSteps) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) static_cast<A*>(a.last)[column + v] = state[v];
+    }
+    if (a.shared && (chunk + 1) % kGroup == 0 && warp == warps - 1 && chunk + 1 < a.chunks) {
+      const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        static_cast<A*>(a.bases)[(chunk + 1) / kGroup * padded + static_cast<int64_t>(block) * kSlots +
+                                 lane * V + v] = state[v];
+      }
+      publish(a.flags + (a.chunks + (chunk + 1) / kGroup) * a.column_blocks + block);
+    }
+  }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+    columns_backward_kernel(const __grid_constant__ RecurrenceArgs a) {
+  using A = typename Wide<T>::type;
+  constexpr int kSteps = kBackwardSteps, kSlots = 32 * V;
+  __shared__ Map<A> forward[kWarps][kSlots];
+  __shared__ A backward[kWarps][kSlots];  // the flow's map: same factor, own offset
+  __shared__ Map<A> after[kWarps * kSlots];
+  __shared__ unsigned int taken;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warps = blockDim.x >> 5;
+  int block = blockIdx.x;
+  int64_t order = 0, stop = a.chunks;  // chunks from the last to the first
+  if (a.shared) {
+    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u);
+    __syncthreads();
+    order = taken / a.column_blocks;
+    block = static_cast<int>(taken - order * a.column_blocks);
+    stop = order + 1;
+  }
+  const int64_t column = (static_cast<int64_t>(block) * 32 + lane) * V;
+  const bool live = column < a.columns;
+  const int64_t base = live ? column / a.inner * a.steps * a.inner + column % a.inner : 0;
+  A begin[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    begin[v] = live && a.dlast != nullptr ? static_cast<const A*>(a.dlast)[column + v] : A(0);
+  }
+  for (; order < stop; ++order) {
+    const int64_t chunk = a.chunks - 1 - order;
+    const int64_t first = (chunk * warps + warp) * kSteps;
+    const int64_t offset = base + first * a.inner;
+    const int count = live ? steps_here(a.steps - first, kSteps) : 0;
+    Pack<T, V> px[kSteps], pg[kSteps], pd[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      if (i < count) {
+        px[i] = load_pack<T, V>(static_cast<const T*>(a.x) + offset + i * a.inner);
+        pg[i] = load_pack<T, V>(static_cast<const T*>(a.gate) + offset + i * a.inner);
+        if (a.dy != nullptr) {
+          pd[i] = load_pack<T, V>(static_cast<const T*>(a.dy) + offset + i * a.inner);
+        }
+      }
+      if (i >= count || a.dy == nullptr) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) pd[i].v[v] = narrow<T>(A(0));
+      }
+    }
+    A saved[V];  // the state before the chunk
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      saved[v] = live && a.steps > 0
+                     ? static_cast<const A*>(a.states_in)[chunk * a.columns + column + v]
+                     : A(0);
+    }
+    A f[kSteps][V], keep[kSteps][V];
+    Map<A> own[V];
+    A flow[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      own[v] = {A(1), A(0)};
+      flow[v] = A(0);
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        f[i][v] = A(1);
+        keep[i][v] = A(0);
+        if (i < count) {
+          gates<T>(widen(pg[i].v[v]), &f[i][v], &keep[i][v]);
+          own[v] = then(own[v], Map<A>{f[i][v], keep[i][v] * widen(px[i].v[v])});
+        }
+      }
+    }
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) flow[v] = f[i][v] * (widen(pd[i].v[v]) + flow[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      forward[warp][lane * V + v] = own[v];
+      backward[warp][lane * V + v] = flow[v];
+    }
+    __syncthreads();
+    Map<A> later[V];  // the block's warps after this one, walked backwards
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      for (int w = 0; w < warp; ++w) {
+        const Map<A> m = forward[w][lane * V + v];
+        saved[v] = m.a * saved[v] + m.b;
+      }
+      later[v] = {A(1), A(0)};
+      for (int w = warps - 1; w > warp; --w) {
+        later[v] = then(later[v], Map<A>{forward[w][lane * V + v].a, backward[w][lane * V + v]});
+      }
+    }
+    A q[V];
+    if (a.shared) {
+      const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
+      const int64_t at = static_cast<int64_t>(block) * kSlots + lane * V;
+      if (warp == 0 && order + 1 < a.chunks) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          static_cast<Map<A>*>(a.maps)[order * padded + at + v] =
+              then(later[v], Map<A>{own[v].a, flow[v]});
+        }
+        publish(a.flags + order * a.column_blocks + block);
+      }
+      look_back<A, kSlots>(a, order, block, after, kSiteBackward);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        q[v] = carried<A, kSlots>(a, order, block, lane * V + v, after, begin[v]);
+        q[v] = later[v].a * q[v] + later[v].b;
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) q[v] = later[v].a * begin[v] + later[v].b;
+      if (order + 1 < stop) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          for (int w = warp; w >= 0; --w) {
+            later[v] = then(later[v], Map<A>{forward[w][lane * V + v].a, backward[w][lane * V + v]});
+          }
+          begin[v] = later[v].a * begin[v] + later[v].b;
+        }
+        __syncthreads();
+      }
+    }
+    A prior[kSteps][V];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        prior[i][v] = saved[v];
+        if (i < count) saved[v] = f[i][v] * saved[v] + keep[i][v] * widen(px[i].v[v]);
+      }
+    }
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i) {
+      Pack<T, V> dx, dg;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const A total = widen(pd[i].v[v]) + q[v];
+        if (i < count) {
+          dx.v[v] = narrow<T>(keep[i][v] * total);
+          dg.v[v] = narrow<T>(f[i][v] * keep[i][v] * (prior[i][v] - widen(px[i].v[v])) * total);
+          q[v] = f[i][v] * total;
+        }
+      }
+      if (i < count) {
+        if (a.dx != nullptr) {
+          *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.dx) + offset + i * a.inner) = dx;
+        }
+        if (a.dgate != nullptr) {
+          *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.dgate) + offset + i * a.inner) = dg;
+        }
+      }
+    }
+    if (a.dinitial != nullptr && live && first == 0) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) static_cast<A*>(a.dinitial)[column + v] = q[v];
+    }
+    if (a.shared && (order + 1) % kGroup == 0 && warp == 0 && order + 1 < a.chunks) {
+      const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        static_cast<A*>(a.bases)[(order + 1) / kGroup * padded + static_cast<int64_t>(block) * kSlots +
+                                 lane * V + v] = q[v];
+      }
+      publish(a.flags + (a.chunks + (order + 1) / kGroup) * a.column_blocks + block);
+    }
+  }
+}
+
+// ---- step layout -----------------------------------------------------------------------
+
+// A thread's run of kAlongSteps steps: one 16-byte (32 for float32) access where rows are
+// aligned, else single elements.
+template <typename T>
+__device__ __forceinline__ void load_run(const T* p, int count, bool vectors,
+                                         T (&v)[kAlongSteps]) {
+  constexpr int kPer = 16 / sizeof(T);
+  if (vectors && count == kAlongSteps) {
+#pragma unroll
+    for (int i = 0; i < kAlongSteps; i += kPer) {
+      *reinterpret_cast<Pack<T, kPer>*>(v + i) = load_pack<T, kPer>(p + i);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kAlongSteps; ++i) v[i] = i < count ? p[i] : narrow<T>(0);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_run(T* p, int count, bool vectors,
+                                          const T (&v)[kAlongSteps]) {
+  constexpr int kPer = 16 / sizeof(T);
+  if (vectors && count == kAlongSteps) {
+#pragma unroll
+    for (int i = 0; i < kAlongSteps; i += kPer) {
+      *reinterpret_cast<Pack<T, kPer>*>(p + i) = *reinterpret_cast<const Pack<T, kPer>*>(v + i);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kAlongSteps; ++i) {
+      if (i < count) p[i] = v[i];
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kWarps * 32)
+    steps_forward_kernel(const __grid_constant__ RecurrenceArgs a, bool vectors) {
+  using A = typename Wide<T>::type;
+  __shared__ Map<A> maps[kWarps];
+  __shared__ Map<A> before[kWarps];
+  __shared__ unsigned int taken;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warps = blockDim.x >> 5;
+  int64_t column = blockIdx.x, chunk = 0, stop = a.chunks;
+  if (a.shared) {
+    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u);
+    __syncthreads();
+    chunk = taken / a.column_blocks;
+    column = taken - chunk * a.column_blocks;
+    stop = chunk + 1;
+  }
+  A begin = a.initial != nullptr ? static_cast<const A*>(a.initial)[column] : A(0);
+  for (; chunk < stop; ++chunk) {
+    const int64_t first = ((chunk * warps + warp) * 32 + lane) * kAlongSteps;
+    const int64_t offset = column * a.steps + first;
+    const int count = steps_here(a.steps - first, kAlongSteps);
+    alignas(16) T x[kAlongSteps], g[kAlongSteps];
+    load_run(static_cast<const T*>(a.x) + offset, count, vectors, x);
+    load_run(static_cast<const T*>(a.gate) + offset, count, vectors, g);
+    A f[kAlongSteps], b[kAlongSteps];
+    Map<A> own{A(1), A(0)};
+#pragma unroll
+    for (int i = 0; i < kAlongSteps; ++i) {
+      f[i] = A(1);
+      b[i] = A(0);
+      if (i < count) {
+        A keep;
+        gates<T>(widen(g[i]), &f[i], &keep);
+        b[i] = keep * widen(x[i]);
+      }
+      own = then(own, Map<A>{f[i], b[i]});
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const Map<A> m = shuffle_up(own, d);
+      if (lane >= d) own = then(m, own);
+    }
+    if (lane == 31) maps[warp] = own;
+    Map<A> earlier = shuffle_up(own, 1);
+    if (lane == 0) earlier = {A(1), A(0)};
+    __syncthreads();
+    Map<A> lead{A(1), A(0)};  // the block's warps before this one
+    for (int w = 0; w < warp; ++w) lead = then(lead, maps[w]);
+    A state = begin;
+    if (a.shared) {
+      if (warp == warps - 1 && chunk + 1 < a.chunks) {
+        if (lane == 31) {
+          static_cast<Map<A>*>(a.maps)[chunk * a.column_blocks + column] = then(lead, own);
+        }
+        publish(a.flags + chunk * a.column_blocks + column);
+      }
+      look_back<A, 1>(a, chunk, static_cast<int>(column), before, kSiteForward);
+      state = carried<A, 1>(a, chunk, static_cast<int>(column), 0, before, begin);
+    } else if (chunk + 1 < stop) {
+      Map<A> all = lead;
+      for (int w = warp; w < warps; ++w) all = then(all, maps[w]);
+      begin = all.a * begin + all.b;
+      __syncthreads();
+    }
+    state = lead.a * state + lead.b;
+    if (a.states != nullptr && lane == 0 && first < a.steps) {
+      static_cast<A*>(a.states)[first / kAlongBlock * a.columns + column] = state;
+    }
+    state = earlier.a * state + earlier.b;
+    alignas(16) T y[kAlongSteps];
+#pragma unroll
+    for (int i = 0; i < kAlongSteps; ++i) {
+      state = f[i] * state + b[i];
+      y[i] = narrow<T>(state);
+    }
+    store_run(static_cast<T*>(a.y) + offset, count, vectors, y);
+    const int64_t end = a.steps > 0 ? a.steps - 1 : 0;
+    if (first <= end && end < first + kAlongSteps) static_cast<A*>(a.last)[column] = state;
+    if (a.shared && (chunk + 1) % kGroup == 0 && warp == warps - 1 && chunk + 1 < a.chunks) {
+      if (lane == 31) {
+        static_cast<A*>(a.bases)[(chunk + 1) / kGroup * a.column_blocks + column] = state;
+      }
+      publish(a.flags + (a.chunks + (chunk + 1) / kGroup) * a.column_blocks + column);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kWarps * 32)
+    steps_backward_kernel(const __grid_constant__ RecurrenceArgs a, bool vectors) {
+  using A = typename Wide<T>::type;
+  __shared__ Map<A> maps[kWarps];
+  __shared__ Map<A> after[kWarps];
+  __shared__ unsigned int taken;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warps = blockDim.x >> 5;
+  int64_t column = blockIdx.x, order = 0, stop = a.chunks;
+  if (a.shared) {
+    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u);
+    __syncthreads();
+    order = taken / a.column_blocks;
+    column = taken - order * a.column_blocks;
+    stop = order + 1;
+  }
+  A begin = a.dlast != nullptr ? static_cast<const A*>(a.dlast)[column] : A(0);
+  for (; order < stop; ++order) {
+    const int64_t chunk = a.chunks - 1 - order;
+    const int64_t first = ((chunk * warps + warp) * 32 + lane) * kAlongSteps;
+    const int64_t offset = column * a.steps + first;
+    const int count = steps_here(a.steps - first, kAlongSteps);
+    alignas(16) T x[kAlongSteps], g[kAlongSteps], d[kAlongSteps];
+    load_run(static_cast<const T*>(a.x) + offset, count, vectors, x);
+    load_run(static_cast<const T*>(a.gate) + offset, count, vectors, g);
+    load_run(static_cast<const T*>(a.dy) + offset, a.dy != nullptr ? count : 0, vectors, d);
+    const int64_t warp_first = first - lane * kAlongSteps;
+    A state = warp_first < a.steps
+                  ? static_cast<const A*>(a.states_in)[warp_first / kAlongBlock * a.columns + column]
+                  : A(0);
+    A f[kAlongSteps], keep[kAlongSteps];
+    Map<A> own{A(1), A(0)};
+#pragma unroll
+    for (int i = 0; i < kAlongSteps; ++i) {
+      f[i] = A(1);
+      keep[i] = A(0);
+      if (i < count) {
+        gates<T>(widen(g[i]), &f[i], &keep[i]);
+        own = then(own, Map<A>{f[i], keep[i] * widen(x[i])});
+      }
+    }
+    Map<A> back{own.a, A(0)};
+#pragma unroll
+    for (int i = kAlongSteps - 1; i >= 0; --i) back.b = f[i] * (widen(d[i]) + back.b);
+#pragma unroll
+    for (int k = 1; k < 32; k *= 2) {
+      const Map<A> m = shuffle_up(own, k);
+      if (lane >= k) own = then(m, own);
+      const Map<A> n = shuffle_down(back, k);
+      if (lane < 32 - k) back = then(n, back);
+    }
+    if (lane == 0) maps[warp] = back;
+    Map<A> earlier = shuffle_up(own, 1), later = shuffle_down(back, 1);
+    if (lane > 0) state = earlier.a * state + earlier.b;
+    if (lane == 31) later = {A(1), A(0)};
+    __syncthreads();
+    Map<A> lead{A(1), A(0)};  // the block's warps after this one
+    for (int w = warps - 1; w > warp; --w) lead = then(lead, maps[w]);
+    A q = begin;
+    if (a.shared) {
+      if (warp == 0 && order + 1 < a.chunks) {
+        if (lane == 0) {
+          static_cast<Map<A>*>(a.maps)[order * a.column_blocks + column] = then(lead, back);
+        }
+        publish(a.flags + order * a.column_blocks + column);
+      }
+      look_back<A, 1>(a, order, static_cast<int>(column), after, kSiteBackward);
+      q = carried<A, 1>(a, order, static_cast<int>(column), 0, after, begin);
+    } else if (order + 1 < stop) {
+      Map<A> all = lead;
+      for (int w = warp; w >= 0; --w) all = then(all, maps[w]);
+      begin = all.a * begin + all.b;
+      __syncthreads();
+    }
+    q = lead.a * q + lead.b;
+    q = later.a * q + later.b;
+    A prior[kAlongSteps];
+#pragma unroll
+    for (int i = 0; i < kAlongSteps; ++i) {
+      prior[i] = state;
+      if (i < count) state = f[i] * state + keep[i] * widen(x[i]);
+    }
+    alignas(16) T dx[kAlongSteps], dg[kAlongSteps];
+#pragma unroll
+    for (int i = kAlongSteps - 1; i >= 0; --i) {
+      const A total = widen(d[i]) + q;
+      dx[i] = narrow<T>(keep[i] * total);
+      dg[i] = narrow<T>(f[i] * keep[i] * (prior[i] - widen(x[i])) * total);
+      if (i < count) q = f[i] * total;
+    }
+    if (a.dx != nullptr) store_run(static_cast<T*>(a.dx) + offset, count, vectors, dx);
+    if (a.dgate != nullptr) store_run(static_cast<T*>(a.dgate) + offset, count, vectors, dg);
+    if (a.dinitial != nullptr && first == 0) static_cast<A*>(a.dinitial)[column] = q;
+    if (a.shared && (order + 1) % kGroup == 0 && warp == 0 && order + 1 < a.chunks) {
+      if (lane == 0) static_cast<A*>(a.bases)[(order + 1) / kGroup * a.column_blocks + column] = q;
+      publish(a.flags + (a.chunks + (order + 1) / kGroup) * a.column_blocks + column);
+    }
+  }
+}
+
+// ---- choice of kernel and layout of the workspace --------------------------------------
+
+struct RecurrencePlan {
+  bool along;          // step layout
+  int vector, warps;   // columns a lane, warps a block
+  int64_t chunks;
+  int64_t column_blocks;
+  bool shared;
+  size_t maps = 0, bases = 0, flags = 0, flag_bytes = 0, total = 0;
+};
+
+// Column blocks as wide as the widest vector allows; a pass over 16-bit columns of odd
+// extent takes narrower ones (`narrow_columns`), which the workspace covers too.
+RecurrencePlan plan_recurrence(int dtype, int64_t outer, int64_t steps, int64_t inner,
+                               bool backward, bool narrow_columns) {
+  RecurrencePlan p{};
+  const int64_t columns = outer * inner;
+  p.along = inner == 1 && steps > 1;
+  p.vector = !p.along && element_size(dtype) == 2 && inner % 2 == 0 && !narrow_columns ? 2 : 1;
+  const int64_t per_warp = p.along ? kAlongBlock : backward ? kBackwardSteps : kForwardSteps;
+  p.warps = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kWarps, (steps + per_warp - 1) / per_warp)));
+  p.chunks = std::max<int64_t>(1, (steps + p.warps * per_warp - 1) / (p.warps * per_warp));
+  p.column_blocks = p.along ? columns : (columns + 32 * p.vector - 1) / (32 * p.vector);
+  // Blocks of eight warps, at most three on an SM: with fewer than 2 blocks an SM, sharing the
+  // time axis fills the machine.
+  p.shared = p.chunks > 1 && p.column_blocks < 2 * 148;
+  if (p.shared) {
+    const int64_t padded = p.along ? columns : p.column_blocks * 32 * p.vector;
+    const int64_t groups = (p.chunks + kGroup - 1) / kGroup;
+    const size_t wide = dtype == CND_F64 ? 8 : 4;
+    const auto take = [&](size_t bytes) {
+      const size_t at = p.total;
+      p.total += (bytes + 255) / 256 * 256;
+      return at;
+    };
+    p.flag_bytes = static_cast<size_t>((p.chunks + groups) * p.column_blocks + 1) * sizeof(unsigned int);
+    p.flags = take(p.flag_bytes);
+    p.maps = take(static_cast<size_t>(p.chunks * padded) * 2 * wide);
+    p.bases = take(static_cast<size_t>(groups * padded) * wide);
+  }
+  return p;
+}
+
+uint64_t wait_timeout() {
+  static const uint64_t value = [] {
+    const char* env = std::getenv("CND_WAIT_TIMEOUT_MS");
+    const long long parsed = env != nullptr ? std::atoll(env) : 0;
+    return (parsed > 0 ? static_cast<uint64_t>(parsed) : uint64_t{2000}) * 1000000u;
+  }();
+  return value;
+}
+
+// Binds the exchange area and clears its flags and ticket.
+int bind_exchange(const char* who, const RecurrencePlan& p, void* workspace, size_t bytes,
+                  RecurrenceArgs* a, cudaStream_t stream) {
+  a->chunks = p.chunks;
+  a->column_blocks = static_cast<int>(p.column_blocks);
+  a->shared = p.shared;
+  if (p.column_blocks > INT32_MAX) {
+    return fail(CND_ERR_UNSUPPORTED, "%s: too many columns", who);
+  }
+  if (!p.shared) return CND_OK;
+  if (workspace == nullptr || bytes < p.total) {
+    return fail(CND_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who,
+                workspace == nullptr ? size_t{0} : bytes, p.total);
+  }
+  char* base = static_cast<char*>(workspace);
+  a->maps = base + p.maps;
+  a->bases = base + p.bases;
+  a->flags = reinterpret_cast<unsigned int*>(base + p.flags);
+  a->ticket = a->flags + p.flag_bytes / sizeof(unsigned int) - 1;
+  a->error = device_error_word();
+  a->timeout_ns = wait_timeout();
+  if (a->error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
+  if (cudaMemsetAsync(a->flags, 0, p.flag_bytes, stream) != cudaSuccess) return launch_status(who);
+  return CND_OK;
+}
+
+unsigned recurrence_grid(const RecurrencePlan& p) {
+  return static_cast<unsigned>(p.shared ? p.column_blocks * p.chunks : p.column_blocks);
+}
+
+// Whether packs of two 16-bit columns may be read and written at these addresses.
+bool pairs_aligned(std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers) {
+    if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return false;
+  }
+  return true;
+}
+
+bool runs_aligned(int dtype, int64_t steps, std::initializer_list<const void*> pointers) {
+  if (steps * element_size(dtype) % 16 != 0) return false;
+  for (const void* p : pointers) {
+    if (!aligned16(p)) return false;
+  }
+  return true;
 }
 
 int check_recurrence(const char* who, int dtype, int64_t outer, int64_t steps, int64_t inner) {
@@ -128,17 +875,25 @@ extern "C" {
 int64_t cnd_gated_recurrence_blocks(int32_t dtype, int64_t outer, int64_t steps, int64_t inner) {
   (void)dtype;
   (void)outer;
-  (void)inner;
-  return steps <= 0 ? 0 : (steps - 1) / cnd::layers::kBlockSteps + 1;
+  using namespace cnd::layers;
+  const int64_t block = inner == 1 && steps > 1 ? kAlongBlock : kStateBlock;
+  return steps <= 0 ? 0 : (steps - 1) / block + 1;
 }
 
 size_t cnd_gated_recurrence_workspace_size(int32_t dtype, int64_t outer, int64_t steps,
                                            int64_t inner) {
-  (void)dtype;
-  (void)outer;
-  (void)steps;
-  (void)inner;
-  return 0;
+  using namespace cnd::layers;
+  if (check_recurrence("cnd_gated_recurrence", dtype, outer, steps, inner) != CND_OK ||
+      outer == 0 || inner == 0) {
+    return 0;
+  }
+  size_t bytes = 0;
+  for (const bool backward : {false, true}) {
+    for (const bool narrow : {false, true}) {
+      bytes = std::max(bytes, plan_recurrence(dtype, outer, steps, inner, backward, narrow).total);
+    }
+  }
+  return bytes;
 }
 
 int cnd_gated_recurrence_forward(int32_t dtype, int64_t outer, int64_t steps, int64_t inner,
@@ -147,10 +902,8 @@ int cnd_gated_recurrence_forward(int32_t dtype, int64_t outer, int64_t steps, in
                                  size_t workspace_bytes, void* stream_handle) {
   using namespace cnd;
   using namespace cnd::layers;
-  (void)workspace;
-  (void)workspace_bytes;
   clear_error();
-  const int rc = check_recurrence("cnd_gated_recurrence_forward", dtype, outer, steps, inner);
+  int rc = check_recurrence("cnd_gated_recurrence_forward", dtype, outer, steps, inner);
   if (rc != CND_OK) return rc;
   const int64_t columns = outer * inner;
   if (columns == 0) return CND_OK;
@@ -168,9 +921,26 @@ int cnd_gated_recurrence_forward(int32_t dtype, int64_t outer, int64_t steps, in
   a.outer = outer;
   a.steps = steps;
   a.inner = inner;
+  a.columns = columns;
+  const RecurrencePlan p = plan_recurrence(dtype, outer, steps, inner, false,
+                                           !pairs_aligned({x, gate, y}));
+  rc = bind_exchange("cnd_gated_recurrence_forward", p, workspace, workspace_bytes, &a, stream);
+  if (rc != CND_OK) return rc;
+  const unsigned grid = recurrence_grid(p);
+  const bool vectors = runs_aligned(dtype, steps, {x, gate, y});
   with_dtype(dtype, [&](auto zero) {
-    recurrence_forward_kernel<decltype(zero)>
-        <<<static_cast<unsigned>((columns + kThreads - 1) / kThreads), kThreads, 0, stream>>>(a);
+    using T = decltype(zero);
+    if (p.along) {
+      steps_forward_kernel<T><<<grid, p.warps * 32, 0, stream>>>(a, vectors);
+      return;
+    }
+    if constexpr (sizeof(T) == 2) {
+      if (p.vector == 2) {
+        columns_forward_kernel<T, 2><<<grid, p.warps * 32, 0, stream>>>(a);
+        return;
+      }
+    }
+    columns_forward_kernel<T, 1><<<grid, p.warps * 32, 0, stream>>>(a);
   });
   count_launch();
   return launch_status("cnd_gated_recurrence_forward");
@@ -183,10 +953,8 @@ int cnd_gated_recurrence_backward(int32_t dtype, int64_t outer, int64_t steps, i
                                   size_t workspace_bytes, void* stream_handle) {
   using namespace cnd;
   using namespace cnd::layers;
-  (void)workspace;
-  (void)workspace_bytes;
   clear_error();
-  const int rc = check_recurrence("cnd_gated_recurrence_backward", dtype, outer, steps, inner);
+  int rc = check_recurrence("cnd_gated_recurrence_backward", dtype, outer, steps, inner);
   if (rc != CND_OK) return rc;
   if (output_mask == nullptr) {
     return fail(CND_ERR_INVALID, "cnd_gated_recurrence_backward: output_mask must not be NULL");
@@ -211,9 +979,26 @@ int cnd_gated_recurrence_backward(int32_t dtype, int64_t outer, int64_t steps, i
   a.outer = outer;
   a.steps = steps;
   a.inner = inner;
+  a.columns = columns;
+  const RecurrencePlan p = plan_recurrence(dtype, outer, steps, inner, true,
+                                           !pairs_aligned({x, gate, dy, dx, dgate}));
+  rc = bind_exchange("cnd_gated_recurrence_backward", p, workspace, workspace_bytes, &a, stream);
+  if (rc != CND_OK) return rc;
+  const unsigned grid = recurrence_grid(p);
+  const bool vectors = runs_aligned(dtype, steps, {x, gate, dy, dx, dgate});
   with_dtype(dtype, [&](auto zero) {
-    recurrence_backward_kernel<decltype(zero)>
-        <<<static_cast<unsigned>((columns + kThreads - 1) / kThreads), kThreads, 0, stream>>>(a);
+    using T = decltype(zero);
+    if (p.along) {
+      steps_backward_kernel<T><<<grid, p.warps * 32, 0, stream>>>(a, vectors);
+      return;
+    }
+    if constexpr (sizeof(T) == 2) {
+      if (p.vector == 2) {
+        columns_backward_kernel<T, 2><<<grid, p.warps * 32, 0, stream>>>(a);
+        return;
+      }
+    }
+    columns_backward_kernel<T, 1><<<grid, p.warps * 32, 0, stream>>>(a);
   });
   count_launch();
   return launch_status("cnd_gated_recurrence_backward");
