@@ -21,7 +21,9 @@
 // so whoever a block waits for is already running; each chunk composes the maps of the
 // chunks before it in its group of kGroup, in order, with the state that the last chunk
 // of the group before published. The association is fixed, so repeated calls give the
-// same bits. Waits are bounded and end at once when any wait has expired.
+// same bits. The exchange area starts as all ones, a NaN that no arithmetic produces, and a
+// map (a state) is stored at once, so a reader polls the value itself: no flag, no fence, one
+// trip to L2. Waits are bounded and end at once when any wait has expired.
 //
 // The forward keeps the state before each block of 64 steps (256 in step layout), from which
 // the backward recomputes the others in float32: it reads x, g and dy only, and its states
@@ -62,11 +64,12 @@ struct RecurrenceArgs {
   int64_t outer, steps, inner, columns;
   int64_t chunks;
   int column_blocks;
+  int balanced;  // steps a thread takes when one chunk holds them all, 0: the most it can
   // exchange between chunks (shared != 0): maps [chunks][padded], states [groups][padded],
-  // flags [chunks + groups][column_blocks], one ticket counter
+  // one ticket counter; all bits set at the start
   int shared;
   void *maps, *bases;
-  unsigned int *flags, *ticket, *error;
+  unsigned int *ticket, *error;
   uint64_t timeout_ns;
 };
 
@@ -84,57 +87,107 @@ __device__ __forceinline__ void gates(A g, A* f, A* keep) {
     r = __fdividef(1.0f, 1.0f + e);
   } else {
     e = exp(-fabs(g));
-    r = A(1) / (A(1) + e);
+    const A d = A(1) + e;
+    if constexpr (sizeof(T) == 4) {
+      // d is in [1, 2]: the approximate reciprocal and one Newton step
+      r = __fdividef(1.0f, d);
+      r = fmaf(r, fmaf(-d, r, 1.0f), r);
+    } else {
+      r = A(1) / d;
+    }
   }
   const A s = e * r;
   *f = g >= A(0) ? r : s;
   *keep = g >= A(0) ? s : r;
 }
 
-__device__ __forceinline__ unsigned int load_acquire(const unsigned int* p) {
-  unsigned int v;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+// Values of the exchange area, read and written at once: 32 bits (a float32 state), 64
+// bits (a float32 map, a float64).
+template <typename Bits>
+__device__ __forceinline__ Bits load_exchange(const Bits* p) {
+  Bits v;
+  if constexpr (sizeof(Bits) == 4) {
+    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  } else {
+    asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  }
   return v;
 }
 
-__device__ __forceinline__ void store_release(unsigned int* p, unsigned int v) {
-  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+template <typename Bits>
+__device__ __forceinline__ void store_exchange(Bits* p, Bits v) {
+  if constexpr (sizeof(Bits) == 4) {
+    asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+  } else {
+    asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
+  }
 }
 
-// Waits, a whole warp, until *flag is set. Gives up (error word set) after the timeout, or
+// Reads *p again until it has been written. Gives up (error word set) after the timeout, or
 // as soon as another wait has.
-__device__ __forceinline__ void wait_flag(const unsigned int* flag, const RecurrenceArgs& a,
-                                          unsigned int site) {
-  if ((threadIdx.x & 31) == 0 && load_acquire(flag) == 0) {
-    const uint64_t start = dev::global_timer_ns();
-    for (uint32_t spin = 1; load_acquire(flag) == 0; ++spin) {
-      if (spin % 64 == 0) {
-        if (*static_cast<volatile unsigned int*>(a.error) != 0) break;
-        if (dev::global_timer_ns() - start > a.timeout_ns) {
-          atomicCAS(a.error, 0u, site);
-          break;
-        }
+template <typename Bits>
+__device__ __forceinline__ Bits settle(const Bits* p, Bits v, const RecurrenceArgs& a,
+                                       unsigned int site) {
+  if (v != ~Bits{0}) return v;
+  const uint64_t start = dev::global_timer_ns();
+  for (uint32_t spin = 1;; ++spin) {
+    v = load_exchange(p);
+    if (v != ~Bits{0}) return v;
+    if (spin % 64 == 0) {
+      if (*static_cast<volatile unsigned int*>(a.error) != 0) return v;
+      if (dev::global_timer_ns() - start > a.timeout_ns) {
+        atomicCAS(a.error, 0u, site);
+        return v;
       }
     }
   }
-  __syncwarp();
 }
 
-// Sets *flag after the warp's earlier stores.
-__device__ __forceinline__ void publish(unsigned int* flag) {
-  __threadfence();
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) store_release(flag, 1u);
+// Words of a map: one of 64 bits for float32, two for float64.
+template <typename A>
+constexpr int kMapWords = sizeof(A) / 4;
+
+template <typename A>
+__device__ __forceinline__ void store_map(void* maps, int64_t i, const Map<A>& m) {
+  auto* p = static_cast<unsigned long long*>(maps) + i * kMapWords<A>;
+  if constexpr (sizeof(A) == 4) {
+    store_exchange(p, static_cast<unsigned long long>(__float_as_uint(m.a)) |
+                          static_cast<unsigned long long>(__float_as_uint(m.b)) << 32);
+  } else {
+    store_exchange(p, static_cast<unsigned long long>(__double_as_longlong(m.a)));
+    store_exchange(p + 1, static_cast<unsigned long long>(__double_as_longlong(m.b)));
+  }
 }
 
 template <typename A>
-__device__ __forceinline__ Map<A> load_map(const void* maps, int64_t i) {
+__device__ __forceinline__ Map<A> map_of(const unsigned long long (&w)[kMapWords<A>]) {
   if constexpr (sizeof(A) == 4) {
-    const float2 v = __ldcg(static_cast<const float2*>(maps) + i);
-    return {v.x, v.y};
+    return {__uint_as_float(static_cast<unsigned int>(w[0])),
+            __uint_as_float(static_cast<unsigned int>(w[0] >> 32))};
   } else {
-    const double2 v = __ldcg(static_cast<const double2*>(maps) + i);
-    return {v.x, v.y};
+    return {__longlong_as_double(static_cast<long long>(w[0])),
+            __longlong_as_double(static_cast<long long>(w[1]))};
+  }
+}
+
+template <typename A>
+__device__ __forceinline__ void store_base(void* bases, int64_t i, A v) {
+  if constexpr (sizeof(A) == 4) {
+    store_exchange(static_cast<unsigned int*>(bases) + i, __float_as_uint(v));
+  } else {
+    store_exchange(static_cast<unsigned long long*>(bases) + i,
+                   static_cast<unsigned long long>(__double_as_longlong(v)));
+  }
+}
+
+template <typename A>
+__device__ __forceinline__ A load_base(const RecurrenceArgs& a, int64_t i, unsigned int site) {
+  if constexpr (sizeof(A) == 4) {
+    const auto* p = static_cast<const unsigned int*>(a.bases) + i;
+    return __uint_as_float(settle(p, load_exchange(p), a, site));
+  } else {
+    const auto* p = static_cast<const unsigned long long*>(a.bases) + i;
+    return __longlong_as_double(static_cast<long long>(settle(p, load_exchange(p), a, site)));
   }
 }
 
@@ -153,59 +206,73 @@ __device__ __forceinline__ Map<A> shuffle_down(const Map<A>& m, int d) {
   return {__shfl_down_sync(0xffffffffu, m.a, d), __shfl_down_sync(0xffffffffu, m.b, d)};
 }
 
-// The state at this chunk's start, for column slot `slot` of `slots` of the block, from
-// the chunks before it (order = 0, 1, ... in the direction of the walk). `scratch`:
-// [kWarps][slots] maps. `begin` is the state before the first chunk. Every thread of the
-// block calls it; warp w composes the 4 maps w * 4 ... of the group.
-template <typename A, int kSlots>
-__device__ __forceinline__ void look_back(const RecurrenceArgs& a, int64_t order, int block,
-                                          Map<A>* scratch, unsigned int site) {
-  constexpr int kEach = kGroup / kWarps;
-  constexpr int kPer = kSlots > 32 ? kSlots / 32 : 1;
+// The state before this chunk for the block's column slots lane * kPer ... (kSlots = 32 kPer
+// slots, or the one slot of step layout), from the chunks before it (order = 0, 1, ... in the
+// direction of the walk) and `begin`, the state before the first. `scratch`: [kWarps][kSlots]
+// maps. The whole block calls it: warp w composes maps w * 4 ... of the group.
+template <typename A, int kSlots, int kPer>
+__device__ __forceinline__ void carry_in(const RecurrenceArgs& a, int64_t order, int64_t block,
+                                         Map<A>* scratch, unsigned int site, A (&state)[kPer]) {
+  constexpr int kEach = kGroup / kWarps, kWords = kMapWords<A>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t first = order / kGroup * kGroup;
+  const int64_t group = order / kGroup;
   const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
-  Map<A> m[kPer];
-#pragma unroll
-  for (int v = 0; v < kPer; ++v) m[v] = {A(1), A(0)};
+  const int64_t slot = block * kSlots + (kSlots == 1 ? 0 : lane * kPer);
+  const auto* maps = static_cast<const unsigned long long*>(a.maps);
+  unsigned long long raw[kEach][kPer][kWords];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    const int64_t at = first + warp * kEach + i;
+    const int64_t at = group * kGroup + warp * kEach + i;
     if (at < order) {
-      wait_flag(a.flags + at * a.column_blocks + block, a, site);
 #pragma unroll
       for (int v = 0; v < kPer; ++v) {
-        const int slot = kSlots == 1 ? 0 : lane * kPer + v;
-        m[v] = then(m[v], load_map<A>(a.maps, at * padded + static_cast<int64_t>(block) * kSlots + slot));
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+          raw[i][v][k] = load_exchange(maps + (at * padded + slot + v) * kWords + k);
+        }
       }
     }
   }
+  if (group > 0) {
+#pragma unroll
+    for (int v = 0; v < kPer; ++v) state[v] = load_base<A>(a, group * padded + slot + v, site);
+  }
 #pragma unroll
   for (int v = 0; v < kPer; ++v) {
-    if (kSlots > 1 || lane == 0) scratch[warp * kSlots + (kSlots == 1 ? 0 : lane * kPer + v)] = m[v];
-  }
-  if (first > 0 && warp == 0) {
-    wait_flag(a.flags + (a.chunks + order / kGroup) * a.column_blocks + block, a, site);
+    Map<A> m{A(1), A(0)};
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int64_t at = group * kGroup + warp * kEach + i;
+      if (at < order) {
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+          raw[i][v][k] = settle(maps + (at * padded + slot + v) * kWords + k, raw[i][v][k], a, site);
+        }
+        m = then(m, map_of<A>(raw[i][v]));
+      }
+    }
+    if (kSlots > 1 || lane == 0) scratch[warp * kSlots + (kSlots == 1 ? 0 : lane * kPer + v)] = m;
   }
   __syncthreads();
+#pragma unroll
+  for (int v = 0; v < kPer; ++v) {
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const Map<A> m = scratch[w * kSlots + (kSlots == 1 ? 0 : lane * kPer + v)];
+      state[v] = m.a * state[v] + m.b;
+    }
+  }
 }
 
-// State before this chunk: the group's first state through the maps left in `scratch`.
-template <typename A, int kSlots>
-__device__ __forceinline__ A carried(const RecurrenceArgs& a, int64_t order, int block, int slot,
-                                     const Map<A>* scratch, A begin) {
-  const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
-  A h = begin;
-  if (order >= kGroup) {
-    h = __ldcg(static_cast<const A*>(a.bases) + order / kGroup * padded +
-               static_cast<int64_t>(block) * kSlots + slot);
+// Column `column`'s first element in [outer][steps][inner].
+__device__ __forceinline__ int64_t column_base(const RecurrenceArgs& a, int64_t column) {
+  int64_t outer;
+  if (a.columns <= INT32_MAX) {
+    outer = static_cast<uint32_t>(column) / static_cast<uint32_t>(a.inner);
+  } else {
+    outer = column / a.inner;
   }
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const Map<A> m = scratch[w * kSlots + slot];
-    h = m.a * h + m.b;
-  }
-  return h;
+  return outer * a.steps * a.inner + (column - outer * a.inner);
 }
 
 // ---- column layout ---------------------------------------------------------------------
@@ -223,7 +290,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   int block = blockIdx.x;
   int64_t chunk = 0, stop = a.chunks;
   if (a.shared) {
-    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u);
+    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u) + 1u;
     __syncthreads();
     chunk = taken / a.column_blocks;
     block = static_cast<int>(taken - chunk * a.column_blocks);
@@ -231,17 +298,18 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   }
   const int64_t column = (static_cast<int64_t>(block) * 32 + lane) * V;
   const bool live = column < a.columns;
-  const int64_t base = live ? column / a.inner * a.steps * a.inner + column % a.inner : 0;
+  const int64_t base = live ? column_base(a, column) : 0;
   A begin[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     begin[v] = live && a.initial != nullptr ? static_cast<const A*>(a.initial)[column + v] : A(0);
   }
   for (; chunk < stop; ++chunk) {
-    const int64_t first = (chunk * warps + warp) * kSteps;
+    const int most = a.balanced ? a.balanced : kSteps;
+    const int64_t first = (chunk * warps + warp) * most;
     const T* x = static_cast<const T*>(a.x) + base + first * a.inner;
     const T* gate = static_cast<const T*>(a.gate) + base + first * a.inner;
-    const int count = live ? steps_here(a.steps - first, kSteps) : 0;
+    const int count = live ? steps_here(a.steps - first, most) : 0;
     Pack<T, V> px[kSteps], pg[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
@@ -281,18 +349,23 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     if (a.shared) {
       const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
       const int64_t at = static_cast<int64_t>(block) * kSlots + lane * V;
-      if (warp == warps - 1 && chunk + 1 < a.chunks) {
+      const bool sends = warp == warps - 1 && chunk + 1 < a.chunks;
+      if (sends) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          static_cast<Map<A>*>(a.maps)[chunk * padded + at + v] = then(earlier[v], own[v]);
+          store_map<A>(a.maps, chunk * padded + at + v, then(earlier[v], own[v]));
         }
-        publish(a.flags + chunk * a.column_blocks + block);
       }
-      look_back<A, kSlots>(a, chunk, block, before, kSiteForward);
+#pragma unroll
+      for (int v = 0; v < V; ++v) state[v] = begin[v];
+      carry_in<A, kSlots, V>(a, chunk, block, before, kSiteForward, state);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        state[v] = carried<A, kSlots>(a, chunk, block, lane * V + v, before, begin[v]);
         state[v] = earlier[v].a * state[v] + earlier[v].b;
+        if (sends && (chunk + 1) % kGroup == 0) {
+          store_base<A>(a.bases, (chunk + 1) / kGroup * padded + at + v,
+                        own[v].a * state[v] + own[v].b);
+        }
       }
     } else {
 #pragma unroll
@@ -326,18 +399,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       if (i < count) *reinterpret_cast<Pack<T, V>*>(y + i * a.inner) = out;
     }
     const int64_t end = a.steps > 0 ? a.steps - 1 : 0;
-    if (live && first <= end && end < first + kSteps) {
+    if (live && first <= end && end < first + most) {
 #pragma unroll
       for (int v = 0; v < V; ++v) static_cast<A*>(a.last)[column + v] = state[v];
-    }
-    if (a.shared && (chunk + 1) % kGroup == 0 && warp == warps - 1 && chunk + 1 < a.chunks) {
-      const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        static_cast<A*>(a.bases)[(chunk + 1) / kGroup * padded + static_cast<int64_t>(block) * kSlots +
-                                 lane * V + v] = state[v];
-      }
-      publish(a.flags + (a.chunks + (chunk + 1) / kGroup) * a.column_blocks + block);
     }
   }
 }
@@ -356,7 +420,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   int block = blockIdx.x;
   int64_t order = 0, stop = a.chunks;  // chunks from the last to the first
   if (a.shared) {
-    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u);
+    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u) + 1u;
     __syncthreads();
     order = taken / a.column_blocks;
     block = static_cast<int>(taken - order * a.column_blocks);
@@ -364,7 +428,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   }
   const int64_t column = (static_cast<int64_t>(block) * 32 + lane) * V;
   const bool live = column < a.columns;
-  const int64_t base = live ? column / a.inner * a.steps * a.inner + column % a.inner : 0;
+  const int64_t base = live ? column_base(a, column) : 0;
   A begin[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -372,9 +436,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   }
   for (; order < stop; ++order) {
     const int64_t chunk = a.chunks - 1 - order;
-    const int64_t first = (chunk * warps + warp) * kSteps;
+    const int most = a.balanced ? a.balanced : kSteps;
+    const int64_t first = (chunk * warps + warp) * most;
     const int64_t offset = base + first * a.inner;
-    const int count = live ? steps_here(a.steps - first, kSteps) : 0;
+    const int count = live ? steps_here(a.steps - first, most) : 0;
     Pack<T, V> px[kSteps], pg[kSteps], pd[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
@@ -444,19 +509,22 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     if (a.shared) {
       const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
       const int64_t at = static_cast<int64_t>(block) * kSlots + lane * V;
-      if (warp == 0 && order + 1 < a.chunks) {
+      const bool sends = warp == 0 && order + 1 < a.chunks;
+      if (sends) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          static_cast<Map<A>*>(a.maps)[order * padded + at + v] =
-              then(later[v], Map<A>{own[v].a, flow[v]});
+          store_map<A>(a.maps, order * padded + at + v, then(later[v], Map<A>{own[v].a, flow[v]}));
         }
-        publish(a.flags + order * a.column_blocks + block);
       }
-      look_back<A, kSlots>(a, order, block, after, kSiteBackward);
+#pragma unroll
+      for (int v = 0; v < V; ++v) q[v] = begin[v];
+      carry_in<A, kSlots, V>(a, order, block, after, kSiteBackward, q);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        q[v] = carried<A, kSlots>(a, order, block, lane * V + v, after, begin[v]);
         q[v] = later[v].a * q[v] + later[v].b;
+        if (sends && (order + 1) % kGroup == 0) {
+          store_base<A>(a.bases, (order + 1) / kGroup * padded + at + v, own[v].a * q[v] + flow[v]);
+        }
       }
     } else {
 #pragma unroll
@@ -505,15 +573,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     if (a.dinitial != nullptr && live && first == 0) {
 #pragma unroll
       for (int v = 0; v < V; ++v) static_cast<A*>(a.dinitial)[column + v] = q[v];
-    }
-    if (a.shared && (order + 1) % kGroup == 0 && warp == 0 && order + 1 < a.chunks) {
-      const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        static_cast<A*>(a.bases)[(order + 1) / kGroup * padded + static_cast<int64_t>(block) * kSlots +
-                                 lane * V + v] = q[v];
-      }
-      publish(a.flags + (a.chunks + (order + 1) / kGroup) * a.column_blocks + block);
     }
   }
 }
@@ -565,7 +624,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int warps = blockDim.x >> 5;
   int64_t column = blockIdx.x, chunk = 0, stop = a.chunks;
   if (a.shared) {
-    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u);
+    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u) + 1u;
     __syncthreads();
     chunk = taken / a.column_blocks;
     column = taken - chunk * a.column_blocks;
@@ -605,14 +664,15 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (int w = 0; w < warp; ++w) lead = then(lead, maps[w]);
     A state = begin;
     if (a.shared) {
-      if (warp == warps - 1 && chunk + 1 < a.chunks) {
-        if (lane == 31) {
-          static_cast<Map<A>*>(a.maps)[chunk * a.column_blocks + column] = then(lead, own);
-        }
-        publish(a.flags + chunk * a.column_blocks + column);
+      const bool sends = warp == warps - 1 && lane == 31 && chunk + 1 < a.chunks;
+      if (sends) store_map<A>(a.maps, chunk * a.column_blocks + column, then(lead, own));
+      A carried[1] = {begin};
+      carry_in<A, 1, 1>(a, chunk, column, before, kSiteForward, carried);
+      state = carried[0];
+      if (sends && (chunk + 1) % kGroup == 0) {
+        const Map<A> all = then(lead, own);
+        store_base<A>(a.bases, (chunk + 1) / kGroup * a.column_blocks + column, all.a * state + all.b);
       }
-      look_back<A, 1>(a, chunk, static_cast<int>(column), before, kSiteForward);
-      state = carried<A, 1>(a, chunk, static_cast<int>(column), 0, before, begin);
     } else if (chunk + 1 < stop) {
       Map<A> all = lead;
       for (int w = warp; w < warps; ++w) all = then(all, maps[w]);
@@ -633,12 +693,6 @@ __global__ void __launch_bounds__(kWarps * 32)
     store_run(static_cast<T*>(a.y) + offset, count, vectors, y);
     const int64_t end = a.steps > 0 ? a.steps - 1 : 0;
     if (first <= end && end < first + kAlongSteps) static_cast<A*>(a.last)[column] = state;
-    if (a.shared && (chunk + 1) % kGroup == 0 && warp == warps - 1 && chunk + 1 < a.chunks) {
-      if (lane == 31) {
-        static_cast<A*>(a.bases)[(chunk + 1) / kGroup * a.column_blocks + column] = state;
-      }
-      publish(a.flags + (a.chunks + (chunk + 1) / kGroup) * a.column_blocks + column);
-    }
   }
 }
 
@@ -653,7 +707,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int warps = blockDim.x >> 5;
   int64_t column = blockIdx.x, order = 0, stop = a.chunks;
   if (a.shared) {
-    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u);
+    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u) + 1u;
     __syncthreads();
     order = taken / a.column_blocks;
     column = taken - order * a.column_blocks;
@@ -703,14 +757,15 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (int w = warps - 1; w > warp; --w) lead = then(lead, maps[w]);
     A q = begin;
     if (a.shared) {
-      if (warp == 0 && order + 1 < a.chunks) {
-        if (lane == 0) {
-          static_cast<Map<A>*>(a.maps)[order * a.column_blocks + column] = then(lead, back);
-        }
-        publish(a.flags + order * a.column_blocks + column);
+      const bool sends = warp == 0 && lane == 0 && order + 1 < a.chunks;
+      if (sends) store_map<A>(a.maps, order * a.column_blocks + column, then(lead, back));
+      A carried[1] = {begin};
+      carry_in<A, 1, 1>(a, order, column, after, kSiteBackward, carried);
+      q = carried[0];
+      if (sends && (order + 1) % kGroup == 0) {
+        const Map<A> all = then(lead, back);
+        store_base<A>(a.bases, (order + 1) / kGroup * a.column_blocks + column, all.a * q + all.b);
       }
-      look_back<A, 1>(a, order, static_cast<int>(column), after, kSiteBackward);
-      q = carried<A, 1>(a, order, static_cast<int>(column), 0, after, begin);
     } else if (order + 1 < stop) {
       Map<A> all = lead;
       for (int w = warp; w >= 0; --w) all = then(all, maps[w]);
@@ -736,10 +791,6 @@ __global__ void __launch_bounds__(kWarps * 32)
     if (a.dx != nullptr) store_run(static_cast<T*>(a.dx) + offset, count, vectors, dx);
     if (a.dgate != nullptr) store_run(static_cast<T*>(a.dgate) + offset, count, vectors, dg);
     if (a.dinitial != nullptr && first == 0) static_cast<A*>(a.dinitial)[column] = q;
-    if (a.shared && (order + 1) % kGroup == 0 && warp == 0 && order + 1 < a.chunks) {
-      if (lane == 0) static_cast<A*>(a.bases)[(order + 1) / kGroup * a.column_blocks + column] = q;
-      publish(a.flags + (a.chunks + (order + 1) / kGroup) * a.column_blocks + column);
-    }
   }
 }
 
@@ -750,8 +801,9 @@ struct RecurrencePlan {
   int vector, warps;   // columns a lane, warps a block
   int64_t chunks;
   int64_t column_blocks;
+  int balanced;
   bool shared;
-  size_t maps = 0, bases = 0, flags = 0, flag_bytes = 0, total = 0;
+  size_t maps = 0, bases = 0, ticket = 0, total = 0;
 };
 
 // Column blocks as wide as the widest vector allows; a pass over 16-bit columns of odd
@@ -765,6 +817,8 @@ RecurrencePlan plan_recurrence(int dtype, int64_t outer, int64_t steps, int64_t 
   const int64_t per_warp = p.along ? kAlongBlock : backward ? kBackwardSteps : kForwardSteps;
   p.warps = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kWarps, (steps + per_warp - 1) / per_warp)));
   p.chunks = std::max<int64_t>(1, (steps + p.warps * per_warp - 1) / (p.warps * per_warp));
+  // Up to 64 steps (one kept state), the warps share them evenly: 33 steps as 11 + 11 + 11.
+  if (!p.along && steps <= kStateBlock) p.balanced = static_cast<int>((steps + p.warps - 1) / p.warps);
   p.column_blocks = p.along ? columns : (columns + 32 * p.vector - 1) / (32 * p.vector);
   // Blocks of eight warps, at most three on an SM: with fewer than 2 blocks an SM, sharing the
   // time axis fills the machine.
@@ -778,8 +832,7 @@ RecurrencePlan plan_recurrence(int dtype, int64_t outer, int64_t steps, int64_t 
       p.total += (bytes + 255) / 256 * 256;
       return at;
     };
-    p.flag_bytes = static_cast<size_t>((p.chunks + groups) * p.column_blocks + 1) * sizeof(unsigned int);
-    p.flags = take(p.flag_bytes);
+    p.ticket = take(sizeof(unsigned int));
     p.maps = take(static_cast<size_t>(p.chunks * padded) * 2 * wide);
     p.bases = take(static_cast<size_t>(groups * padded) * wide);
   }
@@ -795,12 +848,13 @@ uint64_t wait_timeout() {
   return value;
 }
 
-// Binds the exchange area and clears its flags and ticket.
+// Binds the exchange area and sets its bits.
 int bind_exchange(const char* who, const RecurrencePlan& p, void* workspace, size_t bytes,
                   RecurrenceArgs* a, cudaStream_t stream) {
   a->chunks = p.chunks;
   a->column_blocks = static_cast<int>(p.column_blocks);
   a->shared = p.shared;
+  a->balanced = p.balanced;
   if (p.column_blocks > INT32_MAX) {
     return fail(CND_ERR_UNSUPPORTED, "%s: too many columns", who);
   }
@@ -812,12 +866,11 @@ int bind_exchange(const char* who, const RecurrencePlan& p, void* workspace, siz
   char* base = static_cast<char*>(workspace);
   a->maps = base + p.maps;
   a->bases = base + p.bases;
-  a->flags = reinterpret_cast<unsigned int*>(base + p.flags);
-  a->ticket = a->flags + p.flag_bytes / sizeof(unsigned int) - 1;
+  a->ticket = reinterpret_cast<unsigned int*>(base + p.ticket);
   a->error = device_error_word();
   a->timeout_ns = wait_timeout();
   if (a->error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
-  if (cudaMemsetAsync(a->flags, 0, p.flag_bytes, stream) != cudaSuccess) return launch_status(who);
+  if (cudaMemsetAsync(workspace, 0xff, p.total, stream) != cudaSuccess) return launch_status(who);
   return CND_OK;
 }
 
