@@ -197,6 +197,19 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   return *reinterpret_cast<const Pack<T, V>*>(p);
 }
 
+// The same where `valid`, else `other` everywhere. A step past the end is given the gate
+// +inf and x = dy = 0: it holds the state and passes the flow on, so the walks need no
+// branches (a branch per step had kept the exponentials of different steps from
+// overlapping).
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p, bool valid, float other) {
+  Pack<T, V> v;
+#pragma unroll
+  for (int i = 0; i < V; ++i) v.v[i] = narrow<T>(static_cast<typename Wide<T>::type>(other));
+  if (valid) v = *reinterpret_cast<const Pack<T, V>*>(p);
+  return v;
+}
+
 template <typename A>
 __device__ __forceinline__ Map<A> shuffle_up(const Map<A>& m, int d) {
   return {__shfl_up_sync(0xffffffffu, m.a, d), __shfl_up_sync(0xffffffffu, m.b, d)};
@@ -313,10 +326,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     Pack<T, V> px[kSteps], pg[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      if (i < count) {
-        px[i] = load_pack<T, V>(x + i * a.inner);
-        pg[i] = load_pack<T, V>(gate + i * a.inner);
-      }
+      px[i] = load_pack<T, V>(x + i * a.inner, i < count, 0.0f);
+      pg[i] = load_pack<T, V>(gate + i * a.inner, i < count, INFINITY);
     }
     A f[kSteps][V], b[kSteps][V];
     Map<A> own[V];
@@ -326,13 +337,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        f[i][v] = A(1);
-        b[i][v] = A(0);
-        if (i < count) {
-          A keep;
-          gates<T>(widen(pg[i].v[v]), &f[i][v], &keep);
-          b[i][v] = keep * widen(px[i].v[v]);
-        }
+        A keep;
+        gates<T>(widen(pg[i].v[v]), &f[i][v], &keep);
+        b[i][v] = keep * widen(px[i].v[v]);
         own[v] = then(own[v], Map<A>{f[i][v], b[i][v]});
       }
     }
@@ -443,17 +450,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     Pack<T, V> px[kSteps], pg[kSteps], pd[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      if (i < count) {
-        px[i] = load_pack<T, V>(static_cast<const T*>(a.x) + offset + i * a.inner);
-        pg[i] = load_pack<T, V>(static_cast<const T*>(a.gate) + offset + i * a.inner);
-        if (a.dy != nullptr) {
-          pd[i] = load_pack<T, V>(static_cast<const T*>(a.dy) + offset + i * a.inner);
-        }
-      }
-      if (i >= count || a.dy == nullptr) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) pd[i].v[v] = narrow<T>(A(0));
-      }
+      const int64_t at = offset + i * a.inner;
+      px[i] = load_pack<T, V>(static_cast<const T*>(a.x) + at, i < count, 0.0f);
+      pg[i] = load_pack<T, V>(static_cast<const T*>(a.gate) + at, i < count, INFINITY);
+      pd[i] = load_pack<T, V>(static_cast<const T*>(a.dy) + at, i < count && a.dy != nullptr, 0.0f);
     }
     A saved[V];  // the state before the chunk
 #pragma unroll
@@ -474,12 +474,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        f[i][v] = A(1);
-        keep[i][v] = A(0);
-        if (i < count) {
-          gates<T>(widen(pg[i].v[v]), &f[i][v], &keep[i][v]);
-          own[v] = then(own[v], Map<A>{f[i][v], keep[i][v] * widen(px[i].v[v])});
-        }
+        gates<T>(widen(pg[i].v[v]), &f[i][v], &keep[i][v]);
+        own[v] = then(own[v], Map<A>{f[i][v], keep[i][v] * widen(px[i].v[v])});
       }
     }
 #pragma unroll
@@ -546,7 +542,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         prior[i][v] = saved[v];
-        if (i < count) saved[v] = f[i][v] * saved[v] + keep[i][v] * widen(px[i].v[v]);
+        saved[v] = f[i][v] * saved[v] + keep[i][v] * widen(px[i].v[v]);
       }
     }
 #pragma unroll
@@ -555,11 +551,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const A total = widen(pd[i].v[v]) + q[v];
-        if (i < count) {
-          dx.v[v] = narrow<T>(keep[i][v] * total);
-          dg.v[v] = narrow<T>(f[i][v] * keep[i][v] * (prior[i][v] - widen(px[i].v[v])) * total);
-          q[v] = f[i][v] * total;
-        }
+        dx.v[v] = narrow<T>(keep[i][v] * total);
+        dg.v[v] = narrow<T>(f[i][v] * keep[i][v] * (prior[i][v] - widen(px[i].v[v])) * total);
+        q[v] = f[i][v] * total;
       }
       if (i < count) {
         if (a.dx != nullptr) {
@@ -582,7 +576,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 // A thread's run of kAlongSteps steps: one 16-byte (32 for float32) access where rows are
 // aligned, else single elements.
 template <typename T>
-__device__ __forceinline__ void load_run(const T* p, int count, bool vectors,
+__device__ __forceinline__ void load_run(const T* p, int count, bool vectors, float other,
                                          T (&v)[kAlongSteps]) {
   constexpr int kPer = 16 / sizeof(T);
   if (vectors && count == kAlongSteps) {
@@ -592,7 +586,10 @@ __device__ __forceinline__ void load_run(const T* p, int count, bool vectors,
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kAlongSteps; ++i) v[i] = i < count ? p[i] : narrow<T>(0);
+    for (int i = 0; i < kAlongSteps; ++i) {
+      v[i] = narrow<T>(static_cast<typename Wide<T>::type>(other));
+      if (i < count) v[i] = p[i];
+    }
   }
 }
 
@@ -636,19 +633,15 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int64_t offset = column * a.steps + first;
     const int count = steps_here(a.steps - first, kAlongSteps);
     alignas(16) T x[kAlongSteps], g[kAlongSteps];
-    load_run(static_cast<const T*>(a.x) + offset, count, vectors, x);
-    load_run(static_cast<const T*>(a.gate) + offset, count, vectors, g);
+    load_run(static_cast<const T*>(a.x) + offset, count, vectors, 0.0f, x);
+    load_run(static_cast<const T*>(a.gate) + offset, count, vectors, INFINITY, g);
     A f[kAlongSteps], b[kAlongSteps];
     Map<A> own{A(1), A(0)};
 #pragma unroll
     for (int i = 0; i < kAlongSteps; ++i) {
-      f[i] = A(1);
-      b[i] = A(0);
-      if (i < count) {
-        A keep;
-        gates<T>(widen(g[i]), &f[i], &keep);
-        b[i] = keep * widen(x[i]);
-      }
+      A keep;
+      gates<T>(widen(g[i]), &f[i], &keep);
+      b[i] = keep * widen(x[i]);
       own = then(own, Map<A>{f[i], b[i]});
     }
 #pragma unroll
@@ -720,9 +713,9 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int64_t offset = column * a.steps + first;
     const int count = steps_here(a.steps - first, kAlongSteps);
     alignas(16) T x[kAlongSteps], g[kAlongSteps], d[kAlongSteps];
-    load_run(static_cast<const T*>(a.x) + offset, count, vectors, x);
-    load_run(static_cast<const T*>(a.gate) + offset, count, vectors, g);
-    load_run(static_cast<const T*>(a.dy) + offset, a.dy != nullptr ? count : 0, vectors, d);
+    load_run(static_cast<const T*>(a.x) + offset, count, vectors, 0.0f, x);
+    load_run(static_cast<const T*>(a.gate) + offset, count, vectors, INFINITY, g);
+    load_run(static_cast<const T*>(a.dy) + offset, a.dy != nullptr ? count : 0, vectors, 0.0f, d);
     const int64_t warp_first = first - lane * kAlongSteps;
     A state = warp_first < a.steps
                   ? static_cast<const A*>(a.states_in)[warp_first / kAlongBlock * a.columns + column]
@@ -731,12 +724,8 @@ __global__ void __launch_bounds__(kWarps * 32)
     Map<A> own{A(1), A(0)};
 #pragma unroll
     for (int i = 0; i < kAlongSteps; ++i) {
-      f[i] = A(1);
-      keep[i] = A(0);
-      if (i < count) {
-        gates<T>(widen(g[i]), &f[i], &keep[i]);
-        own = then(own, Map<A>{f[i], keep[i] * widen(x[i])});
-      }
+      gates<T>(widen(g[i]), &f[i], &keep[i]);
+      own = then(own, Map<A>{f[i], keep[i] * widen(x[i])});
     }
     Map<A> back{own.a, A(0)};
 #pragma unroll
@@ -778,7 +767,7 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
     for (int i = 0; i < kAlongSteps; ++i) {
       prior[i] = state;
-      if (i < count) state = f[i] * state + keep[i] * widen(x[i]);
+      state = f[i] * state + keep[i] * widen(x[i]);
     }
     alignas(16) T dx[kAlongSteps], dg[kAlongSteps];
 #pragma unroll
@@ -786,7 +775,7 @@ __global__ void __launch_bounds__(kWarps * 32)
       const A total = widen(d[i]) + q;
       dx[i] = narrow<T>(keep[i] * total);
       dg[i] = narrow<T>(f[i] * keep[i] * (prior[i] - widen(x[i])) * total);
-      if (i < count) q = f[i] * total;
+      q = f[i] * total;
     }
     if (a.dx != nullptr) store_run(static_cast<T*>(a.dx) + offset, count, vectors, dx);
     if (a.dgate != nullptr) store_run(static_cast<T*>(a.dgate) + offset, count, vectors, dg);
