@@ -8,61 +8,127 @@
 namespace cnd {
 namespace layers {
 
-// Phi(v) and exp(-v^2 / 2) by Abramowitz and Stegun, Handbook of Mathematical Functions,
-// formula 7.1.26: erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by at most
-// 1.5e-7. Used where the result is rounded to 16 bits: it costs half of erff and shares
-// its exponential with phi.
-__device__ __forceinline__ float normal_cdf_16(float v, float* gauss) {
-  const float x = fabsf(v) * 0.70710678f;
-  const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
-  const float e = __expf(-x * x);
-  float p = fmaf(1.061405429f, t, -1.453152027f);
-  p = fmaf(p, t, 1.421413741f);
-  p = fmaf(p, t, -0.284496736f);
-  p = fmaf(p, t, 0.254829592f);
-  const float tail = 0.5f * p * t * e;  // Phi(-|v|)
-  *gauss = e;
-  return v < 0.0f ? tail : 1.0f - tail;
+// Two float32 values in one 64-bit register pair: sm_100 multiplies and adds them with one
+// instruction.
+struct Two {
+  unsigned long long bits;
+};
+
+__device__ __forceinline__ Two two(float lo, float hi) {
+  Two t;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(t.bits) : "f"(lo), "f"(hi));
+  return t;
+}
+__device__ __forceinline__ void unpack(Two t, float* lo, float* hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*lo), "=f"(*hi) : "l"(t.bits));
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return d;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
+  return d;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
+  return d;
+}
+__device__ __forceinline__ Two same(float v) { return two(v, v); }
+
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 
-// kExact: results of float32 or float64 accuracy; else good to well below 16-bit rounding.
-template <bool kExact, typename A>
-__device__ __forceinline__ A activate(A v, int act) {
+// Phi(-|v|) and exp(-v^2 / 2) of two values, with |v| cut at 64 in `size`, by Abramowitz and
+// Stegun, Handbook of Mathematical Functions, formula 7.1.26:
+//   erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + p x), x >= 0,
+// off by at most 1.5e-7. Used where the result is rounded to 16 bits: the polynomial is
+// half an instruction a value and step, and phi shares the exponential.
+__device__ __forceinline__ Two normal_tail(Two v, Two* size, Two* gauss) {
+  float lo, hi;
+  unpack(v, &lo, &hi);
+  *size = two(fminf(fabsf(lo), 64.0f), fminf(fabsf(hi), 64.0f));
+  // exp(-v^2 / 2) = 2^(-v^2 / (2 ln 2))
+  float e0, e1, d0, d1;
+  unpack(mul2(mul2(v, v), same(-0.72134752044f)), &e0, &e1);
+  *gauss = two(exp2_fast(e0), exp2_fast(e1));
+  unpack(fma2(*size, same(0.3275911f * 0.70710678119f), same(1.0f)), &d0, &d1);
+  const Two t = two(reciprocal_fast(d0), reciprocal_fast(d1));
+  Two p = fma2(t, same(0.5f * 1.061405429f), same(0.5f * -1.453152027f));
+  p = fma2(p, t, same(0.5f * 1.421413741f));
+  p = fma2(p, t, same(0.5f * -0.284496736f));
+  p = fma2(p, t, same(0.5f * 0.254829592f));
+  return mul2(mul2(p, t), *gauss);
+}
+
+// act(v) of two values, good to well below 16-bit rounding. GELU(v) = max(v, 0) - |v| Phi(-|v|)
+// for either sign; its value at -infinity is the limit, 0.
+__device__ __forceinline__ Two activate2(Two v, int act) {
   if (act == CND_ACT_GELU) {
-    if constexpr (kExact) {
-      return A(0.5) * v * (A(1) + erf(v * A(0.70710678118654752440)));
-    } else {
-      float gauss;
-      const float cdf = normal_cdf_16(v, &gauss);
-      return v == -INFINITY ? 0.0f * v : v * cdf;
-    }
+    Two size, gauss;
+    const Two tail = normal_tail(v, &size, &gauss);
+    float lo, hi;
+    unpack(v, &lo, &hi);
+    return fma2(mul2(size, same(-1.0f)), tail, two(fmaxf(lo, 0.0f), fmaxf(hi, 0.0f)));
   }
   if (act == CND_ACT_SILU) {
-    if constexpr (kExact) return v / (A(1) + exp(-v));
-    return __fdividef(v, 1.0f + __expf(-v));
+    float lo, hi, e0, e1;
+    unpack(v, &lo, &hi);
+    unpack(mul2(v, same(-1.44269504089f)), &e0, &e1);
+    return two(__fdividef(lo, 1.0f + exp2_fast(e0)), __fdividef(hi, 1.0f + exp2_fast(e1)));
   }
   return v;
 }
 
-template <bool kExact, typename A>
-__device__ __forceinline__ A activation_slope(A v, int act) {
+// act'(v) of two values, likewise.
+__device__ __forceinline__ Two slope2(Two v, int act) {
+  float lo, hi;
+  unpack(v, &lo, &hi);
   if (act == CND_ACT_GELU) {
-    if constexpr (kExact) {
-      const A cdf = A(0.5) * (A(1) + erf(v * A(0.70710678118654752440)));
-      return cdf + v * exp(A(-0.5) * v * v) * A(0.39894228040143267794);
-    } else {
-      float gauss;
-      const float cdf = normal_cdf_16(v, &gauss);
-      return fmaf(v * gauss, 0.39894228f, cdf);
-    }
+    Two size, gauss;
+    // Phi(v) = 1/2 + copysign(1/2 - Phi(-|v|), v)
+    float s0, s1;
+    unpack(fma2(normal_tail(v, &size, &gauss), same(-1.0f), same(0.5f)), &s0, &s1);
+    const Two cdf = add2(two(copysignf(s0, lo), copysignf(s1, hi)), same(0.5f));
+    return fma2(mul2(two(copysignf(1.0f, lo), copysignf(1.0f, hi)), mul2(size, gauss)),
+                same(0.39894228040f), cdf);
   }
   if (act == CND_ACT_SILU) {
-    A s;
-    if constexpr (kExact) {
-      s = A(1) / (A(1) + exp(-v));
-    } else {
-      s = __fdividef(1.0f, 1.0f + __expf(-v));
-    }
+    float e0, e1;
+    unpack(mul2(v, same(-1.44269504089f)), &e0, &e1);
+    const Two s = two(reciprocal_fast(1.0f + exp2_fast(e0)), reciprocal_fast(1.0f + exp2_fast(e1)));
+    return mul2(s, fma2(v, fma2(s, same(-1.0f), same(1.0f)), same(1.0f)));
+  }
+  return same(1.0f);
+}
+
+// To the accuracy of float32 and float64.
+template <typename A>
+__device__ __forceinline__ A activate(A v, int act) {
+  if (act == CND_ACT_GELU) return A(0.5) * v * (A(1) + erf(v * A(0.70710678118654752440)));
+  if (act == CND_ACT_SILU) return v / (A(1) + exp(-v));
+  return v;
+}
+
+template <typename A>
+__device__ __forceinline__ A activation_slope(A v, int act) {
+  if (act == CND_ACT_GELU) {
+    const A cdf = A(0.5) * (A(1) + erf(v * A(0.70710678118654752440)));
+    return cdf + v * exp(A(-0.5) * v * v) * A(0.39894228040143267794);
+  }
+  if (act == CND_ACT_SILU) {
+    const A s = A(1) / (A(1) + exp(-v));
     return s * (A(1) + v * (A(1) - s));
   }
   return A(1);

@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256) double_product_kernel(const DoubleProduct
       double v = sum[i][j];
       if (p.bias != nullptr) v += p.bias[n];
       if (p.pre != nullptr) p.pre[m * p.n + n] = v;
-      v = activate<true>(v, p.act);
+      v = activate(v, p.act);
       if (p.residual != nullptr) v += p.residual[m * p.n + n];
       p.d[m * p.n + n] = v;
     }
@@ -100,7 +100,6 @@ constexpr int kPrepareColumns = 256;  // columns of a block: 32 lanes of 8
 template <typename T>
 __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
   using A = typename Wide<T>::type;
-  constexpr bool kExact = sizeof(T) >= 4;
   constexpr int kLoad = sizeof(T) == 2 ? 8 : 16 / sizeof(T);
   __shared__ A part[8][kPrepareColumns];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -134,12 +133,22 @@ __global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = widen(v[i]);
       if (a.pre != nullptr) {
+        const auto apply = [&](int act) {
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            if constexpr (sizeof(T) == 2) {
+              unpack(mul2(two(w[i], w[i + 1]), slope2(two(widen(z[i]), widen(z[i + 1])), act)), &w[i],
+                    &w[i + 1]);
+            } else {
+              w[i] *= activation_slope<A>(widen(z[i]), act);
+              w[i + 1] *= activation_slope<A>(widen(z[i + 1]), act);
+            }
+          }
+        };
         if (a.act == CND_ACT_GELU) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] *= activation_slope<kExact>(widen(z[i]), CND_ACT_GELU);
+          apply(CND_ACT_GELU);
         } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] *= activation_slope<kExact>(widen(z[i]), CND_ACT_SILU);
+          apply(CND_ACT_SILU);
         }
       }
 #pragma unroll

@@ -28,6 +28,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdlib>
+#include <cstring>
 
 #include "activation.cuh"
 #include "layers.cuh"
@@ -55,7 +56,8 @@ struct Maps {
 struct KernelArgs {
   int64_t m, n;
   int tiles_m, tiles_n, splits, k_blocks;
-  int stages, buffers;  // operand stages; staging tiles per epilogue group
+  int stages;         // operand stages
+  int buffers, sets;  // staging tiles of an epilogue group; how many units they hold
   uint32_t idesc;
   uint32_t a_step, b_step;  // descriptor units (16 bytes) per 16 of k
   uint32_t a_lbo, b_lbo;
@@ -106,19 +108,54 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, dev::E
   return __all_sync(0xffffffffu, wait<kPair>(bar, parity, err, site, timeout_ns)) != 0;
 }
 
+template <typename Out>
+__device__ __forceinline__ uint32_t narrow2(Two v) {
+  float lo, hi;
+  unpack(v, &lo, &hi);
+  uint32_t bits;
+  if constexpr (sizeof(Out) == 2) {
+    Pack<Out, 2> p;
+    p.v[0] = narrow<Out>(lo);
+    p.v[1] = narrow<Out>(hi);
+    memcpy(&bits, &p, 4);
+  }
+  return bits;
+}
+template <>
+__device__ __forceinline__ uint32_t narrow2<__nv_bfloat16>(Two v) {
+  float lo, hi;
+  unpack(v, &lo, &hi);
+  uint32_t bits;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(bits) : "f"(hi), "f"(lo));
+  return bits;
+}
+template <>
+__device__ __forceinline__ uint32_t narrow2<__half>(Two v) {
+  float lo, hi;
+  unpack(v, &lo, &hi);
+  uint32_t bits;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(bits) : "f"(hi), "f"(lo));
+  return bits;
+}
+
 // Writes 32 values of a row (columns half * 32 ... of a unit) into a 128-byte-wide staging
 // tile with the 128-byte TMA swizzle (16-byte chunk c of row r at chunk c ^ (r & 7)).
 template <typename Out>
-__device__ __forceinline__ void stage_row(uint8_t* tile, int row, int half, const float (&v)[32]) {
-  constexpr int kPerChunk = 16 / sizeof(Out);
-  constexpr int kChunks = 32 / kPerChunk;
+__device__ __forceinline__ void stage_row(uint8_t* tile, int row, int half, const Two (&v)[16]) {
   uint8_t* base = tile + row * 128;
+  if constexpr (sizeof(Out) == 4) {
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    Pack<Out, kPerChunk> p;
+    for (int c = 0; c < 8; ++c) {
+      *reinterpret_cast<ulonglong2*>(base + ((c ^ (row & 7)) * 16)) =
+          make_ulonglong2(v[2 * c].bits, v[2 * c + 1].bits);
+    }
+  } else {
 #pragma unroll
-    for (int i = 0; i < kPerChunk; ++i) p.v[i] = narrow<Out>(v[c * kPerChunk + i]);
-    *reinterpret_cast<Pack<Out, kPerChunk>*>(base + (((half * kChunks + c) ^ (row & 7)) * 16)) = p;
+    for (int c = 0; c < 4; ++c) {
+      *reinterpret_cast<uint4*>(base + (((half * 4 + c) ^ (row & 7)) * 16)) =
+          make_uint4(narrow2<Out>(v[4 * c]), narrow2<Out>(v[4 * c + 1]),
+                     narrow2<Out>(v[4 * c + 2]), narrow2<Out>(v[4 * c + 3]));
+    }
   }
 }
 
@@ -140,30 +177,35 @@ __device__ __forceinline__ void copy_unit(const uint8_t* tile, Out* d, int64_t r
   }
 }
 
+// 32 residual values of a row, zero outside the matrix.
 template <typename Out>
-__device__ __forceinline__ void load_residual(const KernelArgs& a, int64_t row, int64_t col,
-                                              float (&r)[32]) {
-  constexpr int kPer = 16 / sizeof(Out);
-  const Out* p = static_cast<const Out*>(a.residual) + row * a.n + col;
+struct Residual {
+  static constexpr int kPer = 16 / sizeof(Out);
+  Pack<Out, kPer> q[32 / kPer];
+
+  __device__ __forceinline__ void load(const KernelArgs& a, int64_t row, int64_t col) {
+    const Out* p = static_cast<const Out*>(a.residual) + row * a.n + col;
 #pragma unroll
-  for (int c = 0; c < 32 / kPer; ++c) {
-    Pack<Out, kPer> q;
-    if (a.vector_residual) {
-      if (row < a.m && col + c * kPer < a.n) {
-        q = *reinterpret_cast<const Pack<Out, kPer>*>(p + c * kPer);
+    for (int c = 0; c < 32 / kPer; ++c) {
+      q[c] = Pack<Out, kPer>{};
+      if (a.vector_residual) {
+        if (row < a.m && col + c * kPer < a.n) {
+          q[c] = *reinterpret_cast<const Pack<Out, kPer>*>(p + c * kPer);
+        }
       } else {
-        q = Pack<Out, kPer>{};
-      }
-    } else {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        q.v[i] = row < a.m && col + c * kPer + i < a.n ? p[c * kPer + i] : narrow<Out>(0.0f);
+        for (int i = 0; i < kPer; ++i) {
+          if (row < a.m && col + c * kPer + i < a.n) q[c].v[i] = p[c * kPer + i];
+        }
       }
     }
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) r[c * kPer + i] = widen(q.v[i]);
   }
-}
+
+  __device__ __forceinline__ Two pair(int i) const {
+    return two(widen(q[2 * i / kPer].v[2 * i % kPer]),
+               widen(q[(2 * i + 1) / kPer].v[(2 * i + 1) % kPer]));
+  }
+};
 
 template <int kPair, int kBN, int kParts, typename Out>
 __global__ void __launch_bounds__(kBlockThreads, 1)
@@ -401,6 +443,10 @@ __global__ void __launch_bounds__(kBlockThreads, 1)
                         : 0.0f;
       }
       dev::named_barrier(1, 32 * kEpilogueWarps);
+      Residual<Out> residual[kParts == 1 ? 2 : 1];
+      if (kParts == 1 && a.residual != nullptr && works) {
+        residual[0].load(a, row0 + row, col0);
+      }
 
       float sums[kParts == 3 ? kHalves : 1][32];
       if constexpr (kParts == 3) {
@@ -449,14 +495,17 @@ __global__ void __launch_bounds__(kBlockThreads, 1)
 
       const uint32_t acc = tmem + lanes + set * kBN + group * kGroupCols;
       uint8_t *tile = own, *pre_tile = own;
+      uint32_t raw[kParts == 1 ? 2 : 1][32];
+      if (kParts == 1 && works) dev::tmem_load32(acc, raw[0]);
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
         constexpr int kHalvesPerUnit = kUnit / 32;
         if (!works) break;
         if (h % kHalvesPerUnit == 0) {
-          // a free staging tile for this unit (and one for its pre-activation)
+          // a free staging tile for this unit (and one for its pre-activation): the stores of
+          // all but the other sets of tiles have read their shared memory
           if (leader) {
-            if (a.buffers == 2 && a.pre == nullptr) {
+            if (a.sets == 2) {
               dev::bulk_wait_group_read<1>();
             } else {
               dev::bulk_wait_group_read<0>();
@@ -464,32 +513,36 @@ __global__ void __launch_bounds__(kBlockThreads, 1)
           }
           dev::named_barrier(2 + group, kGroupThreads);
           tile = own + buffer * kUnitBytes;
-          pre_tile = own + (a.buffers - 1) * kUnitBytes;
-          if (a.buffers == 2 && a.pre == nullptr) buffer ^= 1;
+          pre_tile = own + (buffer + a.sets) * kUnitBytes;
+          if (a.buffers == 1) pre_tile = tile;
+          if (a.sets == 2) buffer ^= 1;
         }
-        float v[32], r[32];
-        if (kParts == 1 && a.residual != nullptr) {
-          load_residual<Out>(a, row0 + row, col0 + h * 32, r);
-        }
+        Two v[16];
         if constexpr (kParts == 3) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = sums[h][i];
+          for (int i = 0; i < 16; ++i) v[i] = two(sums[h][2 * i], sums[h][2 * i + 1]);
         } else {
-          uint32_t raw[32];
-          dev::tmem_load32(acc + h * 32, raw);
+          // the next 32 columns are on their way while these are worked on
           dev::tmem_load_wait();
+          if (h + 1 < kHalves) {
+            dev::tmem_load32(acc + (h + 1) * 32, raw[(h + 1) & 1]);
+            if (a.residual != nullptr) {
+              residual[(h + 1) & 1].load(a, row0 + row, col0 + (h + 1) * 32);
+            }
+          } else {
+            free_set(acc_empty, release, set);
+          }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
-          if (h == kHalves - 1) free_set(acc_empty, release, set);
+          for (int i = 0; i < 16; ++i) {
+            v[i] = two(__uint_as_float(raw[h & 1][2 * i]), __uint_as_float(raw[h & 1][2 * i + 1]));
+          }
         }
         const float* bias = bias_s + group * kGroupCols + h * 32;
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 b4 = *reinterpret_cast<const float4*>(bias + i);
-          v[i] += b4.x;
-          v[i + 1] += b4.y;
-          v[i + 2] += b4.z;
-          v[i + 3] += b4.w;
+        for (int i = 0; i < 16; i += 2) {
+          const ulonglong2 b2 = *reinterpret_cast<const ulonglong2*>(bias + 2 * i);
+          v[i] = add2(v[i], Two{b2.x});
+          v[i + 1] = add2(v[i + 1], Two{b2.y});
         }
         const int64_t unit_col = col0 + (h / kHalvesPerUnit) * kUnit;
         const bool unit_done = h % kHalvesPerUnit == kHalvesPerUnit - 1;
@@ -514,17 +567,27 @@ __global__ void __launch_bounds__(kBlockThreads, 1)
             dev::named_barrier(2 + group, kGroupThreads);
           }
         }
+        const auto apply = [&](int act) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if constexpr (kExact) {
+              float lo, hi;
+              unpack(v[i], &lo, &hi);
+              v[i] = two(activate(lo, act), activate(hi, act));
+            } else {
+              v[i] = activate2(v[i], act);
+            }
+          }
+        };
         if (a.act == CND_ACT_GELU) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = activate<kExact>(v[i], CND_ACT_GELU);
+          apply(CND_ACT_GELU);
         } else if (a.act == CND_ACT_SILU) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = activate<kExact>(v[i], CND_ACT_SILU);
+          apply(CND_ACT_SILU);
         }
         if (a.residual != nullptr) {
-          if (kParts == 3) load_residual<Out>(a, row0 + row, col0 + h * 32, r);
+          if (kParts == 3) residual[0].load(a, row0 + row, col0 + h * 32);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] += r[i];
+          for (int i = 0; i < 16; ++i) v[i] = add2(v[i], residual[kParts == 1 ? h & 1 : 0].pair(i));
         }
         stage_row<Out>(tile, row, h % kHalvesPerUnit, v);
         if (unit_done) {
@@ -536,7 +599,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1)
               const int y = static_cast<int>(row0) + split * a.tiles_m * kPair * kBM;
               if (row0 < a.m) {
                 dev::tma_store_2d(&maps.out, tile, static_cast<int>(unit_col), y);
-                if (a.pre != nullptr && a.buffers == 2) {
+                if (a.pre != nullptr && a.buffers > 1) {
                   dev::tma_store_2d(&maps.pre, pre_tile, static_cast<int>(unit_col),
                                     static_cast<int>(row0));
                 }
@@ -545,7 +608,7 @@ __global__ void __launch_bounds__(kBlockThreads, 1)
             if (leader) dev::bulk_commit_group();
           } else {
             copy_unit<Out>(tile, static_cast<Out*>(a.d), row0, unit_col, a.m, a.n, quarter, lane);
-            if (a.pre != nullptr && a.buffers == 2) {
+            if (a.pre != nullptr && a.buffers > 1) {
               copy_unit<Out>(pre_tile, static_cast<Out*>(a.pre), row0, unit_col, a.m, a.n, quarter,
                              lane);
             }
@@ -580,7 +643,6 @@ template <typename Out>
 __global__ void __launch_bounds__(256)
     join_kernel(const float* partials, int splits, int64_t split_stride, int64_t pitch, int64_t m,
                 int64_t n, const void* bias, const void* residual, void* d, void* pre, int act) {
-  constexpr bool kExact = sizeof(Out) == 4;
   const int64_t quads = pitch / 4, count = m * quads;
   const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += step) {
@@ -603,7 +665,7 @@ __global__ void __launch_bounds__(256)
       float v = v4[j];
       if (bias != nullptr) v += widen(static_cast<const Out*>(bias)[c]);
       if (pre != nullptr) static_cast<Out*>(pre)[row * n + c] = narrow<Out>(v);
-      v = activate<kExact>(v, act);
+      v = activate(v, act);
       if (residual != nullptr) v += widen(static_cast<const Out*>(residual)[row * n + c]);
       static_cast<Out*>(d)[row * n + c] = narrow<Out>(v);
     }
@@ -680,9 +742,9 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 }  // namespace
 
 ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts) {
-  // Times in cycles of one SM: an operand block of 64 by bn columns takes bn * 2 cycles of
-  // the tensor core (six products: 12), an epilogue 10 per column, a launch that joins splits
-  // the time of its traffic.
+  // Times in cycles of one SM. A block of 64 of k takes the tensor core 2 cycles a column
+  // (six products: 12) and its operands 1 cycle per 60 bytes from L2, an epilogue about 12
+  // cycles a column; a launch that joins splits takes its traffic.
   const int64_t sms = 148, blocks = (k + kBK - 1) / kBK;
   ProductPlan best{1, 64, 1};
   double best_cost = 0;
@@ -694,9 +756,10 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts) {
       for (int64_t splits = 1; splits <= 64; ++splits) {
         if (splits > 1 && (blocks / splits < 4 || tiles * splits > 2 * slots)) break;
         const int64_t waves = (tiles * splits + slots - 1) / slots;
-        const double main = static_cast<double>((blocks + splits - 1) / splits) * bn * 2 *
-                            (parts == 3 ? 6 : 1) * (bn == 64 ? 1.5 : 1.0);
-        const double tail = 10.0 * bn + 1500;
+        const double per_block = std::max(2.0 * bn * (parts == 3 ? 6 : 1),
+                                          (kBM + bn / pair) * 128.0 * parts / 60.0);
+        const double main = static_cast<double>((blocks + splits - 1) / splits) * per_block;
+        const double tail = 12.0 * bn + 1000;
         double cost = waves * std::max(main, tail) + std::min(main, tail) + 1500;
         if (splits > 1) {
           cost += 6000 + static_cast<double>(splits + 1) * m * n * 4 / 3000.0;
@@ -737,7 +800,12 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
     return fail(CND_ERR_UNSUPPORTED, "linear: too many tiles");
   }
   const int out_dtype = split ? static_cast<int>(CND_F32) : p.dtype;
-  a.buffers = p.parts == 3 ? 1 : 2;
+  // Two units of staging hide the stores' latency behind the next unit; with a
+  // pre-activation that takes four tiles, which a short main loop can spare operand stages
+  // for (1M x 64 -> 256 GELU: 585 us with two, 0.5 of that with four).
+  const bool wants_pre = !split && p.pre != nullptr;
+  a.buffers = p.parts == 3 ? 1 : wants_pre && a.k_blocks <= 8 ? 4 : 2;
+  a.sets = wants_pre ? std::max(1, a.buffers / 2) : a.buffers;
   const uint32_t stage = p.parts * (kBM + plan.bn / plan.pair) * 128;
   const uint32_t fixed = 1024 + 2 * a.buffers * kUnitBytes + plan.bn * sizeof(float) + 256;
   a.stages = static_cast<int>(std::min<uint32_t>((kSharedLimit - fixed) / stage, kMostStages));
