@@ -3,7 +3,7 @@
 //   D[m][n] = act(sum_k A(m, k) B(n, k) + bias[n]) + residual[m][n]
 //
 // A persistent kernel: one warp loads 64-deep operand tiles by TMA into a ring of shared
-// memory stages, one warp issues the MMAs into TMEM accumulators, eight warps read them
+// memory stages, one warp issues the MMAs into TMEM accumulators, warps of an epilogue read them
 // back, apply the epilogue and hand finished 128-byte wide tiles to TMA stores. Two
 // accumulator sets let the epilogue of one tile run under the main loop of the next. Either
 // operand may be K-major or MN-major (dx reads W, dW reads dz and x as they lie in memory).
@@ -40,8 +40,8 @@ namespace layers {
 namespace {
 
 constexpr int kBM = 128, kBK = 64;
-constexpr int kEpilogueWarps = 8, kGroupThreads = 128;
-constexpr int kBlockThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kGroupThreads = 128, kGroupCols = 64;  // an epilogue group: four warps, 64 columns
+constexpr int block_threads(int bn) { return 64 + bn / kGroupCols * kGroupThreads; }
 constexpr uint32_t kUnitBytes = kBM * 128;  // staging tile: 128 rows of 128 bytes
 constexpr uint32_t kSharedLimit = 232448;
 constexpr int kMostStages = 8;
@@ -208,21 +208,22 @@ struct Residual {
 };
 
 template <int kPair, int kBN, int kParts, typename Out>
-__global__ void __launch_bounds__(kBlockThreads, 1)
+__global__ void __launch_bounds__(block_threads(kBN), 1)
     product_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ KernelArgs a) {
   constexpr bool kExact = sizeof(Out) == 4;
   constexpr int kColsB = kBN / kPair;  // rows of B that this CTA holds
   constexpr uint32_t kPartA = kBM * 128, kPartB = kColsB * 128;
   constexpr uint32_t kStageBytes = kParts * (kPartA + kPartB);
   constexpr int kUnit = 128 / sizeof(Out);      // columns of a staging tile
-  constexpr int kGroupCols = kBN / 2 < kUnit ? kUnit : kBN / 2;  // columns of a group
+  constexpr int kGroups = kBN / kGroupCols;
+  constexpr int kEpilogueWarps = 4 * kGroups;
   constexpr int kHalves = kGroupCols / 32;
   constexpr uint32_t kColumns = kParts == 1 ? 2 * kBN : 512;
 
   extern __shared__ __align__(1024) uint8_t shared[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(shared) + 1023) & ~uintptr_t{1023});
   uint8_t* staging = smem + a.stages * kStageBytes;
-  float* bias_s = reinterpret_cast<float*>(staging + 2 * a.buffers * kUnitBytes);
+  float* bias_s = reinterpret_cast<float*>(staging + kGroups * a.buffers * kUnitBytes);
   uint64_t* full = reinterpret_cast<uint64_t*>(bias_s + kBN);
   uint64_t* empty = full + kMostStages;
   uint64_t* acc_full = empty + kMostStages;
@@ -404,12 +405,13 @@ __global__ void __launch_bounds__(kBlockThreads, 1)
       }
     }
   } else {
-    // ---- epilogue: two groups of four warps, each a half of the tile's columns ----
+    // ---- epilogue: a group of four warps for every 64 columns. Four groups (256 columns)
+    // put four warps on a scheduler: with two, waiting for TMEM, the exponentials and the
+    // staging barriers left it issuing 27 % of the time (1M x 64 -> 256 GELU).
     const int group = (warp - 2) >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int epi = threadIdx.x - 64;
     const bool leader = (epi & (kGroupThreads - 1)) == 0;
-    const bool works = group * kGroupCols < kBN;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t release = kPair == 2 ? dev::map_to_rank(&acc_empty[0], 0) : 0;
     const uint32_t release_cross = kPair == 2 ? dev::map_to_rank(&cross_empty[0], 0) : 0;
@@ -443,10 +445,8 @@ __global__ void __launch_bounds__(kBlockThreads, 1)
                         : 0.0f;
       }
       dev::named_barrier(1, 32 * kEpilogueWarps);
-      Residual<Out> residual[kParts == 1 ? 2 : 1];
-      if (kParts == 1 && a.residual != nullptr && works) {
-        residual[0].load(a, row0 + row, col0);
-      }
+      Residual<Out> residual;
+      if (kParts == 1 && a.residual != nullptr) residual.load(a, row0 + row, col0);
 
       float sums[kParts == 3 ? kHalves : 1][32];
       if constexpr (kParts == 3) {
@@ -495,12 +495,9 @@ __global__ void __launch_bounds__(kBlockThreads, 1)
 
       const uint32_t acc = tmem + lanes + set * kBN + group * kGroupCols;
       uint8_t *tile = own, *pre_tile = own;
-      uint32_t raw[kParts == 1 ? 2 : 1][32];
-      if (kParts == 1 && works) dev::tmem_load32(acc, raw[0]);
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
         constexpr int kHalvesPerUnit = kUnit / 32;
-        if (!works) break;
         if (h % kHalvesPerUnit == 0) {
           // a free staging tile for this unit (and one for its pre-activation): the stores of
           // all but the other sets of tiles have read their shared memory
@@ -522,19 +519,14 @@ __global__ void __launch_bounds__(kBlockThreads, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = two(sums[h][2 * i], sums[h][2 * i + 1]);
         } else {
-          // the next 32 columns are on their way while these are worked on
+          uint32_t raw[32];
+          dev::tmem_load32(acc + h * 32, raw);
+          if (h > 0 && a.residual != nullptr) residual.load(a, row0 + row, col0 + h * 32);
           dev::tmem_load_wait();
-          if (h + 1 < kHalves) {
-            dev::tmem_load32(acc + (h + 1) * 32, raw[(h + 1) & 1]);
-            if (a.residual != nullptr) {
-              residual[(h + 1) & 1].load(a, row0 + row, col0 + (h + 1) * 32);
-            }
-          } else {
-            free_set(acc_empty, release, set);
-          }
+          if (h + 1 == kHalves) free_set(acc_empty, release, set);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            v[i] = two(__uint_as_float(raw[h & 1][2 * i]), __uint_as_float(raw[h & 1][2 * i + 1]));
+            v[i] = two(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
           }
         }
         const float* bias = bias_s + group * kGroupCols + h * 32;
@@ -585,9 +577,9 @@ __global__ void __launch_bounds__(kBlockThreads, 1)
           apply(CND_ACT_SILU);
         }
         if (a.residual != nullptr) {
-          if (kParts == 3) residual[0].load(a, row0 + row, col0 + h * 32);
+          if (kParts == 3) residual.load(a, row0 + row, col0 + h * 32);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = add2(v[i], residual[kParts == 1 ? h & 1 : 0].pair(i));
+          for (int i = 0; i < 16; ++i) v[i] = add2(v[i], residual.pair(i));
         }
         stage_row<Out>(tile, row, h % kHalvesPerUnit, v);
         if (unit_done) {
@@ -616,7 +608,6 @@ __global__ void __launch_bounds__(kBlockThreads, 1)
         }
       }
       if constexpr (kParts == 1) {
-        if (!works) free_set(acc_empty, release, set);
         if (++set == 2) {
           set = 0;
           set_phase ^= 1u;
@@ -800,14 +791,16 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
     return fail(CND_ERR_UNSUPPORTED, "linear: too many tiles");
   }
   const int out_dtype = split ? static_cast<int>(CND_F32) : p.dtype;
-  // Two units of staging hide the stores' latency behind the next unit; with a
-  // pre-activation that takes four tiles, which a short main loop can spare operand stages
-  // for (1M x 64 -> 256 GELU: 585 us with two, 0.5 of that with four).
+  // A second unit of staging hides the stores' latency behind the next unit. With a
+  // pre-activation a unit takes two tiles; where the main loop is short and the tiles few, two
+  // such units (64 KB a group) leave the operands enough stages.
   const bool wants_pre = !split && p.pre != nullptr;
-  a.buffers = p.parts == 3 ? 1 : wants_pre && a.k_blocks <= 8 ? 4 : 2;
+  const int groups = plan.bn / kGroupCols;
+  a.buffers = p.parts == 3 ? 1 : wants_pre && groups <= 2 ? 4 : 2;
+  if (groups == 4 && !wants_pre && a.k_blocks > 8) a.buffers = 1;
   a.sets = wants_pre ? std::max(1, a.buffers / 2) : a.buffers;
   const uint32_t stage = p.parts * (kBM + plan.bn / plan.pair) * 128;
-  const uint32_t fixed = 1024 + 2 * a.buffers * kUnitBytes + plan.bn * sizeof(float) + 256;
+  const uint32_t fixed = 1024 + groups * a.buffers * kUnitBytes + plan.bn * sizeof(float) + 256;
   a.stages = static_cast<int>(std::min<uint32_t>((kSharedLimit - fixed) / stage, kMostStages));
   const uint32_t shared = fixed + a.stages * stage;
   a.idesc = (1u << 4) | ((p.bf16 ? 1u : 0u) << 7) | ((p.bf16 ? 1u : 0u) << 10) |
@@ -857,7 +850,7 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
   const int slots = sm_count() / plan.pair;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(std::min(items, slots) * plan.pair));
-  config.blockDim = dim3(kBlockThreads);
+  config.blockDim = dim3(block_threads(plan.bn));
   config.dynamicSmemBytes = shared;
   config.stream = stream;
   cudaLaunchAttribute attribute{};
