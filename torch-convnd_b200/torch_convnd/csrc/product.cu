@@ -40,8 +40,8 @@ namespace layers {
 namespace {
 
 constexpr int kBM = 128, kBK = 64;
-constexpr int kGroupThreads = 128, kGroupCols = 64;  // an epilogue group: four warps, 64 columns
-constexpr int block_threads(int bn) { return 64 + bn / kGroupCols * kGroupThreads; }
+constexpr int kGroupThreads = 128;  // an epilogue group: four warps
+constexpr int block_threads(int groups) { return 64 + groups * kGroupThreads; }
 constexpr uint32_t kUnitBytes = kBM * 128;  // staging tile: 128 rows of 128 bytes
 constexpr uint32_t kSharedLimit = 232448;
 constexpr int kMostStages = 8;
@@ -207,15 +207,15 @@ struct Residual {
   }
 };
 
-template <int kPair, int kBN, int kParts, typename Out>
-__global__ void __launch_bounds__(block_threads(kBN), 1)
+template <int kPair, int kBN, int kParts, int kGroups, typename Out>
+__global__ void __launch_bounds__(block_threads(kGroups), 1)
     product_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ KernelArgs a) {
   constexpr bool kExact = sizeof(Out) == 4;
   constexpr int kColsB = kBN / kPair;  // rows of B that this CTA holds
   constexpr uint32_t kPartA = kBM * 128, kPartB = kColsB * 128;
   constexpr uint32_t kStageBytes = kParts * (kPartA + kPartB);
   constexpr int kUnit = 128 / sizeof(Out);      // columns of a staging tile
-  constexpr int kGroups = kBN / kGroupCols;
+  constexpr int kGroupCols = kBN / kGroups;     // columns of an epilogue group
   constexpr int kEpilogueWarps = 4 * kGroups;
   constexpr int kHalves = kGroupCols / 32;
   constexpr uint32_t kColumns = kParts == 1 ? 2 * kBN : 512;
@@ -405,9 +405,7 @@ __global__ void __launch_bounds__(block_threads(kBN), 1)
       }
     }
   } else {
-    // ---- epilogue: a group of four warps for every 64 columns. Four groups (256 columns)
-    // put four warps on a scheduler: with two, waiting for TMEM, the exponentials and the
-    // staging barriers left it issuing 27 % of the time (1M x 64 -> 256 GELU).
+    // ---- epilogue: groups of four warps, each kGroupCols columns of the tile ----
     const int group = (warp - 2) >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int epi = threadIdx.x - 64;
@@ -713,10 +711,14 @@ using Kernel = void (*)(Maps, KernelArgs);
 template <typename Out>
 Kernel pick(const ProductPlan& plan, int parts) {
   if constexpr (sizeof(Out) == 4) {
-    if (parts == 3) return product_tc_kernel<1, 128, 3, Out>;
+    if (parts == 3) return product_tc_kernel<1, 128, 3, 2, Out>;
   }
-  if (plan.pair == 2) return product_tc_kernel<2, 256, 1, Out>;
-  return plan.bn == 128 ? product_tc_kernel<1, 128, 1, Out> : product_tc_kernel<1, 64, 1, Out>;
+  if (plan.pair == 2) {
+    return plan.groups == 4 ? product_tc_kernel<2, 256, 1, 4, Out>
+                            : product_tc_kernel<2, 256, 1, 2, Out>;
+  }
+  return plan.bn == 128 ? product_tc_kernel<1, 128, 1, 2, Out>
+                        : product_tc_kernel<1, 64, 1, 1, Out>;
 }
 
 uint64_t wait_timeout() {
@@ -737,7 +739,7 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts) {
   // (six products: 12) and its operands 1 cycle per 60 bytes from L2, an epilogue about 12
   // cycles a column; a launch that joins splits takes its traffic.
   const int64_t sms = 148, blocks = (k + kBK - 1) / kBK;
-  ProductPlan best{1, 64, 1};
+  ProductPlan best{1, 64, 1, 1};
   double best_cost = 0;
   for (int pair = 2; pair >= 1; --pair) {
     for (int bn : {256, 128, 64}) {
@@ -757,7 +759,11 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts) {
         }
         if (best_cost == 0 || cost < best_cost) {
           best_cost = cost;
-          best = ProductPlan{pair, bn, static_cast<int>(splits)};
+          // Four epilogue groups (four warps a scheduler) where the epilogue is the longer part:
+          // with two, waits for TMEM, exponentials and staging left a scheduler issuing 27 %
+          // of the time (1M x 64 -> 256 GELU: 428 us against 320).
+          const int groups = bn == 64 ? 1 : bn == 256 && main < 2 * tail ? 4 : 2;
+          best = ProductPlan{pair, bn, static_cast<int>(splits), groups};
         }
       }
     }
@@ -791,16 +797,20 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
     return fail(CND_ERR_UNSUPPORTED, "linear: too many tiles");
   }
   const int out_dtype = split ? static_cast<int>(CND_F32) : p.dtype;
-  // A second unit of staging hides the stores' latency behind the next unit. With a
-  // pre-activation a unit takes two tiles; where the main loop is short and the tiles few, two
-  // such units (64 KB a group) leave the operands enough stages.
+  // A second unit of staging hides the stores' latency behind the next unit; a unit with a
+  // pre-activation takes two tiles. Two groups on a pair have main loops long enough to
+  // hide it: there the room goes to a sixth operand stage.
   const bool wants_pre = !split && p.pre != nullptr;
-  const int groups = plan.bn / kGroupCols;
-  a.buffers = p.parts == 3 ? 1 : wants_pre && groups <= 2 ? 4 : 2;
-  if (groups == 4 && !wants_pre && a.k_blocks > 8) a.buffers = 1;
+  if (p.parts == 3) {
+    a.buffers = 1;
+  } else if (plan.pair == 2) {
+    a.buffers = plan.groups == 4 || wants_pre ? 2 : 1;
+  } else {
+    a.buffers = wants_pre ? 4 : 2;
+  }
   a.sets = wants_pre ? std::max(1, a.buffers / 2) : a.buffers;
   const uint32_t stage = p.parts * (kBM + plan.bn / plan.pair) * 128;
-  const uint32_t fixed = 1024 + groups * a.buffers * kUnitBytes + plan.bn * sizeof(float) + 256;
+  const uint32_t fixed = 1024 + plan.groups * a.buffers * kUnitBytes + plan.bn * sizeof(float) + 256;
   a.stages = static_cast<int>(std::min<uint32_t>((kSharedLimit - fixed) / stage, kMostStages));
   const uint32_t shared = fixed + a.stages * stage;
   a.idesc = (1u << 4) | ((p.bf16 ? 1u : 0u) << 7) | ((p.bf16 ? 1u : 0u) << 10) |
@@ -850,7 +860,7 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
   const int slots = sm_count() / plan.pair;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(std::min(items, slots) * plan.pair));
-  config.blockDim = dim3(block_threads(plan.bn));
+  config.blockDim = dim3(block_threads(plan.groups));
   config.dynamicSmemBytes = shared;
   config.stream = stream;
   cudaLaunchAttribute attribute{};

@@ -31,9 +31,10 @@ struct Product {
   int act;
 };
 
-// How a product is cut: CTA pairs or single CTAs, tile width, splits of the k axis.
+// How a product is cut: CTA pairs or single CTAs, tile width, splits of the k axis, epilogue
+// groups.
 struct ProductPlan {
-  int pair, bn, splits;
+  int pair, bn, splits, groups;
 };
 
 ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts);
