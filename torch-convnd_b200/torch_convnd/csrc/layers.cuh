@@ -95,5 +95,8 @@ inline int launch_status(const char* what) {
 // SMs of the current device.
 int sm_count();
 
+// Limit of every wait inside a kernel (CND_WAIT_TIMEOUT_MS, 2 s).
+uint64_t wait_timeout_ns();
+
 }  // namespace layers
 }  // namespace cnd

@@ -13,9 +13,10 @@
 // block and leaves as one partial row per block, summed in order by a second launch. Rows
 // wider than the register kernels take are walked in chunks and read again for each pass.
 #include <algorithm>
-#include <cstring>
+#include <cstdlib>
 
 #include "layers.cuh"
+#include "pair.cuh"
 
 namespace cnd {
 namespace layers {
@@ -29,6 +30,15 @@ int sm_count() {
     return 148;
   }
   return count;
+}
+
+uint64_t wait_timeout_ns() {
+  static const uint64_t value = [] {
+    const char* env = std::getenv("CND_WAIT_TIMEOUT_MS");
+    const long long parsed = env != nullptr ? std::atoll(env) : 0;
+    return (parsed > 0 ? static_cast<uint64_t>(parsed) : uint64_t{2000}) * 1000000u;
+  }();
+  return value;
 }
 
 namespace {
@@ -65,180 +75,258 @@ __device__ __forceinline__ A group_sum(A v, A* scratch) {
   return v;
 }
 
-// Block size of the register kernels: 256 threads, or the G of one row when it needs more.
-template <int G>
-constexpr int block_size() {
-  return G > 256 ? G : (G > 32 ? G : 256);
+// R sums at once: the same for every one, with one pair of block barriers.
+template <int G, int R>
+__device__ __forceinline__ void group_sums(float (&v)[R], float (*scratch)[32]) {
+#pragma unroll
+  for (int d = (G < 32 ? G : 32) / 2; d > 0; d /= 2) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] += __shfl_xor_sync(0xffffffffu, v[r], d);
+  }
+  if constexpr (G > 32) {
+    constexpr int kWarps = G / 32;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) scratch[r][threadIdx.x >> 5] = v[r];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      v[r] = scratch[r][threadIdx.x & (kWarps - 1)];
+#pragma unroll
+      for (int d = kWarps / 2; d > 0; d /= 2) v[r] += __shfl_xor_sync(0xffffffffu, v[r], d);
+    }
+    __syncthreads();
+  }
 }
 
+// A thread's parameters, in float32 registers for all its rows: `absent` where there are none.
 template <typename T, int V, int NV, int G>
+__device__ __forceinline__ void load_params(const void* p, bool is_f32, int64_t width, int lane,
+                                            float absent, float (&v)[NV][V]) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (k * G + lane) * V + i;
+      v[k][i] = p != nullptr && c < width ? load_param<T>(p, is_f32, c) : absent;
+    }
+  }
+}
+
+// Block size of the register kernels: 256 threads, or one row's when it takes more than a warp.
+template <int G>
+constexpr int block_size() {
+  return G > 32 ? G : 256;
+}
+
+// Writes a block's column sums, held by groups of G <= 32 lanes, as one partial row: rows of
+// one warp first (lanes of the same columns), then the warps in order. `columns`: [2][width].
+template <typename T, int V, int NV, int G>
+__device__ __forceinline__ void block_columns(const NormArgs& a, float (&dw)[NV][V],
+                                              float (&db)[NV][V], float* columns) {
+  const int lane = threadIdx.x % G;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+      for (int d = G; d < 32; d *= 2) {
+        dw[k][i] += __shfl_xor_sync(0xffffffffu, dw[k][i], d);
+        db[k][i] += __shfl_xor_sync(0xffffffffu, db[k][i], d);
+      }
+    }
+  }
+  for (int w = 0; w < static_cast<int>(blockDim.x) / 32; ++w) {
+    if (static_cast<int>(threadIdx.x) / 32 == w && (threadIdx.x & 31) < G) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int64_t c = static_cast<int64_t>(k * G + lane) * V;
+        if (c < a.width) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            columns[c + i] = w == 0 ? dw[k][i] : columns[c + i] + dw[k][i];
+            columns[a.width + c + i] = w == 0 ? db[k][i] : columns[a.width + c + i] + db[k][i];
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+  float* partial = static_cast<float*>(a.partials) + static_cast<int64_t>(blockIdx.x) * 2 * a.width;
+  for (int64_t c = threadIdx.x; c < 2 * a.width; c += blockDim.x) partial[c] = columns[c];
+}
+
+// R rows of a group are in flight at once: their loads are issued before the first is summed,
+// and their sums share the reductions' latency.
+template <typename T, int V, int NV, int G, int R>
 __global__ void __launch_bounds__(block_size<G>())
     norm_forward_kernel(const NormArgs a) {
   constexpr int kRows = block_size<G>() / G;
-  __shared__ float scratch[32];
+  __shared__ float scratch[R][32];
   const int lane = threadIdx.x % G;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows * R;
   const float inverse = 1.0f / static_cast<float>(a.width);
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.rows; base += step) {
-    const int64_t row = base + threadIdx.x / G;
-    const bool live = row < a.rows;
-    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-    Pack<T, V> raw[NV];
-    float sum = 0.0f;
+  float w[NV][V], b[NV][V];
+  load_params<T, V, NV, G>(a.weight, a.param_f32, a.width, lane, 1.0f, w);
+  load_params<T, V, NV, G>(a.bias, a.param_f32, a.width, lane, 0.0f, b);
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows * R; base < a.rows; base += step) {
+    const int64_t row0 = base + threadIdx.x / G;
+    Pack<T, V> raw[R][NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int64_t c = static_cast<int64_t>(k * G + lane) * V;
-      if (live && c < a.width) {
-        raw[k] = *reinterpret_cast<const Pack<T, V>*>(x + c);
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = row0 + r * kRows;
+      const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum += widen(raw[k].v[i]);
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * G + lane) * V;
+        if (row < a.rows && c < a.width) raw[r][k] = *reinterpret_cast<const Pack<T, V>*>(x + c);
       }
     }
-    const float mean = group_sum<G>(sum, scratch) * inverse;
-    float squares = 0.0f;
+    float mean[R], squares[R];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int64_t c = static_cast<int64_t>(k * G + lane) * V;
-      if (live && c < a.width) {
+    for (int r = 0; r < R; ++r) {
+      mean[r] = squares[r] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = widen(raw[k].v[i]) - mean;
-          squares += d * d;
+      for (int k = 0; k < NV; ++k) {
+        if ((k * G + lane) * V < a.width) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) mean[r] += widen(raw[r][k].v[i]);
         }
       }
     }
-    const float variance = group_sum<G>(squares, scratch) * inverse;
-    const float rstd = rsqrtf(variance + static_cast<float>(a.eps));
-    if (!live) continue;
-    if (a.stats != nullptr && lane == 0) {
-      static_cast<float*>(a.stats)[row] = mean;
-      static_cast<float*>(a.stats)[a.rows + row] = rstd;
-    }
-    T* y = static_cast<T*>(a.y) + row * a.width;
+    group_sums<G, R>(mean, scratch);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int64_t c = static_cast<int64_t>(k * G + lane) * V;
-      if (c < a.width) {
-        Pack<T, V> out;
+    for (int r = 0; r < R; ++r) {
+      mean[r] *= inverse;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float v = (widen(raw[k].v[i]) - mean) * rstd;
-          if (a.weight != nullptr) v *= load_param<T>(a.weight, a.param_f32, c + i);
-          if (a.bias != nullptr) v += load_param<T>(a.bias, a.param_f32, c + i);
-          out.v[i] = narrow<T>(v);
+      for (int k = 0; k < NV; ++k) {
+        if ((k * G + lane) * V < a.width) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float d = widen(raw[r][k].v[i]) - mean[r];
+            squares[r] += d * d;
+          }
         }
-        *reinterpret_cast<Pack<T, V>*>(y + c) = out;
+      }
+    }
+    group_sums<G, R>(squares, scratch);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = row0 + r * kRows;
+      if (row >= a.rows) continue;
+      const float rstd = rsqrtf(squares[r] * inverse + static_cast<float>(a.eps));
+      if (a.stats != nullptr && lane == 0) {
+        static_cast<float*>(a.stats)[row] = mean[r];
+        static_cast<float*>(a.stats)[a.rows + row] = rstd;
+      }
+      T* y = static_cast<T*>(a.y) + row * a.width;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * G + lane) * V;
+        if (c < a.width) {
+          Pack<T, V> out;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            out.v[i] = narrow<T>((widen(raw[r][k].v[i]) - mean[r]) * rstd * w[k][i] + b[k][i]);
+          }
+          *reinterpret_cast<Pack<T, V>*>(y + c) = out;
+        }
       }
     }
   }
 }
 
-template <typename T, int V, int NV, int G>
+template <typename T, int V, int NV, int G, int R>
 __global__ void __launch_bounds__(block_size<G>())
     norm_backward_kernel(const NormArgs a) {
   constexpr int kThreads = block_size<G>();
   constexpr int kRows = kThreads / G;
   extern __shared__ float columns[];  // [2][width], only when kRows > 1
-  __shared__ float scratch[32];
+  __shared__ float scratch[2 * R][32];
   const int lane = threadIdx.x % G;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows * R;
   const float inverse = 1.0f / static_cast<float>(a.width);
   const float* means = static_cast<const float*>(a.stats);
-  float dw[NV][V], db[NV][V];
+  float w[NV][V], dw[NV][V], db[NV][V];
+  load_params<T, V, NV, G>(a.weight, a.param_f32, a.width, lane, 1.0f, w);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
 #pragma unroll
     for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.0f;
   }
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows; base < a.rows; base += step) {
-    const int64_t row = base + threadIdx.x / G;
-    const bool live = row < a.rows;
-    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-    const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
-    const float mean = live ? means[row] : 0.0f;
-    const float rstd = live ? means[a.rows + row] : 0.0f;
-    Pack<T, V> rx[NV], rd[NV];
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kRows * R; base < a.rows; base += step) {
+    const int64_t row0 = base + threadIdx.x / G;
+    Pack<T, V> rx[R][NV], rd[R][NV];
+    float mean[R], rstd[R];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int64_t c = static_cast<int64_t>(k * G + lane) * V;
-      if (live && c < a.width) {
-        rx[k] = *reinterpret_cast<const Pack<T, V>*>(x + c);
-        rd[k] = *reinterpret_cast<const Pack<T, V>*>(dy + c);
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = row0 + r * kRows;
+      const bool live = row < a.rows;
+      const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+      const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
+      mean[r] = live ? means[row] : 0.0f;
+      rstd[r] = live ? means[a.rows + row] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * G + lane) * V;
+        if (live && c < a.width) {
+          rx[r][k] = *reinterpret_cast<const Pack<T, V>*>(x + c);
+          rd[r][k] = *reinterpret_cast<const Pack<T, V>*>(dy + c);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) rx[r][k].v[i] = rd[r][k].v[i] = narrow<T>(0.0f);
+        }
       }
     }
-    float sum_g = 0.0f, sum_gu = 0.0f;
+    float sums[2 * R];
+#pragma unroll
+    for (int r = 0; r < 2 * R; ++r) sums[r] = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t c = static_cast<int64_t>(k * G + lane) * V;
-      if (live && c < a.width) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float d = widen(rd[k].v[i]);
-          const float u = (widen(rx[k].v[i]) - mean) * rstd;
-          const float g =
-              a.weight != nullptr ? d * load_param<T>(a.weight, a.param_f32, c + i) : d;
-          sum_g += g;
-          sum_gu += g * u;
+          const float d = widen(rd[r][k].v[i]);
+          const float u = (widen(rx[r][k].v[i]) - mean[r]) * rstd[r];
+          const float g = d * w[k][i];
+          sums[2 * r] += g;
+          sums[2 * r + 1] += g * u;
           dw[k][i] += d * u;
           db[k][i] += d;
         }
       }
     }
     if (!a.want_dx) continue;
-    const float mean_g = group_sum<G>(sum_g, scratch) * inverse;
-    const float mean_gu = group_sum<G>(sum_gu, scratch) * inverse;
-    if (!live) continue;
-    T* dx = static_cast<T*>(a.y) + row * a.width;
+    group_sums<G, 2 * R>(sums, scratch);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int64_t c = static_cast<int64_t>(k * G + lane) * V;
-      if (c < a.width) {
-        Pack<T, V> out;
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = row0 + r * kRows;
+      if (row >= a.rows) continue;
+      const float mean_g = sums[2 * r] * inverse, mean_gu = sums[2 * r + 1] * inverse;
+      T* dx = static_cast<T*>(a.y) + row * a.width;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = widen(rd[k].v[i]);
-          const float u = (widen(rx[k].v[i]) - mean) * rstd;
-          const float g =
-              a.weight != nullptr ? d * load_param<T>(a.weight, a.param_f32, c + i) : d;
-          out.v[i] = narrow<T>(rstd * (g - mean_g - u * mean_gu));
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * G + lane) * V;
+        if (c < a.width) {
+          Pack<T, V> out;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float d = widen(rd[r][k].v[i]);
+            const float u = (widen(rx[r][k].v[i]) - mean[r]) * rstd[r];
+            out.v[i] = narrow<T>(rstd[r] * (d * w[k][i] - mean_g - u * mean_gu));
+          }
+          *reinterpret_cast<Pack<T, V>*>(dx + c) = out;
         }
-        *reinterpret_cast<Pack<T, V>*>(dx + c) = out;
       }
     }
   }
   if (!a.want_params) return;
-  float* partial = static_cast<float*>(a.partials) + static_cast<int64_t>(blockIdx.x) * 2 * a.width;
   if constexpr (kRows > 1) {
-    // Rows of one warp first (lanes of the same columns), then the warps in order.
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-#pragma unroll
-        for (int d = G; d < 32; d *= 2) {
-          dw[k][i] += __shfl_xor_sync(0xffffffffu, dw[k][i], d);
-          db[k][i] += __shfl_xor_sync(0xffffffffu, db[k][i], d);
-        }
-      }
-    }
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (static_cast<int>(threadIdx.x) / 32 == w && (threadIdx.x & 31) < G) {
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          const int64_t c = static_cast<int64_t>(k * G + lane) * V;
-          if (c < a.width) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              columns[c + i] = w == 0 ? dw[k][i] : columns[c + i] + dw[k][i];
-              columns[a.width + c + i] = w == 0 ? db[k][i] : columns[a.width + c + i] + db[k][i];
-            }
-          }
-        }
-      }
-      __syncthreads();
-    }
-    for (int64_t c = threadIdx.x; c < 2 * a.width; c += kThreads) partial[c] = columns[c];
+    block_columns<T, V, NV, G>(a, dw, db, columns);
   } else {
+    float* partial = static_cast<float*>(a.partials) + static_cast<int64_t>(blockIdx.x) * 2 * a.width;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int64_t c = static_cast<int64_t>(k * G + lane) * V;
@@ -251,6 +339,398 @@ __global__ void __launch_bounds__(block_size<G>())
       }
     }
   }
+}
+
+// ---- long aligned rows: a ring of rows in shared memory -----------------------------------
+
+// A block of G threads walks rows that bulk copies bring into a ring of stages ahead of it (x,
+// and dy behind it in the backward), so the loads in flight depend neither on registers
+// nor on the block's barriers: holding 16 KB rows in registers had left the memory system at
+// 2.8 TB/s. A row is read again from shared memory for each of its passes. The stage
+// of one row is refilled after the first barrier of the next: by then every thread has
+// finished with it. Short rows that lie back to back come by the tile, whose rows the
+// block's warps share, with one barrier a tile.
+struct Ring {
+  int stages, tile;  // stages; rows of a stage
+  uint32_t row_bytes, stage_bytes;
+  unsigned int* error;
+  uint64_t timeout_ns;
+};
+
+constexpr uint32_t kSiteRing = 0x701;
+
+template <int G, bool kBackward>
+struct RowRing {
+  const NormArgs& a;
+  const Ring& ring;
+  uint8_t* data;
+  uint64_t* full;
+  int64_t next;  // the next row to ask for (thread 0)
+  int fill = 0, stage = 0;
+  uint32_t phase = 0;
+  bool dead = false;
+
+  __device__ __forceinline__ void ask(int es) {
+    // thread 0: rows `next` ... into stage `fill`
+    if (next >= a.rows || dead) return;
+    const int64_t left = a.rows - next;
+    const uint32_t bytes = ring.row_bytes * static_cast<uint32_t>(left < ring.tile ? left : ring.tile);
+    dev::mbar_arrive_expect_tx(&full[fill], kBackward ? 2 * bytes : bytes);
+    uint8_t* dst = data + fill * ring.stage_bytes;
+    dev::bulk_load(dst, static_cast<const char*>(a.x) + next * a.x_stride * es, bytes, &full[fill]);
+    if (kBackward) {
+      dev::bulk_load(dst + ring.stage_bytes / 2,
+                     static_cast<const char*>(a.dy) + next * a.dy_stride * es, bytes, &full[fill]);
+    }
+    next += static_cast<int64_t>(gridDim.x) * ring.tile;
+    if (++fill == ring.stages) fill = 0;
+  }
+
+  // Waits for the current stage. After a wait that expired no other one waits or asks.
+  __device__ __forceinline__ const uint8_t* wait() {
+    if (!dead && !dev::mbar_wait(&full[stage], phase, dev::ErrorWord{ring.error}, kSiteRing,
+                                 ring.timeout_ns)) {
+      dead = true;
+    }
+    return data + stage * ring.stage_bytes;
+  }
+
+  __device__ __forceinline__ void advance() {
+    if (++stage == ring.stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+template <typename T, int V, int NV, int G>
+__global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
+    norm_forward_ring_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Ring ring_args) {
+  extern __shared__ __align__(128) uint8_t shared[];
+  __shared__ float scratch[1][32];
+  __shared__ uint64_t full[16];
+  const int lane = threadIdx.x;
+  const float inverse = 1.0f / static_cast<float>(a.width);
+  if (lane == 0) {
+    for (int s = 0; s < ring_args.stages; ++s) dev::mbar_init(&full[s], 1);
+    dev::fence_barrier_init();
+  }
+  __syncthreads();
+  RowRing<G, false> ring{a, ring_args, shared, full, blockIdx.x};
+  if (lane == 0) {
+    for (int s = 0; s < ring_args.stages; ++s) ring.ask(sizeof(T));
+  }
+  float w[NV][V], b[NV][V];
+  load_params<T, V, NV, G>(a.weight, a.param_f32, a.width, lane, 1.0f, w);
+  load_params<T, V, NV, G>(a.bias, a.param_f32, a.width, lane, 0.0f, b);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const Pack<T, V>* x = reinterpret_cast<const Pack<T, V>*>(ring.wait());
+    float sum[1] = {0.0f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if ((k * G + lane) * V < a.width) {
+        const Pack<T, V> p = x[k * G + lane];
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[0] += widen(p.v[i]);
+      }
+    }
+    group_sums<G, 1>(sum, scratch);
+    // every thread has passed the previous row: its stage is free
+    if (lane == 0 && row != blockIdx.x) ring.ask(sizeof(T));
+    const float mean = sum[0] * inverse;
+    float squares[1] = {0.0f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if ((k * G + lane) * V < a.width) {
+        const Pack<T, V> p = x[k * G + lane];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float d = widen(p.v[i]) - mean;
+          squares[0] += d * d;
+        }
+      }
+    }
+    group_sums<G, 1>(squares, scratch);
+    const float rstd = rsqrtf(squares[0] * inverse + static_cast<float>(a.eps));
+    if (a.stats != nullptr && lane == 0) {
+      static_cast<float*>(a.stats)[row] = mean;
+      static_cast<float*>(a.stats)[a.rows + row] = rstd;
+    }
+    Pack<T, V>* y = reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * a.width);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if ((k * G + lane) * V < a.width) {
+        const Pack<T, V> p = x[k * G + lane];
+        Pack<T, V> out;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          out.v[i] = narrow<T>((widen(p.v[i]) - mean) * rstd * w[k][i] + b[k][i]);
+        }
+        y[k * G + lane] = out;
+      }
+    }
+    ring.advance();
+  }
+}
+
+template <typename T, int V, int NV, int G>
+__global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
+    norm_backward_ring_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Ring ring_args) {
+  extern __shared__ __align__(128) uint8_t shared[];
+  __shared__ float scratch[2][32];
+  __shared__ uint64_t full[16];
+  const int lane = threadIdx.x;
+  const float inverse = 1.0f / static_cast<float>(a.width);
+  const float* means = static_cast<const float*>(a.stats);
+  if (lane == 0) {
+    for (int s = 0; s < ring_args.stages; ++s) dev::mbar_init(&full[s], 1);
+    dev::fence_barrier_init();
+  }
+  __syncthreads();
+  RowRing<G, true> ring{a, ring_args, shared, full, blockIdx.x};
+  if (lane == 0) {
+    for (int s = 0; s < ring_args.stages; ++s) ring.ask(sizeof(T));
+  }
+  float w[NV][V], dw[NV][V], db[NV][V];
+  load_params<T, V, NV, G>(a.weight, a.param_f32, a.width, lane, 1.0f, w);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.0f;
+  }
+  float next_mean = blockIdx.x < a.rows ? means[blockIdx.x] : 0.0f;
+  float next_rstd = blockIdx.x < a.rows ? means[a.rows + blockIdx.x] : 0.0f;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float mean = next_mean, rstd = next_rstd;
+    if (row + gridDim.x < a.rows) {
+      next_mean = means[row + gridDim.x];
+      next_rstd = means[a.rows + row + gridDim.x];
+    }
+    const uint8_t* at = ring.wait();
+    const Pack<T, V>* x = reinterpret_cast<const Pack<T, V>*>(at);
+    const Pack<T, V>* dy = reinterpret_cast<const Pack<T, V>*>(at + ring_args.row_bytes);
+    float sums[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if ((k * G + lane) * V < a.width) {
+        const Pack<T, V> px = x[k * G + lane], pd = dy[k * G + lane];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float d = widen(pd.v[i]);
+          const float u = (widen(px.v[i]) - mean) * rstd;
+          const float g = d * w[k][i];
+          sums[0] += g;
+          sums[1] += g * u;
+          dw[k][i] += d * u;
+          db[k][i] += d;
+        }
+      }
+    }
+    group_sums<G, 2>(sums, scratch);
+    if (lane == 0 && row != blockIdx.x) ring.ask(sizeof(T));
+    if (a.want_dx) {
+      const float mean_g = sums[0] * inverse, mean_gu = sums[1] * inverse;
+      Pack<T, V>* dx = reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * a.width);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        if ((k * G + lane) * V < a.width) {
+          const Pack<T, V> px = x[k * G + lane], pd = dy[k * G + lane];
+          Pack<T, V> out;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float u = (widen(px.v[i]) - mean) * rstd;
+            out.v[i] = narrow<T>(rstd * (widen(pd.v[i]) * w[k][i] - mean_g - u * mean_gu));
+          }
+          dx[k * G + lane] = out;
+        }
+      }
+    }
+    ring.advance();
+  }
+  if (!a.want_params) return;
+  float* partial = static_cast<float*>(a.partials) + static_cast<int64_t>(blockIdx.x) * 2 * a.width;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int64_t c = static_cast<int64_t>(k * G + lane) * V;
+    if (c < a.width) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        partial[c + i] = dw[k][i];
+        partial[a.width + c + i] = db[k][i];
+      }
+    }
+  }
+}
+
+// Short rows in tiles: G lanes of a warp to a row, as in the register kernels.
+constexpr int kTileThreads = 256, kMostTile = 256;
+
+template <typename T, int V, int NV, int G>
+__global__ void __launch_bounds__(kTileThreads, 4)
+    norm_forward_tile_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Ring ring_args) {
+  constexpr int kGroups = kTileThreads / G;
+  extern __shared__ __align__(128) uint8_t shared[];
+  __shared__ uint64_t full[16];
+  const int lane = threadIdx.x % G, group = threadIdx.x / G;
+  const int width = static_cast<int>(a.width), tile = ring_args.tile;
+  const float inverse = 1.0f / static_cast<float>(width);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ring_args.stages; ++s) dev::mbar_init(&full[s], 1);
+    dev::fence_barrier_init();
+  }
+  __syncthreads();
+  RowRing<G, false> ring{a, ring_args, shared, full, static_cast<int64_t>(blockIdx.x) * tile};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ring_args.stages; ++s) ring.ask(sizeof(T));
+  }
+  float w[NV][V], b[NV][V];
+  load_params<T, V, NV, G>(a.weight, a.param_f32, width, lane, 1.0f, w);
+  load_params<T, V, NV, G>(a.bias, a.param_f32, width, lane, 0.0f, b);
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * tile; row0 < a.rows;
+       row0 += static_cast<int64_t>(gridDim.x) * tile) {
+    const T* data = reinterpret_cast<const T*>(ring.wait());
+    for (int i0 = 0; i0 < tile; i0 += kGroups) {
+      const int64_t row = row0 + i0 + group;
+      const bool live = i0 + group < tile && row < a.rows;
+      Pack<T, V> raw[NV];
+      float mean = 0.0f, squares = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * G + lane) * V;
+        if (live && c < width) {
+          raw[k] = *reinterpret_cast<const Pack<T, V>*>(data + (i0 + group) * width + c);
+#pragma unroll
+          for (int i = 0; i < V; ++i) mean += widen(raw[k].v[i]);
+        }
+      }
+      mean = group_sum<G, float>(mean, nullptr) * inverse;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        if (live && (k * G + lane) * V < width) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float d = widen(raw[k].v[i]) - mean;
+            squares += d * d;
+          }
+        }
+      }
+      squares = group_sum<G, float>(squares, nullptr);
+      if (!live) continue;
+      const float rstd = rsqrtf(squares * inverse + static_cast<float>(a.eps));
+      if (a.stats != nullptr && lane == 0) {
+        static_cast<float*>(a.stats)[row] = mean;
+        static_cast<float*>(a.stats)[a.rows + row] = rstd;
+      }
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * G + lane) * V;
+        if (c < width) {
+          Pack<T, V> out;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            out.v[i] = narrow<T>((widen(raw[k].v[i]) - mean) * rstd * w[k][i] + b[k][i]);
+          }
+          *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * width + c) = out;
+        }
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) ring.ask(sizeof(T));
+    ring.advance();
+  }
+}
+
+template <typename T, int V, int NV, int G>
+__global__ void __launch_bounds__(kTileThreads, NV == 1 ? 3 : 2)
+    norm_backward_tile_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Ring ring_args) {
+  constexpr int kGroups = kTileThreads / G;
+  extern __shared__ __align__(128) uint8_t shared[];
+  __shared__ uint64_t full[16];
+  __shared__ float2 stats[2][kMostTile];  // of this tile and the next
+  const int lane = threadIdx.x % G, group = threadIdx.x / G;
+  const int width = static_cast<int>(a.width), tile = ring_args.tile;
+  const float inverse = 1.0f / static_cast<float>(width);
+  const float* means = static_cast<const float*>(a.stats);
+  const auto fetch = [&](int64_t row0, int slot) {
+    const int64_t row = row0 + threadIdx.x;
+    if (static_cast<int>(threadIdx.x) < tile && row < a.rows) {
+      stats[slot][threadIdx.x] = make_float2(means[row], means[a.rows + row]);
+    }
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ring_args.stages; ++s) dev::mbar_init(&full[s], 1);
+    dev::fence_barrier_init();
+  }
+  fetch(static_cast<int64_t>(blockIdx.x) * tile, 0);
+  __syncthreads();
+  RowRing<G, true> ring{a, ring_args, shared, full, static_cast<int64_t>(blockIdx.x) * tile};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ring_args.stages; ++s) ring.ask(sizeof(T));
+  }
+  float w[NV][V], dw[NV][V], db[NV][V];
+  load_params<T, V, NV, G>(a.weight, a.param_f32, width, lane, 1.0f, w);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.0f;
+  }
+  int slot = 0;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * tile;
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * tile; row0 < a.rows; row0 += step) {
+    fetch(row0 + step, slot ^ 1);
+    const uint8_t* at = ring.wait();
+    const T* xs = reinterpret_cast<const T*>(at);
+    const T* ds = reinterpret_cast<const T*>(at + ring_args.stage_bytes / 2);
+    for (int i0 = 0; i0 < tile; i0 += kGroups) {
+      const int64_t row = row0 + i0 + group;
+      const bool live = i0 + group < tile && row < a.rows;
+      const float2 s = live ? stats[slot][i0 + group] : make_float2(0.0f, 0.0f);
+      Pack<T, V> px[NV], pd[NV];
+      float sums[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * G + lane) * V;
+        if (live && c < width) {
+          px[k] = *reinterpret_cast<const Pack<T, V>*>(xs + (i0 + group) * width + c);
+          pd[k] = *reinterpret_cast<const Pack<T, V>*>(ds + (i0 + group) * width + c);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float d = widen(pd[k].v[i]);
+            const float u = (widen(px[k].v[i]) - s.x) * s.y;
+            const float g = d * w[k][i];
+            sums[0] += g;
+            sums[1] += g * u;
+            dw[k][i] += d * u;
+            db[k][i] += d;
+          }
+        }
+      }
+      if (!a.want_dx) continue;
+      group_sums<G, 2>(sums, nullptr);
+      if (!live) continue;
+      const float mean_g = sums[0] * inverse, mean_gu = sums[1] * inverse;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (k * G + lane) * V;
+        if (c < width) {
+          Pack<T, V> out;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float u = (widen(px[k].v[i]) - s.x) * s.y;
+            out.v[i] = narrow<T>(s.y * (widen(pd[k].v[i]) * w[k][i] - mean_g - u * mean_gu));
+          }
+          *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * width + c) = out;
+        }
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) ring.ask(sizeof(T));
+    ring.advance();
+    slot ^= 1;
+  }
+  if (!a.want_params) return;
+  __syncthreads();
+  block_columns<T, V, NV, G>(a, dw, db, reinterpret_cast<float*>(shared));
 }
 
 // ---- rows of any width and type --------------------------------------------------------
@@ -338,27 +818,28 @@ __global__ void __launch_bounds__(128) norm_columns_kernel(const NormArgs a) {
   partial[a.width + c] = db;
 }
 
-// Partial rows [blocks][2][width] summed in order: a block takes 32 columns, its 8 warps
+// Partial rows [blocks][2][width] summed in order: a block takes 32 columns, its 32 warps
 // contiguous ranges of the rows, and the range sums are added in range order.
+constexpr int kReduceWarps = 32;
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kReduceWarps * 32)
     norm_reduce_kernel(const void* partials, int blocks, int64_t width, void* dweight,
                        void* dbias, int param_f32) {
   using A = typename Wide<T>::type;
-  __shared__ A part[8][32];
+  __shared__ A part[kReduceWarps][32];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   A sum = 0;
   if (j < 2 * width) {
     const A* p = static_cast<const A*>(partials) + j;
-    const int last = blocks * (warp + 1) / 8;
+    const int last = blocks * (warp + 1) / kReduceWarps;
 #pragma unroll 8
-    for (int b = blocks * warp / 8; b < last; ++b) sum += p[static_cast<int64_t>(b) * 2 * width];
+    for (int b = blocks * warp / kReduceWarps; b < last; ++b) sum += p[static_cast<int64_t>(b) * 2 * width];
   }
   part[warp][lane] = sum;
   __syncthreads();
   if (warp != 0 || j >= 2 * width) return;
-  for (int w = 1; w < 8; ++w) sum += part[w][lane];
+  for (int w = 1; w < kReduceWarps; ++w) sum += part[w][lane];
   if (j < width) {
     if (dweight != nullptr) store_param<T>(dweight, param_f32, j, sum);
   } else if (dbias != nullptr) {
@@ -371,7 +852,8 @@ __global__ void __launch_bounds__(256)
 struct NormShape {
   int vector;   // elements per load: 16 bytes, or 1 where rows are not 16-byte aligned
   int chunks;   // vectors per row
-  bool loops;   // wider than the register kernels (or float64)
+  bool loops;   // wider than the block kernels (or float64)
+  bool ring;    // 16-byte vectors and rows of more than 64 of them
 };
 
 constexpr int kMostChunks = 2048;
@@ -382,14 +864,29 @@ NormShape norm_shape(int dtype, int64_t width, bool aligned) {
   s.vector = aligned && width % wide == 0 ? wide : 1;
   s.loops = dtype == CND_F64 || width / s.vector > kMostChunks;
   s.chunks = s.loops ? 0 : static_cast<int>(width / s.vector);
+  s.ring = s.vector > 1 && s.chunks > 64;
   return s;
 }
+
+// Blocks an SM of the ring kernels: 768 threads (85 registers each), at least one block.
+int ring_threads(int chunks) {
+  return chunks <= 128 ? 64 : chunks <= 256 ? 128 : chunks <= 512 ? 256 : chunks <= 1024 ? 512 : 1024;
+}
+int ring_blocks(int chunks) { return std::max(1, 768 / ring_threads(chunks)); }
 
 int norm_rows_per_block(const NormShape& s) {
   if (s.chunks <= 4) return 64;
   if (s.chunks <= 8) return 32;
   if (s.chunks <= 16) return 16;
-  return s.chunks <= 128 ? 8 : 1;
+  return s.chunks <= 64 ? 8 : 1;
+}
+
+// Short aligned rows back to back, enough of them to fill the SMs' rings (fewer rows gain nothing
+// from a ring and start faster in registers).
+bool norm_tiles(const NormShape& s, int64_t rows, int64_t width, int64_t x_stride,
+                int64_t dy_stride) {
+  return !s.loops && !s.ring && s.vector > 1 && x_stride == width && dy_stride == width &&
+         rows * s.chunks >= int64_t{148} * 4 * 512;
 }
 
 // Blocks of the backward (one partial row each): enough to fill the SMs, no more than rows.
@@ -400,56 +897,144 @@ int norm_backward_blocks(const NormShape& s, int64_t rows, int64_t width) {
     const int64_t across = (width + 127) / 128;
     return static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, 8 * 148 / across)));
   }
+  if (s.ring) return static_cast<int>(std::min<int64_t>(rows, 148 * ring_blocks(s.chunks)));
   const int per_block = norm_rows_per_block(s);
   const int64_t need = (rows + per_block - 1) / per_block;
   return static_cast<int>(std::min<int64_t>(need, 4 * 148));
 }
 
-template <typename T, int V, typename F>
+// Vectors a thread, threads a row, rows in flight.
+template <bool kBackward, typename T, int V, typename F>
 void with_shape(const NormShape& s, F&& f) {
+  constexpr int kThin = kBackward ? 2 : 4;
   if (s.chunks <= 4) {
-    f.template operator()<T, V, 1, 4>();
+    f.template operator()<T, V, 1, 4, kThin>();
   } else if (s.chunks <= 8) {
-    f.template operator()<T, V, 1, 8>();
+    f.template operator()<T, V, 1, 8, kThin>();
   } else if (s.chunks <= 16) {
-    f.template operator()<T, V, 1, 16>();
+    f.template operator()<T, V, 1, 16, kThin>();
   } else if (s.chunks <= 32) {
-    f.template operator()<T, V, 1, 32>();
-  } else if (s.chunks <= 64) {
-    f.template operator()<T, V, 2, 32>();
-  } else if (s.chunks <= 128) {
-    f.template operator()<T, V, 4, 32>();
-  } else if (s.chunks <= 256) {
-    f.template operator()<T, V, 2, 128>();
-  } else if (s.chunks <= 512) {
-    f.template operator()<T, V, 2, 256>();
-  } else if (s.chunks <= 1024) {
-    f.template operator()<T, V, 2, 512>();
+    f.template operator()<T, V, 1, 32, kThin>();
+  } else if (V > 1 || s.chunks <= 64) {
+    f.template operator()<T, V, 2, 32, 2>();
+  } else if constexpr (V == 1) {  // longer rows of vectors run on the ring kernels
+    if (s.chunks <= 128) {
+      f.template operator()<T, V, 2, 64, 2>();
+    } else if (s.chunks <= 256) {
+      f.template operator()<T, V, 2, 128, 2>();
+    } else if (s.chunks <= 512) {
+      f.template operator()<T, V, 2, 256, 2>();
+    } else if (s.chunks <= 1024) {
+      f.template operator()<T, V, 2, 512, 2>();
+    } else {
+      f.template operator()<T, V, 2, 1024, 2>();
+    }
+  }
+}
+
+template <bool kBackward, typename F>
+void with_kernel(int dtype, const NormShape& s, F&& f) {
+  if (dtype == CND_F32) {
+    s.vector == 1 ? with_shape<kBackward, float, 1>(s, f) : with_shape<kBackward, float, 4>(s, f);
+  } else if (dtype == CND_BF16) {
+    s.vector == 1 ? with_shape<kBackward, __nv_bfloat16, 1>(s, f) : with_shape<kBackward, __nv_bfloat16, 8>(s, f);
   } else {
-    f.template operator()<T, V, 2, 1024>();
+    s.vector == 1 ? with_shape<kBackward, __half, 1>(s, f) : with_shape<kBackward, __half, 8>(s, f);
+  }
+}
+
+// Blocks an SM of the tile kernels.
+int tile_blocks(const NormShape& s, bool backward) {
+  return !backward ? 4 : s.chunks <= 32 ? 3 : 2;
+}
+
+// The ring of a block: its share of 200 KB, at most 16 stages. Tiles of short rows are 8 KB.
+Ring make_ring(const NormShape& s, bool backward) {
+  Ring r{};
+  r.row_bytes = static_cast<uint32_t>(s.chunks) * 16;
+  r.tile = s.ring ? 1 : static_cast<int>(std::min<uint32_t>(kMostTile, 8192 / r.row_bytes));
+  r.stage_bytes = r.row_bytes * r.tile * (backward ? 2 : 1);
+  const uint32_t share = 200 * 1024 / (s.ring ? ring_blocks(s.chunks) : tile_blocks(s, backward));
+  r.stages = static_cast<int>(std::min<uint32_t>(16, std::max<uint32_t>(2, share / r.stage_bytes)));
+  r.error = device_error_word();
+  r.timeout_ns = wait_timeout_ns();
+  return r;
+}
+
+template <typename T, int V, typename F>
+void with_ring(const NormShape& s, F&& f) {
+  switch (ring_threads(s.chunks)) {
+    case 64:
+      return f.template operator()<T, V, 2, 64>();
+    case 128:
+      return f.template operator()<T, V, 2, 128>();
+    case 256:
+      return f.template operator()<T, V, 2, 256>();
+    case 512:
+      return f.template operator()<T, V, 2, 512>();
+    default:
+      return f.template operator()<T, V, 2, 1024>();
   }
 }
 
 template <typename F>
-void with_kernel(int dtype, const NormShape& s, F&& f) {
+void with_ring_dtype(int dtype, const NormShape& s, F&& f) {
   if (dtype == CND_F32) {
-    s.vector == 1 ? with_shape<float, 1>(s, f) : with_shape<float, 4>(s, f);
+    with_ring<float, 4>(s, f);
   } else if (dtype == CND_BF16) {
-    s.vector == 1 ? with_shape<__nv_bfloat16, 1>(s, f) : with_shape<__nv_bfloat16, 8>(s, f);
+    with_ring<__nv_bfloat16, 8>(s, f);
   } else {
-    s.vector == 1 ? with_shape<__half, 1>(s, f) : with_shape<__half, 8>(s, f);
+    with_ring<__half, 8>(s, f);
   }
 }
+
+template <bool kBackward>
+struct LaunchTile {
+  const NormArgs& a;
+  const Ring& ring;
+  int blocks;
+  cudaStream_t stream;
+  // R (rows in flight) is the register kernels': a tile kernel's are in its ring
+  template <typename T, int V, int NV, int G, int R>
+  void operator()() const {
+    if constexpr (V > 1 && G <= 32) {
+      const auto kernel = kBackward ? norm_backward_tile_kernel<T, V, NV, G>
+                                    : norm_forward_tile_kernel<T, V, NV, G>;
+      const uint32_t bytes = std::max<uint32_t>(ring.stage_bytes * ring.stages,
+                                                static_cast<uint32_t>(a.width) * 2 * sizeof(float));
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(bytes));
+      kernel<<<blocks, kTileThreads, bytes, stream>>>(a, ring);
+    }
+  }
+};
+
+template <bool kBackward>
+struct LaunchRing {
+  const NormArgs& a;
+  const Ring& ring;
+  int blocks;
+  cudaStream_t stream;
+  template <typename T, int V, int NV, int G>
+  void operator()() const {
+    const auto kernel = kBackward ? norm_backward_ring_kernel<T, V, NV, G>
+                                  : norm_forward_ring_kernel<T, V, NV, G>;
+    const uint32_t bytes = ring.stage_bytes * ring.stages;
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         static_cast<int>(bytes));
+    kernel<<<blocks, G, bytes, stream>>>(a, ring);
+  }
+};
 
 struct LaunchForward {
   const NormArgs& a;
   cudaStream_t stream;
-  template <typename T, int V, int NV, int G>
+  template <typename T, int V, int NV, int G, int R>
   void operator()() const {
-    constexpr int kRows = block_size<G>() / G;
+    constexpr int kRows = block_size<G>() / G * R;
     const int64_t need = (a.rows + kRows - 1) / kRows;
     const int64_t most = static_cast<int64_t>(sm_count()) * (2048 / block_size<G>()) * 4;
-    norm_forward_kernel<T, V, NV, G>
+    norm_forward_kernel<T, V, NV, G, R>
         <<<static_cast<unsigned>(std::min(need, most)), block_size<G>(), 0, stream>>>(a);
   }
 };
@@ -458,11 +1043,11 @@ struct LaunchBackward {
   const NormArgs& a;
   int blocks;
   cudaStream_t stream;
-  template <typename T, int V, int NV, int G>
+  template <typename T, int V, int NV, int G, int R>
   void operator()() const {
     constexpr int kRows = block_size<G>() / G;
     const size_t shared = kRows > 1 ? static_cast<size_t>(a.width) * 2 * sizeof(float) : 0;
-    norm_backward_kernel<T, V, NV, G><<<blocks, block_size<G>(), shared, stream>>>(a);
+    norm_backward_kernel<T, V, NV, G, R><<<blocks, block_size<G>(), shared, stream>>>(a);
   }
 };
 
@@ -530,8 +1115,20 @@ int cnd_layer_norm_forward(int32_t dtype, int32_t param_dtype, int64_t rows, int
     } else {
       norm_forward_loop_kernel<__half><<<blocks, kLoopThreads, 0, stream>>>(a);
     }
+  } else if (s.ring) {
+    const Ring ring = make_ring(s, false);
+    if (ring.error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
+    const int blocks = static_cast<int>(std::min<int64_t>(rows, sm_count() * ring_blocks(s.chunks)));
+    with_ring_dtype(dtype, s, LaunchRing<false>{a, ring, blocks, stream});
+  } else if (norm_tiles(s, rows, width, x_stride, width)) {
+    const Ring ring = make_ring(s, false);
+    if (ring.error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
+    const int64_t tiles = (rows + ring.tile - 1) / ring.tile;
+    const int blocks =
+        static_cast<int>(std::min<int64_t>(tiles, sm_count() * tile_blocks(s, false)));
+    with_kernel<false>(dtype, s, LaunchTile<false>{a, ring, blocks, stream});
   } else {
-    with_kernel(dtype, s, LaunchForward{a, stream});
+    with_kernel<false>(dtype, s, LaunchForward{a, stream});
   }
   count_launch();
   return launch_status("cnd_layer_norm_forward");
@@ -604,7 +1201,7 @@ int cnd_layer_norm_backward(int32_t dtype, int32_t param_dtype, int64_t rows, in
   const bool aligned = rows_aligned(dtype, x, x_stride) && rows_aligned(dtype, dy, dy_stride) &&
                        (!a.want_dx || aligned16(dx));
   const NormShape s = norm_shape(dtype, width, aligned);
-  const int blocks = norm_backward_blocks(s, rows, width);
+  int blocks = norm_backward_blocks(s, rows, width);
   if (s.loops) {
     const unsigned grid =
         static_cast<unsigned>(std::min<int64_t>(rows, static_cast<int64_t>(sm_count()) * 16));
@@ -629,8 +1226,19 @@ int cnd_layer_norm_backward(int32_t dtype, int32_t param_dtype, int64_t rows, in
     } else {
       run(__half{});
     }
+  } else if (s.ring) {
+    const Ring ring = make_ring(s, true);
+    if (ring.error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
+    with_ring_dtype(dtype, s, LaunchRing<true>{a, ring, blocks, stream});
+    count_launch();
+  } else if (norm_tiles(s, rows, width, x_stride, dy_stride)) {
+    const Ring ring = make_ring(s, true);
+    if (ring.error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
+    blocks = std::min(blocks, sm_count() * tile_blocks(s, true));
+    with_kernel<true>(dtype, s, LaunchTile<true>{a, ring, blocks, stream});
+    count_launch();
   } else {
-    with_kernel(dtype, s, LaunchBackward{a, blocks, stream});
+    with_kernel<true>(dtype, s, LaunchBackward{a, blocks, stream});
     count_launch();
   }
   if (params) {
@@ -638,13 +1246,13 @@ int cnd_layer_norm_backward(int32_t dtype, int32_t param_dtype, int64_t rows, in
     void* w = output_mask[1] ? dweight : nullptr;
     void* b = output_mask[2] ? dbias : nullptr;
     if (dtype == CND_F64) {
-      norm_reduce_kernel<double><<<grid, 256, 0, stream>>>(workspace, blocks, width, w, b, 0);
+      norm_reduce_kernel<double><<<grid, kReduceWarps * 32, 0, stream>>>(workspace, blocks, width, w, b, 0);
     } else if (dtype == CND_F32 || a.param_f32) {
-      norm_reduce_kernel<float><<<grid, 256, 0, stream>>>(workspace, blocks, width, w, b, 1);
+      norm_reduce_kernel<float><<<grid, kReduceWarps * 32, 0, stream>>>(workspace, blocks, width, w, b, 1);
     } else if (dtype == CND_BF16) {
-      norm_reduce_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(workspace, blocks, width, w, b, 0);
+      norm_reduce_kernel<__nv_bfloat16><<<grid, kReduceWarps * 32, 0, stream>>>(workspace, blocks, width, w, b, 0);
     } else {
-      norm_reduce_kernel<__half><<<grid, 256, 0, stream>>>(workspace, blocks, width, w, b, 0);
+      norm_reduce_kernel<__half><<<grid, kReduceWarps * 32, 0, stream>>>(workspace, blocks, width, w, b, 0);
     }
     count_launch();
   }

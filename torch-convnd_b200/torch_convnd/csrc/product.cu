@@ -39,13 +39,16 @@ namespace cnd {
 namespace layers {
 namespace {
 
-constexpr int kBM = 128, kBK = 64;
+constexpr int kBM = 128;
+// Depth of an operand stage. Three-term operands take 32: six tiles of 64 leave room for two
+// stages only.
+constexpr int block_depth(int parts) { return parts == 3 ? 32 : 64; }
 constexpr int kGroupThreads = 128;  // an epilogue group: four warps
 constexpr int block_threads(int groups) { return 64 + groups * kGroupThreads; }
 constexpr uint32_t kUnitBytes = kBM * 128;  // staging tile: 128 rows of 128 bytes
 constexpr uint32_t kSharedLimit = 232448;
 constexpr int kMostStages = 8;
-constexpr int kChunkBlocks = 4;  // k blocks per float32 accumulation (three-term operands)
+constexpr int kChunkBlocks = 8;  // k blocks per float32 accumulation (three-term operands)
 constexpr uint32_t kSiteLoad = 0x501, kSiteMma = 0x502, kSiteAccumulator = 0x503,
                    kSiteEpilogue = 0x504, kSiteDrain = 0x505;
 
@@ -61,6 +64,7 @@ struct KernelArgs {
   uint32_t idesc;
   uint32_t a_step, b_step;  // descriptor units (16 bytes) per 16 of k
   uint32_t a_lbo, b_lbo;
+  uint32_t a_sbo, b_sbo, a_swizzle, b_swizzle;
   int a_k_major, b_k_major;
   int act, tma_out, vector_residual;
   const void* bias;
@@ -212,7 +216,8 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
     product_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ KernelArgs a) {
   constexpr bool kExact = sizeof(Out) == 4;
   constexpr int kColsB = kBN / kPair;  // rows of B that this CTA holds
-  constexpr uint32_t kPartA = kBM * 128, kPartB = kColsB * 128;
+  constexpr int kBK = block_depth(kParts);
+  constexpr uint32_t kPartA = kBM * kBK * 2, kPartB = kColsB * kBK * 2;
   constexpr uint32_t kStageBytes = kParts * (kPartA + kPartB);
   constexpr int kUnit = 128 / sizeof(Out);      // columns of a staging tile
   constexpr int kGroupCols = kBN / kGroups;     // columns of an epilogue group
@@ -265,76 +270,84 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
   const int items = a.tiles_m * a.tiles_n * a.splits;
 
   if (warp == 0) {
-    // ---- TMA loads: one lane ----
+    // ---- TMA loads: the converged warp, elect.sync issues ----
     if (lane == 0) {
       dev::prefetch_tensormap(&maps.a);
       dev::prefetch_tensormap(&maps.b);
-      int stage = 0;
-      uint32_t phase = 0, issued = 0;
-      bool ok = true;
-      for (int item = worker; item < items && ok; item += workers) {
-        const int split = item % a.splits;
-        int tm, tn;
-        tile_of(a, item / a.splits, &tm, &tn);
-        const int m0 = (tm * kPair + static_cast<int>(rank)) * kBM;
-        const int n0 = tn * kBN + static_cast<int>(rank) * kColsB;
-        const int first = static_cast<int>(static_cast<int64_t>(a.k_blocks) * split / a.splits);
-        const int last = static_cast<int>(static_cast<int64_t>(a.k_blocks) * (split + 1) / a.splits);
-        for (int kb = first; kb < last; ++kb) {
-          if (!wait<kPair>(&empty[stage], phase ^ 1u, err, kSiteLoad, a.timeout_ns)) {
-            ok = false;
-            break;
-          }
-          if (rank == 0) dev::mbar_arrive_expect_tx(&full[stage], kPair * kStageBytes);
-          const uint32_t bar =
-              kPair == 2 ? dev::map_to_rank(&full[stage], 0) : dev::smem_u32(&full[stage]);
-          uint8_t* dst = smem + stage * kStageBytes;
+    }
+    __syncwarp();
+    const uint32_t full_here = dev::smem_u32(full);
+    const uint32_t full_signal = kPair == 2 ? dev::map_to_rank(full, 0) : full_here;
+    const uint32_t stages_at = dev::smem_u32(smem);
+    int stage = 0;
+    uint32_t phase = 0, issued = 0;
+    bool ok = true;
+    for (int item = worker; item < items && ok; item += workers) {
+      const int split = item % a.splits;
+      int tm, tn;
+      tile_of(a, item / a.splits, &tm, &tn);
+      const int m0 = (tm * kPair + static_cast<int>(rank)) * kBM;
+      const int n0 = tn * kBN + static_cast<int>(rank) * kColsB;
+      const int first = static_cast<int>(static_cast<int64_t>(a.k_blocks) * split / a.splits);
+      const int last = static_cast<int>(static_cast<int64_t>(a.k_blocks) * (split + 1) / a.splits);
+      for (int kb = first; kb < last; ++kb) {
+        if (!wait_warp<kPair>(&empty[stage], phase ^ 1u, err, kSiteLoad, a.timeout_ns)) {
+          ok = false;
+          break;
+        }
+        if (rank == 0) dev::mbar_expect_tx_warp(full_here + 8 * stage, kPair * kStageBytes);
+        const uint32_t bar = full_signal + 8 * stage;
+        const uint32_t dst = stages_at + stage * kStageBytes;
+        const int k0 = kb * kBK;
+        if (a.a_k_major) {
 #pragma unroll
           for (int p = 0; p < kParts; ++p) {
-            if (a.a_k_major) {
-              dev::tma_load_3d_to<kPair>(dst, &maps.a, bar, kb * kBK, m0, p);
-            } else {
-#pragma unroll
-              for (int i = 0; i < kBM / 64; ++i) {
-                dev::tma_load_3d_to<kPair>(dst + i * (kBK * 128), &maps.a, bar, m0 + 64 * i,
-                                           kb * kBK, p);
-              }
-            }
-            dst += kPartA;
+            dev::tma_load_3d_to<kPair>(dst + p * kPartA, &maps.a, bar, k0, m0, p);
           }
+        } else {
 #pragma unroll
           for (int p = 0; p < kParts; ++p) {
-            if (a.b_k_major) {
-              dev::tma_load_3d_to<kPair>(dst, &maps.b, bar, kb * kBK, n0, p);
-            } else {
 #pragma unroll
-              for (int i = 0; i < kColsB / 64; ++i) {
-                dev::tma_load_3d_to<kPair>(dst + i * (kBK * 128), &maps.b, bar, n0 + 64 * i,
-                                           kb * kBK, p);
-              }
+            for (int i = 0; i < kBM / 64; ++i) {
+              dev::tma_load_3d_to<kPair>(dst + p * kPartA + i * (kBK * 128), &maps.a, bar,
+                                         m0 + 64 * i, k0, p);
             }
-            dst += kPartB;
-          }
-          ++issued;
-          if (++stage == a.stages) {
-            stage = 0;
-            phase ^= 1u;
           }
         }
+        if (a.b_k_major) {
+#pragma unroll
+          for (int p = 0; p < kParts; ++p) {
+            dev::tma_load_3d_to<kPair>(dst + kParts * kPartA + p * kPartB, &maps.b, bar, k0, n0, p);
+          }
+        } else {
+#pragma unroll
+          for (int p = 0; p < kParts; ++p) {
+#pragma unroll
+            for (int i = 0; i < kColsB / 64; ++i) {
+              dev::tma_load_3d_to<kPair>(dst + kParts * kPartA + p * kPartB + i * (kBK * 128),
+                                         &maps.b, bar, n0 + 64 * i, k0, p);
+            }
+          }
+        }
+        ++issued;
+        if (++stage == a.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
       }
-      if (!ok && issued > 0 && rank == 0) {
-        // give loads in flight a bounded time to land before the block may exit
-        const int previous = stage == 0 ? a.stages - 1 : stage - 1;
-        wait<kPair>(&full[previous], stage == 0 ? phase ^ 1u : phase, err, kSiteDrain,
-                    a.timeout_ns / 8 + 1);
-      }
+    }
+    if (!ok && issued > 0 && rank == 0) {
+      // give loads in flight a bounded time to land before the block may exit
+      const int previous = stage == 0 ? a.stages - 1 : stage - 1;
+      wait_warp<kPair>(&full[previous], stage == 0 ? phase ^ 1u : phase, err, kSiteDrain,
+                       a.timeout_ns / 8 + 1);
     }
   } else if (warp == 1) {
     // ---- MMAs: the leader CTA's warp, converged; elect.sync issues ----
     if (rank == 0) {
       const uint32_t base = dev::warp_uniform(tmem);
-      const uint64_t a_hi = dev::make_smem_desc(0, a.a_lbo, 1024, 2);
-      const uint64_t b_hi = dev::make_smem_desc(0, a.b_lbo, 1024, 2);
+      const uint64_t a_hi = dev::make_smem_desc(0, a.a_lbo, a.a_sbo, a.a_swizzle);
+      const uint64_t b_hi = dev::make_smem_desc(0, a.b_lbo, a.b_sbo, a.b_swizzle);
       int stage = 0;
       uint32_t phase = 0;
       int set = 0, cross = 0;
@@ -677,17 +690,20 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
 
 bool encode_operand(CUtensorMap* map, const Operand& o, int64_t rows, int64_t k, int parts,
                     bool bf16, int box_rows) {
+  const int depth = block_depth(parts);
   const cuuint64_t inner = static_cast<cuuint64_t>(o.k_major ? k : rows);
   const cuuint64_t outer = static_cast<cuuint64_t>(o.k_major ? rows : k);
   const cuuint64_t dims[3] = {inner, outer, static_cast<cuuint64_t>(parts)};
   const int64_t plane = parts > 1 ? o.plane : o.pitch * static_cast<int64_t>(outer);
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(o.pitch) * 2,
                                  static_cast<cuuint64_t>(plane) * 2};
-  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(o.k_major ? box_rows : kBK), 1};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(o.k_major ? depth : 64),
+                             static_cast<cuuint32_t>(o.k_major ? box_rows : depth), 1};
   const cuuint32_t ones[3] = {1, 1, 1};
   return encoder()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                    3, const_cast<void*>(o.data), dims, strides, box, ones,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -711,7 +727,10 @@ using Kernel = void (*)(Maps, KernelArgs);
 template <typename Out>
 Kernel pick(const ProductPlan& plan, int parts) {
   if constexpr (sizeof(Out) == 4) {
-    if (parts == 3) return product_tc_kernel<1, 128, 3, 2, Out>;
+    if (parts == 3) {
+      return plan.pair == 2 ? product_tc_kernel<2, 128, 3, 2, Out>
+                            : product_tc_kernel<1, 128, 3, 2, Out>;
+    }
   }
   if (plan.pair == 2) {
     return plan.groups == 4 ? product_tc_kernel<2, 256, 1, 4, Out>
@@ -721,50 +740,48 @@ Kernel pick(const ProductPlan& plan, int parts) {
                         : product_tc_kernel<1, 64, 1, 1, Out>;
 }
 
-uint64_t wait_timeout() {
-  static const uint64_t value = [] {
-    const char* env = std::getenv("CND_WAIT_TIMEOUT_MS");
-    const long long parsed = env != nullptr ? std::atoll(env) : 0;
-    return (parsed > 0 ? static_cast<uint64_t>(parsed) : uint64_t{2000}) * 1000000u;
-  }();
-  return value;
-}
-
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 }  // namespace
 
 ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts) {
-  // Times in cycles of one SM. A block of 64 of k takes the tensor core 2 cycles a column
-  // (six products: 12) and its operands 1 cycle per 60 bytes from L2, an epilogue about 12
-  // cycles a column; a launch that joins splits takes its traffic.
-  const int64_t sms = 148, blocks = (k + kBK - 1) / kBK;
+  // Microseconds, fitted to runs over 16 to 4096 rows and 1024 or 4096 of n and k: a launch,
+  // a block of k, and the epilogue of a tile (which runs under the next tile's main loop);
+  // joining splits costs a launch and its traffic. The fit is within a few percent where two
+  // cuts are close; the wrong one of a pair far apart costs half again (4096^3: 99 us on
+  // pairs, 132 on single CTAs; 16 x 4096 -> 1024: 10.1 in 8 splits, 20 in one).
+  struct Cut {
+    int parts, pair, bn;
+    double launch, block, tail;
+  };
+  static constexpr Cut kCuts[] = {
+      {1, 2, 256, 8.5, 0.32, 5.5}, {1, 1, 128, 5.0, 0.27, 3.0}, {1, 1, 64, 4.3, 0.25, 1.9},
+      {3, 2, 128, 8.0, 0.72, 4.0}, {3, 1, 128, 5.0, 0.77, 3.0},
+  };
+  const int64_t sms = 148, blocks = (k + block_depth(parts) - 1) / block_depth(parts);
   ProductPlan best{1, 64, 1, 1};
   double best_cost = 0;
-  for (int pair = 2; pair >= 1; --pair) {
-    for (int bn : {256, 128, 64}) {
-      if ((pair == 2) != (bn == 256) || (parts == 3 && bn != 128)) continue;
-      const int64_t tiles = ((m + kBM * pair - 1) / (kBM * pair)) * ((n + bn - 1) / bn);
-      const int64_t slots = sms / pair;
-      for (int64_t splits = 1; splits <= 64; ++splits) {
-        if (splits > 1 && (blocks / splits < 4 || tiles * splits > 2 * slots)) break;
-        const int64_t waves = (tiles * splits + slots - 1) / slots;
-        const double per_block = std::max(2.0 * bn * (parts == 3 ? 6 : 1),
-                                          (kBM + bn / pair) * 128.0 * parts / 60.0);
-        const double main = static_cast<double>((blocks + splits - 1) / splits) * per_block;
-        const double tail = 12.0 * bn + 1000;
-        double cost = waves * std::max(main, tail) + std::min(main, tail) + 1500;
-        if (splits > 1) {
-          cost += 6000 + static_cast<double>(splits + 1) * m * n * 4 / 3000.0;
-        }
-        if (best_cost == 0 || cost < best_cost) {
-          best_cost = cost;
-          // Four epilogue groups (four warps a scheduler) where the epilogue is the longer part:
-          // with two, waits for TMEM, exponentials and staging left a scheduler issuing 27 %
-          // of the time (1M x 64 -> 256 GELU: 428 us against 320).
-          const int groups = bn == 64 ? 1 : bn == 256 && main < 2 * tail ? 4 : 2;
-          best = ProductPlan{pair, bn, static_cast<int>(splits), groups};
-        }
+  for (const Cut& c : kCuts) {
+    if (c.parts != parts) continue;
+    const int64_t rows = kBM * c.pair;
+    const int64_t tiles = ((m + rows - 1) / rows) * ((n + c.bn - 1) / c.bn);
+    const int64_t slots = sms / c.pair;
+    for (int64_t splits = 1; splits <= 64; ++splits) {
+      if (splits > 1 && (blocks / splits < 2 || tiles * splits > 2 * slots)) break;
+      const int64_t waves = (tiles * splits + slots - 1) / slots;
+      const double main = static_cast<double>((blocks + splits - 1) / splits) * c.block;
+      double cost = c.launch + (waves - 1) * std::max(main, c.tail) + main;
+      if (splits > 1) {
+        cost += 2.2 + 0.3e-6 * static_cast<double>(splits) * ((m + rows - 1) / rows * rows) * n * 4;
+      }
+      if (best_cost == 0 || cost < best_cost) {
+        best_cost = cost;
+        // Four epilogue groups (four warps a scheduler) where the epilogue is the longer part:
+        // with two, waits for TMEM, exponentials and staging left a scheduler issuing 27 % of
+        // the time (1M x 64 -> 256 GELU: 428 us against 320). From a depth of 1024 on two
+        // groups and a sixth stage win (4096 x 1024 -> 4096: 30.6 us against 36.4).
+        const int groups = c.bn == 64 ? 1 : c.bn == 256 && blocks / splits <= 8 ? 4 : 2;
+        best = ProductPlan{c.pair, c.bn, static_cast<int>(splits), groups};
       }
     }
   }
@@ -782,6 +799,7 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
   if (encoder() == nullptr) return fail(CND_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const int bm = kBM * plan.pair;
   const bool split = plan.splits > 1;
+  const int depth = block_depth(p.parts);
   if (round_up(p.m, bm) * plan.splits > INT32_MAX || p.n > INT32_MAX - 256 ||
       p.k > INT32_MAX - 64) {
     return fail(CND_ERR_UNSUPPORTED, "linear: a matrix dimension exceeds 2^31");
@@ -792,7 +810,7 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
   a.tiles_m = static_cast<int>((p.m + bm - 1) / bm);
   a.tiles_n = static_cast<int>((p.n + plan.bn - 1) / plan.bn);
   a.splits = plan.splits;
-  a.k_blocks = static_cast<int>((p.k + kBK - 1) / kBK);
+  a.k_blocks = static_cast<int>((p.k + depth - 1) / depth);
   if (static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits > INT32_MAX) {
     return fail(CND_ERR_UNSUPPORTED, "linear: too many tiles");
   }
@@ -809,7 +827,7 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
     a.buffers = wants_pre ? 4 : 2;
   }
   a.sets = wants_pre ? std::max(1, a.buffers / 2) : a.buffers;
-  const uint32_t stage = p.parts * (kBM + plan.bn / plan.pair) * 128;
+  const uint32_t stage = p.parts * (kBM + plan.bn / plan.pair) * depth * 2;
   const uint32_t fixed = 1024 + plan.groups * a.buffers * kUnitBytes + plan.bn * sizeof(float) + 256;
   a.stages = static_cast<int>(std::min<uint32_t>((kSharedLimit - fixed) / stage, kMostStages));
   const uint32_t shared = fixed + a.stages * stage;
@@ -820,10 +838,16 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
   a.b_k_major = p.b.k_major;
   a.a_step = (p.a.k_major ? 32 : 16 * 128) >> 4;
   a.b_step = (p.b.k_major ? 32 : 16 * 128) >> 4;
-  a.a_lbo = p.a.k_major ? 16 : kBK * 128;
-  a.b_lbo = p.b.k_major ? 16 : kBK * 128;
+  a.a_lbo = p.a.k_major ? 16 : depth * 128;
+  a.b_lbo = p.b.k_major ? 16 : depth * 128;
+  // eight rows of a swizzle atom: 128 bytes wide, or 64 (K-major blocks 32 deep)
+  const uint32_t narrow_rows = depth == 32;
+  a.a_sbo = p.a.k_major && narrow_rows ? 512 : 1024;
+  a.b_sbo = p.b.k_major && narrow_rows ? 512 : 1024;
+  a.a_swizzle = p.a.k_major && narrow_rows ? 4 : 2;
+  a.b_swizzle = p.b.k_major && narrow_rows ? 4 : 2;
   a.error = device_error_word();
-  a.timeout_ns = wait_timeout();
+  a.timeout_ns = wait_timeout_ns();
   if (a.error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
   Maps maps{};
   if (!encode_operand(&maps.a, p.a, p.m, p.k, p.parts, p.bf16, kBM) ||

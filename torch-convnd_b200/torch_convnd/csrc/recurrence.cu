@@ -828,15 +828,6 @@ RecurrencePlan plan_recurrence(int dtype, int64_t outer, int64_t steps, int64_t 
   return p;
 }
 
-uint64_t wait_timeout() {
-  static const uint64_t value = [] {
-    const char* env = std::getenv("CND_WAIT_TIMEOUT_MS");
-    const long long parsed = env != nullptr ? std::atoll(env) : 0;
-    return (parsed > 0 ? static_cast<uint64_t>(parsed) : uint64_t{2000}) * 1000000u;
-  }();
-  return value;
-}
-
 // Binds the exchange area and sets its bits.
 int bind_exchange(const char* who, const RecurrencePlan& p, void* workspace, size_t bytes,
                   RecurrenceArgs* a, cudaStream_t stream) {
@@ -857,7 +848,7 @@ int bind_exchange(const char* who, const RecurrencePlan& p, void* workspace, siz
   a->bases = base + p.bases;
   a->ticket = reinterpret_cast<unsigned int*>(base + p.ticket);
   a->error = device_error_word();
-  a->timeout_ns = wait_timeout();
+  a->timeout_ns = wait_timeout_ns();
   if (a->error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
   if (cudaMemsetAsync(workspace, 0xff, p.total, stream) != cudaSuccess) return launch_status(who);
   return CND_OK;
