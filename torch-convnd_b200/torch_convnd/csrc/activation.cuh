@@ -8,37 +8,6 @@
 namespace cnd {
 namespace layers {
 
-// Two float32 values in one 64-bit register pair: sm_100 multiplies and adds them with one
-// instruction.
-struct Two {
-  unsigned long long bits;
-};
-
-__device__ __forceinline__ Two two(float lo, float hi) {
-  Two t;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(t.bits) : "f"(lo), "f"(hi));
-  return t;
-}
-__device__ __forceinline__ void unpack(Two t, float* lo, float* hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(*lo), "=f"(*hi) : "l"(t.bits));
-}
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
-  Two d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
-  return d;
-}
-__device__ __forceinline__ Two mul2(Two a, Two b) {
-  Two d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
-  return d;
-}
-__device__ __forceinline__ Two add2(Two a, Two b) {
-  Two d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
-  return d;
-}
-__device__ __forceinline__ Two same(float v) { return two(v, v); }
-
 __device__ __forceinline__ float exp2_fast(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "convnd_b200_layers.h"
 #include "internal.h"
@@ -55,6 +56,88 @@ template <typename T, int V>
 struct alignas(V * sizeof(T)) Pack {
   T v[V];
 };
+
+// Two float32 values in one 64-bit register pair: sm_100 multiplies and adds them with one
+// instruction.
+struct Two {
+  unsigned long long bits;
+};
+
+__device__ __forceinline__ Two two(float lo, float hi) {
+  Two t;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(t.bits) : "f"(lo), "f"(hi));
+  return t;
+}
+__device__ __forceinline__ void unpack(Two t, float* lo, float* hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*lo), "=f"(*hi) : "l"(t.bits));
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return d;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
+  return d;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
+  return d;
+}
+__device__ __forceinline__ Two same(float v) { return two(v, v); }
+
+// V elements at a 16-byte aligned address as pairs, and back (rounded once).
+template <typename T, int V>
+__device__ __forceinline__ void load_twos(const void* p, Two (&v)[V / 2]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      const ulonglong2 q = static_cast<const ulonglong2*>(p)[i];
+      v[2 * i] = Two{q.x};
+      v[2 * i + 1] = Two{q.y};
+    }
+  } else {
+    uint32_t q[V / 2];
+    *reinterpret_cast<uint4*>(q) = *static_cast<const uint4*>(p);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        v[i] = two(__uint_as_float(q[i] << 16), __uint_as_float(q[i] & 0xffff0000u));
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[i]));
+        v[i] = two(f.x, f.y);
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t narrow2(Two v) {
+  float lo, hi;
+  unpack(v, &lo, &hi);
+  uint32_t bits = 0;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(bits) : "f"(hi), "f"(lo));
+  } else if constexpr (std::is_same_v<T, __half>) {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(bits) : "f"(hi), "f"(lo));
+  }
+  return bits;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_twos(void* p, const Two (&v)[V / 2]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      static_cast<ulonglong2*>(p)[i] = make_ulonglong2(v[2 * i].bits, v[2 * i + 1].bits);
+    }
+  } else {
+    *static_cast<uint4*>(p) =
+        make_uint4(narrow2<T>(v[0]), narrow2<T>(v[1]), narrow2<T>(v[2]), narrow2<T>(v[3]));
+  }
+}
 
 // Vector parameter element i of `type` T or float32 (uniform flag), 0-d when absent.
 template <typename T>

@@ -120,6 +120,81 @@ constexpr int block_size() {
   return G > 32 ? G : 256;
 }
 
+// The same as pairs.
+template <typename T, int V, int NV, int G>
+__device__ __forceinline__ void load_param_pairs(const void* p, bool is_f32, int64_t width,
+                                                 int lane, float absent, Two (&v)[NV][V / 2]) {
+  float f[NV][V];
+  load_params<T, V, NV, G>(p, is_f32, width, lane, absent, f);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) v[k][i] = two(f[k][2 * i], f[k][2 * i + 1]);
+  }
+}
+
+__device__ __forceinline__ float both(Two v) {
+  float lo, hi;
+  unpack(v, &lo, &hi);
+  return lo + hi;
+}
+
+// The arithmetic of a row's thread on vectors of V elements, two at a time: one instruction a
+// pair where scalar code had the schedulers issuing more than half of the time.
+template <typename T, int V, int NV, int G>
+struct RowMath {
+  static constexpr int kPairs = V / 2;
+
+  static __device__ __forceinline__ float sum(const Two (&x)[kPairs]) {
+    Two s = x[0];
+#pragma unroll
+    for (int i = 1; i < kPairs; ++i) s = add2(s, x[i]);
+    return both(s);
+  }
+  static __device__ __forceinline__ float squares(const Two (&x)[kPairs], float mean) {
+    Two s = same(0.0f);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const Two d = add2(x[i], same(-mean));
+      s = fma2(d, d, s);
+    }
+    return both(s);
+  }
+  static __device__ __forceinline__ void normalise(Two (&x)[kPairs], float mean, float rstd,
+                                                   const Two (&w)[kPairs], const Two (&b)[kPairs]) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      x[i] = fma2(mul2(add2(x[i], same(-mean)), same(rstd)), w[i], b[i]);
+    }
+  }
+  // sums += (g, g u); dw += dy u, db += dy
+  static __device__ __forceinline__ void collect(const Two (&x)[kPairs], const Two (&dy)[kPairs],
+                                                 float mean, float rstd, const Two (&w)[kPairs],
+                                                 Two (&sums)[2], Two (&dw)[kPairs],
+                                                 Two (&db)[kPairs]) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const Two u = mul2(add2(x[i], same(-mean)), same(rstd));
+      const Two g = mul2(dy[i], w[i]);
+      sums[0] = add2(sums[0], g);
+      sums[1] = fma2(g, u, sums[1]);
+      dw[i] = fma2(dy[i], u, dw[i]);
+      db[i] = add2(db[i], dy[i]);
+    }
+  }
+  // dy becomes rstd (g - mean_g - u mean_gu)
+  static __device__ __forceinline__ void gradient(const Two (&x)[kPairs], Two (&dy)[kPairs],
+                                                  float mean, float rstd, const Two (&w)[kPairs],
+                                                  float mean_g, float mean_gu) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const Two u = mul2(add2(x[i], same(-mean)), same(rstd));
+      const Two t = fma2(dy[i], w[i], same(-mean_g));
+      dy[i] = mul2(fma2(u, same(-mean_gu), t), same(rstd));
+    }
+  }
+};
+
 // Writes a block's column sums, held by groups of G <= 32 lanes, as one partial row: rows of
 // one warp first (lanes of the same columns), then the warps in order. `columns`: [2][width].
 template <typename T, int V, int NV, int G>
@@ -420,18 +495,19 @@ __global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
   if (lane == 0) {
     for (int s = 0; s < ring_args.stages; ++s) ring.ask(sizeof(T));
   }
-  float w[NV][V], b[NV][V];
-  load_params<T, V, NV, G>(a.weight, a.param_f32, a.width, lane, 1.0f, w);
-  load_params<T, V, NV, G>(a.bias, a.param_f32, a.width, lane, 0.0f, b);
+  using M = RowMath<T, V, NV, G>;
+  Two w[NV][V / 2], b[NV][V / 2];
+  load_param_pairs<T, V, NV, G>(a.weight, a.param_f32, a.width, lane, 1.0f, w);
+  load_param_pairs<T, V, NV, G>(a.bias, a.param_f32, a.width, lane, 0.0f, b);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const Pack<T, V>* x = reinterpret_cast<const Pack<T, V>*>(ring.wait());
+    const T* data = reinterpret_cast<const T*>(ring.wait());
+    Two x[NV][V / 2];
     float sum[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if ((k * G + lane) * V < a.width) {
-        const Pack<T, V> p = x[k * G + lane];
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum[0] += widen(p.v[i]);
+        load_twos<T, V>(data + (k * G + lane) * V, x[k]);
+        sum[0] += M::sum(x[k]);
       }
     }
     group_sums<G, 1>(sum, scratch);
@@ -441,14 +517,7 @@ __global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
     float squares[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if ((k * G + lane) * V < a.width) {
-        const Pack<T, V> p = x[k * G + lane];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = widen(p.v[i]) - mean;
-          squares[0] += d * d;
-        }
-      }
+      if ((k * G + lane) * V < a.width) squares[0] += M::squares(x[k], mean);
     }
     group_sums<G, 1>(squares, scratch);
     const float rstd = rsqrtf(squares[0] * inverse + static_cast<float>(a.eps));
@@ -456,17 +525,12 @@ __global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
       static_cast<float*>(a.stats)[row] = mean;
       static_cast<float*>(a.stats)[a.rows + row] = rstd;
     }
-    Pack<T, V>* y = reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * a.width);
+    T* y = static_cast<T*>(a.y) + row * a.width;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if ((k * G + lane) * V < a.width) {
-        const Pack<T, V> p = x[k * G + lane];
-        Pack<T, V> out;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          out.v[i] = narrow<T>((widen(p.v[i]) - mean) * rstd * w[k][i] + b[k][i]);
-        }
-        y[k * G + lane] = out;
+        M::normalise(x[k], mean, rstd, w[k], b[k]);
+        store_twos<T, V>(y + (k * G + lane) * V, x[k]);
       }
     }
     ring.advance();
@@ -491,12 +555,13 @@ __global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
   if (lane == 0) {
     for (int s = 0; s < ring_args.stages; ++s) ring.ask(sizeof(T));
   }
-  float w[NV][V], dw[NV][V], db[NV][V];
-  load_params<T, V, NV, G>(a.weight, a.param_f32, a.width, lane, 1.0f, w);
+  using M = RowMath<T, V, NV, G>;
+  Two w[NV][V / 2], dw[NV][V / 2], db[NV][V / 2];
+  load_param_pairs<T, V, NV, G>(a.weight, a.param_f32, a.width, lane, 1.0f, w);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.0f;
+    for (int i = 0; i < V / 2; ++i) dw[k][i] = db[k][i] = same(0.0f);
   }
   float next_mean = blockIdx.x < a.rows ? means[blockIdx.x] : 0.0f;
   float next_rstd = blockIdx.x < a.rows ? means[a.rows + blockIdx.x] : 0.0f;
@@ -507,41 +572,31 @@ __global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
       next_rstd = means[a.rows + row + gridDim.x];
     }
     const uint8_t* at = ring.wait();
-    const Pack<T, V>* x = reinterpret_cast<const Pack<T, V>*>(at);
-    const Pack<T, V>* dy = reinterpret_cast<const Pack<T, V>*>(at + ring_args.row_bytes);
-    float sums[2] = {0.0f, 0.0f};
+    const T* xs = reinterpret_cast<const T*>(at);
+    const T* ds = reinterpret_cast<const T*>(at + ring_args.row_bytes);
+    Two pairs[2] = {same(0.0f), same(0.0f)};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if ((k * G + lane) * V < a.width) {
-        const Pack<T, V> px = x[k * G + lane], pd = dy[k * G + lane];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = widen(pd.v[i]);
-          const float u = (widen(px.v[i]) - mean) * rstd;
-          const float g = d * w[k][i];
-          sums[0] += g;
-          sums[1] += g * u;
-          dw[k][i] += d * u;
-          db[k][i] += d;
-        }
+        Two x[V / 2], dy[V / 2];
+        load_twos<T, V>(xs + (k * G + lane) * V, x);
+        load_twos<T, V>(ds + (k * G + lane) * V, dy);
+        M::collect(x, dy, mean, rstd, w[k], pairs, dw[k], db[k]);
       }
     }
+    float sums[2] = {both(pairs[0]), both(pairs[1])};
     group_sums<G, 2>(sums, scratch);
     if (lane == 0 && row != blockIdx.x) ring.ask(sizeof(T));
     if (a.want_dx) {
-      const float mean_g = sums[0] * inverse, mean_gu = sums[1] * inverse;
-      Pack<T, V>* dx = reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * a.width);
+      T* dx = static_cast<T*>(a.y) + row * a.width;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         if ((k * G + lane) * V < a.width) {
-          const Pack<T, V> px = x[k * G + lane], pd = dy[k * G + lane];
-          Pack<T, V> out;
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float u = (widen(px.v[i]) - mean) * rstd;
-            out.v[i] = narrow<T>(rstd * (widen(pd.v[i]) * w[k][i] - mean_g - u * mean_gu));
-          }
-          dx[k * G + lane] = out;
+          Two x[V / 2], dy[V / 2];
+          load_twos<T, V>(xs + (k * G + lane) * V, x);
+          load_twos<T, V>(ds + (k * G + lane) * V, dy);
+          M::gradient(x, dy, mean, rstd, w[k], sums[0] * inverse, sums[1] * inverse);
+          store_twos<T, V>(dx + (k * G + lane) * V, dy);
         }
       }
     }
@@ -554,9 +609,9 @@ __global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
     const int64_t c = static_cast<int64_t>(k * G + lane) * V;
     if (c < a.width) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        partial[c + i] = dw[k][i];
-        partial[a.width + c + i] = db[k][i];
+      for (int i = 0; i < V / 2; ++i) {
+        unpack(dw[k][i], partial + c + 2 * i, partial + c + 2 * i + 1);
+        unpack(db[k][i], partial + a.width + c + 2 * i, partial + a.width + c + 2 * i + 1);
       }
     }
   }
@@ -583,36 +638,31 @@ __global__ void __launch_bounds__(kTileThreads, 4)
   if (threadIdx.x == 0) {
     for (int s = 0; s < ring_args.stages; ++s) ring.ask(sizeof(T));
   }
-  float w[NV][V], b[NV][V];
-  load_params<T, V, NV, G>(a.weight, a.param_f32, width, lane, 1.0f, w);
-  load_params<T, V, NV, G>(a.bias, a.param_f32, width, lane, 0.0f, b);
+  using M = RowMath<T, V, NV, G>;
+  Two w[NV][V / 2], b[NV][V / 2];
+  load_param_pairs<T, V, NV, G>(a.weight, a.param_f32, width, lane, 1.0f, w);
+  load_param_pairs<T, V, NV, G>(a.bias, a.param_f32, width, lane, 0.0f, b);
   for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * tile; row0 < a.rows;
        row0 += static_cast<int64_t>(gridDim.x) * tile) {
     const T* data = reinterpret_cast<const T*>(ring.wait());
+#pragma unroll 2
     for (int i0 = 0; i0 < tile; i0 += kGroups) {
       const int64_t row = row0 + i0 + group;
       const bool live = i0 + group < tile && row < a.rows;
-      Pack<T, V> raw[NV];
+      Two x[NV][V / 2];
       float mean = 0.0f, squares = 0.0f;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = (k * G + lane) * V;
         if (live && c < width) {
-          raw[k] = *reinterpret_cast<const Pack<T, V>*>(data + (i0 + group) * width + c);
-#pragma unroll
-          for (int i = 0; i < V; ++i) mean += widen(raw[k].v[i]);
+          load_twos<T, V>(data + (i0 + group) * width + c, x[k]);
+          mean += M::sum(x[k]);
         }
       }
       mean = group_sum<G, float>(mean, nullptr) * inverse;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        if (live && (k * G + lane) * V < width) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float d = widen(raw[k].v[i]) - mean;
-            squares += d * d;
-          }
-        }
+        if (live && (k * G + lane) * V < width) squares += M::squares(x[k], mean);
       }
       squares = group_sum<G, float>(squares, nullptr);
       if (!live) continue;
@@ -625,12 +675,8 @@ __global__ void __launch_bounds__(kTileThreads, 4)
       for (int k = 0; k < NV; ++k) {
         const int c = (k * G + lane) * V;
         if (c < width) {
-          Pack<T, V> out;
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            out.v[i] = narrow<T>((widen(raw[k].v[i]) - mean) * rstd * w[k][i] + b[k][i]);
-          }
-          *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * width + c) = out;
+          M::normalise(x[k], mean, rstd, w[k], b[k]);
+          store_twos<T, V>(static_cast<T*>(a.y) + row * width + c, x[k]);
         }
       }
     }
@@ -667,12 +713,13 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 3 : 2)
   if (threadIdx.x == 0) {
     for (int s = 0; s < ring_args.stages; ++s) ring.ask(sizeof(T));
   }
-  float w[NV][V], dw[NV][V], db[NV][V];
-  load_params<T, V, NV, G>(a.weight, a.param_f32, width, lane, 1.0f, w);
+  using M = RowMath<T, V, NV, G>;
+  Two w[NV][V / 2], dw[NV][V / 2], db[NV][V / 2];
+  load_param_pairs<T, V, NV, G>(a.weight, a.param_f32, width, lane, 1.0f, w);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.0f;
+    for (int i = 0; i < V / 2; ++i) dw[k][i] = db[k][i] = same(0.0f);
   }
   int slot = 0;
   const int64_t step = static_cast<int64_t>(gridDim.x) * tile;
@@ -681,45 +728,32 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 3 : 2)
     const uint8_t* at = ring.wait();
     const T* xs = reinterpret_cast<const T*>(at);
     const T* ds = reinterpret_cast<const T*>(at + ring_args.stage_bytes / 2);
+#pragma unroll 2
     for (int i0 = 0; i0 < tile; i0 += kGroups) {
       const int64_t row = row0 + i0 + group;
       const bool live = i0 + group < tile && row < a.rows;
       const float2 s = live ? stats[slot][i0 + group] : make_float2(0.0f, 0.0f);
-      Pack<T, V> px[NV], pd[NV];
-      float sums[2] = {0.0f, 0.0f};
+      Two x[NV][V / 2], dy[NV][V / 2];
+      Two pairs[2] = {same(0.0f), same(0.0f)};
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = (k * G + lane) * V;
         if (live && c < width) {
-          px[k] = *reinterpret_cast<const Pack<T, V>*>(xs + (i0 + group) * width + c);
-          pd[k] = *reinterpret_cast<const Pack<T, V>*>(ds + (i0 + group) * width + c);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float d = widen(pd[k].v[i]);
-            const float u = (widen(px[k].v[i]) - s.x) * s.y;
-            const float g = d * w[k][i];
-            sums[0] += g;
-            sums[1] += g * u;
-            dw[k][i] += d * u;
-            db[k][i] += d;
-          }
+          load_twos<T, V>(xs + (i0 + group) * width + c, x[k]);
+          load_twos<T, V>(ds + (i0 + group) * width + c, dy[k]);
+          M::collect(x[k], dy[k], s.x, s.y, w[k], pairs, dw[k], db[k]);
         }
       }
       if (!a.want_dx) continue;
+      float sums[2] = {both(pairs[0]), both(pairs[1])};
       group_sums<G, 2>(sums, nullptr);
       if (!live) continue;
-      const float mean_g = sums[0] * inverse, mean_gu = sums[1] * inverse;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = (k * G + lane) * V;
         if (c < width) {
-          Pack<T, V> out;
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float u = (widen(px[k].v[i]) - s.x) * s.y;
-            out.v[i] = narrow<T>(s.y * (widen(pd[k].v[i]) * w[k][i] - mean_g - u * mean_gu));
-          }
-          *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * width + c) = out;
+          M::gradient(x[k], dy[k], s.x, s.y, w[k], sums[0] * inverse, sums[1] * inverse);
+          store_twos<T, V>(static_cast<T*>(a.y) + row * width + c, dy[k]);
         }
       }
     }
@@ -730,7 +764,16 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 3 : 2)
   }
   if (!a.want_params) return;
   __syncthreads();
-  block_columns<T, V, NV, G>(a, dw, db, reinterpret_cast<float*>(shared));
+  float wide_dw[NV][V], wide_db[NV][V];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      unpack(dw[k][i], &wide_dw[k][2 * i], &wide_dw[k][2 * i + 1]);
+      unpack(db[k][i], &wide_db[k][2 * i], &wide_db[k][2 * i + 1]);
+    }
+  }
+  block_columns<T, V, NV, G>(a, wide_dw, wide_db, reinterpret_cast<float*>(shared));
 }
 
 // ---- rows of any width and type --------------------------------------------------------

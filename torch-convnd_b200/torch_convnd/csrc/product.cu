@@ -112,36 +112,6 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, dev::E
   return __all_sync(0xffffffffu, wait<kPair>(bar, parity, err, site, timeout_ns)) != 0;
 }
 
-template <typename Out>
-__device__ __forceinline__ uint32_t narrow2(Two v) {
-  float lo, hi;
-  unpack(v, &lo, &hi);
-  uint32_t bits;
-  if constexpr (sizeof(Out) == 2) {
-    Pack<Out, 2> p;
-    p.v[0] = narrow<Out>(lo);
-    p.v[1] = narrow<Out>(hi);
-    memcpy(&bits, &p, 4);
-  }
-  return bits;
-}
-template <>
-__device__ __forceinline__ uint32_t narrow2<__nv_bfloat16>(Two v) {
-  float lo, hi;
-  unpack(v, &lo, &hi);
-  uint32_t bits;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(bits) : "f"(hi), "f"(lo));
-  return bits;
-}
-template <>
-__device__ __forceinline__ uint32_t narrow2<__half>(Two v) {
-  float lo, hi;
-  unpack(v, &lo, &hi);
-  uint32_t bits;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(bits) : "f"(hi), "f"(lo));
-  return bits;
-}
-
 // Writes 32 values of a row (columns half * 32 ... of a unit) into a 128-byte-wide staging
 // tile with the 128-byte TMA swizzle (16-byte chunk c of row r at chunk c ^ (r & 7)).
 template <typename Out>
