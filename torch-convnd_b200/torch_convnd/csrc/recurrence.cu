@@ -43,7 +43,7 @@ constexpr int kGroup = 32;      // chunks that are composed without an intermedi
 constexpr uint32_t kSiteForward = 0x601, kSiteBackward = 0x602;
 
 // Steps a thread holds: forward and backward in column layout, both in step layout.
-constexpr int kForwardSteps = 16, kBackwardSteps = 8, kAlongSteps = 8;
+constexpr int kForwardSteps = 8, kBackwardSteps = 8, kAlongSteps = 8;
 constexpr int kStateBlock = kBackwardSteps * kWarps;  // 64
 constexpr int kAlongBlock = 32 * kAlongSteps;         // 256
 
@@ -291,7 +291,7 @@ __device__ __forceinline__ int64_t column_base(const RecurrenceArgs& a, int64_t 
 // ---- column layout ---------------------------------------------------------------------
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kWarps * 32, 2)
+__global__ void __launch_bounds__(kWarps * 32, 3)
     columns_forward_kernel(const __grid_constant__ RecurrenceArgs a) {
   using A = typename Wide<T>::type;
   constexpr int kSteps = kForwardSteps, kSlots = 32 * V;
@@ -536,13 +536,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         __syncthreads();
       }
     }
-    A prior[kSteps][V];
+    A slope[kSteps][V];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        prior[i][v] = saved[v];
-        saved[v] = f[i][v] * saved[v] + keep[i][v] * widen(px[i].v[v]);
+        // f (1 - f) (h_{t-1} - x), what the gate's gradient takes of the flow
+        const A x = widen(px[i].v[v]);
+        slope[i][v] = f[i][v] * keep[i][v] * (saved[v] - x);
+        saved[v] = f[i][v] * saved[v] + keep[i][v] * x;
       }
     }
 #pragma unroll
@@ -552,7 +554,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       for (int v = 0; v < V; ++v) {
         const A total = widen(pd[i].v[v]) + q[v];
         dx.v[v] = narrow<T>(keep[i][v] * total);
-        dg.v[v] = narrow<T>(f[i][v] * keep[i][v] * (prior[i][v] - widen(px[i].v[v])) * total);
+        dg.v[v] = narrow<T>(slope[i][v] * total);
         q[v] = f[i][v] * total;
       }
       if (i < count) {
