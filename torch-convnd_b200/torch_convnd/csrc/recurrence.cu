@@ -43,7 +43,7 @@ constexpr int kGroup = 32;      // chunks that are composed without an intermedi
 constexpr uint32_t kSiteForward = 0x601, kSiteBackward = 0x602;
 
 // Steps a thread holds: forward and backward in column layout, both in step layout.
-constexpr int kForwardSteps = 8, kBackwardSteps = 8, kAlongSteps = 8;
+constexpr int kForwardSteps = 16, kBackwardSteps = 8, kAlongSteps = 8;
 constexpr int kStateBlock = kBackwardSteps * kWarps;  // 64
 constexpr int kAlongBlock = 32 * kAlongSteps;         // 256
 
@@ -197,18 +197,9 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   return *reinterpret_cast<const Pack<T, V>*>(p);
 }
 
-// The same where `valid`, else `other` everywhere. A step past the end is given the gate
-// +inf and x = dy = 0: it holds the state and passes the flow on, so the walks need no
-// branches (a branch per step had kept the exponentials of different steps from
-// overlapping).
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_pack(const T* p, bool valid, float other) {
-  Pack<T, V> v;
-#pragma unroll
-  for (int i = 0; i < V; ++i) v.v[i] = narrow<T>(static_cast<typename Wide<T>::type>(other));
-  if (valid) v = *reinterpret_cast<const Pack<T, V>*>(p);
-  return v;
-}
+// A step past the end is given the gate +inf and x = dy = 0: it holds the state and passes the
+// flow on, so the walks need no branches (a branch per step had kept the exponentials of
+// different steps from overlapping).
 
 template <typename A>
 __device__ __forceinline__ Map<A> shuffle_up(const Map<A>& m, int d) {
@@ -288,10 +279,37 @@ __device__ __forceinline__ int64_t column_base(const RecurrenceArgs& a, int64_t 
   return outer * a.steps * a.inner + (column - outer * a.inner);
 }
 
-// ---- column layout ---------------------------------------------------------------------
+// The addresses of a thread's steps: step i of every tensor lies i strides behind the same
+// element offset. Offset: uint32_t bytes where the tensors are below 4 GB (one 32-bit
+// addition serves all tensors, whose bases stay in uniform registers), else int64_t.
+template <typename T, typename Offset>
+struct Steps {
+  Offset first, stride;
+  __device__ __forceinline__ Steps(int64_t element, int64_t inner)
+      : first(static_cast<Offset>(element * static_cast<int64_t>(sizeof(T)))),
+        stride(static_cast<Offset>(inner * static_cast<int64_t>(sizeof(T)))) {}
+  template <int V>
+  __device__ __forceinline__ const Pack<T, V>& read(const void* base, int i) const {
+    return *reinterpret_cast<const Pack<T, V>*>(static_cast<const char*>(base) + (first + i * stride));
+  }
+  template <int V>
+  __device__ __forceinline__ void write(void* base, int i, const Pack<T, V>& v) const {
+    *reinterpret_cast<Pack<T, V>*>(static_cast<char*>(base) + (first + i * stride)) = v;
+  }
+};
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kWarps * 32, 3)
+__device__ __forceinline__ Pack<T, V> all_of(float value) {
+  Pack<T, V> p;
+#pragma unroll
+  for (int v = 0; v < V; ++v) p.v[v] = narrow<T>(static_cast<typename Wide<T>::type>(value));
+  return p;
+}
+
+// ---- column layout ---------------------------------------------------------------------
+
+template <typename T, int V, typename Offset>
+__global__ void __launch_bounds__(kWarps * 32, 2)
     columns_forward_kernel(const __grid_constant__ RecurrenceArgs a) {
   using A = typename Wide<T>::type;
   constexpr int kSteps = kForwardSteps, kSlots = 32 * V;
@@ -320,14 +338,25 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
   for (; chunk < stop; ++chunk) {
     const int most = a.balanced ? a.balanced : kSteps;
     const int64_t first = (chunk * warps + warp) * most;
-    const T* x = static_cast<const T*>(a.x) + base + first * a.inner;
-    const T* gate = static_cast<const T*>(a.gate) + base + first * a.inner;
+    const Steps<T, Offset> at(base + first * a.inner, a.inner);
     const int count = live ? steps_here(a.steps - first, most) : 0;
     Pack<T, V> px[kSteps], pg[kSteps];
+    if (count == kSteps) {
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      px[i] = load_pack<T, V>(x + i * a.inner, i < count, 0.0f);
-      pg[i] = load_pack<T, V>(gate + i * a.inner, i < count, INFINITY);
+      for (int i = 0; i < kSteps; ++i) {
+        px[i] = at.template read<V>(a.x, i);
+        pg[i] = at.template read<V>(a.gate, i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        px[i] = all_of<T, V>(0.0f);
+        pg[i] = all_of<T, V>(INFINITY);
+        if (i < count) {
+          px[i] = at.template read<V>(a.x, i);
+          pg[i] = at.template read<V>(a.gate, i);
+        }
+      }
     }
     A f[kSteps][V], b[kSteps][V];
     Map<A> own[V];
@@ -394,7 +423,6 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
         static_cast<A*>(a.states)[first / kStateBlock * a.columns + column + v] = state[v];
       }
     }
-    T* y = static_cast<T*>(a.y) + base + first * a.inner;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       Pack<T, V> out;
@@ -403,7 +431,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
         state[v] = f[i][v] * state[v] + b[i][v];
         out.v[v] = narrow<T>(state[v]);
       }
-      if (i < count) *reinterpret_cast<Pack<T, V>*>(y + i * a.inner) = out;
+      if (i < count) at.template write<V>(a.y, i, out);
     }
     const int64_t end = a.steps > 0 ? a.steps - 1 : 0;
     if (live && first <= end && end < first + most) {
@@ -413,7 +441,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, typename Offset>
 __global__ void __launch_bounds__(kWarps * 32, 2)
     columns_backward_kernel(const __grid_constant__ RecurrenceArgs a) {
   using A = typename Wide<T>::type;
@@ -445,15 +473,27 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     const int64_t chunk = a.chunks - 1 - order;
     const int most = a.balanced ? a.balanced : kSteps;
     const int64_t first = (chunk * warps + warp) * most;
-    const int64_t offset = base + first * a.inner;
+    const Steps<T, Offset> at(base + first * a.inner, a.inner);
     const int count = live ? steps_here(a.steps - first, most) : 0;
     Pack<T, V> px[kSteps], pg[kSteps], pd[kSteps];
+    if (count == kSteps && a.dy != nullptr) {
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int64_t at = offset + i * a.inner;
-      px[i] = load_pack<T, V>(static_cast<const T*>(a.x) + at, i < count, 0.0f);
-      pg[i] = load_pack<T, V>(static_cast<const T*>(a.gate) + at, i < count, INFINITY);
-      pd[i] = load_pack<T, V>(static_cast<const T*>(a.dy) + at, i < count && a.dy != nullptr, 0.0f);
+      for (int i = 0; i < kSteps; ++i) {
+        px[i] = at.template read<V>(a.x, i);
+        pg[i] = at.template read<V>(a.gate, i);
+        pd[i] = at.template read<V>(a.dy, i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        px[i] = pd[i] = all_of<T, V>(0.0f);
+        pg[i] = all_of<T, V>(INFINITY);
+        if (i < count) {
+          px[i] = at.template read<V>(a.x, i);
+          pg[i] = at.template read<V>(a.gate, i);
+          if (a.dy != nullptr) pd[i] = at.template read<V>(a.dy, i);
+        }
+      }
     }
     A saved[V];  // the state before the chunk
 #pragma unroll
@@ -558,12 +598,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         q[v] = f[i][v] * total;
       }
       if (i < count) {
-        if (a.dx != nullptr) {
-          *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.dx) + offset + i * a.inner) = dx;
-        }
-        if (a.dgate != nullptr) {
-          *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.dgate) + offset + i * a.inner) = dg;
-        }
+        if (a.dx != nullptr) at.template write<V>(a.dx, i, dx);
+        if (a.dgate != nullptr) at.template write<V>(a.dgate, i, dg);
       }
     }
     if (a.dinitial != nullptr && live && first == 0) {
@@ -963,19 +999,21 @@ int cnd_gated_recurrence_forward(int32_t dtype, int64_t outer, int64_t steps, in
   if (rc != CND_OK) return rc;
   const unsigned grid = recurrence_grid(p);
   const bool vectors = runs_aligned(dtype, steps, {x, gate, y});
+  const bool small = columns * std::max<int64_t>(steps, 1) * element_size(dtype) <= UINT32_MAX;
   with_dtype(dtype, [&](auto zero) {
     using T = decltype(zero);
     if (p.along) {
       steps_forward_kernel<T><<<grid, p.warps * 32, 0, stream>>>(a, vectors);
       return;
     }
+    const auto run = [&](auto kernel) { kernel<<<grid, p.warps * 32, 0, stream>>>(a); };
     if constexpr (sizeof(T) == 2) {
       if (p.vector == 2) {
-        columns_forward_kernel<T, 2><<<grid, p.warps * 32, 0, stream>>>(a);
-        return;
+        return small ? run(columns_forward_kernel<T, 2, uint32_t>)
+                     : run(columns_forward_kernel<T, 2, int64_t>);
       }
     }
-    columns_forward_kernel<T, 1><<<grid, p.warps * 32, 0, stream>>>(a);
+    small ? run(columns_forward_kernel<T, 1, uint32_t>) : run(columns_forward_kernel<T, 1, int64_t>);
   });
   count_launch();
   return launch_status("cnd_gated_recurrence_forward");
@@ -1021,19 +1059,22 @@ int cnd_gated_recurrence_backward(int32_t dtype, int64_t outer, int64_t steps, i
   if (rc != CND_OK) return rc;
   const unsigned grid = recurrence_grid(p);
   const bool vectors = runs_aligned(dtype, steps, {x, gate, dy, dx, dgate});
+  const bool small = columns * std::max<int64_t>(steps, 1) * element_size(dtype) <= UINT32_MAX;
   with_dtype(dtype, [&](auto zero) {
     using T = decltype(zero);
     if (p.along) {
       steps_backward_kernel<T><<<grid, p.warps * 32, 0, stream>>>(a, vectors);
       return;
     }
+    const auto run = [&](auto kernel) { kernel<<<grid, p.warps * 32, 0, stream>>>(a); };
     if constexpr (sizeof(T) == 2) {
       if (p.vector == 2) {
-        columns_backward_kernel<T, 2><<<grid, p.warps * 32, 0, stream>>>(a);
-        return;
+        return small ? run(columns_backward_kernel<T, 2, uint32_t>)
+                     : run(columns_backward_kernel<T, 2, int64_t>);
       }
     }
-    columns_backward_kernel<T, 1><<<grid, p.warps * 32, 0, stream>>>(a);
+    small ? run(columns_backward_kernel<T, 1, uint32_t>)
+          : run(columns_backward_kernel<T, 1, int64_t>);
   });
   count_launch();
   return launch_status("cnd_gated_recurrence_backward");
