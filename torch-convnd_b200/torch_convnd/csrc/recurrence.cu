@@ -11,8 +11,8 @@
 // read once and stay in registers between the two walks. The work is bound by memory
 // traffic: 3 elements a step forward, 5 backward.
 //
-// Column layout (inner > 1): the lanes of a warp hold neighbouring columns, the warps of a
-// block follow one another in time. Step layout (inner = 1, steps contiguous): the lanes of a
+// Column layout (inner > 1): the lanes of a warp hold two columns each, in packed float32
+// pairs, the warps of a block follow one another in time. Step layout (inner = 1, steps contiguous): the lanes of a
 // warp hold neighbouring runs of steps of one column and compose their maps by shuffles.
 //
 // A block that has its columns to itself loops over the chunks of the time axis. Where
@@ -31,6 +31,8 @@
 #include <algorithm>
 #include <cstdlib>
 
+#include <type_traits>
+
 #include "layers.cuh"
 #include "ptx.cuh"
 
@@ -42,8 +44,10 @@ constexpr int kWarps = 8;       // most warps of a block
 constexpr int kGroup = 32;      // chunks that are composed without an intermediate state
 constexpr uint32_t kSiteForward = 0x601, kSiteBackward = 0x602;
 
-// Steps a thread holds: forward and backward in column layout, both in step layout.
-constexpr int kForwardSteps = 16, kBackwardSteps = 8, kAlongSteps = 8;
+// Steps a thread holds: forward (by element size: what its registers take of two columns) and
+// backward in column layout, both in step layout.
+constexpr int forward_steps(size_t size) { return size == 2 ? 16 : 8; }
+constexpr int kBackwardSteps = 8, kAlongSteps = 8;
 constexpr int kStateBlock = kBackwardSteps * kWarps;  // 64
 constexpr int kAlongBlock = 32 * kAlongSteps;         // 256
 
@@ -210,59 +214,76 @@ __device__ __forceinline__ Map<A> shuffle_down(const Map<A>& m, int d) {
   return {__shfl_down_sync(0xffffffffu, m.a, d), __shfl_down_sync(0xffffffffu, m.b, d)};
 }
 
-// The state before this chunk for the block's column slots lane * kPer ... (kSlots = 32 kPer
-// slots, or the one slot of step layout), from the chunks before it (order = 0, 1, ... in the
-// direction of the walk) and `begin`, the state before the first. `scratch`: [kWarps][kSlots]
-// maps. The whole block calls it: warp w composes maps w * 4 ... of the group.
-template <typename A, int kSlots, int kPer>
+// The one column of a block in step layout, as Steps are the columns of the other.
+struct OneColumn {
+  static constexpr int kColumns = 1;
+  static __device__ __forceinline__ int slot(int, int) { return 0; }
+};
+template <typename S>
+constexpr int slots_of() {
+  if constexpr (std::is_same_v<S, OneColumn>) {
+    return 1;
+  } else {
+    return 32 * S::kColumns;
+  }
+}
+
+// The state before this chunk, for the columns a lane holds (S::slot of them), from the chunks
+// before it (order = 0, 1, ... in the direction of the walk) and `state`, the state before
+// the first. `scratch`: [kWarps][slots] maps. The whole block calls it: warp w composes maps
+// w * 4 ... of the group.
+template <typename A, typename S>
 __device__ __forceinline__ void carry_in(const RecurrenceArgs& a, int64_t order, int64_t block,
-                                         Map<A>* scratch, unsigned int site, A (&state)[kPer]) {
-  constexpr int kEach = kGroup / kWarps, kWords = kMapWords<A>;
+                                         Map<A>* scratch, unsigned int site,
+                                         A (&state)[S::kColumns]) {
+  constexpr int kEach = kGroup / kWarps, kWords = kMapWords<A>, kPer = S::kColumns;
+  constexpr int kSlots = slots_of<S>();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t group = order / kGroup;
   const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
-  const int64_t slot = block * kSlots + (kSlots == 1 ? 0 : lane * kPer);
   const auto* maps = static_cast<const unsigned long long*>(a.maps);
   unsigned long long raw[kEach][kPer][kWords];
+  const auto place = [&](int i, int v) {
+    return ((group * kGroup + warp * kEach + i) * padded + block * kSlots + S::slot(lane, v)) * kWords;
+  };
+  const int known = static_cast<int>(order - group * kGroup) - warp * kEach;  // maps of this warp
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    const int64_t at = group * kGroup + warp * kEach + i;
-    if (at < order) {
+    if (i < known) {
 #pragma unroll
       for (int v = 0; v < kPer; ++v) {
 #pragma unroll
-        for (int k = 0; k < kWords; ++k) {
-          raw[i][v][k] = load_exchange(maps + (at * padded + slot + v) * kWords + k);
-        }
+        for (int k = 0; k < kWords; ++k) raw[i][v][k] = load_exchange(maps + place(i, v) + k);
       }
     }
   }
   if (group > 0) {
 #pragma unroll
-    for (int v = 0; v < kPer; ++v) state[v] = load_base<A>(a, group * padded + slot + v, site);
+    for (int v = 0; v < kPer; ++v) {
+      state[v] = load_base<A>(a, group * padded + block * kSlots + S::slot(lane, v), site);
+    }
   }
 #pragma unroll
   for (int v = 0; v < kPer; ++v) {
     Map<A> m{A(1), A(0)};
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int64_t at = group * kGroup + warp * kEach + i;
-      if (at < order) {
+      if (i < known) {
 #pragma unroll
         for (int k = 0; k < kWords; ++k) {
-          raw[i][v][k] = settle(maps + (at * padded + slot + v) * kWords + k, raw[i][v][k], a, site);
+          raw[i][v][k] = settle(maps + place(i, v) + k, raw[i][v][k], a, site);
         }
         m = then(m, map_of<A>(raw[i][v]));
       }
     }
-    if (kSlots > 1 || lane == 0) scratch[warp * kSlots + (kSlots == 1 ? 0 : lane * kPer + v)] = m;
+    if (kSlots > 1 || lane == 0) scratch[warp * kSlots + S::slot(lane, v)] = m;
   }
   __syncthreads();
 #pragma unroll
   for (int v = 0; v < kPer; ++v) {
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const Map<A> m = scratch[w * kSlots + (kSlots == 1 ? 0 : lane * kPer + v)];
+      const Map<A> m = scratch[w * kSlots + S::slot(lane, v)];
       state[v] = m.a * state[v] + m.b;
     }
   }
@@ -279,332 +300,417 @@ __device__ __forceinline__ int64_t column_base(const RecurrenceArgs& a, int64_t 
   return outer * a.steps * a.inner + (column - outer * a.inner);
 }
 
-// The addresses of a thread's steps: step i of every tensor lies i strides behind the same
-// element offset. Offset: uint32_t bytes where the tensors are below 4 GB (one 32-bit
-// addition serves all tensors, whose bases stay in uniform registers), else int64_t.
-template <typename T, typename Offset>
+// What a lane holds of a step: two columns (of float32 arithmetic, in packed pairs) or, for
+// float64, one.
+template <typename T>
+struct Held {
+  using P = Two;
+  static constexpr int kColumns = 2;
+  static __device__ __forceinline__ P value(float v) { return same(v); }
+  static __device__ __forceinline__ P join(const float (&v)[2]) { return two(v[0], v[1]); }
+  static __device__ __forceinline__ void part(P p, float (&v)[2]) { unpack(p, &v[0], &v[1]); }
+  static __device__ __forceinline__ P mad(P a, P b, P c) { return fma2(a, b, c); }
+  static __device__ __forceinline__ P mul(P a, P b) { return mul2(a, b); }
+  static __device__ __forceinline__ P add(P a, P b) { return add2(a, b); }
+};
+template <>
+struct Held<double> {
+  using P = double;
+  static constexpr int kColumns = 1;
+  static __device__ __forceinline__ P value(double v) { return v; }
+  static __device__ __forceinline__ P join(const double (&v)[1]) { return v[0]; }
+  static __device__ __forceinline__ void part(P p, double (&v)[1]) { v[0] = p; }
+  static __device__ __forceinline__ P mad(P a, P b, P c) { return fma(a, b, c); }
+  static __device__ __forceinline__ P mul(P a, P b) { return a * b; }
+  static __device__ __forceinline__ P add(P a, P b) { return a + b; }
+};
+
+// A map of the held columns.
+template <typename T>
+struct HeldMap {
+  typename Held<T>::P a, b;
+};
+template <typename T>
+__device__ __forceinline__ HeldMap<T> then(const HeldMap<T>& first, const HeldMap<T>& second) {
+  using H = Held<T>;
+  return {H::mul(first.a, second.a), H::mad(second.a, first.b, second.b)};
+}
+
+// The addresses of a thread's steps. Adjacent: its columns are neighbours read at once (two
+// 16-bit columns are 4 bytes); else they lie 32 apart, each warp reading 32 neighbours, which
+// needs no alignment. Step i of every tensor lies i strides behind the same offset.
+// Offset: uint32_t bytes where the tensors are below 4 GB (one 32-bit addition serves all
+// tensors, whose bases stay in uniform registers), else int64_t.
+template <typename T, bool kAdjacent, typename Offset>
 struct Steps {
-  Offset first, stride;
-  __device__ __forceinline__ Steps(int64_t element, int64_t inner)
-      : first(static_cast<Offset>(element * static_cast<int64_t>(sizeof(T)))),
-        stride(static_cast<Offset>(inner * static_cast<int64_t>(sizeof(T)))) {}
-  template <int V>
-  __device__ __forceinline__ const Pack<T, V>& read(const void* base, int i) const {
-    return *reinterpret_cast<const Pack<T, V>*>(static_cast<const char*>(base) + (first + i * stride));
+  static constexpr int kColumns = Held<T>::kColumns, kParts = kAdjacent ? 1 : kColumns;
+  Offset first[kParts], stride;
+  bool live[kParts];
+
+  __device__ __forceinline__ Steps(const RecurrenceArgs& a, int64_t block, int lane)
+      : stride(static_cast<Offset>(a.inner * static_cast<int64_t>(sizeof(T)))) {
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      const int64_t c = column(block, lane, p);
+      live[p] = c < a.columns;
+      first[p] = live[p] ? static_cast<Offset>(column_base(a, c) * static_cast<int64_t>(sizeof(T)))
+                         : Offset(0);
+    }
   }
-  template <int V>
-  __device__ __forceinline__ void write(void* base, int i, const Pack<T, V>& v) const {
-    *reinterpret_cast<Pack<T, V>*>(static_cast<char*>(base) + (first + i * stride)) = v;
+  // Column of held column `i`.
+  static __device__ __forceinline__ int64_t column(int64_t block, int lane, int i) {
+    return block * 32 * kColumns + (kAdjacent ? lane * kColumns + i : i * 32 + lane);
+  }
+  // Slot of held column `i` among the block's.
+  static __device__ __forceinline__ int slot(int lane, int i) {
+    return kAdjacent ? lane * kColumns + i : i * 32 + lane;
+  }
+  __device__ __forceinline__ bool lives(int i) const { return live[kAdjacent ? 0 : i]; }
+
+  __device__ __forceinline__ Pack<T, kColumns> read(const void* base, Offset ahead) const {
+    Pack<T, kColumns> v;
+    if constexpr (kAdjacent) {
+      v = *reinterpret_cast<const Pack<T, kColumns>*>(static_cast<const char*>(base) + (first[0] + ahead));
+    } else {
+#pragma unroll
+      for (int p = 0; p < kColumns; ++p) {
+        v.v[p] = *reinterpret_cast<const T*>(static_cast<const char*>(base) + (first[p] + ahead));
+      }
+    }
+    return v;
+  }
+  // The held columns that exist, `other` for the rest.
+  __device__ __forceinline__ Pack<T, kColumns> read_live(const void* base, Offset ahead,
+                                                         float other) const {
+    Pack<T, kColumns> v;
+#pragma unroll
+    for (int i = 0; i < kColumns; ++i) {
+      v.v[i] = narrow<T>(static_cast<typename Wide<T>::type>(other));
+    }
+    if constexpr (kAdjacent) {
+      if (live[0]) v = read(base, ahead);
+    } else {
+#pragma unroll
+      for (int p = 0; p < kColumns; ++p) {
+        if (live[p]) {
+          v.v[p] = *reinterpret_cast<const T*>(static_cast<const char*>(base) + (first[p] + ahead));
+        }
+      }
+    }
+    return v;
+  }
+  __device__ __forceinline__ void write(void* base, Offset ahead, typename Held<T>::P value) const {
+    typename Wide<T>::type w[kColumns];
+    Held<T>::part(value, w);
+    if constexpr (kAdjacent) {
+      if (!live[0]) return;
+      Pack<T, kColumns> v;
+#pragma unroll
+      for (int i = 0; i < kColumns; ++i) v.v[i] = narrow<T>(w[i]);
+      *reinterpret_cast<Pack<T, kColumns>*>(static_cast<char*>(base) + (first[0] + ahead)) = v;
+    } else {
+#pragma unroll
+      for (int p = 0; p < kColumns; ++p) {
+        if (live[p]) {
+          *reinterpret_cast<T*>(static_cast<char*>(base) + (first[p] + ahead)) = narrow<T>(w[p]);
+        }
+      }
+    }
+  }
+  // A step's pack past the end of the steps.
+  static __device__ __forceinline__ Pack<T, kColumns> all(float value) {
+    Pack<T, kColumns> v;
+#pragma unroll
+    for (int i = 0; i < kColumns; ++i) {
+      v.v[i] = narrow<T>(static_cast<typename Wide<T>::type>(value));
+    }
+    return v;
   }
 };
 
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> all_of(float value) {
-  Pack<T, V> p;
+template <typename T, int N>
+__device__ __forceinline__ typename Held<T>::P held(const Pack<T, N>& p) {
+  typename Wide<T>::type w[N];
 #pragma unroll
-  for (int v = 0; v < V; ++v) p.v[v] = narrow<T>(static_cast<typename Wide<T>::type>(value));
-  return p;
+  for (int i = 0; i < N; ++i) w[i] = widen(p.v[i]);
+  return Held<T>::join(w);
 }
 
-// ---- column layout ---------------------------------------------------------------------
+// f and 1 - f of the held columns.
+template <typename T, int N>
+__device__ __forceinline__ void held_gates(const Pack<T, N>& g, typename Held<T>::P* f,
+                                           typename Held<T>::P* keep) {
+  typename Wide<T>::type w[N], v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) gates<T>(widen(g.v[i]), &w[i], &v[i]);
+  *f = Held<T>::join(w);
+  *keep = Held<T>::join(v);
+}
 
-template <typename T, int V, typename Offset>
+// Values kept per column ([..][columns] of type Wide<T>), zero where there are none.
+template <typename T, typename S>
+__device__ __forceinline__ typename Held<T>::P load_columns(const void* p, const S& at,
+                                                            const RecurrenceArgs& a, int64_t row,
+                                                            int64_t block, int lane) {
+  using A = typename Wide<T>::type;
+  A w[S::kColumns];
+#pragma unroll
+  for (int i = 0; i < S::kColumns; ++i) {
+    w[i] = p != nullptr && at.lives(i)
+               ? static_cast<const A*>(p)[row * a.columns + S::column(block, lane, i)]
+               : A(0);
+  }
+  return Held<T>::join(w);
+}
+
+template <typename T, typename S>
+__device__ __forceinline__ void store_columns(void* p, const S& at, const RecurrenceArgs& a,
+                                              int64_t row, int64_t block, int lane,
+                                              typename Held<T>::P value) {
+  using A = typename Wide<T>::type;
+  A w[S::kColumns];
+  Held<T>::part(value, w);
+#pragma unroll
+  for (int i = 0; i < S::kColumns; ++i) {
+    if (at.lives(i)) static_cast<A*>(p)[row * a.columns + S::column(block, lane, i)] = w[i];
+  }
+}
+
+// Sends this chunk's map (and, from the last chunk of a group, the state behind it) and returns
+// the state before the chunk.
+template <typename T, typename S>
+__device__ __forceinline__ typename Held<T>::P exchange(const RecurrenceArgs& a, int64_t order,
+                                                        int64_t block, int lane, bool sends,
+                                                        const HeldMap<T>& whole,
+                                                        typename Held<T>::P begin,
+                                                        Map<typename Wide<T>::type>* scratch,
+                                                        unsigned int site) {
+  using A = typename Wide<T>::type;
+  constexpr int kSlots = 32 * S::kColumns;
+  const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
+  A map_a[S::kColumns], map_b[S::kColumns], state[S::kColumns];
+  Held<T>::part(whole.a, map_a);
+  Held<T>::part(whole.b, map_b);
+  Held<T>::part(begin, state);
+  if (sends) {
+#pragma unroll
+    for (int i = 0; i < S::kColumns; ++i) {
+      store_map<A>(a.maps, order * padded + block * kSlots + S::slot(lane, i),
+                   Map<A>{map_a[i], map_b[i]});
+    }
+  }
+  carry_in<A, S>(a, order, block, scratch, site, state);
+  if (sends && (order + 1) % kGroup == 0) {
+#pragma unroll
+    for (int i = 0; i < S::kColumns; ++i) {
+      store_base<A>(a.bases, (order + 1) / kGroup * padded + block * kSlots + S::slot(lane, i),
+                    map_a[i] * state[i] + map_b[i]);
+    }
+  }
+  return Held<T>::join(state);
+}
+
+template <typename T, bool kAdjacent, typename Offset>
 __global__ void __launch_bounds__(kWarps * 32, 2)
     columns_forward_kernel(const __grid_constant__ RecurrenceArgs a) {
+  using H = Held<T>;
+  using S = Steps<T, kAdjacent, Offset>;
   using A = typename Wide<T>::type;
-  constexpr int kSteps = kForwardSteps, kSlots = 32 * V;
-  __shared__ Map<A> maps[kWarps][kSlots];
-  __shared__ Map<A> before[kWarps * kSlots];
+  using P = typename H::P;
+  constexpr int kSteps = forward_steps(sizeof(T)), kColumns = H::kColumns;
+  __shared__ HeldMap<T> maps[kWarps][32];
+  __shared__ Map<A> before[kWarps * 32 * kColumns];
   __shared__ unsigned int taken;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int warps = blockDim.x >> 5;
-  int block = blockIdx.x;
-  int64_t chunk = 0, stop = a.chunks;
+  int64_t block = blockIdx.x, chunk = 0, stop = a.chunks;
   if (a.shared) {
     if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u) + 1u;
     __syncthreads();
     chunk = taken / a.column_blocks;
-    block = static_cast<int>(taken - chunk * a.column_blocks);
+    block = taken - static_cast<uint32_t>(chunk) * a.column_blocks;
     stop = chunk + 1;
   }
-  const int64_t column = (static_cast<int64_t>(block) * 32 + lane) * V;
-  const bool live = column < a.columns;
-  const int64_t base = live ? column_base(a, column) : 0;
-  A begin[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    begin[v] = live && a.initial != nullptr ? static_cast<const A*>(a.initial)[column + v] : A(0);
-  }
+  const S at(a, block, lane);
+  P begin = load_columns<T>(a.initial, at, a, 0, block, lane);
   for (; chunk < stop; ++chunk) {
     const int most = a.balanced ? a.balanced : kSteps;
     const int64_t first = (chunk * warps + warp) * most;
-    const Steps<T, Offset> at(base + first * a.inner, a.inner);
-    const int count = live ? steps_here(a.steps - first, most) : 0;
-    Pack<T, V> px[kSteps], pg[kSteps];
-    if (count == kSteps) {
+    const Offset offset = static_cast<Offset>(first) * at.stride;
+    const int count = steps_here(a.steps - first, most);
+    Pack<T, kColumns> px[kSteps], pg[kSteps];
+    if (count == kSteps && at.lives(0) && at.lives(kColumns - 1)) {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        px[i] = at.template read<V>(a.x, i);
-        pg[i] = at.template read<V>(a.gate, i);
+        px[i] = at.read(a.x, offset + i * at.stride);
+        pg[i] = at.read(a.gate, offset + i * at.stride);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        px[i] = all_of<T, V>(0.0f);
-        pg[i] = all_of<T, V>(INFINITY);
+        px[i] = S::all(0.0f);
+        pg[i] = S::all(INFINITY);
         if (i < count) {
-          px[i] = at.template read<V>(a.x, i);
-          pg[i] = at.template read<V>(a.gate, i);
+          px[i] = at.read_live(a.x, offset + i * at.stride, 0.0f);
+          pg[i] = at.read_live(a.gate, offset + i * at.stride, INFINITY);
         }
       }
     }
-    A f[kSteps][V], b[kSteps][V];
-    Map<A> own[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) own[v] = {A(1), A(0)};
+    P f[kSteps], b[kSteps];
+    HeldMap<T> own{H::value(1), H::value(0)};
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        A keep;
-        gates<T>(widen(pg[i].v[v]), &f[i][v], &keep);
-        b[i][v] = keep * widen(px[i].v[v]);
-        own[v] = then(own[v], Map<A>{f[i][v], b[i][v]});
-      }
+      P keep;
+      held_gates<T>(pg[i], &f[i], &keep);
+      b[i] = H::mul(keep, held<T>(px[i]));
+      own = then<T>(own, HeldMap<T>{f[i], b[i]});
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v) maps[warp][lane * V + v] = own[v];
+    maps[warp][lane] = own;
     __syncthreads();
-    Map<A> earlier[V];  // the block's warps before this one
+    HeldMap<T> earlier{H::value(1), H::value(0)};  // the block's warps before this one
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      earlier[v] = {A(1), A(0)};
-      for (int w = 0; w < warp; ++w) earlier[v] = then(earlier[v], maps[w][lane * V + v]);
+    for (int w = 0; w < kWarps - 1; ++w) {
+      if (w < warp) earlier = then<T>(earlier, maps[w][lane]);
     }
-    A state[V];
+    P state;
     if (a.shared) {
-      const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
-      const int64_t at = static_cast<int64_t>(block) * kSlots + lane * V;
-      const bool sends = warp == warps - 1 && chunk + 1 < a.chunks;
-      if (sends) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          store_map<A>(a.maps, chunk * padded + at + v, then(earlier[v], own[v]));
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) state[v] = begin[v];
-      carry_in<A, kSlots, V>(a, chunk, block, before, kSiteForward, state);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        state[v] = earlier[v].a * state[v] + earlier[v].b;
-        if (sends && (chunk + 1) % kGroup == 0) {
-          store_base<A>(a.bases, (chunk + 1) / kGroup * padded + at + v,
-                        own[v].a * state[v] + own[v].b);
-        }
-      }
+      state = exchange<T, S>(a, chunk, block, lane, warp == warps - 1 && chunk + 1 < a.chunks,
+                             then<T>(earlier, own), begin, before, kSiteForward);
     } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) state[v] = earlier[v].a * begin[v] + earlier[v].b;
+      state = begin;
       if (chunk + 1 < stop) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          for (int w = warp; w < warps; ++w) {
-            earlier[v] = then(earlier[v], maps[w][lane * V + v]);
-          }
-          begin[v] = earlier[v].a * begin[v] + earlier[v].b;
-        }
+        HeldMap<T> all = earlier;
+        for (int w = warp; w < warps; ++w) all = then<T>(all, maps[w][lane]);
+        begin = H::mad(all.a, begin, all.b);
         __syncthreads();
       }
     }
-    if (a.states != nullptr && live && first < a.steps && first % kStateBlock == 0) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        static_cast<A*>(a.states)[first / kStateBlock * a.columns + column + v] = state[v];
-      }
+    state = H::mad(earlier.a, state, earlier.b);
+    if (a.states != nullptr && first < a.steps && first % kStateBlock == 0) {
+      store_columns<T>(a.states, at, a, first / kStateBlock, block, lane, state);
     }
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      Pack<T, V> out;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        state[v] = f[i][v] * state[v] + b[i][v];
-        out.v[v] = narrow<T>(state[v]);
-      }
-      if (i < count) at.template write<V>(a.y, i, out);
+      state = H::mad(f[i], state, b[i]);
+      if (i < count) at.write(a.y, offset + i * at.stride, state);
     }
     const int64_t end = a.steps > 0 ? a.steps - 1 : 0;
-    if (live && first <= end && end < first + most) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) static_cast<A*>(a.last)[column + v] = state[v];
-    }
+    if (first <= end && end < first + most) store_columns<T>(a.last, at, a, 0, block, lane, state);
   }
 }
 
-template <typename T, int V, typename Offset>
+template <typename T, bool kAdjacent, typename Offset>
 __global__ void __launch_bounds__(kWarps * 32, 2)
     columns_backward_kernel(const __grid_constant__ RecurrenceArgs a) {
+  using H = Held<T>;
+  using S = Steps<T, kAdjacent, Offset>;
   using A = typename Wide<T>::type;
-  constexpr int kSteps = kBackwardSteps, kSlots = 32 * V;
-  __shared__ Map<A> forward[kWarps][kSlots];
-  __shared__ A backward[kWarps][kSlots];  // the flow's map: same factor, own offset
-  __shared__ Map<A> after[kWarps * kSlots];
+  using P = typename H::P;
+  constexpr int kSteps = kBackwardSteps, kColumns = H::kColumns;
+  __shared__ HeldMap<T> forward[kWarps][32];
+  __shared__ P backward[kWarps][32];  // the flow's map: same factor, own offset
+  __shared__ Map<A> after[kWarps * 32 * kColumns];
   __shared__ unsigned int taken;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int warps = blockDim.x >> 5;
-  int block = blockIdx.x;
-  int64_t order = 0, stop = a.chunks;  // chunks from the last to the first
+  int64_t block = blockIdx.x, order = 0, stop = a.chunks;  // chunks from the last to the first
   if (a.shared) {
     if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u) + 1u;
     __syncthreads();
     order = taken / a.column_blocks;
-    block = static_cast<int>(taken - order * a.column_blocks);
+    block = taken - static_cast<uint32_t>(order) * a.column_blocks;
     stop = order + 1;
   }
-  const int64_t column = (static_cast<int64_t>(block) * 32 + lane) * V;
-  const bool live = column < a.columns;
-  const int64_t base = live ? column_base(a, column) : 0;
-  A begin[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    begin[v] = live && a.dlast != nullptr ? static_cast<const A*>(a.dlast)[column + v] : A(0);
-  }
+  const S at(a, block, lane);
+  P begin = load_columns<T>(a.dlast, at, a, 0, block, lane);
   for (; order < stop; ++order) {
     const int64_t chunk = a.chunks - 1 - order;
     const int most = a.balanced ? a.balanced : kSteps;
     const int64_t first = (chunk * warps + warp) * most;
-    const Steps<T, Offset> at(base + first * a.inner, a.inner);
-    const int count = live ? steps_here(a.steps - first, most) : 0;
-    Pack<T, V> px[kSteps], pg[kSteps], pd[kSteps];
-    if (count == kSteps && a.dy != nullptr) {
+    const Offset offset = static_cast<Offset>(first) * at.stride;
+    const int count = steps_here(a.steps - first, most);
+    Pack<T, kColumns> px[kSteps], pg[kSteps], pd[kSteps];
+    if (count == kSteps && a.dy != nullptr && at.lives(0) && at.lives(kColumns - 1)) {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        px[i] = at.template read<V>(a.x, i);
-        pg[i] = at.template read<V>(a.gate, i);
-        pd[i] = at.template read<V>(a.dy, i);
+        px[i] = at.read(a.x, offset + i * at.stride);
+        pg[i] = at.read(a.gate, offset + i * at.stride);
+        pd[i] = at.read(a.dy, offset + i * at.stride);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        px[i] = pd[i] = all_of<T, V>(0.0f);
-        pg[i] = all_of<T, V>(INFINITY);
+        px[i] = pd[i] = S::all(0.0f);
+        pg[i] = S::all(INFINITY);
         if (i < count) {
-          px[i] = at.template read<V>(a.x, i);
-          pg[i] = at.template read<V>(a.gate, i);
-          if (a.dy != nullptr) pd[i] = at.template read<V>(a.dy, i);
+          px[i] = at.read_live(a.x, offset + i * at.stride, 0.0f);
+          pg[i] = at.read_live(a.gate, offset + i * at.stride, INFINITY);
+          if (a.dy != nullptr) pd[i] = at.read_live(a.dy, offset + i * at.stride, 0.0f);
         }
       }
     }
-    A saved[V];  // the state before the chunk
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      saved[v] = live && a.steps > 0
-                     ? static_cast<const A*>(a.states_in)[chunk * a.columns + column + v]
-                     : A(0);
-    }
-    A f[kSteps][V], keep[kSteps][V];
-    Map<A> own[V];
-    A flow[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      own[v] = {A(1), A(0)};
-      flow[v] = A(0);
-    }
+    // the state before the chunk
+    P state = a.steps > 0 ? load_columns<T>(a.states_in, at, a, chunk, block, lane) : H::value(0);
+    P f[kSteps], keep[kSteps];
+    HeldMap<T> own{H::value(1), H::value(0)};
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        gates<T>(widen(pg[i].v[v]), &f[i][v], &keep[i][v]);
-        own[v] = then(own[v], Map<A>{f[i][v], keep[i][v] * widen(px[i].v[v])});
-      }
+      held_gates<T>(pg[i], &f[i], &keep[i]);
+      own = then<T>(own, HeldMap<T>{f[i], H::mul(keep[i], held<T>(px[i]))});
     }
+    P flow = H::value(0);
 #pragma unroll
-    for (int i = kSteps - 1; i >= 0; --i) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) flow[v] = f[i][v] * (widen(pd[i].v[v]) + flow[v]);
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      forward[warp][lane * V + v] = own[v];
-      backward[warp][lane * V + v] = flow[v];
-    }
+    for (int i = kSteps - 1; i >= 0; --i) flow = H::mul(f[i], H::add(held<T>(pd[i]), flow));
+    forward[warp][lane] = own;
+    backward[warp][lane] = flow;
     __syncthreads();
-    Map<A> later[V];  // the block's warps after this one, walked backwards
+    HeldMap<T> later{H::value(1), H::value(0)};  // the block's warps after this one, backwards
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      for (int w = 0; w < warp; ++w) {
-        const Map<A> m = forward[w][lane * V + v];
-        saved[v] = m.a * saved[v] + m.b;
-      }
-      later[v] = {A(1), A(0)};
-      for (int w = warps - 1; w > warp; --w) {
-        later[v] = then(later[v], Map<A>{forward[w][lane * V + v].a, backward[w][lane * V + v]});
+    for (int w = 0; w < kWarps - 1; ++w) {
+      if (w < warp) state = H::mad(forward[w][lane].a, state, forward[w][lane].b);
+    }
+#pragma unroll
+    for (int w = kWarps - 1; w > 0; --w) {
+      if (w > warp && w < warps) {
+        later = then<T>(later, HeldMap<T>{forward[w][lane].a, backward[w][lane]});
       }
     }
-    A q[V];
+    P q;
     if (a.shared) {
-      const int64_t padded = static_cast<int64_t>(a.column_blocks) * kSlots;
-      const int64_t at = static_cast<int64_t>(block) * kSlots + lane * V;
-      const bool sends = warp == 0 && order + 1 < a.chunks;
-      if (sends) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          store_map<A>(a.maps, order * padded + at + v, then(later[v], Map<A>{own[v].a, flow[v]}));
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) q[v] = begin[v];
-      carry_in<A, kSlots, V>(a, order, block, after, kSiteBackward, q);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        q[v] = later[v].a * q[v] + later[v].b;
-        if (sends && (order + 1) % kGroup == 0) {
-          store_base<A>(a.bases, (order + 1) / kGroup * padded + at + v, own[v].a * q[v] + flow[v]);
-        }
-      }
+      q = exchange<T, S>(a, order, block, lane, warp == 0 && order + 1 < a.chunks,
+                         then<T>(later, HeldMap<T>{own.a, flow}), begin, after, kSiteBackward);
     } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) q[v] = later[v].a * begin[v] + later[v].b;
+      q = begin;
       if (order + 1 < stop) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          for (int w = warp; w >= 0; --w) {
-            later[v] = then(later[v], Map<A>{forward[w][lane * V + v].a, backward[w][lane * V + v]});
-          }
-          begin[v] = later[v].a * begin[v] + later[v].b;
+        HeldMap<T> all = later;
+        for (int w = warp; w >= 0; --w) {
+          all = then<T>(all, HeldMap<T>{forward[w][lane].a, backward[w][lane]});
         }
+        begin = H::mad(all.a, begin, all.b);
         __syncthreads();
       }
     }
-    A slope[kSteps][V];
+    q = H::mad(later.a, q, later.b);
+    P slope[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        // f (1 - f) (h_{t-1} - x), what the gate's gradient takes of the flow
-        const A x = widen(px[i].v[v]);
-        slope[i][v] = f[i][v] * keep[i][v] * (saved[v] - x);
-        saved[v] = f[i][v] * saved[v] + keep[i][v] * x;
-      }
+      // f (1 - f) (h_{t-1} - x), what the gate's gradient takes of the flow
+      const P x = held<T>(px[i]);
+      const P difference = H::mad(x, H::value(-1), state);
+      slope[i] = H::mul(H::mul(f[i], keep[i]), difference);
+      state = H::mad(f[i], state, H::mul(keep[i], x));
     }
 #pragma unroll
     for (int i = kSteps - 1; i >= 0; --i) {
-      Pack<T, V> dx, dg;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const A total = widen(pd[i].v[v]) + q[v];
-        dx.v[v] = narrow<T>(keep[i][v] * total);
-        dg.v[v] = narrow<T>(slope[i][v] * total);
-        q[v] = f[i][v] * total;
-      }
+      const P total = H::add(held<T>(pd[i]), q);
+      q = H::mul(f[i], total);
       if (i < count) {
-        if (a.dx != nullptr) at.template write<V>(a.dx, i, dx);
-        if (a.dgate != nullptr) at.template write<V>(a.dgate, i, dg);
+        if (a.dx != nullptr) at.write(a.dx, offset + i * at.stride, H::mul(keep[i], total));
+        if (a.dgate != nullptr) at.write(a.dgate, offset + i * at.stride, H::mul(slope[i], total));
       }
     }
-    if (a.dinitial != nullptr && live && first == 0) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) static_cast<A*>(a.dinitial)[column + v] = q[v];
+    if (a.dinitial != nullptr && first == 0) {
+      store_columns<T>(a.dinitial, at, a, 0, block, lane, q);
     }
   }
 }
@@ -698,7 +804,7 @@ __global__ void __launch_bounds__(kWarps * 32)
       const bool sends = warp == warps - 1 && lane == 31 && chunk + 1 < a.chunks;
       if (sends) store_map<A>(a.maps, chunk * a.column_blocks + column, then(lead, own));
       A carried[1] = {begin};
-      carry_in<A, 1, 1>(a, chunk, column, before, kSiteForward, carried);
+      carry_in<A, OneColumn>(a, chunk, column, before, kSiteForward, carried);
       state = carried[0];
       if (sends && (chunk + 1) % kGroup == 0) {
         const Map<A> all = then(lead, own);
@@ -787,7 +893,7 @@ __global__ void __launch_bounds__(kWarps * 32)
       const bool sends = warp == 0 && lane == 0 && order + 1 < a.chunks;
       if (sends) store_map<A>(a.maps, order * a.column_blocks + column, then(lead, back));
       A carried[1] = {begin};
-      carry_in<A, 1, 1>(a, order, column, after, kSiteBackward, carried);
+      carry_in<A, OneColumn>(a, order, column, after, kSiteBackward, carried);
       q = carried[0];
       if (sends && (order + 1) % kGroup == 0) {
         const Map<A> all = then(lead, back);
@@ -824,8 +930,8 @@ __global__ void __launch_bounds__(kWarps * 32)
 // ---- choice of kernel and layout of the workspace --------------------------------------
 
 struct RecurrencePlan {
-  bool along;          // step layout
-  int vector, warps;   // columns a lane, warps a block
+  bool along;  // step layout
+  int warps;   // warps a block
   int64_t chunks;
   int64_t column_blocks;
   int balanced;
@@ -833,25 +939,25 @@ struct RecurrencePlan {
   size_t maps = 0, bases = 0, ticket = 0, total = 0;
 };
 
-// Column blocks as wide as the widest vector allows; a pass over 16-bit columns of odd
-// extent takes narrower ones (`narrow_columns`), which the workspace covers too.
 RecurrencePlan plan_recurrence(int dtype, int64_t outer, int64_t steps, int64_t inner,
-                               bool backward, bool narrow_columns) {
+                               bool backward) {
   RecurrencePlan p{};
   const int64_t columns = outer * inner;
+  const int held = dtype == CND_F64 ? 1 : 2;  // columns a lane
   p.along = inner == 1 && steps > 1;
-  p.vector = !p.along && element_size(dtype) == 2 && inner % 2 == 0 && !narrow_columns ? 2 : 1;
-  const int64_t per_warp = p.along ? kAlongBlock : backward ? kBackwardSteps : kForwardSteps;
+  const int64_t per_warp = p.along    ? kAlongBlock
+                           : backward ? kBackwardSteps
+                                      : forward_steps(element_size(dtype));
   p.warps = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kWarps, (steps + per_warp - 1) / per_warp)));
   p.chunks = std::max<int64_t>(1, (steps + p.warps * per_warp - 1) / (p.warps * per_warp));
   // Up to 64 steps (one kept state), the warps share them evenly: 33 steps as 11 + 11 + 11.
   if (!p.along && steps <= kStateBlock) p.balanced = static_cast<int>((steps + p.warps - 1) / p.warps);
-  p.column_blocks = p.along ? columns : (columns + 32 * p.vector - 1) / (32 * p.vector);
+  p.column_blocks = p.along ? columns : (columns + 32 * held - 1) / (32 * held);
   // Blocks of eight warps, at most three on an SM: with fewer than 2 blocks an SM, sharing the
   // time axis fills the machine.
   p.shared = p.chunks > 1 && p.column_blocks < 2 * 148;
   if (p.shared) {
-    const int64_t padded = p.along ? columns : p.column_blocks * 32 * p.vector;
+    const int64_t padded = p.along ? columns : p.column_blocks * 32 * held;
     const int64_t groups = (p.chunks + kGroup - 1) / kGroup;
     const size_t wide = dtype == CND_F64 ? 8 : 4;
     const auto take = [&](size_t bytes) {
@@ -896,10 +1002,11 @@ unsigned recurrence_grid(const RecurrencePlan& p) {
   return static_cast<unsigned>(p.shared ? p.column_blocks * p.chunks : p.column_blocks);
 }
 
-// Whether packs of two 16-bit columns may be read and written at these addresses.
-bool pairs_aligned(std::initializer_list<const void*> pointers) {
+// Whether two neighbouring columns can be read and written at once.
+bool pairs_aligned(int dtype, int64_t inner, std::initializer_list<const void*> pointers) {
+  if (inner % 2 != 0) return false;
   for (const void* p : pointers) {
-    if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return false;
+    if (reinterpret_cast<uintptr_t>(p) % (2 * element_size(dtype)) != 0) return false;
   }
   return true;
 }
@@ -960,9 +1067,7 @@ size_t cnd_gated_recurrence_workspace_size(int32_t dtype, int64_t outer, int64_t
   }
   size_t bytes = 0;
   for (const bool backward : {false, true}) {
-    for (const bool narrow : {false, true}) {
-      bytes = std::max(bytes, plan_recurrence(dtype, outer, steps, inner, backward, narrow).total);
-    }
+    bytes = std::max(bytes, plan_recurrence(dtype, outer, steps, inner, backward).total);
   }
   return bytes;
 }
@@ -993,8 +1098,7 @@ int cnd_gated_recurrence_forward(int32_t dtype, int64_t outer, int64_t steps, in
   a.steps = steps;
   a.inner = inner;
   a.columns = columns;
-  const RecurrencePlan p = plan_recurrence(dtype, outer, steps, inner, false,
-                                           !pairs_aligned({x, gate, y}));
+  const RecurrencePlan p = plan_recurrence(dtype, outer, steps, inner, false);
   rc = bind_exchange("cnd_gated_recurrence_forward", p, workspace, workspace_bytes, &a, stream);
   if (rc != CND_OK) return rc;
   const unsigned grid = recurrence_grid(p);
@@ -1007,13 +1111,12 @@ int cnd_gated_recurrence_forward(int32_t dtype, int64_t outer, int64_t steps, in
       return;
     }
     const auto run = [&](auto kernel) { kernel<<<grid, p.warps * 32, 0, stream>>>(a); };
-    if constexpr (sizeof(T) == 2) {
-      if (p.vector == 2) {
-        return small ? run(columns_forward_kernel<T, 2, uint32_t>)
-                     : run(columns_forward_kernel<T, 2, int64_t>);
-      }
+    if (sizeof(T) < 8 && pairs_aligned(dtype, inner, {x, gate, y})) {
+      return small ? run(columns_forward_kernel<T, true, uint32_t>)
+                   : run(columns_forward_kernel<T, true, int64_t>);
     }
-    small ? run(columns_forward_kernel<T, 1, uint32_t>) : run(columns_forward_kernel<T, 1, int64_t>);
+    small ? run(columns_forward_kernel<T, false, uint32_t>)
+          : run(columns_forward_kernel<T, false, int64_t>);
   });
   count_launch();
   return launch_status("cnd_gated_recurrence_forward");
@@ -1053,8 +1156,7 @@ int cnd_gated_recurrence_backward(int32_t dtype, int64_t outer, int64_t steps, i
   a.steps = steps;
   a.inner = inner;
   a.columns = columns;
-  const RecurrencePlan p = plan_recurrence(dtype, outer, steps, inner, true,
-                                           !pairs_aligned({x, gate, dy, dx, dgate}));
+  const RecurrencePlan p = plan_recurrence(dtype, outer, steps, inner, true);
   rc = bind_exchange("cnd_gated_recurrence_backward", p, workspace, workspace_bytes, &a, stream);
   if (rc != CND_OK) return rc;
   const unsigned grid = recurrence_grid(p);
@@ -1067,14 +1169,12 @@ int cnd_gated_recurrence_backward(int32_t dtype, int64_t outer, int64_t steps, i
       return;
     }
     const auto run = [&](auto kernel) { kernel<<<grid, p.warps * 32, 0, stream>>>(a); };
-    if constexpr (sizeof(T) == 2) {
-      if (p.vector == 2) {
-        return small ? run(columns_backward_kernel<T, 2, uint32_t>)
-                     : run(columns_backward_kernel<T, 2, int64_t>);
-      }
+    if (sizeof(T) < 8 && pairs_aligned(dtype, inner, {x, gate, dy, dx, dgate})) {
+      return small ? run(columns_backward_kernel<T, true, uint32_t>)
+                   : run(columns_backward_kernel<T, true, int64_t>);
     }
-    small ? run(columns_backward_kernel<T, 1, uint32_t>)
-          : run(columns_backward_kernel<T, 1, int64_t>);
+    small ? run(columns_backward_kernel<T, false, uint32_t>)
+          : run(columns_backward_kernel<T, false, int64_t>);
   });
   count_launch();
   return launch_status("cnd_gated_recurrence_backward");
