@@ -90,28 +90,13 @@ struct PrepareArgs {
   void* dst;        // NULL: column sums only
   void* sums;       // [gridDim.y][width] partial column sums, or NULL
   int64_t rows, width, src_stride, pitch, plane;
-  int act, vectors;
+  int act;
 };
 
 constexpr int kPrepareColumns = 256;  // columns of a block: 32 lanes of 8
 
-// w *= act'(z), 8 values.
-template <typename T, typename A>
-__device__ __forceinline__ void times_slope(A (&w)[8], const T (&z)[8], int act) {
-#pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    if constexpr (sizeof(T) == 2) {
-      unpack(mul2(two(w[i], w[i + 1]), slope2(two(widen(z[i]), widen(z[i + 1])), act)), &w[i],
-             &w[i + 1]);
-    } else {
-      w[i] *= activation_slope<A>(widen(z[i]), act);
-      w[i + 1] *= activation_slope<A>(widen(z[i + 1]), act);
-    }
-  }
-}
-
-// Writes 8 columns of a row as an operand: rounded to 16 bits, split into three bfloat16
-// terms (float32), or as they are (float64).
+// Writes 8 columns of a row as an operand: split into three bfloat16 terms (float32), or as they
+// are (float64).
 template <typename T, typename A>
 __device__ __forceinline__ void store_operand(const PrepareArgs& a, int64_t row, int64_t col,
                                               const A (&w)[8]) {
@@ -120,7 +105,7 @@ __device__ __forceinline__ void store_operand(const PrepareArgs& a, int64_t row,
     for (int i = 0; i < 8; ++i) {
       if (col + i < a.width) static_cast<T*>(a.dst)[row * a.pitch + col + i] = w[i];
     }
-  } else if constexpr (sizeof(T) == 4) {
+  } else {
     // x = x0 + x1 + x2, each the nearest bfloat16 of what is left; an infinity or NaN is x0
     // alone
     Pack<__nv_bfloat16, 8> t[3];
@@ -141,20 +126,15 @@ __device__ __forceinline__ void store_operand(const PrepareArgs& a, int64_t row,
     for (int p = 0; p < 3; ++p) {
       *reinterpret_cast<Pack<__nv_bfloat16, 8>*>(dst + p * a.plane) = t[p];
     }
-  } else {
-    Pack<T, 8> t;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t.v[i] = narrow<T>(w[i]);
-    *reinterpret_cast<Pack<T, 8>*>(static_cast<T*>(a.dst) + row * a.pitch + col) = t;
   }
 }
 
 // T: source type. A block takes 256 columns and a range of rows, a warp one row of it at a
 // time, a lane 8 consecutive columns: 16-byte loads and stores where rows allow them.
-template <typename T>
-__global__ void __launch_bounds__(256, 2) prepare_kernel(const PrepareArgs a) {
+template <typename T, bool kVectors>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) prepare_kernel(const PrepareArgs a) {
   using A = typename Wide<T>::type;
-  constexpr int kBatch = sizeof(T) == 2 ? 4 : 2;
+  constexpr int kBatch = 2;
   constexpr int kLoad = sizeof(T) == 2 ? 8 : 16 / sizeof(T);
   __shared__ A part[8][kPrepareColumns];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -162,9 +142,10 @@ __global__ void __launch_bounds__(256, 2) prepare_kernel(const PrepareArgs a) {
   const int64_t first = a.rows * blockIdx.y / gridDim.y;
   const int64_t last = a.rows * (blockIdx.y + 1) / gridDim.y;
   A sum[8] = {};
+  Two sums[4] = {same(0.0f), same(0.0f), same(0.0f), same(0.0f)};
   if (col < a.width) {
-    // kBatch rows are loaded before the first is worked on: one row at a time had left the
-    // memory system at 3.8 TB/s.
+    // Two rows are loaded before the first is worked on, and four blocks fit an SM: 4.8 TB/s on
+    // 1M x 256 bf16; four rows in twice the registers reached 4.2.
     for (int64_t row0 = first + warp; row0 < last; row0 += 8 * kBatch) {
       alignas(16) T v[kBatch][8], z[kBatch][8];
 #pragma unroll
@@ -173,7 +154,7 @@ __global__ void __launch_bounds__(256, 2) prepare_kernel(const PrepareArgs a) {
         const bool live = row < last;
         const T* src = static_cast<const T*>(a.src) + row * a.src_stride + col;
         const T* pre = static_cast<const T*>(a.pre) + row * a.width + col;
-        if (a.vectors) {
+        if constexpr (kVectors) {
 #pragma unroll
           for (int i = 0; i < 8; i += kLoad) {
             if (live) {
@@ -200,22 +181,42 @@ __global__ void __launch_bounds__(256, 2) prepare_kernel(const PrepareArgs a) {
       for (int j = 0; j < kBatch; ++j) {
         const int64_t row = row0 + 8 * j;
         if (row < last) {
-          A w[8];
+          if constexpr (sizeof(T) == 2) {
+            Two w[4];
+            load_twos<T, 8>(v[j], w);
+            if (a.pre != nullptr) {
+              Two pre[4];
+              load_twos<T, 8>(z[j], pre);
+              if (a.act == CND_ACT_GELU) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = widen(v[j][i]);
-          if (a.pre != nullptr) {
-            if (a.act == CND_ACT_GELU) {
-              times_slope<T>(w, z[j], CND_ACT_GELU);
-            } else {
-              times_slope<T>(w, z[j], CND_ACT_SILU);
+                for (int i = 0; i < 4; ++i) w[i] = mul2(w[i], slope2(pre[i], CND_ACT_GELU));
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = mul2(w[i], slope2(pre[i], CND_ACT_SILU));
+              }
             }
-          }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) sum[i] += w[i];
-          if (a.dst != nullptr) store_operand<T>(a, row, col, w);
+            for (int i = 0; i < 4; ++i) sums[i] = add2(sums[i], w[i]);
+            if (a.dst != nullptr) store_twos<T, 8>(static_cast<T*>(a.dst) + row * a.pitch + col, w);
+          } else {
+            A w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = widen(v[j][i]);
+            if (a.pre != nullptr) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) w[i] *= activation_slope<A>(widen(z[j][i]), a.act);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += w[i];
+            if (a.dst != nullptr) store_operand<T>(a, row, col, w);
+          }
         }
       }
     }
+  }
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack(sums[i], &sum[2 * i], &sum[2 * i + 1]);
   }
   if (a.sums == nullptr) return;
 #pragma unroll
@@ -293,12 +294,14 @@ void prepare(int dtype, const void* src, const void* pre, int act, int64_t rows,
   a.pitch = pitch;
   a.plane = rows * pitch;
   a.act = act;
-  a.vectors = width % 8 == 0 && stride * element_size(dtype) % 16 == 0 && aligned16(src) &&
-              aligned16(pre);
+  const bool vectors = width % 8 == 0 && stride * element_size(dtype) % 16 == 0 &&
+                       aligned16(src) && aligned16(pre);
   const dim3 grid(static_cast<unsigned>((width + kPrepareColumns - 1) / kPrepareColumns),
                   static_cast<unsigned>(prepare_ranges(rows, width)));
   with_dtype(dtype, [&](auto zero) {
-    prepare_kernel<decltype(zero)><<<grid, 256, 0, stream>>>(a);
+    using T = decltype(zero);
+    vectors ? prepare_kernel<T, true><<<grid, 256, 0, stream>>>(a)
+            : prepare_kernel<T, false><<<grid, 256, 0, stream>>>(a);
   });
   count_launch();
 }
