@@ -230,25 +230,26 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) prepare_kernel(co
   static_cast<A*>(a.sums)[blockIdx.y * a.width + c] = total;
 }
 
-// Partial column sums [count][width] added in order: a block takes 32 columns, its warps
+// Partial column sums [count][width] added in order: a block takes 32 columns, its 32 warps
 // contiguous ranges of the partial rows, and the range sums are added in range order.
+constexpr int kJoinWarps = 32;
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kJoinWarps * 32)
     column_join_kernel(const void* sums, int count, int64_t width, T* out) {
   using A = typename Wide<T>::type;
-  __shared__ A part[8][32];
+  __shared__ A part[kJoinWarps][32];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   A sum = 0;
   if (c < width) {
     const A* p = static_cast<const A*>(sums) + c;
 #pragma unroll 8
-    for (int r = count * warp / 8; r < count * (warp + 1) / 8; ++r) sum += p[r * width];
+    for (int r = count * warp / kJoinWarps; r < count * (warp + 1) / kJoinWarps; ++r) sum += p[r * width];
   }
   part[warp][lane] = sum;
   __syncthreads();
   if (warp != 0 || c >= width) return;
-  for (int w = 1; w < 8; ++w) sum += part[w][lane];
+  for (int w = 1; w < kJoinWarps; ++w) sum += part[w][lane];
   out[c] = narrow<T>(sum);
 }
 
@@ -549,7 +550,7 @@ int cnd_linear_backward(const cnd_linear* problem, const void* dy, const void* p
   if (want_b) {
     with_dtype(q.dtype, [&](auto zero) {
       using T = decltype(zero);
-      column_join_kernel<T><<<static_cast<unsigned>((out + 31) / 32), 256, 0, stream>>>(
+      column_join_kernel<T><<<static_cast<unsigned>((out + 31) / 32), kJoinWarps * 32, 0, stream>>>(
           base + l.sums, prepare_ranges(rows, out), out, static_cast<T*>(dbias));
     });
     count_launch();

@@ -133,19 +133,40 @@ __device__ __forceinline__ void stage_row(uint8_t* tile, int row, int half, cons
   }
 }
 
-// Copies a staging tile to rows of a matrix that TMA cannot address, a warp per row.
-template <typename Out>
-__device__ __forceinline__ void copy_unit(const uint8_t* tile, Out* d, int64_t row0, int64_t col0,
+// Copies between a staging tile and rows of a matrix that TMA cannot address, a warp per row
+// and eight rows in flight: neighbouring lanes hold neighbouring columns.
+template <bool kStore, typename Out>
+__device__ __forceinline__ void copy_unit(uint8_t* tile, Out* d, int64_t row0, int64_t col0,
                                           int64_t m, int64_t n, int warp, int lane) {
-  constexpr int kColumns = 128 / sizeof(Out);
-  for (int r = warp; r < kBM; r += 4) {
-    if (row0 + r >= m) break;
+  constexpr int kColumns = 128 / sizeof(Out), kEach = kColumns / 32;
+  for (int r0 = warp; r0 < kBM && row0 + r0 < m; r0 += 32) {
+    Out v[8][kEach];
 #pragma unroll
-    for (int c = lane; c < kColumns; c += 32) {
-      if (col0 + c < n) {
-        const int byte = c * static_cast<int>(sizeof(Out));
-        d[(row0 + r) * n + col0 + c] =
-            *reinterpret_cast<const Out*>(tile + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int r = r0 + 4 * j, c = e * 32 + lane, byte = c * static_cast<int>(sizeof(Out));
+        Out* at = reinterpret_cast<Out*>(tile + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
+        const bool inside = row0 + r < m && col0 + c < n;
+        if constexpr (kStore) {
+          v[j][e] = *at;
+        } else {
+          v[j][e] = inside ? d[(row0 + r) * n + col0 + c] : narrow<Out>(0.0f);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int r = r0 + 4 * j, c = e * 32 + lane, byte = c * static_cast<int>(sizeof(Out));
+        Out* at = reinterpret_cast<Out*>(tile + r * 128 + (((byte >> 4) ^ (r & 7)) << 4) + (byte & 15));
+        const bool inside = row0 + r < m && col0 + c < n;
+        if constexpr (kStore) {
+          if (inside) d[(row0 + r) * n + col0 + c] = v[j][e];
+        } else {
+          *at = v[j][e];
+        }
       }
     }
   }
@@ -162,16 +183,19 @@ struct Residual {
 #pragma unroll
     for (int c = 0; c < 32 / kPer; ++c) {
       q[c] = Pack<Out, kPer>{};
-      if (a.vector_residual) {
-        if (row < a.m && col + c * kPer < a.n) {
-          q[c] = *reinterpret_cast<const Pack<Out, kPer>*>(p + c * kPer);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          if (row < a.m && col + c * kPer + i < a.n) q[c].v[i] = p[c * kPer + i];
-        }
+      if (row < a.m && col + c * kPer < a.n) {
+        q[c] = *reinterpret_cast<const Pack<Out, kPer>*>(p + c * kPer);
       }
+    }
+  }
+
+  // From a staging tile that copy_unit filled.
+  __device__ __forceinline__ void take(const uint8_t* tile, int row, int half) {
+    constexpr int kChunks = 32 / kPer;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      q[c] = *reinterpret_cast<const Pack<Out, kPer>*>(
+          tile + row * 128 + (((half * kChunks + c) ^ (row & 7)) * 16));
     }
   }
 
@@ -427,7 +451,8 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
       }
       dev::named_barrier(1, 32 * kEpilogueWarps);
       Residual<Out> residual;
-      if (kParts == 1 && a.residual != nullptr) residual.load(a, row0 + row, col0);
+      const bool direct = a.residual != nullptr && a.vector_residual;
+      if (kParts == 1 && direct) residual.load(a, row0 + row, col0);
 
       float sums[kParts == 3 ? kHalves : 1][32];
       if constexpr (kParts == 3) {
@@ -502,7 +527,7 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
         } else {
           uint32_t raw[32];
           dev::tmem_load32(acc + h * 32, raw);
-          if (h > 0 && a.residual != nullptr) residual.load(a, row0 + row, col0 + h * 32);
+          if (h > 0 && direct) residual.load(a, row0 + row, col0 + h * 32);
           dev::tmem_load_wait();
           if (h + 1 == kHalves) free_set(acc_empty, release, set);
 #pragma unroll
@@ -534,7 +559,7 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
                 dev::bulk_wait_group_read<0>();
               }
             } else {
-              copy_unit<Out>(pre_tile, static_cast<Out*>(a.pre), row0, unit_col, a.m, a.n, quarter,
+              copy_unit<true, Out>(pre_tile, static_cast<Out*>(a.pre), row0, unit_col, a.m, a.n, quarter,
                              lane);
             }
             dev::named_barrier(2 + group, kGroupThreads);
@@ -558,7 +583,17 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
           apply(CND_ACT_SILU);
         }
         if (a.residual != nullptr) {
-          if (kParts == 3) residual.load(a, row0 + row, col0 + h * 32);
+          if (!a.vector_residual) {
+            // rows that are not 16-byte aligned come through the staging tile
+            if (h % kHalvesPerUnit == 0) {
+              copy_unit<false, Out>(tile, const_cast<Out*>(static_cast<const Out*>(a.residual)), row0,
+                                    unit_col, a.m, a.n, quarter, lane);
+              dev::named_barrier(2 + group, kGroupThreads);
+            }
+            residual.take(tile, row, h % kHalvesPerUnit);
+          } else if (kParts == 3) {
+            residual.load(a, row0 + row, col0 + h * 32);
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = add2(v[i], residual.pair(i));
         }
@@ -580,9 +615,9 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
             }
             if (leader) dev::bulk_commit_group();
           } else {
-            copy_unit<Out>(tile, static_cast<Out*>(a.d), row0, unit_col, a.m, a.n, quarter, lane);
+            copy_unit<true, Out>(tile, static_cast<Out*>(a.d), row0, unit_col, a.m, a.n, quarter, lane);
             if (a.pre != nullptr && a.buffers > 1) {
-              copy_unit<Out>(pre_tile, static_cast<Out*>(a.pre), row0, unit_col, a.m, a.n, quarter,
+              copy_unit<true, Out>(pre_tile, static_cast<Out*>(a.pre), row0, unit_col, a.m, a.n, quarter,
                              lane);
             }
           }
@@ -610,25 +645,51 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
   }
 }
 
-// Adds the partial tiles of a split product in split order and applies the epilogue.
-template <typename Out>
+// Adds the partial tiles of a split product and applies the epilogue. A thread takes four
+// columns and one of kRanges contiguous ranges of the splits, in split order; the ranges are
+// added in order. (148 splits of 256 x 64: 14 us in one range.)
+template <typename Out, int kRanges>
 __global__ void __launch_bounds__(256)
     join_kernel(const float* partials, int splits, int64_t split_stride, int64_t pitch, int64_t m,
                 int64_t n, const void* bias, const void* residual, void* d, void* pre, int act) {
+  constexpr int kQuads = 256 / kRanges;
+  __shared__ float4 part[kRanges][kQuads];
   const int64_t quads = pitch / 4, count = m * quads;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += step) {
+  const int range = threadIdx.x / kQuads, at = threadIdx.x % kQuads;
+  const int first = splits * range / kRanges, last = splits * (range + 1) / kRanges;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kQuads; base < count;
+       base += static_cast<int64_t>(gridDim.x) * kQuads) {
+    const int64_t i = base + at;
     const int64_t row = i / quads, col = i % quads * 4;
-    const float* p = partials + row * pitch + col;
-    float4 sum = *reinterpret_cast<const float4*>(p);
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (i < count) {
+      const float* p = partials + row * pitch + col;
 #pragma unroll 4
-    for (int s = 1; s < splits; ++s) {
-      const float4 v = *reinterpret_cast<const float4*>(p + s * split_stride);
-      sum.x += v.x;
-      sum.y += v.y;
-      sum.z += v.z;
-      sum.w += v.w;
+      for (int s = first; s < last; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(p + s * split_stride);
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+      }
     }
+    if constexpr (kRanges > 1) {
+      part[range][at] = sum;
+      __syncthreads();
+      if (range == 0) {
+#pragma unroll
+        for (int r = 1; r < kRanges; ++r) {
+          const float4 v = part[r][at];
+          sum.x += v.x;
+          sum.y += v.y;
+          sum.z += v.z;
+          sum.w += v.w;
+        }
+      }
+      __syncthreads();
+      if (range != 0) continue;
+    }
+    if (i >= count) continue;
     const float v4[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -698,8 +759,9 @@ template <typename Out>
 Kernel pick(const ProductPlan& plan, int parts) {
   if constexpr (sizeof(Out) == 4) {
     if (parts == 3) {
-      return plan.pair == 2 ? product_tc_kernel<2, 128, 3, 2, Out>
-                            : product_tc_kernel<1, 128, 3, 2, Out>;
+      return plan.pair == 2   ? product_tc_kernel<2, 128, 3, 2, Out>
+             : plan.bn == 128 ? product_tc_kernel<1, 128, 3, 2, Out>
+                              : product_tc_kernel<1, 64, 3, 1, Out>;
     }
   }
   if (plan.pair == 2) {
@@ -726,7 +788,7 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts) {
   };
   static constexpr Cut kCuts[] = {
       {1, 2, 256, 8.5, 0.32, 5.5}, {1, 1, 128, 5.0, 0.27, 3.0}, {1, 1, 64, 4.3, 0.25, 1.9},
-      {3, 2, 128, 8.0, 0.72, 4.0}, {3, 1, 128, 5.0, 0.77, 3.0},
+      {3, 2, 128, 8.0, 0.52, 4.0}, {3, 1, 128, 5.0, 0.62, 3.0}, {3, 1, 64, 4.3, 0.47, 2.0},
   };
   const int64_t sms = 148, blocks = (k + block_depth(parts) - 1) / block_depth(parts);
   ProductPlan best{1, 64, 1, 1};
@@ -873,8 +935,10 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
   count_launch();
   if (split) {
     const int64_t quads = p.m * (pitch / 4);
-    const unsigned grid = static_cast<unsigned>(
-        std::min<int64_t>((quads + 255) / 256, static_cast<int64_t>(sm_count()) * 8));
+    const bool many = plan.splits >= 16;
+    const int per_block = many ? 32 : 256;
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(
+        (quads + per_block - 1) / per_block, static_cast<int64_t>(sm_count()) * 8));
     const int64_t stride = round_up(p.m, bm) * pitch;
     const float* partials = static_cast<const float*>(workspace);
     const auto join = [&](auto* kernel_join) {
@@ -882,11 +946,11 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
                                             p.residual, p.d, p.pre, p.act);
     };
     if (p.dtype == CND_F32) {
-      join(join_kernel<float>);
+      many ? join(join_kernel<float, 8>) : join(join_kernel<float, 1>);
     } else if (p.dtype == CND_BF16) {
-      join(join_kernel<__nv_bfloat16>);
+      many ? join(join_kernel<__nv_bfloat16, 8>) : join(join_kernel<__nv_bfloat16, 1>);
     } else {
-      join(join_kernel<__half>);
+      many ? join(join_kernel<__half, 8>) : join(join_kernel<__half, 1>);
     }
     count_launch();
   }
