@@ -91,9 +91,10 @@ struct PrepareArgs {
   void* sums;       // [gridDim.y][width] partial column sums, or NULL
   int64_t rows, width, src_stride, pitch, plane;
   int act;
+  int lanes;  // lanes of a row (8 columns each): a power of two, all 32 from 256 columns on
 };
 
-constexpr int kPrepareColumns = 256;  // columns of a block: 32 lanes of 8
+constexpr int kPrepareColumns = 256;  // most columns of a block: 32 lanes of 8
 
 // Writes 8 columns of a row as an operand: split into three bfloat16 terms (float32), or as they
 // are (float64).
@@ -129,15 +130,17 @@ __device__ __forceinline__ void store_operand(const PrepareArgs& a, int64_t row,
   }
 }
 
-// T: source type. A block takes 256 columns and a range of rows, a warp one row of it at a
-// time, a lane 8 consecutive columns: 16-byte loads and stores where rows allow them.
+// T: source type. A block takes up to 256 columns and a range of rows, a lane 8 consecutive
+// columns of a row: 16-byte loads and stores where rows allow them. A warp takes one row at a
+// time, or several narrow ones.
 template <typename T, bool kVectors>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) prepare_kernel(const PrepareArgs a) {
   using A = typename Wide<T>::type;
   constexpr int kBatch = 2;
   constexpr int kLoad = sizeof(T) == 2 ? 8 : 16 / sizeof(T);
   __shared__ A part[8][kPrepareColumns];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % a.lanes;
+  const int rows = 256 / a.lanes, row_of = threadIdx.x / a.lanes;  // rows of the block at once
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kPrepareColumns + lane * 8;
   const int64_t first = a.rows * blockIdx.y / gridDim.y;
   const int64_t last = a.rows * (blockIdx.y + 1) / gridDim.y;
@@ -146,11 +149,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) prepare_kernel(co
   if (col < a.width) {
     // Two rows are loaded before the first is worked on, and four blocks fit an SM: 4.8 TB/s on
     // 1M x 256 bf16; four rows in twice the registers reached 4.2.
-    for (int64_t row0 = first + warp; row0 < last; row0 += 8 * kBatch) {
+    for (int64_t row0 = first + row_of; row0 < last; row0 += rows * kBatch) {
       alignas(16) T v[kBatch][8], z[kBatch][8];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        const int64_t row = row0 + 8 * j;
+        const int64_t row = row0 + rows * j;
         const bool live = row < last;
         const T* src = static_cast<const T*>(a.src) + row * a.src_stride + col;
         const T* pre = static_cast<const T*>(a.pre) + row * a.width + col;
@@ -179,7 +182,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) prepare_kernel(co
       }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        const int64_t row = row0 + 8 * j;
+        const int64_t row = row0 + rows * j;
         if (row < last) {
           if constexpr (sizeof(T) == 2) {
             Two w[4];
@@ -220,13 +223,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) prepare_kernel(co
   }
   if (a.sums == nullptr) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) part[warp][lane * 8 + i] = sum[i];
+  for (int i = 0; i < 8; ++i) part[warp][threadIdx.x % 32 * 8 + i] = sum[i];
   __syncthreads();
   const int64_t c = static_cast<int64_t>(blockIdx.x) * kPrepareColumns + threadIdx.x;
-  if (c >= a.width) return;
+  if (c >= a.width || static_cast<int>(threadIdx.x) >= a.lanes * 8) return;
   A total = 0;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) total += part[w][threadIdx.x];
+  for (int w = 0; w < 8; ++w) {
+    for (int r = 0; r < 32 / a.lanes; ++r) total += part[w][r * a.lanes * 8 + threadIdx.x];
+  }
   static_cast<A*>(a.sums)[blockIdx.y * a.width + c] = total;
 }
 
@@ -297,6 +301,8 @@ void prepare(int dtype, const void* src, const void* pre, int act, int64_t rows,
   a.act = act;
   const bool vectors = width % 8 == 0 && stride * element_size(dtype) % 16 == 0 &&
                        aligned16(src) && aligned16(pre);
+  a.lanes = 1;
+  while (a.lanes < 32 && a.lanes * 8 < width) a.lanes *= 2;
   const dim3 grid(static_cast<unsigned>((width + kPrepareColumns - 1) / kPrepareColumns),
                   static_cast<unsigned>(prepare_ranges(rows, width)));
   with_dtype(dtype, [&](auto zero) {

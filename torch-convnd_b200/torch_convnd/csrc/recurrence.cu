@@ -510,8 +510,9 @@ __device__ __forceinline__ typename Held<T>::P exchange(const RecurrenceArgs& a,
   return Held<T>::join(state);
 }
 
+// Blocks an SM: what two columns of forward_steps() cost in registers.
 template <typename T, bool kAdjacent, typename Offset>
-__global__ void __launch_bounds__(kWarps * 32, 2)
+__global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 4 ? 4 : 2)
     columns_forward_kernel(const __grid_constant__ RecurrenceArgs a) {
   using H = Held<T>;
   using S = Steps<T, kAdjacent, Offset>;
@@ -539,11 +540,20 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     const Offset offset = static_cast<Offset>(first) * at.stride;
     const int count = steps_here(a.steps - first, most);
     Pack<T, kColumns> px[kSteps], pg[kSteps];
-    if (count == kSteps && at.lives(0) && at.lives(kColumns - 1)) {
+    if (count > 0 && at.lives(0) && at.lives(kColumns - 1)) {
+      // steps past the end read the last one again: no branches between the loads
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        px[i] = at.read(a.x, offset + i * at.stride);
-        pg[i] = at.read(a.gate, offset + i * at.stride);
+        const Offset ahead = offset + min(i, count - 1) * at.stride;
+        px[i] = at.read(a.x, ahead);
+        pg[i] = at.read(a.gate, ahead);
+      }
+      if (count < kSteps) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          px[i] = i < count ? px[i] : S::all(0.0f);
+          pg[i] = i < count ? pg[i] : S::all(INFINITY);
+        }
       }
     } else {
 #pragma unroll
@@ -630,12 +640,21 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     const Offset offset = static_cast<Offset>(first) * at.stride;
     const int count = steps_here(a.steps - first, most);
     Pack<T, kColumns> px[kSteps], pg[kSteps], pd[kSteps];
-    if (count == kSteps && a.dy != nullptr && at.lives(0) && at.lives(kColumns - 1)) {
+    if (count > 0 && a.dy != nullptr && at.lives(0) && at.lives(kColumns - 1)) {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        px[i] = at.read(a.x, offset + i * at.stride);
-        pg[i] = at.read(a.gate, offset + i * at.stride);
-        pd[i] = at.read(a.dy, offset + i * at.stride);
+        const Offset ahead = offset + min(i, count - 1) * at.stride;
+        px[i] = at.read(a.x, ahead);
+        pg[i] = at.read(a.gate, ahead);
+        pd[i] = at.read(a.dy, ahead);
+      }
+      if (count < kSteps) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          px[i] = i < count ? px[i] : S::all(0.0f);
+          pg[i] = i < count ? pg[i] : S::all(INFINITY);
+          pd[i] = i < count ? pd[i] : S::all(0.0f);
+        }
       }
     } else {
 #pragma unroll
