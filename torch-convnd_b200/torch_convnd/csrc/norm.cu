@@ -55,6 +55,7 @@ struct NormArgs {
   double eps;
   int param_f32;
   int want_dx, want_params;
+  int shift;  // rows shifted against 16-byte boundaries (ring and tile kernels)
 };
 
 // Sum over the G threads of a row's group; every thread gets it. G <= 32: lanes of one
@@ -118,19 +119,6 @@ __device__ __forceinline__ void load_params(const void* p, bool is_f32, int64_t 
 template <int G>
 constexpr int block_size() {
   return G > 32 ? G : 256;
-}
-
-// The same as pairs.
-template <typename T, int V, int NV, int G>
-__device__ __forceinline__ void load_param_pairs(const void* p, bool is_f32, int64_t width,
-                                                 int lane, float absent, Two (&v)[NV][V / 2]) {
-  float f[NV][V];
-  load_params<T, V, NV, G>(p, is_f32, width, lane, absent, f);
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) v[k][i] = two(f[k][2 * i], f[k][2 * i + 1]);
-  }
 }
 
 __device__ __forceinline__ float both(Two v) {
@@ -416,7 +404,102 @@ __global__ void __launch_bounds__(block_size<G>())
   }
 }
 
-// ---- long aligned rows: a ring of rows in shared memory -----------------------------------
+// ---- rows in vectors from shared memory ---------------------------------------------------
+//
+// Rows of any width and 16-byte vectors: row r of dense rows starts at element r * width,
+// off a 16-byte boundary by (r * width) % V elements. A thread whose rows are all congruent
+// modulo V (8 for 16 bits, 4 for float32) meets one such shift, so it can read aligned
+// vectors with columns, parameters and column sums fixed in registers as if its rows began
+// `shift` elements earlier; the first and the last vector of a row are masked. (Single
+// elements took 171 + 217 us for 65536 x 1001 bf16.)
+
+// A thread's vector: columns c ... c + V - 1 of which [lo, hi) exist. Without shifts (kShift)
+// a vector exists or does not.
+template <int V, bool kShift>
+struct Span {
+  int c, lo, hi;
+  bool exists;
+  __device__ __forceinline__ Span(int vector, int shift, int width) {
+    c = vector * V - (kShift ? shift : 0);
+    lo = kShift && c < 0 ? -c : 0;
+    hi = kShift && width - c < V ? width - c : V;
+    exists = kShift ? lo < hi : c < width;
+  }
+  __device__ __forceinline__ bool whole() const { return !kShift || (lo == 0 && hi == V); }
+  __device__ __forceinline__ bool any() const { return exists; }
+  // Whether column c + i exists (of a span that may not).
+  __device__ __forceinline__ bool has(int i) const {
+    return kShift ? i >= lo && i < hi : exists;
+  }
+};
+
+template <typename T, int V, bool kShift>
+__device__ __forceinline__ void store_span(T* row, const Span<V, kShift>& s, const Two (&v)[V / 2]) {
+  if (s.whole()) {
+    store_twos<T, V>(row + s.c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      float lo, hi;
+      unpack(v[i / 2], &lo, &hi);
+      if (s.has(i)) row[s.c + i] = narrow<T>(lo);
+      if (s.has(i + 1)) row[s.c + i + 1] = narrow<T>(hi);
+    }
+  }
+}
+
+// Values outside a span become `value`.
+template <int V, bool kShift>
+__device__ __forceinline__ void fill_outside(const Span<V, kShift>& s, float value, Two (&v)[V / 2]) {
+#pragma unroll
+  for (int i = 0; i < V; i += 2) {
+    float lo, hi;
+    unpack(v[i / 2], &lo, &hi);
+    v[i / 2] = two(s.has(i) ? lo : value, s.has(i + 1) ? hi : value);
+  }
+}
+
+template <typename T, int V, bool kShift>
+__device__ __forceinline__ void load_span_params(const void* p, bool is_f32,
+                                                 const Span<V, kShift>& s,
+                                                 float absent, Two (&v)[V / 2]) {
+  float f[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    f[i] = p != nullptr && s.has(i) ? load_param<T>(p, is_f32, s.c + i) : absent;
+  }
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) v[i] = two(f[2 * i], f[2 * i + 1]);
+}
+
+// Elements between the 16-byte boundary before a row and the row.
+template <int V>
+__device__ __forceinline__ int row_shift(int64_t row, int64_t stride) {
+  return static_cast<int>(row % V * (stride % V) % V);
+}
+
+// Adds a span's column sums to `to` ([2][width]), or starts them.
+template <int V, bool kShift>
+__device__ __forceinline__ void add_span(const Span<V, kShift>& s, const Two (&dw)[V / 2],
+                                         const Two (&db)[V / 2], float* to, int width, bool first) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float w2[2], b2[2];
+    unpack(dw[i / 2], &w2[0], &w2[1]);
+    unpack(db[i / 2], &b2[0], &b2[1]);
+    if (s.has(i)) {
+      const int c = s.c + i;
+      to[c] = first ? w2[i % 2] : to[c] + w2[i % 2];
+      to[width + c] = first ? b2[i % 2] : to[width + c] + b2[i % 2];
+    }
+  }
+}
+
+// Blocks an SM of the ring kernels: 768 threads of 80 registers, 512 where the masks of shifted
+// rows take more.
+constexpr int ring_blocks_of(int threads, bool shift) {
+  return threads >= 512 ? 1 : (shift ? 512 : 768) / threads;
+}
 
 // A block of G threads walks rows that bulk copies bring into a ring of stages ahead of it (x,
 // and dy behind it in the backward), so the loads in flight depend neither on registers
@@ -429,14 +512,14 @@ __global__ void __launch_bounds__(block_size<G>())
 // block's warps share, with one barrier a tile.
 struct Ring {
   int stages, tile;  // stages; rows of a stage
-  uint32_t row_bytes, stage_bytes;
+  uint32_t stage_bytes;  // the backward's second half holds dy
   unsigned int* error;
   uint64_t timeout_ns;
 };
 
 constexpr uint32_t kSiteRing = 0x701;
 
-template <int G, bool kBackward>
+template <bool kBackward, bool kShift>
 struct RowRing {
   const NormArgs& a;
   const Ring& ring;
@@ -447,18 +530,53 @@ struct RowRing {
   uint32_t phase = 0;
   bool dead = false;
 
+  // One operand's part of a stage: the 16-byte blocks that hold rows next ... next + count - 1
+  // (they lie back to back where a stage holds several), but none past the tensor's end: what
+  // the last rows have beyond the last whole block is stored element by element. Returns
+  // the bytes that the copy will bring.
+  __device__ __forceinline__ uint32_t bring(uint8_t* dst, const void* base, int64_t stride, int es,
+                                            int count, bool copy) {
+    const int64_t begin = next * stride * es, end = begin + ((count - 1) * stride + a.width) * es;
+    const int64_t first = begin & ~int64_t{15};
+    const int64_t limit = ((a.rows - 1) * stride + a.width) * es;
+    int64_t last = (end + 15) & ~int64_t{15};
+    if (last > limit) last = limit & ~int64_t{15};
+    if (last < first) last = first;
+    const char* src = static_cast<const char*>(base);
+    if (!copy) {
+      for (int64_t at = last; at < end; at += 2) {
+        *reinterpret_cast<uint16_t*>(dst + (at - first)) = *reinterpret_cast<const uint16_t*>(src + at);
+      }
+    } else if (last > first) {
+      dev::bulk_load(dst, src + first, static_cast<uint32_t>(last - first), &full[fill]);
+    }
+    return static_cast<uint32_t>(last - first);
+  }
+
   __device__ __forceinline__ void ask(int es) {
     // thread 0: rows `next` ... into stage `fill`
     if (next >= a.rows || dead) return;
     const int64_t left = a.rows - next;
-    const uint32_t bytes = ring.row_bytes * static_cast<uint32_t>(left < ring.tile ? left : ring.tile);
-    dev::mbar_arrive_expect_tx(&full[fill], kBackward ? 2 * bytes : bytes);
+    const int count = left < ring.tile ? static_cast<int>(left) : ring.tile;
     uint8_t* dst = data + fill * ring.stage_bytes;
-    dev::bulk_load(dst, static_cast<const char*>(a.x) + next * a.x_stride * es, bytes, &full[fill]);
-    if (kBackward) {
-      dev::bulk_load(dst + ring.stage_bytes / 2,
-                     static_cast<const char*>(a.dy) + next * a.dy_stride * es, bytes, &full[fill]);
+    uint8_t* second = dst + ring.stage_bytes / 2;
+    if constexpr (!kShift) {
+      const uint32_t whole = static_cast<uint32_t>(count) * static_cast<uint32_t>(a.width) * es;
+      dev::mbar_arrive_expect_tx(&full[fill], kBackward ? 2 * whole : whole);
+      dev::bulk_load(dst, static_cast<const char*>(a.x) + next * a.x_stride * es, whole, &full[fill]);
+      if (kBackward) {
+        dev::bulk_load(second, static_cast<const char*>(a.dy) + next * a.dy_stride * es, whole,
+                       &full[fill]);
+      }
+      next += static_cast<int64_t>(gridDim.x) * ring.tile;
+      if (++fill == ring.stages) fill = 0;
+      return;
     }
+    uint32_t bytes = bring(dst, a.x, a.x_stride, es, count, false);
+    if (kBackward) bytes += bring(second, a.dy, a.dy_stride, es, count, false);
+    dev::mbar_arrive_expect_tx(&full[fill], bytes);
+    bring(dst, a.x, a.x_stride, es, count, true);
+    if (kBackward) bring(second, a.dy, a.dy_stride, es, count, true);
     next += static_cast<int64_t>(gridDim.x) * ring.tile;
     if (++fill == ring.stages) fill = 0;
   }
@@ -480,8 +598,8 @@ struct RowRing {
   }
 };
 
-template <typename T, int V, int NV, int G>
-__global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
+template <typename T, int V, int NV, int G, bool kShift>
+__global__ void __launch_bounds__(G, ring_blocks_of(G, kShift))
     norm_forward_ring_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Ring ring_args) {
   extern __shared__ __align__(128) uint8_t shared[];
   __shared__ float scratch[1][32];
@@ -493,22 +611,30 @@ __global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
     dev::fence_barrier_init();
   }
   __syncthreads();
-  RowRing<G, false> ring{a, ring_args, shared, full, blockIdx.x};
+  RowRing<false, kShift> ring{a, ring_args, shared, full, blockIdx.x};
   if (lane == 0) {
     for (int s = 0; s < ring_args.stages; ++s) ring.ask(sizeof(T));
   }
   using M = RowMath<T, V, NV, G>;
   Two w[NV][V / 2], b[NV][V / 2];
-  load_param_pairs<T, V, NV, G>(a.weight, a.param_f32, a.width, lane, 1.0f, w);
-  load_param_pairs<T, V, NV, G>(a.bias, a.param_f32, a.width, lane, 0.0f, b);
+  const int width = static_cast<int>(a.width);
+  const int shift = row_shift<V>(blockIdx.x, a.x_stride);  // the same for all the block's rows
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const Span<V, kShift> s(k * G + lane, shift, width);
+    load_span_params<T>(a.weight, a.param_f32, s, 1.0f, w[k]);
+    load_span_params<T>(a.bias, a.param_f32, s, 0.0f, b[k]);
+  }
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* data = reinterpret_cast<const T*>(ring.wait());
     Two x[NV][V / 2];
     float sum[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if ((k * G + lane) * V < a.width) {
+      const Span<V, kShift> s(k * G + lane, shift, width);
+      if (s.any()) {
         load_twos<T, V>(data + (k * G + lane) * V, x[k]);
+        if (!s.whole()) fill_outside(s, 0.0f, x[k]);
         sum[0] += M::sum(x[k]);
       }
     }
@@ -519,7 +645,11 @@ __global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
     float squares[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if ((k * G + lane) * V < a.width) squares[0] += M::squares(x[k], mean);
+      const Span<V, kShift> s(k * G + lane, shift, width);
+      if (s.any()) {
+        if (!s.whole()) fill_outside(s, mean, x[k]);
+        squares[0] += M::squares(x[k], mean);
+      }
     }
     group_sums<G, 1>(squares, scratch);
     const float rstd = rsqrtf(squares[0] * inverse + static_cast<float>(a.eps));
@@ -527,20 +657,21 @@ __global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
       static_cast<float*>(a.stats)[row] = mean;
       static_cast<float*>(a.stats)[a.rows + row] = rstd;
     }
-    T* y = static_cast<T*>(a.y) + row * a.width;
+    T* y = static_cast<T*>(a.y) + row * width;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if ((k * G + lane) * V < a.width) {
+      const Span<V, kShift> s(k * G + lane, shift, width);
+      if (s.any()) {
         M::normalise(x[k], mean, rstd, w[k], b[k]);
-        store_twos<T, V>(y + (k * G + lane) * V, x[k]);
+        store_span<T>(y, s, x[k]);
       }
     }
     ring.advance();
   }
 }
 
-template <typename T, int V, int NV, int G>
-__global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
+template <typename T, int V, int NV, int G, bool kShift>
+__global__ void __launch_bounds__(G, ring_blocks_of(G, kShift))
     norm_backward_ring_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Ring ring_args) {
   extern __shared__ __align__(128) uint8_t shared[];
   __shared__ float scratch[4][32];
@@ -553,15 +684,17 @@ __global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
     dev::fence_barrier_init();
   }
   __syncthreads();
-  RowRing<G, true> ring{a, ring_args, shared, full, blockIdx.x};
+  RowRing<true, kShift> ring{a, ring_args, shared, full, blockIdx.x};
   if (lane == 0) {
     for (int s = 0; s < ring_args.stages; ++s) ring.ask(sizeof(T));
   }
   using M = RowMath<T, V, NV, G>;
+  const int width = static_cast<int>(a.width);
+  const int shift = row_shift<V>(blockIdx.x, a.x_stride);  // the same for all the block's rows
   Two w[NV][V / 2], dw[NV][V / 2], db[NV][V / 2];
-  load_param_pairs<T, V, NV, G>(a.weight, a.param_f32, a.width, lane, 1.0f, w);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
+    load_span_params<T>(a.weight, a.param_f32, Span<V, kShift>(k * G + lane, shift, width), 1.0f, w[k]);
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) dw[k][i] = db[k][i] = same(0.0f);
   }
@@ -590,10 +723,15 @@ __global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
         Two pairs[2] = {same(0.0f), same(0.0f)};
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-          if ((k * G + lane) * V < a.width) {
+          const Span<V, kShift> s(k * G + lane, shift, width);
+          if (s.any()) {
             Two x[V / 2], dy[V / 2];
             load_twos<T, V>(reinterpret_cast<const T*>(at[r]) + (k * G + lane) * V, x);
-            load_twos<T, V>(reinterpret_cast<const T*>(at[r] + ring_args.row_bytes) + (k * G + lane) * V, dy);
+            load_twos<T, V>(reinterpret_cast<const T*>(at[r] + ring_args.stage_bytes / 2) + (k * G + lane) * V, dy);
+            if (!s.whole()) {  // nothing is collected outside the row
+              fill_outside(s, 0.0f, x);
+              fill_outside(s, 0.0f, dy);
+            }
             M::collect(x, dy, stats[r].x, stats[r].y, w[k], pairs, dw[k], db[k]);
           }
         }
@@ -612,40 +750,37 @@ __global__ void __launch_bounds__(G, G == 1024 ? 1 : 768 / G)
     for (int r = 0; r < 2; ++r) {
       const int64_t row = row0 + r * step;
       if (row >= a.rows) break;
-      T* dx = static_cast<T*>(a.y) + row * a.width;
+      T* dx = static_cast<T*>(a.y) + row * width;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        if ((k * G + lane) * V < a.width) {
+        const Span<V, kShift> s(k * G + lane, shift, width);
+        if (s.any()) {
           Two x[V / 2], dy[V / 2];
           load_twos<T, V>(reinterpret_cast<const T*>(at[r]) + (k * G + lane) * V, x);
-          load_twos<T, V>(reinterpret_cast<const T*>(at[r] + ring_args.row_bytes) + (k * G + lane) * V, dy);
+          load_twos<T, V>(reinterpret_cast<const T*>(at[r] + ring_args.stage_bytes / 2) + (k * G + lane) * V, dy);
           M::gradient(x, dy, stats[r].x, stats[r].y, w[k], sums[2 * r] * inverse,
                       sums[2 * r + 1] * inverse);
-          store_twos<T, V>(dx + (k * G + lane) * V, dy);
+          store_span<T>(dx, s, dy);
         }
       }
     }
   }
   if (!a.want_params) return;
-  float* partial = static_cast<float*>(a.partials) + static_cast<int64_t>(blockIdx.x) * 2 * a.width;
+  float* partial = static_cast<float*>(a.partials) + static_cast<int64_t>(blockIdx.x) * 2 * width;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int64_t c = static_cast<int64_t>(k * G + lane) * V;
-    if (c < a.width) {
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) {
-        unpack(dw[k][i], partial + c + 2 * i, partial + c + 2 * i + 1);
-        unpack(db[k][i], partial + a.width + c + 2 * i, partial + a.width + c + 2 * i + 1);
-      }
-    }
+    add_span(Span<V, kShift>(k * G + lane, shift, width), dw[k], db[k], partial, width, true);
   }
 }
 
 // Short rows in tiles: G lanes of a warp to a row, as in the register kernels.
+constexpr int tile_blocks_of(int vectors, bool shift, bool backward) {
+  return backward ? (vectors == 1 && !shift ? 3 : 2) : (vectors == 1 && !shift ? 4 : 3);
+}
 constexpr int kTileThreads = 256, kMostTile = 256;
 
-template <typename T, int V, int NV, int G>
-__global__ void __launch_bounds__(kTileThreads, 4)
+template <typename T, int V, int NV, int G, bool kShift>
+__global__ void __launch_bounds__(kTileThreads, tile_blocks_of(NV, kShift, false))
     norm_forward_tile_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Ring ring_args) {
   constexpr int kGroups = kTileThreads / G;
   extern __shared__ __align__(128) uint8_t shared[];
@@ -658,14 +793,19 @@ __global__ void __launch_bounds__(kTileThreads, 4)
     dev::fence_barrier_init();
   }
   __syncthreads();
-  RowRing<G, false> ring{a, ring_args, shared, full, static_cast<int64_t>(blockIdx.x) * tile};
+  RowRing<false, kShift> ring{a, ring_args, shared, full, static_cast<int64_t>(blockIdx.x) * tile};
   if (threadIdx.x == 0) {
     for (int s = 0; s < ring_args.stages; ++s) ring.ask(sizeof(T));
   }
   using M = RowMath<T, V, NV, G>;
   Two w[NV][V / 2], b[NV][V / 2];
-  load_param_pairs<T, V, NV, G>(a.weight, a.param_f32, width, lane, 1.0f, w);
-  load_param_pairs<T, V, NV, G>(a.bias, a.param_f32, width, lane, 0.0f, b);
+  const int shift = row_shift<V>(group, width);  // tiles and steps are multiples of V rows
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const Span<V, kShift> s(k * G + lane, shift, width);
+    load_span_params<T>(a.weight, a.param_f32, s, 1.0f, w[k]);
+    load_span_params<T>(a.bias, a.param_f32, s, 0.0f, b[k]);
+  }
   for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * tile; row0 < a.rows;
        row0 += static_cast<int64_t>(gridDim.x) * tile) {
     const T* data = reinterpret_cast<const T*>(ring.wait());
@@ -677,16 +817,21 @@ __global__ void __launch_bounds__(kTileThreads, 4)
       float mean = 0.0f, squares = 0.0f;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * G + lane) * V;
-        if (live && c < width) {
-          load_twos<T, V>(data + (i0 + group) * width + c, x[k]);
+        const Span<V, kShift> s(k * G + lane, shift, width);
+        if (live && s.any()) {
+          load_twos<T, V>(data + (i0 + group) * width + s.c, x[k]);
+          if (!s.whole()) fill_outside(s, 0.0f, x[k]);
           mean += M::sum(x[k]);
         }
       }
       mean = group_sum<G, float>(mean, nullptr) * inverse;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        if (live && (k * G + lane) * V < width) squares += M::squares(x[k], mean);
+        const Span<V, kShift> s(k * G + lane, shift, width);
+        if (live && s.any()) {
+          if (!s.whole()) fill_outside(s, mean, x[k]);
+          squares += M::squares(x[k], mean);
+        }
       }
       squares = group_sum<G, float>(squares, nullptr);
       if (!live) continue;
@@ -697,10 +842,10 @@ __global__ void __launch_bounds__(kTileThreads, 4)
       }
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * G + lane) * V;
-        if (c < width) {
+        const Span<V, kShift> s(k * G + lane, shift, width);
+        if (s.any()) {
           M::normalise(x[k], mean, rstd, w[k], b[k]);
-          store_twos<T, V>(static_cast<T*>(a.y) + row * width + c, x[k]);
+          store_span<T>(static_cast<T*>(a.y) + row * width, s, x[k]);
         }
       }
     }
@@ -710,8 +855,8 @@ __global__ void __launch_bounds__(kTileThreads, 4)
   }
 }
 
-template <typename T, int V, int NV, int G>
-__global__ void __launch_bounds__(kTileThreads, NV == 1 ? 3 : 2)
+template <typename T, int V, int NV, int G, bool kShift>
+__global__ void __launch_bounds__(kTileThreads, tile_blocks_of(NV, kShift, true))
     norm_backward_tile_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ Ring ring_args) {
   constexpr int kGroups = kTileThreads / G;
   extern __shared__ __align__(128) uint8_t shared[];
@@ -733,15 +878,16 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 3 : 2)
   }
   fetch(static_cast<int64_t>(blockIdx.x) * tile, 0);
   __syncthreads();
-  RowRing<G, true> ring{a, ring_args, shared, full, static_cast<int64_t>(blockIdx.x) * tile};
+  RowRing<true, kShift> ring{a, ring_args, shared, full, static_cast<int64_t>(blockIdx.x) * tile};
   if (threadIdx.x == 0) {
     for (int s = 0; s < ring_args.stages; ++s) ring.ask(sizeof(T));
   }
   using M = RowMath<T, V, NV, G>;
   Two w[NV][V / 2], dw[NV][V / 2], db[NV][V / 2];
-  load_param_pairs<T, V, NV, G>(a.weight, a.param_f32, width, lane, 1.0f, w);
+  const int shift = row_shift<V>(group, width);  // tiles and steps are multiples of V rows
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
+    load_span_params<T>(a.weight, a.param_f32, Span<V, kShift>(k * G + lane, shift, width), 1.0f, w[k]);
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) dw[k][i] = db[k][i] = same(0.0f);
   }
@@ -756,16 +902,20 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 3 : 2)
     for (int i0 = 0; i0 < tile; i0 += kGroups) {
       const int64_t row = row0 + i0 + group;
       const bool live = i0 + group < tile && row < a.rows;
-      const float2 s = live ? stats[slot][i0 + group] : make_float2(0.0f, 0.0f);
+      const float2 st = live ? stats[slot][i0 + group] : make_float2(0.0f, 0.0f);
       Two x[NV][V / 2], dy[NV][V / 2];
       Two pairs[2] = {same(0.0f), same(0.0f)};
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * G + lane) * V;
-        if (live && c < width) {
-          load_twos<T, V>(xs + (i0 + group) * width + c, x[k]);
-          load_twos<T, V>(ds + (i0 + group) * width + c, dy[k]);
-          M::collect(x[k], dy[k], s.x, s.y, w[k], pairs, dw[k], db[k]);
+        const Span<V, kShift> s(k * G + lane, shift, width);
+        if (live && s.any()) {
+          load_twos<T, V>(xs + (i0 + group) * width + s.c, x[k]);
+          load_twos<T, V>(ds + (i0 + group) * width + s.c, dy[k]);
+          if (!s.whole()) {  // nothing is collected outside the row
+            fill_outside(s, 0.0f, x[k]);
+            fill_outside(s, 0.0f, dy[k]);
+          }
+          M::collect(x[k], dy[k], st.x, st.y, w[k], pairs, dw[k], db[k]);
         }
       }
       if (!a.want_dx) continue;
@@ -774,10 +924,10 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 3 : 2)
       if (!live) continue;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * G + lane) * V;
-        if (c < width) {
-          M::gradient(x[k], dy[k], s.x, s.y, w[k], sums[0] * inverse, sums[1] * inverse);
-          store_twos<T, V>(static_cast<T*>(a.y) + row * width + c, dy[k]);
+        const Span<V, kShift> s(k * G + lane, shift, width);
+        if (s.any()) {
+          M::gradient(x[k], dy[k], st.x, st.y, w[k], sums[0] * inverse, sums[1] * inverse);
+          store_span<T>(static_cast<T*>(a.y) + row * width, s, dy[k]);
         }
       }
     }
@@ -788,16 +938,32 @@ __global__ void __launch_bounds__(kTileThreads, NV == 1 ? 3 : 2)
   }
   if (!a.want_params) return;
   __syncthreads();
-  float wide_dw[NV][V], wide_db[NV][V];
+  float* columns = reinterpret_cast<float*>(shared);
+  if constexpr (kShift) {
+    // the groups' columns are offset against one another, so they add theirs one by one
+    for (int g = 0; g < kGroups; ++g) {
+      if (group == g) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      unpack(dw[k][i], &wide_dw[k][2 * i], &wide_dw[k][2 * i + 1]);
-      unpack(db[k][i], &wide_db[k][2 * i], &wide_db[k][2 * i + 1]);
+        for (int k = 0; k < NV; ++k) {
+          add_span(Span<V, kShift>(k * G + lane, shift, width), dw[k], db[k], columns, width, g == 0);
+        }
+      }
+      __syncthreads();
     }
+    float* partial = static_cast<float*>(a.partials) + static_cast<int64_t>(blockIdx.x) * 2 * width;
+    for (int c = threadIdx.x; c < 2 * width; c += kTileThreads) partial[c] = columns[c];
+  } else {
+    float wide_dw[NV][V], wide_db[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        unpack(dw[k][i], &wide_dw[k][2 * i], &wide_dw[k][2 * i + 1]);
+        unpack(db[k][i], &wide_db[k][2 * i], &wide_db[k][2 * i + 1]);
+      }
+    }
+    block_columns<T, V, NV, G>(a, wide_dw, wide_db, columns);
   }
-  block_columns<T, V, NV, G>(a, wide_dw, wide_db, reinterpret_cast<float*>(shared));
 }
 
 // ---- rows of any width and type --------------------------------------------------------
@@ -920,27 +1086,37 @@ struct NormShape {
   int vector;   // elements per load: 16 bytes, or 1 where rows are not 16-byte aligned
   int chunks;   // vectors per row
   bool loops;   // wider than the block kernels (or float64)
-  bool ring;    // 16-byte vectors and rows of more than 64 of them
+  bool shift;   // dense rows of another width, read in vectors from shifted starts
+  bool ring;    // more than 64 vectors a row
 };
 
 // Four stages of two such rows (28 KB each) fit the ring of the backward.
 constexpr int kMostChunks = 1792;
 
-NormShape norm_shape(int dtype, int64_t width, bool aligned) {
+// aligned: data on 16-byte boundaries; whole: rows a multiple of 16 bytes apart; dense: rows
+// back to back.
+NormShape norm_shape(int dtype, int64_t width, bool aligned, bool whole, bool dense) {
   NormShape s{};
   const int wide = 16 / element_size(dtype);
-  s.vector = aligned && width % wide == 0 ? wide : 1;
+  s.shift = aligned && dense && width % wide != 0 && width > 2 * wide && dtype != CND_F64 &&
+            (width + 2 * wide - 2) / wide <= kMostChunks;
+  if (s.shift) {
+    s.vector = wide;
+    s.chunks = static_cast<int>((width + 2 * wide - 2) / wide);
+    s.ring = s.chunks > 64;
+    return s;
+  }
+  s.vector = aligned && whole && width % wide == 0 ? wide : 1;
   s.loops = dtype == CND_F64 || width / s.vector > kMostChunks;
   s.chunks = s.loops ? 0 : static_cast<int>(width / s.vector);
   s.ring = s.vector > 1 && s.chunks > 64;
   return s;
 }
 
-// Blocks an SM of the ring kernels: 768 threads (85 registers each), at least one block.
 int ring_threads(int chunks) {
   return chunks <= 128 ? 64 : chunks <= 256 ? 128 : chunks <= 512 ? 256 : chunks <= 1024 ? 512 : 1024;
 }
-int ring_blocks(int chunks) { return std::max(1, 768 / ring_threads(chunks)); }
+int ring_blocks(const NormShape& s) { return ring_blocks_of(ring_threads(s.chunks), s.shift); }
 
 int norm_rows_per_block(const NormShape& s) {
   if (s.chunks <= 4) return 64;
@@ -949,12 +1125,12 @@ int norm_rows_per_block(const NormShape& s) {
   return s.chunks <= 64 ? 8 : 1;
 }
 
-// Short aligned rows back to back, enough of them to fill the SMs' rings (fewer rows gain nothing
-// from a ring and start faster in registers).
+// Short rows back to back: shifted ones, or enough to fill the SMs' rings (fewer aligned rows gain
+// nothing from a ring and start faster in registers).
 bool norm_tiles(const NormShape& s, int64_t rows, int64_t width, int64_t x_stride,
                 int64_t dy_stride) {
   return !s.loops && !s.ring && s.vector > 1 && x_stride == width && dy_stride == width &&
-         rows * s.chunks >= int64_t{148} * 4 * 512;
+         (s.shift || rows * s.chunks >= int64_t{148} * 4 * 512);
 }
 
 // Blocks of the backward (one partial row each): enough to fill the SMs, no more than rows.
@@ -965,7 +1141,10 @@ int norm_backward_blocks(const NormShape& s, int64_t rows, int64_t width) {
     const int64_t across = (width + 127) / 128;
     return static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, 8 * 148 / across)));
   }
-  if (s.ring) return static_cast<int>(std::min<int64_t>(rows, 148 * ring_blocks(s.chunks)));
+  if (s.ring) {
+    // a multiple of 8 where blocks take several rows: one shift a block
+    return static_cast<int>(std::min<int64_t>(rows, 148 * ring_blocks(s) / 8 * 8));
+  }
   const int per_block = norm_rows_per_block(s);
   const int64_t need = (rows + per_block - 1) / per_block;
   return static_cast<int>(std::min<int64_t>(need, 4 * 148));
@@ -1013,16 +1192,23 @@ void with_kernel(int dtype, const NormShape& s, F&& f) {
 
 // Blocks an SM of the tile kernels.
 int tile_blocks(const NormShape& s, bool backward) {
-  return !backward ? 4 : s.chunks <= 32 ? 3 : 2;
+  return tile_blocks_of(s.chunks <= 32 ? 1 : 2, s.shift, backward);
 }
 
 // The ring of a block: its share of 200 KB, at most 16 stages. Tiles of short rows are 8 KB.
-Ring make_ring(const NormShape& s, bool backward) {
+Ring make_ring(const NormShape& s, int dtype, int64_t width, bool backward) {
   Ring r{};
-  r.row_bytes = static_cast<uint32_t>(s.chunks) * 16;
-  r.tile = s.ring ? 1 : static_cast<int>(std::min<uint32_t>(kMostTile, 8192 / r.row_bytes));
-  r.stage_bytes = r.row_bytes * r.tile * (backward ? 2 : 1);
-  const uint32_t share = 200 * 1024 / (s.ring ? ring_blocks(s.chunks) : tile_blocks(s, backward));
+  if (s.ring) {
+    r.tile = 1;
+    r.stage_bytes = static_cast<uint32_t>(s.chunks) * 16;
+  } else {
+    // whole multiples of 8 rows; a vector before and behind for the masked ends
+    const uint32_t row = static_cast<uint32_t>(width) * element_size(dtype);
+    r.tile = static_cast<int>(std::max<uint32_t>(8, std::min<uint32_t>(kMostTile, 8192 / row / 8 * 8)));
+    r.stage_bytes = (row * r.tile + 31) / 16 * 16;
+  }
+  if (backward) r.stage_bytes *= 2;
+  const uint32_t share = 200 * 1024 / (s.ring ? ring_blocks(s) : tile_blocks(s, backward));
   r.stages = static_cast<int>(std::min<uint32_t>(16, std::max<uint32_t>(4, share / r.stage_bytes)));
   r.error = device_error_word();
   r.timeout_ns = wait_timeout_ns();
@@ -1066,8 +1252,10 @@ struct LaunchTile {
   template <typename T, int V, int NV, int G, int R>
   void operator()() const {
     if constexpr (V > 1 && G <= 32) {
-      const auto kernel = kBackward ? norm_backward_tile_kernel<T, V, NV, G>
-                                    : norm_forward_tile_kernel<T, V, NV, G>;
+      const auto kernel = a.shift ? (kBackward ? norm_backward_tile_kernel<T, V, NV, G, true>
+                                               : norm_forward_tile_kernel<T, V, NV, G, true>)
+                                  : (kBackward ? norm_backward_tile_kernel<T, V, NV, G, false>
+                                               : norm_forward_tile_kernel<T, V, NV, G, false>);
       const uint32_t bytes = std::max<uint32_t>(ring.stage_bytes * ring.stages,
                                                 static_cast<uint32_t>(a.width) * 2 * sizeof(float));
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1085,8 +1273,10 @@ struct LaunchRing {
   cudaStream_t stream;
   template <typename T, int V, int NV, int G>
   void operator()() const {
-    const auto kernel = kBackward ? norm_backward_ring_kernel<T, V, NV, G>
-                                  : norm_forward_ring_kernel<T, V, NV, G>;
+    const auto kernel = a.shift ? (kBackward ? norm_backward_ring_kernel<T, V, NV, G, true>
+                                             : norm_forward_ring_kernel<T, V, NV, G, true>)
+                                : (kBackward ? norm_backward_ring_kernel<T, V, NV, G, false>
+                                             : norm_forward_ring_kernel<T, V, NV, G, false>);
     const uint32_t bytes = ring.stage_bytes * ring.stages;
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                          static_cast<int>(bytes));
@@ -1136,9 +1326,7 @@ int check_norm(const char* who, int dtype, int param_dtype, int64_t rows, int64_
   return CND_OK;
 }
 
-bool rows_aligned(int dtype, const void* p, int64_t stride) {
-  return aligned16(p) && stride * element_size(dtype) % 16 == 0;
-}
+bool rows_whole(int dtype, int64_t stride) { return stride * element_size(dtype) % 16 == 0; }
 
 }  // namespace
 }  // namespace layers
@@ -1170,7 +1358,9 @@ int cnd_layer_norm_forward(int32_t dtype, int32_t param_dtype, int64_t rows, int
   a.x_stride = x_stride;
   a.eps = eps;
   a.param_f32 = param_dtype == CND_F32;
-  const NormShape s = norm_shape(dtype, width, rows_aligned(dtype, x, x_stride) && aligned16(y));
+  const NormShape s = norm_shape(dtype, width, aligned16(x) && aligned16(y),
+                                 rows_whole(dtype, x_stride), x_stride == width);
+  a.shift = s.shift;
   if (s.loops) {
     const unsigned blocks =
         static_cast<unsigned>(std::min<int64_t>(rows, static_cast<int64_t>(sm_count()) * 16));
@@ -1184,12 +1374,13 @@ int cnd_layer_norm_forward(int32_t dtype, int32_t param_dtype, int64_t rows, int
       norm_forward_loop_kernel<__half><<<blocks, kLoopThreads, 0, stream>>>(a);
     }
   } else if (s.ring) {
-    const Ring ring = make_ring(s, false);
+    const Ring ring = make_ring(s, dtype, width, false);
     if (ring.error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
-    const int blocks = static_cast<int>(std::min<int64_t>(rows, sm_count() * ring_blocks(s.chunks)));
+    const int blocks =
+        static_cast<int>(std::min<int64_t>(rows, sm_count() * ring_blocks(s) / 8 * 8));
     with_ring_dtype(dtype, s, LaunchRing<false>{a, ring, blocks, stream});
   } else if (norm_tiles(s, rows, width, x_stride, width)) {
-    const Ring ring = make_ring(s, false);
+    const Ring ring = make_ring(s, dtype, width, false);
     if (ring.error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
     const int64_t tiles = (rows + ring.tile - 1) / ring.tile;
     const int blocks =
@@ -1207,10 +1398,11 @@ size_t cnd_layer_norm_backward_workspace_size(int32_t dtype, int64_t rows, int64
   using namespace cnd::layers;
   if (!known_dtype(dtype) || rows <= 0 || width <= 0 || output_mask == nullptr) return 0;
   if (!output_mask[1] && !output_mask[2]) return 0;
-  // the larger of what aligned and unaligned rows take
+  // the largest of what the data's alignment can lead to
   int blocks = 0;
-  for (const bool aligned : {false, true}) {
-    blocks = std::max(blocks, norm_backward_blocks(norm_shape(dtype, width, aligned), rows, width));
+  for (int kind = 0; kind < 8; ++kind) {
+    const NormShape s = norm_shape(dtype, width, (kind & 1) != 0, (kind & 2) != 0, (kind & 4) != 0);
+    blocks = std::max(blocks, norm_backward_blocks(s, rows, width));
   }
   return static_cast<size_t>(blocks) * 2 * static_cast<size_t>(width) *
          (dtype == CND_F64 ? sizeof(double) : sizeof(float));
@@ -1266,9 +1458,11 @@ int cnd_layer_norm_backward(int32_t dtype, int32_t param_dtype, int64_t rows, in
   a.param_f32 = param_dtype == CND_F32;
   a.want_dx = output_mask[0] != 0;
   a.want_params = params;
-  const bool aligned = rows_aligned(dtype, x, x_stride) && rows_aligned(dtype, dy, dy_stride) &&
-                       (!a.want_dx || aligned16(dx));
-  const NormShape s = norm_shape(dtype, width, aligned);
+  const NormShape s =
+      norm_shape(dtype, width, aligned16(x) && aligned16(dy) && (!a.want_dx || aligned16(dx)),
+                 rows_whole(dtype, x_stride) && rows_whole(dtype, dy_stride),
+                 x_stride == width && dy_stride == width);
+  a.shift = s.shift;
   int blocks = norm_backward_blocks(s, rows, width);
   if (s.loops) {
     const unsigned grid =
@@ -1295,12 +1489,12 @@ int cnd_layer_norm_backward(int32_t dtype, int32_t param_dtype, int64_t rows, in
       run(__half{});
     }
   } else if (s.ring) {
-    const Ring ring = make_ring(s, true);
+    const Ring ring = make_ring(s, dtype, width, true);
     if (ring.error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
     with_ring_dtype(dtype, s, LaunchRing<true>{a, ring, blocks, stream});
     count_launch();
   } else if (norm_tiles(s, rows, width, x_stride, dy_stride)) {
-    const Ring ring = make_ring(s, true);
+    const Ring ring = make_ring(s, dtype, width, true);
     if (ring.error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
     blocks = std::min(blocks, sm_count() * tile_blocks(s, true));
     with_kernel<true>(dtype, s, LaunchTile<true>{a, ring, blocks, stream});

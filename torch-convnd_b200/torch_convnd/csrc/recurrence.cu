@@ -68,6 +68,7 @@ struct RecurrenceArgs {
   int64_t outer, steps, inner, columns;
   int64_t chunks;
   int column_blocks;
+  int lanes, per_block;  // step layout: lanes of a column, columns of a block
   int balanced;  // steps a thread takes when one chunk holds them all, 0: the most it can
   // exchange between chunks (shared != 0): maps [chunks][padded], states [groups][padded],
   // one ticket counter; all bits set at the start
@@ -193,12 +194,6 @@ __device__ __forceinline__ A load_base(const RecurrenceArgs& a, int64_t i, unsig
     const auto* p = static_cast<const unsigned long long*>(a.bases) + i;
     return __longlong_as_double(static_cast<long long>(settle(p, load_exchange(p), a, site)));
   }
-}
-
-// V columns (or one column's run of steps) of a thread, loaded at once where they lie together.
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
-  return *reinterpret_cast<const Pack<T, V>*>(p);
 }
 
 // A step past the end is given the gate +inf and x = dy = 0: it holds the state and passes the
@@ -736,68 +731,108 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 
 // ---- step layout -----------------------------------------------------------------------
 
-// A thread's run of kAlongSteps steps: one 16-byte (32 for float32) access where rows are
-// aligned, else single elements.
+// Column c starts at element c * steps, off a 16-byte boundary by `shift` elements where steps
+// is no multiple of one. Its runs start `shift` elements earlier, so that every run is read and
+// written in aligned vectors; the column's first run then begins, like its last one ends, with
+// steps that do not exist and hold the state. A column takes `lanes` lanes of a warp (a short
+// column less than a warp, a block then several columns) or a block's warps one behind the
+// other.
 template <typename T>
-__device__ __forceinline__ void load_run(const T* p, int count, bool vectors, float other,
-                                         T (&v)[kAlongSteps]) {
-  constexpr int kPer = 16 / sizeof(T);
-  if (vectors && count == kAlongSteps) {
-#pragma unroll
-    for (int i = 0; i < kAlongSteps; i += kPer) {
-      *reinterpret_cast<Pack<T, kPer>*>(v + i) = load_pack<T, kPer>(p + i);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kAlongSteps; ++i) {
-      v[i] = narrow<T>(static_cast<typename Wide<T>::type>(other));
-      if (i < count) v[i] = p[i];
-    }
-  }
-}
+struct Run {
+  static constexpr int kPer = 16 / sizeof(T);
+  int64_t first;  // step of the run's first element, negative in a shifted column's first run
+  int lo, hi;     // steps of the run that exist
+  bool vectors;   // the column's data start on 16-byte boundaries `shift` elements before it
 
-template <typename T>
-__device__ __forceinline__ void store_run(T* p, int count, bool vectors,
-                                          const T (&v)[kAlongSteps]) {
-  constexpr int kPer = 16 / sizeof(T);
-  if (vectors && count == kAlongSteps) {
+  __device__ __forceinline__ Run(int64_t index, int shift, int64_t steps, bool aligned)
+      : first(index * kAlongSteps - shift) {
+    lo = first < 0 ? static_cast<int>(-first) : 0;
+    hi = steps_here(steps - first, kAlongSteps);
+    vectors = aligned && lo == 0 && hi == kAlongSteps;
+  }
+  __device__ __forceinline__ bool has(int i) const { return i >= lo && i < hi; }
+
+  // `column`: the column's first element.
+  __device__ __forceinline__ void load(const T* column, float other, T (&v)[kAlongSteps]) const {
+    const T* p = column + first;
+    if (vectors) {
 #pragma unroll
-    for (int i = 0; i < kAlongSteps; i += kPer) {
-      *reinterpret_cast<Pack<T, kPer>*>(p + i) = *reinterpret_cast<const Pack<T, kPer>*>(v + i);
-    }
-  } else {
+      for (int i = 0; i < kAlongSteps; i += kPer) {
+        *reinterpret_cast<Pack<T, kPer>*>(v + i) = *reinterpret_cast<const Pack<T, kPer>*>(p + i);
+      }
+    } else {
 #pragma unroll
-    for (int i = 0; i < kAlongSteps; ++i) {
-      if (i < count) p[i] = v[i];
+      for (int i = 0; i < kAlongSteps; ++i) {
+        v[i] = narrow<T>(static_cast<typename Wide<T>::type>(other));
+        if (has(i)) v[i] = p[i];
+      }
     }
   }
-}
+  __device__ __forceinline__ void store(T* column, const T (&v)[kAlongSteps]) const {
+    T* p = column + first;
+    if (vectors) {
+#pragma unroll
+      for (int i = 0; i < kAlongSteps; i += kPer) {
+        *reinterpret_cast<Pack<T, kPer>*>(p + i) = *reinterpret_cast<const Pack<T, kPer>*>(v + i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kAlongSteps; ++i) {
+        if (has(i)) p[i] = v[i];
+      }
+    }
+  }
+};
+
+// Places of a thread in step layout: its column, its lane among the column's and its warp.
+struct Along {
+  int64_t column, chunk;  // chunk: the walk's first
+  int warp, warps, lane, lanes;
+
+  __device__ __forceinline__ Along(const RecurrenceArgs& a, unsigned int* taken) {
+    lanes = a.lanes;
+    chunk = 0;
+    if (a.shared) {
+      if (threadIdx.x == 0) *taken = atomicAdd(a.ticket, 1u) + 1u;
+      __syncthreads();
+      chunk = *taken / a.column_blocks;
+      column = *taken - static_cast<uint32_t>(chunk) * a.column_blocks;
+    } else {
+      column = blockIdx.x;
+    }
+    warp = threadIdx.x >> 5;
+    warps = blockDim.x >> 5;
+    lane = threadIdx.x & 31;
+    if (a.per_block > 1) {  // several columns a block, each within a warp
+      column = static_cast<int64_t>(blockIdx.x) * a.per_block + threadIdx.x / lanes;
+      warp = 0;
+      warps = 1;
+      lane = threadIdx.x % lanes;
+    }
+  }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32)
-    steps_forward_kernel(const __grid_constant__ RecurrenceArgs a, bool vectors) {
+    steps_forward_kernel(const __grid_constant__ RecurrenceArgs a, bool aligned) {
   using A = typename Wide<T>::type;
   __shared__ Map<A> maps[kWarps];
   __shared__ Map<A> before[kWarps];
   __shared__ unsigned int taken;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int warps = blockDim.x >> 5;
-  int64_t column = blockIdx.x, chunk = 0, stop = a.chunks;
-  if (a.shared) {
-    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u) + 1u;
-    __syncthreads();
-    chunk = taken / a.column_blocks;
-    column = taken - chunk * a.column_blocks;
-    stop = chunk + 1;
-  }
+  const Along at(a, &taken);
+  const bool live = at.column < a.columns;
+  const int64_t column = live ? at.column : 0;
+  const int shift = aligned ? static_cast<int>(column * a.steps % Run<T>::kPer) : 0;
+  const int64_t stop = a.shared ? at.chunk + 1 : a.chunks;
+  const T* x_column = static_cast<const T*>(a.x) + column * a.steps;
+  const T* g_column = static_cast<const T*>(a.gate) + column * a.steps;
+  T* y_column = static_cast<T*>(a.y) + column * a.steps;
   A begin = a.initial != nullptr ? static_cast<const A*>(a.initial)[column] : A(0);
-  for (; chunk < stop; ++chunk) {
-    const int64_t first = ((chunk * warps + warp) * 32 + lane) * kAlongSteps;
-    const int64_t offset = column * a.steps + first;
-    const int count = steps_here(a.steps - first, kAlongSteps);
+  for (int64_t chunk = at.chunk; chunk < stop; ++chunk) {
+    const Run<T> run((chunk * at.warps + at.warp) * at.lanes + at.lane, shift, a.steps, aligned);
     alignas(16) T x[kAlongSteps], g[kAlongSteps];
-    load_run(static_cast<const T*>(a.x) + offset, count, vectors, 0.0f, x);
-    load_run(static_cast<const T*>(a.gate) + offset, count, vectors, INFINITY, g);
+    run.load(x_column, 0.0f, x);
+    run.load(g_column, INFINITY, g);
     A f[kAlongSteps], b[kAlongSteps];
     Map<A> own{A(1), A(0)};
 #pragma unroll
@@ -807,20 +842,21 @@ __global__ void __launch_bounds__(kWarps * 32)
       b[i] = keep * widen(x[i]);
       own = then(own, Map<A>{f[i], b[i]});
     }
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
+    for (int d = 1; d < at.lanes; d *= 2) {
       const Map<A> m = shuffle_up(own, d);
-      if (lane >= d) own = then(m, own);
+      if (at.lane >= d) own = then(m, own);
     }
-    if (lane == 31) maps[warp] = own;
     Map<A> earlier = shuffle_up(own, 1);
-    if (lane == 0) earlier = {A(1), A(0)};
-    __syncthreads();
+    if (at.lane == 0) earlier = {A(1), A(0)};
     Map<A> lead{A(1), A(0)};  // the block's warps before this one
-    for (int w = 0; w < warp; ++w) lead = then(lead, maps[w]);
+    if (at.warps > 1) {
+      if (at.lane == 31) maps[at.warp] = own;
+      __syncthreads();
+      for (int w = 0; w < at.warp; ++w) lead = then(lead, maps[w]);
+    }
     A state = begin;
     if (a.shared) {
-      const bool sends = warp == warps - 1 && lane == 31 && chunk + 1 < a.chunks;
+      const bool sends = at.warp == at.warps - 1 && at.lane == 31 && chunk + 1 < a.chunks;
       if (sends) store_map<A>(a.maps, chunk * a.column_blocks + column, then(lead, own));
       A carried[1] = {begin};
       carry_in<A, OneColumn>(a, chunk, column, before, kSiteForward, carried);
@@ -831,13 +867,13 @@ __global__ void __launch_bounds__(kWarps * 32)
       }
     } else if (chunk + 1 < stop) {
       Map<A> all = lead;
-      for (int w = warp; w < warps; ++w) all = then(all, maps[w]);
+      for (int w = at.warp; w < at.warps; ++w) all = then(all, maps[w]);
       begin = all.a * begin + all.b;
       __syncthreads();
     }
     state = lead.a * state + lead.b;
-    if (a.states != nullptr && lane == 0 && first < a.steps) {
-      static_cast<A*>(a.states)[first / kAlongBlock * a.columns + column] = state;
+    if (a.states != nullptr && at.lane == 0 && live && run.first < a.steps) {
+      static_cast<A*>(a.states)[(run.first + shift) / kAlongBlock * a.columns + column] = state;
     }
     state = earlier.a * state + earlier.b;
     alignas(16) T y[kAlongSteps];
@@ -846,42 +882,42 @@ __global__ void __launch_bounds__(kWarps * 32)
       state = f[i] * state + b[i];
       y[i] = narrow<T>(state);
     }
-    store_run(static_cast<T*>(a.y) + offset, count, vectors, y);
-    const int64_t end = a.steps > 0 ? a.steps - 1 : 0;
-    if (first <= end && end < first + kAlongSteps) static_cast<A*>(a.last)[column] = state;
+    if (!live) continue;
+    run.store(y_column, y);
+    const int64_t end = a.steps - 1;
+    if (run.first <= end && end < run.first + kAlongSteps) static_cast<A*>(a.last)[column] = state;
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32)
-    steps_backward_kernel(const __grid_constant__ RecurrenceArgs a, bool vectors) {
+    steps_backward_kernel(const __grid_constant__ RecurrenceArgs a, bool aligned) {
   using A = typename Wide<T>::type;
   __shared__ Map<A> maps[kWarps];
   __shared__ Map<A> after[kWarps];
   __shared__ unsigned int taken;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int warps = blockDim.x >> 5;
-  int64_t column = blockIdx.x, order = 0, stop = a.chunks;
-  if (a.shared) {
-    if (threadIdx.x == 0) taken = atomicAdd(a.ticket, 1u) + 1u;
-    __syncthreads();
-    order = taken / a.column_blocks;
-    column = taken - order * a.column_blocks;
-    stop = order + 1;
-  }
+  const Along at(a, &taken);
+  const bool live = at.column < a.columns;
+  const int64_t column = live ? at.column : 0;
+  const int shift = aligned ? static_cast<int>(column * a.steps % Run<T>::kPer) : 0;
+  const int64_t stop = a.shared ? at.chunk + 1 : a.chunks;
+  const int64_t base = column * a.steps;
   A begin = a.dlast != nullptr ? static_cast<const A*>(a.dlast)[column] : A(0);
-  for (; order < stop; ++order) {
+  for (int64_t order = at.chunk; order < stop; ++order) {
     const int64_t chunk = a.chunks - 1 - order;
-    const int64_t first = ((chunk * warps + warp) * 32 + lane) * kAlongSteps;
-    const int64_t offset = column * a.steps + first;
-    const int count = steps_here(a.steps - first, kAlongSteps);
+    const int64_t warp_run = (chunk * at.warps + at.warp) * at.lanes;
+    const Run<T> run(warp_run + at.lane, shift, a.steps, aligned);
     alignas(16) T x[kAlongSteps], g[kAlongSteps], d[kAlongSteps];
-    load_run(static_cast<const T*>(a.x) + offset, count, vectors, 0.0f, x);
-    load_run(static_cast<const T*>(a.gate) + offset, count, vectors, INFINITY, g);
-    load_run(static_cast<const T*>(a.dy) + offset, a.dy != nullptr ? count : 0, vectors, 0.0f, d);
-    const int64_t warp_first = first - lane * kAlongSteps;
-    A state = warp_first < a.steps
-                  ? static_cast<const A*>(a.states_in)[warp_first / kAlongBlock * a.columns + column]
+    run.load(static_cast<const T*>(a.x) + base, 0.0f, x);
+    run.load(static_cast<const T*>(a.gate) + base, INFINITY, g);
+    if (a.dy != nullptr) {
+      run.load(static_cast<const T*>(a.dy) + base, 0.0f, d);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kAlongSteps; ++i) d[i] = narrow<T>(A(0));
+    }
+    A state = warp_run * kAlongSteps - shift < a.steps
+                  ? static_cast<const A*>(a.states_in)[warp_run * kAlongSteps / kAlongBlock * a.columns + column]
                   : A(0);
     A f[kAlongSteps], keep[kAlongSteps];
     Map<A> own{A(1), A(0)};
@@ -893,23 +929,24 @@ __global__ void __launch_bounds__(kWarps * 32)
     Map<A> back{own.a, A(0)};
 #pragma unroll
     for (int i = kAlongSteps - 1; i >= 0; --i) back.b = f[i] * (widen(d[i]) + back.b);
-#pragma unroll
-    for (int k = 1; k < 32; k *= 2) {
+    for (int k = 1; k < at.lanes; k *= 2) {
       const Map<A> m = shuffle_up(own, k);
-      if (lane >= k) own = then(m, own);
+      if (at.lane >= k) own = then(m, own);
       const Map<A> n = shuffle_down(back, k);
-      if (lane < 32 - k) back = then(n, back);
+      if (at.lane < at.lanes - k) back = then(n, back);
     }
-    if (lane == 0) maps[warp] = back;
     Map<A> earlier = shuffle_up(own, 1), later = shuffle_down(back, 1);
-    if (lane > 0) state = earlier.a * state + earlier.b;
-    if (lane == 31) later = {A(1), A(0)};
-    __syncthreads();
+    if (at.lane > 0) state = earlier.a * state + earlier.b;
+    if (at.lane == at.lanes - 1) later = {A(1), A(0)};
     Map<A> lead{A(1), A(0)};  // the block's warps after this one
-    for (int w = warps - 1; w > warp; --w) lead = then(lead, maps[w]);
+    if (at.warps > 1) {
+      if (at.lane == 0) maps[at.warp] = back;
+      __syncthreads();
+      for (int w = at.warps - 1; w > at.warp; --w) lead = then(lead, maps[w]);
+    }
     A q = begin;
     if (a.shared) {
-      const bool sends = warp == 0 && lane == 0 && order + 1 < a.chunks;
+      const bool sends = at.warp == 0 && at.lane == 0 && order + 1 < a.chunks;
       if (sends) store_map<A>(a.maps, order * a.column_blocks + column, then(lead, back));
       A carried[1] = {begin};
       carry_in<A, OneColumn>(a, order, column, after, kSiteBackward, carried);
@@ -920,29 +957,33 @@ __global__ void __launch_bounds__(kWarps * 32)
       }
     } else if (order + 1 < stop) {
       Map<A> all = lead;
-      for (int w = warp; w >= 0; --w) all = then(all, maps[w]);
+      for (int w = at.warp; w >= 0; --w) all = then(all, maps[w]);
       begin = all.a * begin + all.b;
       __syncthreads();
     }
     q = lead.a * q + lead.b;
     q = later.a * q + later.b;
-    A prior[kAlongSteps];
+    A slope[kAlongSteps];
 #pragma unroll
     for (int i = 0; i < kAlongSteps; ++i) {
-      prior[i] = state;
-      state = f[i] * state + keep[i] * widen(x[i]);
+      const A value = widen(x[i]);
+      slope[i] = f[i] * keep[i] * (state - value);
+      state = f[i] * state + keep[i] * value;
     }
     alignas(16) T dx[kAlongSteps], dg[kAlongSteps];
 #pragma unroll
     for (int i = kAlongSteps - 1; i >= 0; --i) {
       const A total = widen(d[i]) + q;
       dx[i] = narrow<T>(keep[i] * total);
-      dg[i] = narrow<T>(f[i] * keep[i] * (prior[i] - widen(x[i])) * total);
+      dg[i] = narrow<T>(slope[i] * total);
       q = f[i] * total;
     }
-    if (a.dx != nullptr) store_run(static_cast<T*>(a.dx) + offset, count, vectors, dx);
-    if (a.dgate != nullptr) store_run(static_cast<T*>(a.dgate) + offset, count, vectors, dg);
-    if (a.dinitial != nullptr && first == 0) static_cast<A*>(a.dinitial)[column] = q;
+    if (!live) continue;
+    if (a.dx != nullptr) run.store(static_cast<T*>(a.dx) + base, dx);
+    if (a.dgate != nullptr) run.store(static_cast<T*>(a.dgate) + base, dg);
+    if (a.dinitial != nullptr && run.first <= 0 && run.first + kAlongSteps > 0) {
+      static_cast<A*>(a.dinitial)[column] = q;
+    }
   }
 }
 
@@ -953,6 +994,7 @@ struct RecurrencePlan {
   int warps;   // warps a block
   int64_t chunks;
   int64_t column_blocks;
+  int lanes, per_block;  // step layout
   int balanced;
   bool shared;
   size_t maps = 0, bases = 0, ticket = 0, total = 0;
@@ -964,14 +1006,30 @@ RecurrencePlan plan_recurrence(int dtype, int64_t outer, int64_t steps, int64_t 
   const int64_t columns = outer * inner;
   const int held = dtype == CND_F64 ? 1 : 2;  // columns a lane
   p.along = inner == 1 && steps > 1;
-  const int64_t per_warp = p.along    ? kAlongBlock
-                           : backward ? kBackwardSteps
-                                      : forward_steps(element_size(dtype));
-  p.warps = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kWarps, (steps + per_warp - 1) / per_warp)));
-  p.chunks = std::max<int64_t>(1, (steps + p.warps * per_warp - 1) / (p.warps * per_warp));
+  p.lanes = 32;
+  p.per_block = 1;
+  if (p.along) {
+    // runs of a column: one more where its start is shifted
+    const int per = 16 / element_size(dtype);
+    const int64_t ahead = steps % per != 0 ? per - 1 : 0;
+    const int64_t runs = (steps + ahead + kAlongSteps - 1) / kAlongSteps;
+    p.warps = static_cast<int>(std::min<int64_t>(kWarps, (runs + 31) / 32));
+    p.chunks = (runs + p.warps * 32 - 1) / (p.warps * 32);
+    if (runs <= 32) {
+      p.lanes = 1;
+      while (p.lanes < runs) p.lanes *= 2;
+      p.warps = kWarps;
+      p.per_block = kWarps * 32 / p.lanes;
+    }
+  } else {
+    const int64_t per_warp = backward ? kBackwardSteps : forward_steps(element_size(dtype));
+    p.warps = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kWarps, (steps + per_warp - 1) / per_warp)));
+    p.chunks = std::max<int64_t>(1, (steps + p.warps * per_warp - 1) / (p.warps * per_warp));
+  }
   // Up to 64 steps (one kept state), the warps share them evenly: 33 steps as 11 + 11 + 11.
   if (!p.along && steps <= kStateBlock) p.balanced = static_cast<int>((steps + p.warps - 1) / p.warps);
-  p.column_blocks = p.along ? columns : (columns + 32 * held - 1) / (32 * held);
+  p.column_blocks = p.along ? (columns + p.per_block - 1) / p.per_block
+                            : (columns + 32 * held - 1) / (32 * held);
   // Blocks of eight warps, at most three on an SM: with fewer than 2 blocks an SM, sharing the
   // time axis fills the machine.
   p.shared = p.chunks > 1 && p.column_blocks < 2 * 148;
@@ -998,6 +1056,8 @@ int bind_exchange(const char* who, const RecurrencePlan& p, void* workspace, siz
   a->column_blocks = static_cast<int>(p.column_blocks);
   a->shared = p.shared;
   a->balanced = p.balanced;
+  a->lanes = p.lanes;
+  a->per_block = p.per_block;
   if (p.column_blocks > INT32_MAX) {
     return fail(CND_ERR_UNSUPPORTED, "%s: too many columns", who);
   }
@@ -1030,8 +1090,7 @@ bool pairs_aligned(int dtype, int64_t inner, std::initializer_list<const void*> 
   return true;
 }
 
-bool runs_aligned(int dtype, int64_t steps, std::initializer_list<const void*> pointers) {
-  if (steps * element_size(dtype) % 16 != 0) return false;
+bool runs_aligned(std::initializer_list<const void*> pointers) {
   for (const void* p : pointers) {
     if (!aligned16(p)) return false;
   }
@@ -1073,8 +1132,10 @@ int64_t cnd_gated_recurrence_blocks(int32_t dtype, int64_t outer, int64_t steps,
   (void)dtype;
   (void)outer;
   using namespace cnd::layers;
-  const int64_t block = inner == 1 && steps > 1 ? kAlongBlock : kStateBlock;
-  return steps <= 0 ? 0 : (steps - 1) / block + 1;
+  if (steps <= 0) return 0;
+  // in step layout a column's runs may start up to 7 steps before it
+  if (inner == 1 && steps > 1) return (steps + 6) / kAlongBlock + 1;
+  return (steps - 1) / kStateBlock + 1;
 }
 
 size_t cnd_gated_recurrence_workspace_size(int32_t dtype, int64_t outer, int64_t steps,
@@ -1121,7 +1182,7 @@ int cnd_gated_recurrence_forward(int32_t dtype, int64_t outer, int64_t steps, in
   rc = bind_exchange("cnd_gated_recurrence_forward", p, workspace, workspace_bytes, &a, stream);
   if (rc != CND_OK) return rc;
   const unsigned grid = recurrence_grid(p);
-  const bool vectors = runs_aligned(dtype, steps, {x, gate, y});
+  const bool vectors = runs_aligned({x, gate, y});
   const bool small = columns * std::max<int64_t>(steps, 1) * element_size(dtype) <= UINT32_MAX;
   with_dtype(dtype, [&](auto zero) {
     using T = decltype(zero);
@@ -1179,7 +1240,7 @@ int cnd_gated_recurrence_backward(int32_t dtype, int64_t outer, int64_t steps, i
   rc = bind_exchange("cnd_gated_recurrence_backward", p, workspace, workspace_bytes, &a, stream);
   if (rc != CND_OK) return rc;
   const unsigned grid = recurrence_grid(p);
-  const bool vectors = runs_aligned(dtype, steps, {x, gate, dy, dx, dgate});
+  const bool vectors = runs_aligned({x, gate, dy, dx, dgate});
   const bool small = columns * std::max<int64_t>(steps, 1) * element_size(dtype) <= UINT32_MAX;
   with_dtype(dtype, [&](auto zero) {
     using T = decltype(zero);
