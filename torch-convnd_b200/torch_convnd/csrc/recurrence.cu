@@ -842,7 +842,9 @@ __global__ void __launch_bounds__(kWarps * 32)
       b[i] = keep * widen(x[i]);
       own = then(own, Map<A>{f[i], b[i]});
     }
-    for (int d = 1; d < at.lanes; d *= 2) {
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      if (d >= at.lanes) break;
       const Map<A> m = shuffle_up(own, d);
       if (at.lane >= d) own = then(m, own);
     }
@@ -929,7 +931,9 @@ __global__ void __launch_bounds__(kWarps * 32)
     Map<A> back{own.a, A(0)};
 #pragma unroll
     for (int i = kAlongSteps - 1; i >= 0; --i) back.b = f[i] * (widen(d[i]) + back.b);
-    for (int k = 1; k < at.lanes; k *= 2) {
+#pragma unroll
+    for (int k = 1; k < 32; k *= 2) {
+      if (k >= at.lanes) break;
       const Map<A> m = shuffle_up(own, k);
       if (at.lane >= k) own = then(m, own);
       const Map<A> n = shuffle_down(back, k);
