@@ -50,10 +50,10 @@ constexpr uint32_t kSharedLimit = 232448;
 constexpr int kMostStages = 8;
 constexpr int kChunkBlocks = 8;  // k blocks per float32 accumulation (three-term operands)
 constexpr uint32_t kSiteLoad = 0x501, kSiteMma = 0x502, kSiteAccumulator = 0x503,
-                   kSiteEpilogue = 0x504, kSiteDrain = 0x505;
+                   kSiteEpilogue = 0x504, kSiteDrain = 0x505, kSiteResidual = 0x506;
 
 struct Maps {
-  CUtensorMap a, b, out, pre;
+  CUtensorMap a, b, out, pre, residual;
 };
 
 struct KernelArgs {
@@ -66,7 +66,8 @@ struct KernelArgs {
   uint32_t a_lbo, b_lbo;
   uint32_t a_sbo, b_sbo, a_swizzle, b_swizzle;
   int a_k_major, b_k_major;
-  int act, tma_out, vector_residual;
+  int act, tma_out;
+  int tma_residual;  // its rows are 16-byte aligned
   const void* bias;
   const void* residual;
   void* d;
@@ -172,24 +173,12 @@ __device__ __forceinline__ void copy_unit(uint8_t* tile, Out* d, int64_t row0, i
   }
 }
 
-// 32 residual values of a row, zero outside the matrix.
+// 32 residual values of a row, from a staging tile.
 template <typename Out>
 struct Residual {
   static constexpr int kPer = 16 / sizeof(Out);
   Pack<Out, kPer> q[32 / kPer];
 
-  __device__ __forceinline__ void load(const KernelArgs& a, int64_t row, int64_t col) {
-    const Out* p = static_cast<const Out*>(a.residual) + row * a.n + col;
-#pragma unroll
-    for (int c = 0; c < 32 / kPer; ++c) {
-      q[c] = Pack<Out, kPer>{};
-      if (row < a.m && col + c * kPer < a.n) {
-        q[c] = *reinterpret_cast<const Pack<Out, kPer>*>(p + c * kPer);
-      }
-    }
-  }
-
-  // From a staging tile that copy_unit filled.
   __device__ __forceinline__ void take(const uint8_t* tile, int row, int half) {
     constexpr int kChunks = 32 / kPer;
 #pragma unroll
@@ -228,7 +217,8 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
   uint64_t* acc_full = empty + kMostStages;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* cross_empty = acc_empty + 2;  // three-term operands: the small products' sets
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cross_empty + 2);
+  uint64_t* residual_full = cross_empty + 2;  // a group's residual tile has arrived
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(residual_full + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = kPair == 2 ? dev::cluster_rank() : 0;
@@ -239,6 +229,7 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
       dev::mbar_init(&full[s], 1);
       dev::mbar_init(&empty[s], 1);
     }
+    for (int g = 0; g < kGroups; ++g) dev::mbar_init(&residual_full[g], 1);
     for (int s = 0; s < 2; ++s) {
       dev::mbar_init(&acc_full[s], 1);
       dev::mbar_init(&acc_empty[s], kPair * kEpilogueWarps);
@@ -433,8 +424,20 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
       }
     };
     int set = 0, cross = 0, buffer = 0;
-    uint32_t set_phase = 0;
+    uint32_t set_phase = 0, residual_phase = 0;
     bool ok = true;
+    // The residual's tile of a unit comes by TMA into the staging tile that its output will
+    // take: each thread then reads its row's part and writes the output over it. It is asked
+    // for while the unit before is worked on where there is a second tile, else once the
+    // one tile is free. (Read by warps of the epilogue, a row each, it had waited for memory
+    // there: 1M x 64 -> 256 in bf16 475 us, by TMA 260, without a residual 192;
+    // 16384 x 1024 -> 4096 147 us, by TMA 116.)
+    const auto ask_residual = [&](int64_t row0, int64_t col, uint8_t* into) {
+      dev::mbar_arrive_expect_tx(&residual_full[group], kUnitBytes);
+      dev::tma_load_2d(into, &maps.residual, &residual_full[group], static_cast<int>(col),
+                       static_cast<int>(row0));
+    };
+    bool asked = false;  // the coming unit's residual is on its way
     for (int item = worker; item < items && ok; item += workers) {
       const int split = item % a.splits;
       int tm, tn;
@@ -450,10 +453,6 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
                         : 0.0f;
       }
       dev::named_barrier(1, 32 * kEpilogueWarps);
-      Residual<Out> residual;
-      const bool direct = a.residual != nullptr && a.vector_residual;
-      if (kParts == 1 && direct) residual.load(a, row0 + row, col0);
-
       float sums[kParts == 3 ? kHalves : 1][32];
       if constexpr (kParts == 3) {
         const int first = static_cast<int>(static_cast<int64_t>(a.k_blocks) * split / a.splits);
@@ -519,6 +518,11 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
           pre_tile = own + (buffer + a.sets) * kUnitBytes;
           if (a.buffers == 1) pre_tile = tile;
           if (a.sets == 2) buffer ^= 1;
+          // (one tile for all: after the pre-activation has left it)
+          if (a.tma_residual && !asked && leader && !(a.buffers == 1 && a.pre != nullptr)) {
+            ask_residual(row0, col0 + h * 32, tile);
+          }
+          asked = false;
         }
         Two v[16];
         if constexpr (kParts == 3) {
@@ -527,7 +531,6 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
         } else {
           uint32_t raw[32];
           dev::tmem_load32(acc + h * 32, raw);
-          if (h > 0 && direct) residual.load(a, row0 + row, col0 + h * 32);
           dev::tmem_load_wait();
           if (h + 1 == kHalves) free_set(acc_empty, release, set);
 #pragma unroll
@@ -583,22 +586,45 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
           apply(CND_ACT_SILU);
         }
         if (a.residual != nullptr) {
-          if (!a.vector_residual) {
-            // rows that are not 16-byte aligned come through the staging tile
-            if (h % kHalvesPerUnit == 0) {
+          if (h % kHalvesPerUnit == 0) {
+            if (a.tma_residual) {
+              if (a.buffers == 1 && a.pre != nullptr && leader) ask_residual(row0, unit_col, tile);
+              if (!dev::mbar_wait_warp(&residual_full[group], residual_phase, err, kSiteResidual,
+                                       a.timeout_ns)) {
+                ok = false;
+              }
+              residual_phase ^= 1u;
+            } else {
+              // rows that are not 16-byte aligned
               copy_unit<false, Out>(tile, const_cast<Out*>(static_cast<const Out*>(a.residual)), row0,
                                     unit_col, a.m, a.n, quarter, lane);
               dev::named_barrier(2 + group, kGroupThreads);
             }
-            residual.take(tile, row, h % kHalvesPerUnit);
-          } else if (kParts == 3) {
-            residual.load(a, row0 + row, col0 + h * 32);
           }
+          Residual<Out> residual;
+          residual.take(tile, row, h % kHalvesPerUnit);
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = add2(v[i], residual.pair(i));
         }
         stage_row<Out>(tile, row, h % kHalvesPerUnit, v);
         if (unit_done) {
+          if (a.tma_residual && a.sets == 2) {
+            // the next unit's residual: the next of this tile, or the first of the next tile
+            int64_t next_row = row0, next_col = unit_col + kUnit;
+            bool more = h + 1 < kHalves;
+            if (!more && item + workers < items) {
+              int next_m, next_n;
+              tile_of(a, (item + workers) / a.splits, &next_m, &next_n);
+              next_row = static_cast<int64_t>(next_m * kPair + static_cast<int>(rank)) * kBM;
+              next_col = static_cast<int64_t>(next_n) * kBN + group * kGroupCols;
+              more = true;
+            }
+            if (more && leader) {
+              dev::bulk_wait_group_read<0>();  // the other tile's store, a unit ago
+              ask_residual(next_row, next_col, own + buffer * kUnitBytes);
+            }
+            asked = more;
+          }
           dev::fence_proxy_async();
           dev::named_barrier(2 + group, kGroupThreads);
           if (a.tma_out) {
@@ -810,8 +836,9 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts) {
         best_cost = cost;
         // Four epilogue groups (four warps a scheduler) where the epilogue is the longer part:
         // with two, waits for TMEM, exponentials and staging left a scheduler issuing 27 % of
-        // the time (1M x 64 -> 256 GELU: 428 us against 320). From a depth of 1024 on two
-        // groups and a sixth stage win (4096 x 1024 -> 4096: 30.6 us against 36.4).
+        // the time (1M x 64 -> 256 GELU: 383 us against 310). From a depth of 1024 on two
+        // groups and more operand stages win (16384 x 1024 -> 4096 GELU: 123 us against 125,
+        // without an activation 103 against 116).
         const int groups = c.bn == 64 ? 1 : c.bn == 256 && blocks / splits <= 8 ? 4 : 2;
         best = ProductPlan{c.pair, c.bn, static_cast<int>(splits), groups};
       }
@@ -854,7 +881,7 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
   if (p.parts == 3) {
     a.buffers = 1;
   } else if (plan.pair == 2) {
-    a.buffers = plan.groups == 4 || wants_pre ? 2 : 1;
+    a.buffers = plan.groups == 4 || wants_pre || (!split && p.residual != nullptr) ? 2 : 1;
   } else {
     a.buffers = wants_pre ? 4 : 2;
   }
@@ -901,11 +928,15 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
     a.d = p.d;
     a.pre = p.pre;
     a.act = p.act;
-    a.vector_residual = aligned16(p.residual) && p.n * size % 16 == 0;
+    a.tma_residual = p.residual != nullptr && aligned16(p.residual) && p.n * size % 16 == 0;
     a.tma_out = p.n * size % 16 == 0 && aligned16(p.d) && aligned16(p.pre);
     if (a.tma_out &&
         (!encode_output(&maps.out, p.d, p.dtype, p.m, p.n, p.n) ||
          (p.pre != nullptr && !encode_output(&maps.pre, p.pre, p.dtype, p.m, p.n, p.n)))) {
+      return fail(CND_ERR_CUDA, "linear: encoding an output's tensor map failed");
+    }
+    if (a.tma_residual && !encode_output(&maps.residual, const_cast<void*>(p.residual), p.dtype, p.m,
+                                         p.n, p.n)) {
       return fail(CND_ERR_CUDA, "linear: encoding an output's tensor map failed");
     }
   }
