@@ -22,7 +22,8 @@ extern "C" {
  *   mean = sum(x) / width, rstd = 1 / sqrt(sum((x - mean)^2) / width + eps),
  *   y = (x - mean) * rstd * weight + bias.
  * x and dy rows start x_stride / dy_stride elements apart (>= width); y and dx are dense.
- * weight and bias ([width], either may be NULL) have type param_dtype: `dtype`, or CND_F32.
+ * eps >= 0. weight and bias ([width], either may be NULL) have type param_dtype: `dtype`, or
+ * CND_F32.
  * stats receives mean and rstd per row ([2][rows] float32, float64 for CND_F64; NULL in
  * cnd_layer_norm_forward when no backward follows).
  * The backward fills the gradients selected by output_mask = {dx, dweight, dbias}:

@@ -4,7 +4,8 @@ A drop-in for the native backend of lyehe/torch-convnd 0.5.0: the same
 ``torch_convnd::conv_nd`` / ``conv_nd_backward`` operators, the ``ConvNd`` /
 ``Conv1d``..``Conv4d`` modules and the ``conv_nd`` function. Importing the package
 defines the operator schemas and loads the prebuilt native libraries when they exist; it
-never compiles anything.
+never compiles anything. Beside the convolutions stand ``layer_norm``, ``linear`` and
+``gated_recurrence``, and ``RecurrentConvBlock``, which runs them together.
 """
 
 from ._geometry import DEFAULT_WORKSPACE_BYTES
@@ -22,6 +23,7 @@ from ._partial import PartialConvOutput, partial_conv_nd
 from .functional import conv_nd
 from .modules import Conv1d, Conv2d, Conv3d, Conv4d, ConvNd, PartialConvNd
 from .onnx import export_onnx
+from .sequence import RecurrentConvBlock
 
 __version__ = "0.5.0+b200.1"
 
@@ -38,6 +40,7 @@ __all__ = [
     "ConvNd",
     "PartialConvNd",
     "PartialConvOutput",
+    "RecurrentConvBlock",
     "channels_last",
     "conv_nd",
     "device_status",

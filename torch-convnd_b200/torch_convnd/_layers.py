@@ -49,7 +49,7 @@ def layer_norm(
     Statistics and sums are float32 (float64 for a float64 input). ``weight`` and ``bias``
     are vectors of the last dimension's size, of the input's dtype or float32. The result is
     contiguous; an input whose rows have unit stride and one common distance is read in
-    place. First derivatives only.
+    place. ``eps`` must not be negative. First derivatives only.
     """
     if not is_loaded():
         load_native()

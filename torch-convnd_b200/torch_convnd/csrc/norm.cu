@@ -1342,6 +1342,7 @@ int cnd_layer_norm_forward(int32_t dtype, int32_t param_dtype, int64_t rows, int
   clear_error();
   int rc = check_norm("cnd_layer_norm_forward", dtype, param_dtype, rows, width, x_stride);
   if (rc != CND_OK) return rc;
+  if (!(eps >= 0)) return fail(CND_ERR_INVALID, "cnd_layer_norm_forward: eps must be nonnegative");
   if (rows == 0) return CND_OK;
   if (x == nullptr || y == nullptr) {
     return fail(CND_ERR_INVALID, "cnd_layer_norm_forward: x and y must not be NULL");
