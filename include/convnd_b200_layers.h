@@ -51,8 +51,8 @@ CND_API int cnd_layer_norm_backward(int32_t dtype, int32_t param_dtype, int64_t 
  * terms each and the six products above 2^-24 are summed (float32 accuracy; a non-finite
  * operand gives a non-finite result, but an infinity may come out as NaN); float64 runs on
  * the CUDA cores. cnd_linear_forward writes z to `pre` (same shape and type as y) when it is
- * not NULL; the backward of an activation needs it. x, weight, dy and pre are 16-byte aligned
- * (float64: their natural alignment):
+ * not NULL; the backward of an activation needs it. x, weight, dy, pre and dx are 16-byte
+ * aligned (float64: their natural alignment):
  *   dz = dy * act'(z), dx = dz W, dW = dz^T x, dbias = column sums of dz
  * (the residual's gradient is dy itself). `pre` may be NULL for CND_ACT_NONE. The
  * gradients selected by output_mask = {dx, dW, dbias} are written; dy is dense. */

@@ -10,6 +10,7 @@ kept in T (the pre-activation and dz of a 16-bit linear layer) adds eps(T) times
 from __future__ import annotations
 
 import math
+import threading
 
 import pytest
 import torch
@@ -331,6 +332,18 @@ def test_linear_empty_rows_and_frozen_parts():
 
 @gpu
 @pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("m,k,n", [
+    (8192, 64, 256), (8193, 64, 64), (20000, 8, 8), (37889, 40, 200), (50001, 64, 136), (8320, 16, 72)])
+def test_linear_tall_and_thin(m, k, n, act, dtype):
+    x, w, b, _ = linear_inputs(m, k, n, dtype)
+    linear_case(x, w, b, act=act)
+    wide = torch.cat([x, x.flip(0)], 1)
+    linear_case(wide[:, k:], w, act=act, seed=10)  # rows twice as far apart, no bias
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
 def test_linear_nonfinite_rows_stay_alone(dtype):
     x, w, b, _ = linear_inputs(140, 72, 40, dtype)
     clean = torch_convnd.linear(x, w, b)
@@ -585,6 +598,30 @@ def test_repeated_calls_give_the_same_bits_on_any_stream():
             for a, c in zip(first, second):
                 assert torch.equal(a, c), name
     torch_convnd.device_status()
+
+
+@gpu
+@pytest.mark.parametrize("rows", [256, 8192])
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_linear_in_a_new_thread(rows, act):
+    """A thread that has made no CUDA call yet (an autograd worker's first backward)."""
+    x, w, _, _ = linear_inputs(rows, 64, 128, torch.bfloat16)
+    dy = randn((rows, 128), torch.bfloat16, 5)
+    ops = torch.ops.torch_convnd
+    def run():
+        _, pre = ops.linear_train(x, w, None, None, act)
+        return ops.linear_backward(dy, pre, x, w, act, [True, True, False])[:2]
+    def backward_only():
+        found.append(ops.linear_backward(dy, pre, x, w, act, [True, True, False])[:2])
+    found, expected = [], run()
+    _, pre = ops.linear_train(x, w, None, None, act)
+    for target in (backward_only, lambda: found.append(run())):
+        thread = threading.Thread(target=target)
+        thread.start()
+        thread.join()
+    assert len(found) == 2
+    for got in found:
+        assert all(torch.equal(g, e) for g, e in zip(got, expected))
 
 
 @gpu

@@ -31,7 +31,7 @@ SHIM_LIBRARY = LIB_DIR / "_C.so"
 OBJECT_DIR = LIB_DIR / "build"
 
 CORE_SOURCES = ["problem.cpp", "capi.cu", "fprop.cu", "tc_conv.cu", "pack.cu", "generic.cu",
-                "norm.cu", "linear.cu", "product.cu", "recurrence.cu"]
+                "norm.cu", "linear.cu", "product.cu", "thin.cu", "recurrence.cu"]
 SHIM_SOURCES = ["shim.cpp", "shim_layers.cpp"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -6,8 +6,9 @@
 // the products is one kernel here, prepare_kernel: it reads a matrix once and writes it as a
 // product's operand, multiplied by the activation's slope on the way (dz), split into three
 // bfloat16 terms (float32), or with rows padded to 16 bytes (sizes that TMA cannot address),
-// and sums its columns (dbias). Operands that TMA can read as they lie are not copied. float64
-// runs on the CUDA cores.
+// and sums its columns (dbias). Operands that TMA can read as they lie are not copied. The
+// backward of thin 16-bit layers with an activation is one kernel (thin.cu). float64 runs on
+// the CUDA cores.
 #include <algorithm>
 
 #include "activation.cuh"
@@ -270,6 +271,16 @@ void with_dtype(int dtype, F&& f) {
   }
 }
 
+void join_columns(int dtype, const void* sums, int count, int64_t width, void* out,
+                  cudaStream_t stream) {
+  with_dtype(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    column_join_kernel<T><<<static_cast<unsigned>((width + 31) / 32), kJoinWarps * 32, 0, stream>>>(
+        sums, count, width, static_cast<T*>(out));
+  });
+  count_launch();
+}
+
 // Elements between the rows of a prepared operand: whole 16-byte units, and whole 128-byte
 // lines where that costs at most an eighth more (a 64-byte piece of a row that starts off a
 // 32-byte sector is three sectors: float32 1999 x 771 -> 1280 took 46 us, 768 -> 1280 32).
@@ -280,6 +291,11 @@ int64_t row_pitch(int64_t width) {
   }
   return (width + 7) / 8 * 8;
 }
+// Rows from which the one-pass backward of thin layers is taken: two of its tiles. At 512 rows
+// it takes 23 us for 64 -> 256 in bf16 and separate launches 27, at 8192 rows 25 and 33, at
+// 262144 rows 90 and 158; for 8 -> 8 14 and 23, 16 and 29, 41 and 84.
+constexpr int64_t kThinRows = 256;
+
 size_t up1024(size_t v) { return (v + 1023) / 1024 * 1024; }
 
 // Row ranges of prepare_kernel's grid: about eight blocks an SM, 32 rows or more each.
@@ -333,6 +349,14 @@ bool copies_dz(const cnd_linear& p) {
   return p.dtype == CND_F32 || p.activation != CND_ACT_NONE || p.out_features % 8 != 0;
 }
 
+// Whether the backward takes the one-pass kernel of thin layers.
+bool one_pass(const cnd_linear& p, const int32_t mask[3]) {
+  return (p.dtype == CND_BF16 || p.dtype == CND_F16) && p.activation != CND_ACT_NONE && mask[0] &&
+         mask[1] && p.in_features <= kThinIn && p.out_features <= kThinOut &&
+         p.in_features % 8 == 0 && p.out_features % 8 == 0 && p.x_stride % 8 == 0 &&
+         p.rows >= kThinRows && p.rows < INT32_MAX - 128;
+}
+
 // Workspace of a call: byte offsets of its regions.
 struct Layout {
   size_t dz = 0, x = 0, w = 0, sums = 0, splits = 0, total = 0;
@@ -358,6 +382,12 @@ Layout forward_layout(const cnd_linear& p) {
 
 Layout backward_layout(const cnd_linear& p, const int32_t mask[3]) {
   Layout l;
+  if (one_pass(p, mask)) {
+    const size_t blocks = thin_blocks(p.rows), out = p.out_features;
+    if (mask[2]) l.sums = take(&l.total, blocks * out * sizeof(float));
+    l.splits = take(&l.total, blocks * out * p.in_features * sizeof(float));
+    return l;
+  }
   const bool products = mask[0] || mask[1];
   if (p.dtype == CND_F64) {
     if (p.activation != CND_ACT_NONE) {
@@ -548,14 +578,40 @@ int cnd_linear_backward(const cnd_linear* problem, const void* dy, const void* p
     return launch_status("cnd_linear_backward");
   }
   if (q.dtype != CND_F64 && (!aligned16(dy) || !aligned16(pre) || (want_w && !aligned16(x)) ||
-                             (want_x && !aligned16(weight)))) {
+                             (want_x && (!aligned16(weight) || !aligned16(dx))))) {
     return fail(CND_ERR_INVALID,
-                "cnd_linear_backward: dy, pre, x and weight must be 16-byte aligned");
+                "cnd_linear_backward: dy, pre, x, weight and dx must be 16-byte aligned");
   }
   const Layout l = backward_layout(q, output_mask);
   rc = check_workspace("cnd_linear_backward", workspace, workspace_bytes, l.total);
   if (rc != CND_OK) return rc;
   char* base = static_cast<char*>(workspace);
+  if (one_pass(q, output_mask)) {
+    ThinBackward t{};
+    t.dtype = q.dtype;
+    t.act = q.activation;
+    t.rows = rows;
+    t.n = out;
+    t.k = in;
+    t.x_stride = q.x_stride;
+    t.dy = dy;
+    t.z = pre;
+    t.x = x;
+    t.w = weight;
+    t.dx = dx;
+    t.dw = reinterpret_cast<float*>(base + l.splits);
+    t.db = want_b ? reinterpret_cast<float*>(base + l.sums) : nullptr;
+    rc = launch_thin_backward(t, stream);
+    if (rc != CND_OK) return rc;
+    Product p{};
+    p.m = out;
+    p.n = in;
+    p.dtype = q.dtype;
+    p.d = dweight;
+    join_partials(p, t.dw, thin_blocks(rows), out * in, in, stream);
+    if (want_b) join_columns(q.dtype, t.db, thin_blocks(rows), out, dbias, stream);
+    return launch_status("cnd_linear_backward");
+  }
   const bool copy = q.dtype == CND_F64 ? act : (want_x || want_w) && copies_dz(q);
   const int64_t pitch = q.dtype == CND_F64 ? out : row_pitch(out);
   if (copy || want_b) {
@@ -563,12 +619,7 @@ int cnd_linear_backward(const cnd_linear* problem, const void* dy, const void* p
             copy ? base + l.dz : nullptr, pitch, want_b ? base + l.sums : nullptr, stream);
   }
   if (want_b) {
-    with_dtype(q.dtype, [&](auto zero) {
-      using T = decltype(zero);
-      column_join_kernel<T><<<static_cast<unsigned>((out + 31) / 32), kJoinWarps * 32, 0, stream>>>(
-          base + l.sums, prepare_ranges(rows, out), out, static_cast<T*>(dbias));
-    });
-    count_launch();
+    join_columns(q.dtype, base + l.sums, prepare_ranges(rows, out), out, dbias, stream);
   }
   if (q.dtype == CND_F64) {
     DoubleProduct p{};

@@ -425,6 +425,8 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
     };
     int set = 0, cross = 0, buffer = 0;
     uint32_t set_phase = 0, residual_phase = 0;
+    // Once false, on without waiting: the named barriers take all warps of a group, and one that
+    // left them would hold the others for good.
     bool ok = true;
     // The residual's tile of a unit comes by TMA into the staging tile that its output will
     // take: each thread then reads its row's part and writes the output over it. It is asked
@@ -433,12 +435,13 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
     // there: 1M x 64 -> 256 in bf16 475 us, by TMA 260, without a residual 192;
     // 16384 x 1024 -> 4096 147 us, by TMA 116.)
     const auto ask_residual = [&](int64_t row0, int64_t col, uint8_t* into) {
+      if (!ok) return;
       dev::mbar_arrive_expect_tx(&residual_full[group], kUnitBytes);
       dev::tma_load_2d(into, &maps.residual, &residual_full[group], static_cast<int>(col),
                        static_cast<int>(row0));
     };
     bool asked = false;  // the coming unit's residual is on its way
-    for (int item = worker; item < items && ok; item += workers) {
+    for (int item = worker; item < items; item += workers) {
       const int split = item % a.splits;
       int tm, tn;
       tile_of(a, item / a.splits, &tm, &tn);
@@ -458,10 +461,7 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
         const int first = static_cast<int>(static_cast<int64_t>(a.k_blocks) * split / a.splits);
         const int last = static_cast<int>(static_cast<int64_t>(a.k_blocks) * (split + 1) / a.splits);
         for (int kb = first; kb < last; kb += kChunkBlocks) {
-          if (!wait_warp<kPair>(&acc_full[set], set_phase, err, kSiteEpilogue, a.timeout_ns)) {
-            ok = false;
-            break;
-          }
+          ok = ok && wait_warp<kPair>(&acc_full[set], set_phase, err, kSiteEpilogue, a.timeout_ns);
           dev::tc_fence_after();
 #pragma unroll
           for (int h = 0; h < kHalves; ++h) {
@@ -479,7 +479,6 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
             set_phase ^= 1u;
           }
         }
-        if (!ok) break;
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
           uint32_t v[32];
@@ -491,10 +490,7 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
         free_set(cross_empty, release_cross, cross);
         cross ^= 1;
       } else {
-        if (!wait_warp<kPair>(&acc_full[set], set_phase, err, kSiteEpilogue, a.timeout_ns)) {
-          ok = false;
-          break;
-        }
+        ok = ok && wait_warp<kPair>(&acc_full[set], set_phase, err, kSiteEpilogue, a.timeout_ns);
         dev::tc_fence_after();
       }
 
@@ -589,10 +585,8 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
           if (h % kHalvesPerUnit == 0) {
             if (a.tma_residual) {
               if (a.buffers == 1 && a.pre != nullptr && leader) ask_residual(row0, unit_col, tile);
-              if (!dev::mbar_wait_warp(&residual_full[group], residual_phase, err, kSiteResidual,
-                                       a.timeout_ns)) {
-                ok = false;
-              }
+              ok = ok && dev::mbar_wait_warp(&residual_full[group], residual_phase, err,
+                                             kSiteResidual, a.timeout_ns);
               residual_phase ^= 1u;
             } else {
               // rows that are not 16-byte aligned
@@ -655,6 +649,10 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
           set_phase ^= 1u;
         }
       }
+    }
+    if (asked) {  // a wait ran out: the tile on its way has a bounded time to land
+      dev::mbar_wait_warp(&residual_full[group], residual_phase, err, kSiteDrain,
+                          a.timeout_ns / 8 + 1);
     }
     if (leader) dev::bulk_wait_group<0>();
   }
@@ -765,20 +763,6 @@ bool encode_operand(CUtensorMap* map, const Operand& o, int64_t rows, int64_t k,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool encode_output(CUtensorMap* map, void* d, int dtype, int64_t rows, int64_t n, int64_t pitch) {
-  const int size = element_size(dtype);
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch) * size};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), kBM};
-  const cuuint32_t ones[2] = {1, 1};
-  const CUtensorMapDataType type = dtype == CND_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                   : dtype == CND_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  return encoder()(map, type, 2, d, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 using Kernel = void (*)(Maps, KernelArgs);
 
 template <typename Out>
@@ -801,6 +785,23 @@ Kernel pick(const ProductPlan& plan, int parts) {
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 }  // namespace
+
+bool encode_matrix(CUtensorMap* map, void* d, int dtype, int64_t rows, int64_t n, int64_t pitch,
+                   int box_rows) {
+  const int size = element_size(dtype);
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch) * size};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size),
+                             static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t ones[2] = {1, 1};
+  const CUtensorMapDataType type = dtype == CND_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == CND_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (encoder() == nullptr) return false;
+  return encoder()(map, type, 2, d, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts) {
   // Microseconds, fitted to runs over 16 to 4096 rows and 1024 or 4096 of n and k: a launch,
@@ -851,6 +852,27 @@ size_t product_workspace(const ProductPlan& plan, int64_t m, int64_t n) {
   if (plan.splits <= 1) return 0;
   return static_cast<size_t>(plan.splits) * round_up(m, kBM * plan.pair) * round_up(n, 4) *
          sizeof(float);
+}
+
+void join_partials(const Product& p, const float* partials, int splits, int64_t stride,
+                   int64_t pitch, cudaStream_t stream) {
+  const int64_t quads = p.m * (pitch / 4);
+  const bool many = splits >= 16;
+  const int per_block = many ? 32 : 256;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(
+      (quads + per_block - 1) / per_block, static_cast<int64_t>(sm_count()) * 8));
+  const auto join = [&](auto* kernel_join) {
+    kernel_join<<<grid, 256, 0, stream>>>(partials, splits, stride, pitch, p.m, p.n, p.bias,
+                                          p.residual, p.d, p.pre, p.act);
+  };
+  if (p.dtype == CND_F32) {
+    many ? join(join_kernel<float, 8>) : join(join_kernel<float, 1>);
+  } else if (p.dtype == CND_BF16) {
+    many ? join(join_kernel<__nv_bfloat16, 8>) : join(join_kernel<__nv_bfloat16, 1>);
+  } else {
+    many ? join(join_kernel<__half, 8>) : join(join_kernel<__half, 1>);
+  }
+  count_launch();
 }
 
 int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
@@ -908,6 +930,14 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
   a.error = device_error_word();
   a.timeout_ns = wait_timeout_ns();
   if (a.error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
+  const Kernel kernel = out_dtype == CND_F32    ? pick<float>(plan, p.parts)
+                        : out_dtype == CND_BF16 ? pick<__nv_bfloat16>(plan, p.parts)
+                                                : pick<__half>(plan, p.parts);
+  // (a runtime call before the tensor maps: encoding needs the thread to have a context)
+  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(kSharedLimit));
+  if (e != cudaSuccess) return fail(CND_ERR_CUDA, "linear: %s", cudaGetErrorString(e));
   Maps maps{};
   if (!encode_operand(&maps.a, p.a, p.m, p.k, p.parts, p.bf16, kBM) ||
       !encode_operand(&maps.b, p.b, p.n, p.k, p.parts, p.bf16, plan.bn / plan.pair)) {
@@ -917,8 +947,8 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
   if (split) {
     // partial tiles below one another, each split's rows rounded up to whole tiles
     a.tma_out = 1;
-    if (!encode_output(&maps.out, workspace, CND_F32, round_up(p.m, bm) * plan.splits, pitch,
-                       pitch)) {
+    if (!encode_matrix(&maps.out, workspace, CND_F32, round_up(p.m, bm) * plan.splits, pitch,
+                       pitch, kBM)) {
       return fail(CND_ERR_CUDA, "linear: encoding the partial sums' tensor map failed");
     }
   } else {
@@ -931,18 +961,15 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
     a.tma_residual = p.residual != nullptr && aligned16(p.residual) && p.n * size % 16 == 0;
     a.tma_out = p.n * size % 16 == 0 && aligned16(p.d) && aligned16(p.pre);
     if (a.tma_out &&
-        (!encode_output(&maps.out, p.d, p.dtype, p.m, p.n, p.n) ||
-         (p.pre != nullptr && !encode_output(&maps.pre, p.pre, p.dtype, p.m, p.n, p.n)))) {
+        (!encode_matrix(&maps.out, p.d, p.dtype, p.m, p.n, p.n, kBM) ||
+         (p.pre != nullptr && !encode_matrix(&maps.pre, p.pre, p.dtype, p.m, p.n, p.n, kBM)))) {
       return fail(CND_ERR_CUDA, "linear: encoding an output's tensor map failed");
     }
-    if (a.tma_residual && !encode_output(&maps.residual, const_cast<void*>(p.residual), p.dtype, p.m,
-                                         p.n, p.n)) {
+    if (a.tma_residual && !encode_matrix(&maps.residual, const_cast<void*>(p.residual), p.dtype, p.m,
+                                         p.n, p.n, kBM)) {
       return fail(CND_ERR_CUDA, "linear: encoding an output's tensor map failed");
     }
   }
-  const Kernel kernel = out_dtype == CND_F32    ? pick<float>(plan, p.parts)
-                        : out_dtype == CND_BF16 ? pick<__nv_bfloat16>(plan, p.parts)
-                                                : pick<__half>(plan, p.parts);
   const int items = a.tiles_m * a.tiles_n * a.splits;
   const int slots = sm_count() / plan.pair;
   cudaLaunchConfig_t config{};
@@ -958,32 +985,12 @@ int launch_product(const Product& p, const ProductPlan& plan, void* workspace,
     config.attrs = &attribute;
     config.numAttrs = 1;
   }
-  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(kSharedLimit));
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&config, kernel, maps, a);
+  e = cudaLaunchKernelEx(&config, kernel, maps, a);
   if (e != cudaSuccess) return fail(CND_ERR_CUDA, "linear: %s", cudaGetErrorString(e));
   count_launch();
   if (split) {
-    const int64_t quads = p.m * (pitch / 4);
-    const bool many = plan.splits >= 16;
-    const int per_block = many ? 32 : 256;
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(
-        (quads + per_block - 1) / per_block, static_cast<int64_t>(sm_count()) * 8));
-    const int64_t stride = round_up(p.m, bm) * pitch;
-    const float* partials = static_cast<const float*>(workspace);
-    const auto join = [&](auto* kernel_join) {
-      kernel_join<<<grid, 256, 0, stream>>>(partials, plan.splits, stride, pitch, p.m, p.n, p.bias,
-                                            p.residual, p.d, p.pre, p.act);
-    };
-    if (p.dtype == CND_F32) {
-      many ? join(join_kernel<float, 8>) : join(join_kernel<float, 1>);
-    } else if (p.dtype == CND_BF16) {
-      many ? join(join_kernel<__nv_bfloat16, 8>) : join(join_kernel<__nv_bfloat16, 1>);
-    } else {
-      many ? join(join_kernel<__half, 8>) : join(join_kernel<__half, 1>);
-    }
-    count_launch();
+    join_partials(p, static_cast<const float*>(workspace), plan.splits, round_up(p.m, bm) * pitch,
+                  pitch, stream);
   }
   return launch_status("linear");
 }

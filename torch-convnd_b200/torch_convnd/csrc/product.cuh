@@ -2,6 +2,7 @@
 // with bias, activation, pre-activation output and residual in the epilogue.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -41,6 +42,32 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts);
 
 // float32 partial sums of a split product, [splits][m][round up n to 4]; 0 without splits.
 size_t product_workspace(const ProductPlan& plan, int64_t m, int64_t n);
+
+// Adds `splits` float32 partial results [m][pitch], `stride` elements apart, in order and applies
+// the epilogue of `p`.
+void join_partials(const Product& p, const float* partials, int splits, int64_t stride,
+                   int64_t pitch, cudaStream_t stream);
+
+// Tensor map of a [rows][n] matrix, rows `pitch` elements apart: boxes of 128 bytes by box_rows
+// rows with the 128-byte swizzle.
+bool encode_matrix(CUtensorMap* map, void* d, int dtype, int64_t rows, int64_t n, int64_t pitch,
+                   int box_rows);
+
+// The one-pass backward of a 16-bit layer with an activation, up to kThinIn input and kThinOut
+// output features (thin.cu). All addresses and rows are whole 16-byte units.
+constexpr int kThinIn = 64, kThinOut = 256;
+
+struct ThinBackward {
+  int dtype, act;
+  int64_t rows, n, k, x_stride;  // n output features, k input features
+  const void *dy, *z, *x, *w;
+  void* dx;
+  float* dw;  // partial sums [thin_blocks()][n][k]
+  float* db;  // partial sums [thin_blocks()][n], or NULL
+};
+
+int thin_blocks(int64_t rows);
+int launch_thin_backward(const ThinBackward& p, cudaStream_t stream);
 
 int launch_product(const Product& p, const ProductPlan& plan, void* workspace, cudaStream_t stream);
 
