@@ -441,21 +441,26 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
                        static_cast<int>(row0));
     };
     bool asked = false;  // the coming unit's residual is on its way
+    int bias_tile = -1;
     for (int item = worker; item < items; item += workers) {
       const int split = item % a.splits;
       int tm, tn;
       tile_of(a, item / a.splits, &tm, &tn);
       const int64_t row0 = static_cast<int64_t>(tm * kPair + static_cast<int>(rank)) * kBM;
       const int64_t col0 = static_cast<int64_t>(tn) * kBN + group * kGroupCols;
-      // bias of the tile's columns, after every thread has finished the previous tile's
-      dev::named_barrier(1, 32 * kEpilogueWarps);
-      for (int c = epi; c < kBN; c += 32 * kEpilogueWarps) {
-        const int64_t column = static_cast<int64_t>(tn) * kBN + c;
-        bias_s[c] = a.bias != nullptr && column < a.n
-                        ? widen(static_cast<const Out*>(a.bias)[column])
-                        : 0.0f;
+      // bias of the tile's columns, where they change and after every thread has finished the
+      // previous tile's
+      if (tn != bias_tile) {
+        bias_tile = tn;
+        dev::named_barrier(1, 32 * kEpilogueWarps);
+        for (int c = epi; c < kBN; c += 32 * kEpilogueWarps) {
+          const int64_t column = static_cast<int64_t>(tn) * kBN + c;
+          bias_s[c] = a.bias != nullptr && column < a.n
+                          ? widen(static_cast<const Out*>(a.bias)[column])
+                          : 0.0f;
+        }
+        dev::named_barrier(1, 32 * kEpilogueWarps);
       }
-      dev::named_barrier(1, 32 * kEpilogueWarps);
       float sums[kParts == 3 ? kHalves : 1][32];
       if constexpr (kParts == 3) {
         const int first = static_cast<int>(static_cast<int64_t>(a.k_blocks) * split / a.splits);
