@@ -8,17 +8,6 @@
 namespace cnd {
 namespace layers {
 
-__device__ __forceinline__ float exp2_fast(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float reciprocal_fast(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
 // Phi(-|v|) and exp(-v^2 / 2) of two values, with |v| cut at 6 in `size`:
 //   Phi(-a) = Q(a) exp(-a^2 / 2),
 // where Q(a) = erfcx(a / sqrt 2) / 2 is smooth and falls from 0.5 to 0.066 on [0, 6]. Q is the

@@ -88,6 +88,18 @@ __device__ __forceinline__ Two add2(Two a, Two b) {
 }
 __device__ __forceinline__ Two same(float v) { return two(v, v); }
 
+// 2^v and 1 / v to a few units in the last place, results below 2^-126 as zero.
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // V elements at a 16-byte aligned address as pairs, and back (rounded once).
 template <typename T, int V>
 __device__ __forceinline__ void load_twos(const void* p, Two (&v)[V / 2]) {

@@ -83,19 +83,20 @@ __device__ __forceinline__ int steps_here(int64_t left, int most) {
 }
 
 // f = sigmoid(g) and 1 - f, each to full relative accuracy (exact 0 and 1 at +-inf). For
-// 16-bit tensors by the fast exponential and reciprocal, good to 2^-20.
+// 16-bit tensors by the fast exponential and reciprocal, good to 2^-20; what falls below
+// 2^-126 (|g| > 87) is zero.
 template <typename T, typename A>
 __device__ __forceinline__ void gates(A g, A* f, A* keep) {
   A e, r;
   if constexpr (sizeof(T) == 2) {
-    e = __expf(-fabsf(g));
-    r = __fdividef(1.0f, 1.0f + e);
+    e = exp2_fast(-fabsf(g * 1.44269504089f));
+    r = reciprocal_fast(1.0f + e);
   } else {
     e = exp(-fabs(g));
     const A d = A(1) + e;
     if constexpr (sizeof(T) == 4) {
       // d is in [1, 2]: the approximate reciprocal and one Newton step
-      r = __fdividef(1.0f, d);
+      r = reciprocal_fast(d);
       r = fmaf(r, fmaf(-d, r, 1.0f), r);
     } else {
       r = A(1) / d;
@@ -399,10 +400,15 @@ struct Steps {
     Held<T>::part(value, w);
     if constexpr (kAdjacent) {
       if (!live[0]) return;
-      Pack<T, kColumns> v;
+      char* to = static_cast<char*>(base) + (first[0] + ahead);
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint32_t*>(to) = narrow2<T>(value);
+      } else {
+        Pack<T, kColumns> v;
 #pragma unroll
-      for (int i = 0; i < kColumns; ++i) v.v[i] = narrow<T>(w[i]);
-      *reinterpret_cast<Pack<T, kColumns>*>(static_cast<char*>(base) + (first[0] + ahead)) = v;
+        for (int i = 0; i < kColumns; ++i) v.v[i] = narrow<T>(w[i]);
+        *reinterpret_cast<Pack<T, kColumns>*>(to) = v;
+      }
     } else {
 #pragma unroll
       for (int p = 0; p < kColumns; ++p) {
@@ -435,11 +441,26 @@ __device__ __forceinline__ typename Held<T>::P held(const Pack<T, N>& p) {
 template <typename T, int N>
 __device__ __forceinline__ void held_gates(const Pack<T, N>& g, typename Held<T>::P* f,
                                            typename Held<T>::P* keep) {
-  typename Wide<T>::type w[N], v[N];
+  if constexpr (sizeof(T) == 2) {  // gates() in pairs
+    const Two pair = held<T>(g);
+    float lo, hi, m0, m1, r0, r1, s0, s1;
+    unpack(pair, &lo, &hi);
+    unpack(mul2(pair, same(1.44269504089f)), &m0, &m1);
+    const Two e = two(exp2_fast(-fabsf(m0)), exp2_fast(-fabsf(m1)));
+    float d0, d1;
+    unpack(add2(e, same(1.0f)), &d0, &d1);
+    r0 = reciprocal_fast(d0);
+    r1 = reciprocal_fast(d1);
+    unpack(mul2(e, two(r0, r1)), &s0, &s1);
+    *f = two(lo >= 0.0f ? r0 : s0, hi >= 0.0f ? r1 : s1);
+    *keep = two(lo >= 0.0f ? s0 : r0, hi >= 0.0f ? s1 : r1);
+  } else {
+    typename Wide<T>::type w[N], v[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) gates<T>(widen(g.v[i]), &w[i], &v[i]);
-  *f = Held<T>::join(w);
-  *keep = Held<T>::join(v);
+    for (int i = 0; i < N; ++i) gates<T>(widen(g.v[i]), &w[i], &v[i]);
+    *f = Held<T>::join(w);
+    *keep = Held<T>::join(v);
+  }
 }
 
 // Values kept per column ([..][columns] of type Wide<T>), zero where there are none.
