@@ -15,8 +15,8 @@ namespace layers {
 // double-precision erfc by iteratively reweighted least squares at Chebyshev points); beyond
 // 6, Phi(-a) is below 1e-9. Used where the result is rounded to 16 bits (2^-11 and more):
 // half an instruction a value and step and one exponential, shared with phi. A
-// reciprocal beside the exponential costs 3 % more (1M x 64 -> 256 GELU 319 us against 310;
-// 192 without an activation).
+// reciprocal beside the exponential costs 3 % more (1M x 64 -> 256 GELU 319 us against 310,
+// where no activation took 192).
 __device__ __forceinline__ Two normal_tail(Two v, Two* size, Two* gauss) {
   float lo, hi;
   unpack(v, &lo, &hi);

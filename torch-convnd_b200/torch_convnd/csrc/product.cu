@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
     // take: each thread then reads its row's part and writes the output over it. It is asked
     // for while the unit before is worked on where there is a second tile, else once the
     // one tile is free. (Read by warps of the epilogue, a row each, it had waited for memory
-    // there: 1M x 64 -> 256 in bf16 475 us, by TMA 260, without a residual 192;
+    // there: 1M x 64 -> 256 in bf16 475 us, by TMA 253, without a residual 179;
     // 16384 x 1024 -> 4096 147 us, by TMA 116.)
     const auto ask_residual = [&](int64_t row0, int64_t col, uint8_t* into) {
       if (!ok) return;
@@ -449,7 +449,8 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
       const int64_t row0 = static_cast<int64_t>(tm * kPair + static_cast<int>(rank)) * kBM;
       const int64_t col0 = static_cast<int64_t>(tn) * kBN + group * kGroupCols;
       // bias of the tile's columns, where they change and after every thread has finished the
-      // previous tile's
+      // previous tile's (two barriers of all epilogue warps, 15 us of 1M x 64 -> 256's 313 when
+      // done for every tile)
       if (tn != bias_tile) {
         bias_tile = tn;
         dev::named_barrier(1, 32 * kEpilogueWarps);
@@ -842,7 +843,7 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts) {
         best_cost = cost;
         // Four epilogue groups (four warps a scheduler) where the epilogue is the longer part:
         // with two, waits for TMEM, exponentials and staging left a scheduler issuing 27 % of
-        // the time (1M x 64 -> 256 GELU: 383 us against 310). From a depth of 1024 on two
+        // the time (1M x 64 -> 256 GELU: 369 us against 263). From a depth of 1024 on two
         // groups and more operand stages win (16384 x 1024 -> 4096 GELU: 123 us against 125,
         // without an activation 103 against 116).
         const int groups = c.bn == 64 ? 1 : c.bn == 256 && blocks / splits <= 8 ? 4 : 2;

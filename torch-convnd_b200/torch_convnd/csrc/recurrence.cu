@@ -8,12 +8,16 @@
 // (a1, b1) then (a2, b2) is (a1 a2, a2 b1 + b2). So a thread reduces a few consecutive steps
 // to a map, a block composes its threads' maps in shared memory to find the state each of
 // them starts from, and the thread then walks its steps from that state: x, g and dy are
-// read once and stay in registers between the two walks. The work is bound by memory
-// traffic: 3 elements a step forward, 5 backward.
+// read once and stay in registers between the two walks. The traffic is 3 elements a step
+// forward, 5 backward. float32, 8 x 33 x 129600: 100 / 181 us, 4.1 / 3.8 TB/s. What is
+// between that and the 6.55 TB/s of a copy is latency: a block loads, composes, waits and
+// stores one after the other, and 128 registers leave room for two blocks on an SM. Most of
+// it is seen where 16-bit columns share the time axis (65536 x 512 bf16, 87 / 180 us).
 //
 // Column layout (inner > 1): the lanes of a warp hold two columns each, in packed float32
-// pairs, the warps of a block follow one another in time. Step layout (inner = 1, steps contiguous): the lanes of a
-// warp hold neighbouring runs of steps of one column and compose their maps by shuffles.
+// pairs, the warps of a block follow one another in time. Step layout (inner = 1, steps
+// contiguous): the lanes of a warp hold neighbouring runs of steps of one column and compose
+// their maps by shuffles.
 //
 // A block that has its columns to itself loops over the chunks of the time axis. Where
 // the columns are too few to fill the SMs, every (chunk, column block) is a block of its own
@@ -41,7 +45,10 @@ namespace layers {
 namespace {
 
 constexpr int kWarps = 8;       // most warps of a block
-constexpr int kGroup = 32;      // chunks that are composed without an intermediate state
+// Chunks that are composed without an intermediate state. Forward / backward, 65536 steps of
+// 512 and of 64 bf16 columns: 16 chunks 104 / 190 and 70 / 122 us, 32 chunks 103 / 194 and
+// 57 / 93, 64 chunks 121 / 224 and 45 / 73.
+constexpr int kGroup = 32;
 constexpr uint32_t kSiteForward = 0x601, kSiteBackward = 0x602;
 
 // Steps a thread holds: forward (by element size: what its registers take of two columns) and
@@ -334,7 +341,8 @@ __device__ __forceinline__ HeldMap<T> then(const HeldMap<T>& first, const HeldMa
 
 // The addresses of a thread's steps. Adjacent: its columns are neighbours read at once (two
 // 16-bit columns are 4 bytes); else they lie 32 apart, each warp reading 32 neighbours, which
-// needs no alignment. Step i of every tensor lies i strides behind the same offset.
+// needs no alignment (32768 bf16 columns of 1024 steps: forward 76 us adjacent, 87 apart).
+// Step i of every tensor lies i strides behind the same offset.
 // Offset: uint32_t bytes where the tensors are below 4 GB (one 32-bit addition serves all
 // tensors, whose bases stay in uniform registers), else int64_t.
 template <typename T, bool kAdjacent, typename Offset>
@@ -1055,9 +1063,11 @@ RecurrencePlan plan_recurrence(int dtype, int64_t outer, int64_t steps, int64_t 
   if (!p.along && steps <= kStateBlock) p.balanced = static_cast<int>((steps + p.warps - 1) / p.warps);
   p.column_blocks = p.along ? (columns + p.per_block - 1) / p.per_block
                             : (columns + 32 * held - 1) / (32 * held);
-  // Blocks of eight warps, at most three on an SM: with fewer than 2 blocks an SM, sharing the
-  // time axis fills the machine.
-  p.shared = p.chunks > 1 && p.column_blocks < 2 * 148;
+  // Too few column blocks to give each SM more than one share the time axis. bf16, 4096
+  // steps, forward / backward: 128 blocks 114 / 232 us alone and 90 / 180 shared, 160 blocks
+  // 131 / 264 and 106 / 220, 200 blocks 133 / 269 and 129 / 270; 2048 steps, 256 blocks 77 / 146
+  // and 89 / 175.
+  p.shared = p.chunks > 1 && p.column_blocks < 200;
   if (p.shared) {
     const int64_t padded = p.along ? columns : p.column_blocks * 32 * held;
     const int64_t groups = (p.chunks + kGroup - 1) / kGroup;
