@@ -114,7 +114,7 @@ def test_linear_forward_refuses(problem, change):
     ({"dtype": 7}, {}), ({"activation": -1}, {}), ({"rows": -1}, {}), ({"x_stride": 63}, {}),
     ({}, {"dy": None}), ({}, {"pre": None}), ({}, {"x": None}), ({}, {"w": None}),
     ({}, {"dx": None}), ({}, {"dw": None}), ({}, {"db": None}), ({}, {"mask": None}),
-    ({}, {"dy": A + 2})])
+    ({}, {"dy": A + 2}), ({}, {"dx": A + 2}), ({}, {"w": A + 4})])
 def test_linear_backward_refuses(problem, change):
     refused(linear_backward(problem, **change), INVALID, UNSUPPORTED)
 
