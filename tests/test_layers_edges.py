@@ -1,0 +1,148 @@
+"""The layer operators at the edges of their inputs: alignment, gaps, empty axes, tails.
+
+Where two calls do the same arithmetic on the same values the results have to be the same
+bits; elsewhere a bound is derived beside the test.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+import torch_convnd
+from test_layers import check, eps, linear_inputs, randn, recurrence_inputs
+from torch_convnd import _native
+
+gpu = pytest.mark.gpu
+
+
+def off_boundary(t):
+    """The same values, shape and strides (contiguous) one element past a 16-byte boundary."""
+    moved = torch.empty(t.numel() + 1, device=t.device, dtype=t.dtype)[1:].view(t.shape)
+    moved.copy_(t)
+    assert moved.data_ptr() % 16 != 0
+    return moved
+
+
+# ---- gated recurrence along the last axis: steps next to one another ---------------------
+
+
+def recurrence_backward(x, g, h0, dy):
+    leaves = [t.detach().requires_grad_() for t in (x, g, h0)]
+    y, _ = torch_convnd.gated_recurrence(*leaves, dim=x.ndim - 1)
+    return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32, torch.float64])
+@pytest.mark.parametrize("steps", [7, 301, 1001, 5003])
+def test_recurrence_gradients_do_not_depend_on_alignment(steps, dtype):
+    """Kept states lie where the backward looks for them, whatever starts off 16 bytes."""
+    x, g, h0 = recurrence_inputs((3, 7, steps), 2, dtype)
+    dy = randn((3, 7, steps), dtype, 5)
+    expected = recurrence_backward(x, g, h0, dy)
+    for moved in ((3,), (0,), (1,), (0, 1), (0, 1, 3)):
+        inputs = [off_boundary(t) if i in moved else t for i, t in enumerate((x, g, h0, dy))]
+        for name, got, ref in zip(("y", "dx", "dgate", "dinitial"), recurrence_backward(*inputs), expected):
+            assert torch.equal(got, ref), f"{name}, unaligned {moved}"
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_recurrence_gradient_through_concatenation(dtype):
+    """torch.cat hands its second part a gradient that starts inside a larger buffer."""
+    x, g, h0 = recurrence_inputs((1, 7, 1001), 2, dtype)
+    dy = randn((1, 8, 1001), dtype, 5)
+    leaves = [t.detach().requires_grad_() for t in (x, g, h0)]
+    y, _ = torch_convnd.gated_recurrence(*leaves, dim=2)
+    ahead = torch.zeros((1, 1, 1001), device="cuda", dtype=dtype)
+    grads = torch.autograd.grad(torch.cat([ahead, y], 1), leaves, dy)
+    for got, ref in zip(grads, recurrence_backward(x, g, h0, dy[:, 1:].clone())[1:]):
+        assert torch.equal(got, ref)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("steps", [301, 1101])
+def test_recurrence_step_layout_against_definition(steps, dtype):
+    """Bounds that follow each column's own memory: a rounding of step t reaches step t + k
+    times the gates between them, so the sum of those products (`reach`, the same recurrence
+    over ones) times a step's roundings bounds a state's error, and likewise the flow's. A
+    step rounds its gate (2^-20 with the fast exponential, four float32 roundings else),
+    the two products and the sum, and composed maps round each of theirs once more: 16."""
+    x, g, h0 = recurrence_inputs((2, 5, steps), 2, dtype)
+    dy = off_boundary(randn((2, 5, steps), dtype, 5))
+    y, dx, dgate, d0 = recurrence_backward(x, g, h0, dy)
+    u = 16 * (2.0**-20 if dtype == torch.bfloat16 else 2.0**-24)
+    xs, gs, ds = x.double(), g.double(), dy.double()
+    f, keep = torch.sigmoid(gs), torch.sigmoid(-gs)
+    before, states, reach, state, r = [], [], [], h0.double(), torch.zeros_like(h0).double()
+    for t in range(steps):
+        before.append(state)
+        state = f[..., t] * state + keep[..., t] * xs[..., t]
+        r = f[..., t] * r + 1
+        states.append(state)
+        reach.append(r)
+    before, states, reach = (torch.stack(v, -1) for v in (before, states, reach))
+    flow, total, memory, m = torch.zeros_like(state), [], [], torch.zeros_like(state)
+    for t in reversed(range(steps)):
+        total.append(flow + ds[..., t])
+        m = m + 1
+        memory.append(m)
+        flow, m = f[..., t] * total[-1], f[..., t] * m
+    total, memory = (torch.stack(v[::-1], -1) for v in (total, memory))
+    big, largest = max(xs.abs().max(), h0.abs().max()), ds.abs().max()
+    off_state, off_flow = u * big * reach, u * largest * memory
+    check(y, states, off_state, "y")
+    check(dx, total * keep, keep * off_flow + u * (total * keep).abs(), "dx")
+    slope = f * keep
+    check(dgate, total * (before - xs) * slope,
+          slope * (off_flow * (before - xs).abs() + total.abs() * (off_state + u * big)) * 1.01
+          + u * (total * (before - xs) * slope).abs(), "dgate")
+    check(d0, flow, off_flow[..., 0], "dinitial")
+
+
+@gpu
+def test_recurrence_c_abi_buffers_of_any_alignment():
+    """Outputs of another alignment than the inputs, in either pass."""
+    library = _native.core()
+    pointer, size = ctypes.c_void_p, ctypes.c_size_t
+    dims = [ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]
+    library.cnd_gated_recurrence_forward.argtypes = dims + [pointer] * 7 + [size, pointer]
+    library.cnd_gated_recurrence_backward.argtypes = dims + [pointer] * 10 + [size, pointer]
+    library.cnd_gated_recurrence_workspace_size.argtypes = dims
+    library.cnd_gated_recurrence_workspace_size.restype = size
+    columns, steps = 6, 1101
+    x, g, _ = recurrence_inputs((columns, steps), 1, torch.float32, initial=False)
+    dy = randn((columns, steps), torch.float32, 5)
+    problem = (2, columns, steps, 1)
+    blocks = library.cnd_gated_recurrence_blocks(*problem)
+    bytes_ = library.cnd_gated_recurrence_workspace_size(*problem)
+    workspace = torch.empty(max(bytes_, 1), device="cuda", dtype=torch.uint8)
+    stream = pointer(torch.cuda.current_stream().cuda_stream)
+
+    def step(moved):
+        def output():
+            t = torch.zeros_like(x)
+            return off_boundary(t) if moved[0] else t
+        y, last = output(), torch.empty(columns, device="cuda")
+        states = torch.empty((blocks, columns), device="cuda")
+        assert library.cnd_gated_recurrence_forward(
+            *problem, x.data_ptr(), g.data_ptr(), None, y.data_ptr(), last.data_ptr(),
+            states.data_ptr(), workspace.data_ptr(), bytes_, stream) == 0
+        moved = moved[1:]
+        dx, dgate, d0 = output(), output(), torch.empty(columns, device="cuda")
+        mask = (ctypes.c_int32 * 3)(1, 1, 1)
+        assert library.cnd_gated_recurrence_backward(
+            *problem, dy.data_ptr(), None, x.data_ptr(), g.data_ptr(), states.data_ptr(),
+            dx.data_ptr(), dgate.data_ptr(), d0.data_ptr(), mask, workspace.data_ptr(), bytes_,
+            stream) == 0
+        return y, last, dx, dgate, d0
+
+    expected = step((False, False))
+    for moved in ((True, False), (False, True), (True, True)):
+        for got, ref in zip(step(moved), expected):
+            assert torch.equal(got, ref), moved

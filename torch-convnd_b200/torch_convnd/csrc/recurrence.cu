@@ -760,18 +760,20 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 
 // ---- step layout -----------------------------------------------------------------------
 
-// Column c starts at element c * steps, off a 16-byte boundary by `shift` elements where steps
-// is no multiple of one. Its runs start `shift` elements earlier, so that every run is read and
-// written in aligned vectors; the column's first run then begins, like its last one ends, with
-// steps that do not exist and hold the state. A column takes `lanes` lanes of a warp (a short
-// column less than a warp, a block then several columns) or a block's warps one behind the
-// other.
+// Column c starts at element c * steps, off a 16-byte boundary of its tensor by `shift` elements
+// where steps is no multiple of one. Its runs start `shift` elements earlier, so that in an aligned
+// tensor every run is read and written in aligned vectors; the column's first run then begins, like
+// its last one ends, with steps that do not exist and hold the state. The runs lie the same
+// whatever the alignment of the data, which only decides between vectors and single elements: the
+// backward, whose tensors may be aligned otherwise, looks for the kept states where the
+// forward put them. A column takes `lanes` lanes of a warp (a short column less than a warp, a
+// block then several columns) or a block's warps one behind the other.
 template <typename T>
 struct Run {
   static constexpr int kPer = 16 / sizeof(T);
   int64_t first;  // step of the run's first element, negative in a shifted column's first run
   int lo, hi;     // steps of the run that exist
-  bool vectors;   // the column's data start on 16-byte boundaries `shift` elements before it
+  bool vectors;   // whole, of tensors that start on 16-byte boundaries
 
   __device__ __forceinline__ Run(int64_t index, int shift, int64_t steps, bool aligned)
       : first(index * kAlongSteps - shift) {
@@ -851,7 +853,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   const Along at(a, &taken);
   const bool live = at.column < a.columns;
   const int64_t column = live ? at.column : 0;
-  const int shift = aligned ? static_cast<int>(column * a.steps % Run<T>::kPer) : 0;
+  const int shift = static_cast<int>(column * a.steps % Run<T>::kPer);
   const int64_t stop = a.shared ? at.chunk + 1 : a.chunks;
   const T* x_column = static_cast<const T*>(a.x) + column * a.steps;
   const T* g_column = static_cast<const T*>(a.gate) + column * a.steps;
@@ -930,7 +932,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   const Along at(a, &taken);
   const bool live = at.column < a.columns;
   const int64_t column = live ? at.column : 0;
-  const int shift = aligned ? static_cast<int>(column * a.steps % Run<T>::kPer) : 0;
+  const int shift = static_cast<int>(column * a.steps % Run<T>::kPer);
   const int64_t stop = a.shared ? at.chunk + 1 : a.chunks;
   const int64_t base = column * a.steps;
   A begin = a.dlast != nullptr ? static_cast<const A*>(a.dlast)[column] : A(0);
