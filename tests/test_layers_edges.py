@@ -146,3 +146,22 @@ def test_recurrence_c_abi_buffers_of_any_alignment():
     for moved in ((True, False), (False, True), (True, True)):
         for got, ref in zip(step(moved), expected):
             assert torch.equal(got, ref), moved
+
+
+# ---- linear: residual tiles that arrive ahead --------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(60001, 64, 256), (40000, 512, 520), (9000, 64, 128), (3001, 72, 64)])
+def test_linear_residual_tiles_are_waited_for(m, k, n, dtype):
+    """Many tiles a block, each with a residual fetched while the one before is worked on: the
+    same bits call after call, those of the sum taken in float32 outside, and no expired wait."""
+    x, w, b, r = linear_inputs(m, k, n, dtype, residual=True)
+    plain = torch_convnd.linear(x, w, b)
+    y = torch_convnd.linear(x, w, b, residual=r)
+    # the rounding of `plain` is the only difference: half a unit in its last place
+    check(y, plain.double() + r.double(), eps(dtype) * plain.double().abs(), "y")
+    for _ in range(100):
+        assert torch.equal(torch_convnd.linear(x, w, b, residual=r), y)
+    torch_convnd.device_status()

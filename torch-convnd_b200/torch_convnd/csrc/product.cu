@@ -608,8 +608,12 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
         }
         stage_row<Out>(tile, row, h % kHalvesPerUnit, v);
         if (unit_done) {
+          dev::fence_proxy_async();
+          dev::named_barrier(2 + group, kGroupThreads);
           if (a.tma_residual && a.sets == 2) {
-            // the next unit's residual: the next of this tile, or the first of the next tile
+            // The next unit's residual: the next of this tile, or the first of the next tile.
+            // Asked for behind the barrier, when every warp has seen this unit's arrive: a
+            // warp that came to its wait two phases late would wait for the next one.
             int64_t next_row = row0, next_col = unit_col + kUnit;
             bool more = h + 1 < kHalves;
             if (!more && item + workers < items) {
@@ -625,8 +629,6 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
             }
             asked = more;
           }
-          dev::fence_proxy_async();
-          dev::named_barrier(2 + group, kGroupThreads);
           if (a.tma_out) {
             if (leader && unit_col < a.n) {
               // partial tiles of a split lie below one another
