@@ -165,3 +165,49 @@ def test_linear_residual_tiles_are_waited_for(m, k, n, dtype):
     for _ in range(100):
         assert torch.equal(torch_convnd.linear(x, w, b, residual=r), y)
     torch_convnd.device_status()
+
+
+# ---- fake kernels ------------------------------------------------------------------------
+
+GAPS = {  # inputs of gated_recurrence: (make, dim)
+    "rows and columns cut, transposed": (
+        lambda **o: torch.empty((2, 30, 40), **o)[:, ::2, 3:20].transpose(1, 2), 1),
+    "channels-last volume cut": (
+        lambda **o: torch.empty((2, 6, 8, 10), **o).to(memory_format=torch.channels_last)[:, :, :6, ::2], 2),
+    "expanded": (lambda **o: torch.empty((2, 1, 7), **o).expand(2, 300, 7), 1),
+    "long, transposed": (lambda **o: torch.empty((2, 600, 40), **o)[:, 1:-3, ::2].transpose(1, 2), 2),
+    "dense, transposed": (lambda **o: torch.empty((2, 600, 40), **o).transpose(1, 2), 2),
+}
+
+
+@pytest.mark.parametrize("name,strides,last", [
+    ("rows and columns cut, transposed", (255, 15, 1), (15, 1)),
+    ("channels-last volume cut", (180, 30, 5, 1), (30, 5, 1)),
+    ("expanded", (2100, 7, 1), (7, 1)),
+    ("dense, transposed", (24000, 1, 40), (40, 1))])
+def test_recurrence_fake_strides_follow_the_native_rule(name, strides, last):
+    """The input's own strides where it is dense, else contiguous."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    make, dim = GAPS[name]
+    with FakeTensorMode():
+        x = make(device="cuda")
+        y, state = torch_convnd.gated_recurrence(x, x, dim=dim)
+        assert y.stride() == strides and state.stride() == last
+        _, _, states = torch.ops.torch_convnd.gated_recurrence_train(x, x, None, dim)
+        dx, dgate, d0 = torch.ops.torch_convnd.gated_recurrence_backward(
+            y, state, x, x, states, dim, [True, True, True])
+        assert dx.stride() == dgate.stride() == strides and d0.stride() == last
+
+
+@gpu
+@pytest.mark.parametrize("name", list(GAPS))
+def test_recurrence_fake_kernels_agree_with_native(name):
+    make, dim = GAPS[name]
+    x = make(device="cuda").normal_() if name != "expanded" else make(device="cuda")
+    train = torch.ops.torch_convnd.gated_recurrence_train.default
+    torch.library.opcheck(train, (x, x, None, dim), test_utils=("test_schema", "test_faketensor"))
+    y, last, states = train(x, x, None, dim)
+    torch.library.opcheck(
+        torch.ops.torch_convnd.gated_recurrence_backward.default,
+        (y, last, x, x, states, dim, [True, True, True]), test_utils=("test_schema", "test_faketensor"))

@@ -139,8 +139,13 @@ def _fake_linear_backward(grad_output, pre, input, weight, activation, output_ma
 
 
 def _dense_like(input):
-    """An empty tensor in the input's memory order (contiguous unless it is dense)."""
-    return torch.empty_like(input, memory_format=torch.preserve_format)
+    """An empty tensor in the input's memory order, contiguous if the input is not dense."""
+    like = torch.empty_like(input, memory_format=torch.preserve_format)
+    # preserve_format takes a dense input's strides as they are, and packs any other's in the
+    # order of its strides, where the native kernels work on a contiguous copy
+    same = all(size == 1 or ours == theirs
+               for size, ours, theirs in zip(input.shape, like.stride(), input.stride()))
+    return like if same else input.new_empty(input.shape)
 
 
 def _state_like(input, dim):
