@@ -211,3 +211,27 @@ def test_recurrence_fake_kernels_agree_with_native(name):
     torch.library.opcheck(
         torch.ops.torch_convnd.gated_recurrence_backward.default,
         (y, last, x, x, states, dim, [True, True, True]), test_utils=("test_schema", "test_faketensor"))
+
+
+# ---- gated recurrence without steps ------------------------------------------------------
+
+EMPTY = [lambda t: t[:, :0], lambda t: t[:, 2:2], lambda t: t.transpose(0, 2)[:, :0],
+         lambda t: t.permute(2, 1, 0)[::2, :0], lambda t: t[:0]]
+
+
+@gpu
+@pytest.mark.parametrize("cut", EMPTY)
+def test_recurrence_over_an_empty_slice(cut):
+    """A slice without steps keeps the strides of its source; the state is dense all the same."""
+    x = cut(randn((4, 5, 6), torch.float32, 1)).requires_grad_()
+    h0 = randn((x.shape[0], x.shape[2]), torch.float32, 2).requires_grad_()
+    y, last = torch_convnd.gated_recurrence(x, x, h0, dim=1)
+    assert y.shape == x.shape and last.is_contiguous() and torch.equal(last, h0)
+    dlast = randn(tuple(last.shape), torch.float32, 3)
+    d0, dx = torch.autograd.grad(last, (h0, x), dlast)
+    assert torch.equal(d0, dlast) and dx.shape == x.shape
+    _, last = torch_convnd.gated_recurrence(x, x, None, dim=1)
+    assert torch.equal(last, torch.zeros_like(h0))
+    torch.library.opcheck(torch.ops.torch_convnd.gated_recurrence_train.default,
+                          (x.detach(), x.detach(), h0.detach(), 1),
+                          test_utils=("test_schema", "test_faketensor"))

@@ -149,9 +149,11 @@ def _dense_like(input):
 
 
 def _state_like(input, dim):
-    """A state: the input without ``dim``, in the same memory order."""
+    """A state: the input without ``dim``, in the same memory order (contiguous if empty)."""
     dense = _dense_like(input)
     dim = dim % input.ndim
+    if input.numel() == 0:
+        return input.new_empty((*input.shape[:dim], *input.shape[dim + 1:]), dtype=_wide(input))
     steps, own = dense.shape[dim], dense.stride(dim)
     sizes, strides = [], []
     for d in range(input.ndim):

@@ -571,6 +571,15 @@ Columns columns_of(const at::Tensor& input, int64_t dim) {
     c.state_sizes.push_back(size);
     c.state_strides.push_back(outside ? stride / c.steps : stride);
   }
+  if (input.numel() == 0) {
+    // an empty tensor counts as dense whatever its strides (a slice without steps keeps its
+    // source's), so they say nothing about a dense state
+    int64_t next = 1;
+    for (size_t d = c.state_sizes.size(); d-- > 0;) {
+      c.state_strides[d] = next;
+      next *= std::max<int64_t>(c.state_sizes[d], 1);
+    }
+  }
   return c;
 }
 
