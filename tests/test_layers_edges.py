@@ -235,3 +235,56 @@ def test_recurrence_over_an_empty_slice(cut):
     torch.library.opcheck(torch.ops.torch_convnd.gated_recurrence_train.default,
                           (x.detach(), x.detach(), h0.detach(), 1),
                           test_utils=("test_schema", "test_faketensor"))
+
+
+# ---- activations far from zero -----------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_activation_tails_keep_their_digits(act, dtype):
+    """Relative accuracy where the activation is far smaller than its argument. GELU in
+    float32: v^2 / 2 rounds twice, which moves its exponential by v^2 2^-24 of itself, at most
+    2^-17 for |v| = 11, beside 6 units of the tail's own form and three products. SiLU: two units
+    of exp and three roundings. Values below the smallest normal number may be flushed."""
+    low = -11.0 if dtype == torch.float32 else -30.0
+    v = torch.linspace(low, -3, 4001, device="cuda", dtype=dtype)[:, None]
+    one = torch.ones((1, 1), device="cuda", dtype=dtype)
+    y = torch_convnd.linear(v, one, activation=act)
+    leaf = v.clone().requires_grad_()
+    (slope,) = torch.autograd.grad(torch_convnd.linear(leaf, one, activation=act), leaf,
+                                   torch.ones_like(y))
+    z = v.double().cpu()
+    if act == "gelu":
+        cdf = torch.special.erfc(-z / math.sqrt(2)) / 2
+        density = torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+        ref, ref_slope = z * cdf, cdf + z * density
+        terms = cdf + z.abs() * density
+    else:
+        s = torch.exp(z) / (1 + torch.exp(z))
+        ref, ref_slope = z * s, s * (1 + z * (1 - s))
+        terms = s * (1 + z.abs())
+    u = 2.0**-24 if dtype == torch.float32 else 2.0**-53
+    grow = u * (4 * low * low + 32)
+    tiny = torch.finfo(dtype).tiny
+    for got, want, size in ((y, ref, ref.abs()), (slope, ref_slope, terms)):
+        off = (got.double().cpu() - want).abs()
+        assert bool((off <= grow * size + 8 * tiny).all()), float((off / size).max())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32, torch.float64])
+def test_gelu_at_minus_infinity_is_its_limit(dtype):
+    """0, also from a product whose long sum is split and joined by another kernel."""
+    for k in (8, 8192):
+        x = torch.zeros((3, k), device="cuda", dtype=dtype)
+        b = torch.tensor([-math.inf, math.inf, 0.0], device="cuda", dtype=dtype).repeat(3)
+        y = torch_convnd.linear(x, torch.zeros((9, k), device="cuda", dtype=dtype), b,
+                                activation="gelu")
+        assert torch.equal(y[0], torch.tensor([0.0, math.inf, 0.0], device="cuda", dtype=dtype).repeat(3))
+        leaf = b.clone().requires_grad_()
+        out = torch_convnd.linear(x[:1], torch.zeros((9, k), device="cuda", dtype=dtype), leaf,
+                                  activation="gelu")
+        (slope,) = torch.autograd.grad(out, leaf, torch.ones_like(out))
+        assert torch.equal(slope, torch.tensor([0.0, 1.0, 0.5], device="cuda", dtype=dtype).repeat(3))
