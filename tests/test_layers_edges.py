@@ -288,3 +288,22 @@ def test_gelu_at_minus_infinity_is_its_limit(dtype):
                                   activation="gelu")
         (slope,) = torch.autograd.grad(out, leaf, torch.ones_like(out))
         assert torch.equal(slope, torch.tensor([0.0, 1.0, 0.5], device="cuda", dtype=dtype).repeat(3))
+
+
+@gpu
+def test_linear_float64_of_many_features():
+    """More features than a grid's second dimension counts 64-wide tiles (65535)."""
+    n = 65535 * 64 + 70
+    w = randn((n, 1), torch.float64, 1).requires_grad_()
+    x = randn((3, 1), torch.float64, 2).requires_grad_()
+    y = torch_convnd.linear(x, w)
+    assert torch.equal(y, x * w[:, 0])
+    dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    bound = n * 2.0**-53 * w.abs().sum()
+    assert bool(((dx - w.sum()).abs() <= bound).all())
+    check(dw, x.sum().expand_as(dw), 4 * 2.0**-53 * float(x.abs().sum()), "dw")
+    rows = randn((2, n), torch.float64, 3).requires_grad_()
+    up = randn((2, n), torch.float64, 4).requires_grad_()
+    out = torch_convnd.linear(rows, up)
+    dx, dw = torch.autograd.grad(out, (rows, up), torch.eye(2, device="cuda", dtype=torch.float64))
+    assert torch.equal(dx, up) and torch.equal(dw, rows)

@@ -35,50 +35,53 @@ __global__ void __launch_bounds__(256) double_product_kernel(const DoubleProduct
   __shared__ double sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const int64_t m0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.y) * kTile;
-  double sum[4][4] = {};
-  for (int64_t k0 = 0; k0 < p.k; k0 += kDepth) {
-    for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-      const int r = p.a_col == 1 ? i / kDepth : i % kTile;
-      const int k = p.a_col == 1 ? i % kDepth : i / kTile;
-      const bool in = m0 + r < p.m && k0 + k < p.k;
-      sa[k][r] = in ? p.a[(m0 + r) * p.a_row + (k0 + k) * p.a_col] : 0.0;
-    }
-    for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-      const int r = p.b_col == 1 ? i / kDepth : i % kTile;
-      const int k = p.b_col == 1 ? i % kDepth : i / kTile;
-      const bool in = n0 + r < p.n && k0 + k < p.k;
-      sb[k][r] = in ? p.b[(n0 + r) * p.b_row + (k0 + k) * p.b_col] : 0.0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kDepth; ++k) {
-      double u[4], v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u[i] = sa[k][ty * 4 + i];
-        v[i] = sb[k][tx + 16 * i];
+  // a grid has at most 65535 blocks in y
+  for (int64_t n0 = static_cast<int64_t>(blockIdx.y) * kTile; n0 < p.n;
+       n0 += static_cast<int64_t>(gridDim.y) * kTile) {
+    double sum[4][4] = {};
+    for (int64_t k0 = 0; k0 < p.k; k0 += kDepth) {
+      for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
+        const int r = p.a_col == 1 ? i / kDepth : i % kTile;
+        const int k = p.a_col == 1 ? i % kDepth : i / kTile;
+        const bool in = m0 + r < p.m && k0 + k < p.k;
+        sa[k][r] = in ? p.a[(m0 + r) * p.a_row + (k0 + k) * p.a_col] : 0.0;
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum[i][j] += u[i] * v[j];
+      for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
+        const int r = p.b_col == 1 ? i / kDepth : i % kTile;
+        const int k = p.b_col == 1 ? i % kDepth : i / kTile;
+        const bool in = n0 + r < p.n && k0 + k < p.k;
+        sb[k][r] = in ? p.b[(n0 + r) * p.b_row + (k0 + k) * p.b_col] : 0.0;
       }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kDepth; ++k) {
+        double u[4], v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          u[i] = sa[k][ty * 4 + i];
+          v[i] = sb[k][tx + 16 * i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum[i][j] += u[i] * v[j];
+        }
+      }
+      __syncthreads();
     }
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + ty * 4 + i;
-    if (m >= p.m) break;
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = n0 + tx + 16 * j;
-      if (n >= p.n) break;
-      double v = sum[i][j];
-      if (p.bias != nullptr) v += p.bias[n];
-      if (p.pre != nullptr) p.pre[m * p.n + n] = v;
-      v = activate(v, p.act);
-      if (p.residual != nullptr) v += p.residual[m * p.n + n];
-      p.d[m * p.n + n] = v;
+    for (int i = 0; i < 4; ++i) {
+      const int64_t m = m0 + ty * 4 + i;
+      if (m >= p.m) break;
+      for (int j = 0; j < 4; ++j) {
+        const int64_t n = n0 + tx + 16 * j;
+        if (n >= p.n) break;
+        double v = sum[i][j];
+        if (p.bias != nullptr) v += p.bias[n];
+        if (p.pre != nullptr) p.pre[m * p.n + n] = v;
+        v = activate(v, p.act);
+        if (p.residual != nullptr) v += p.residual[m * p.n + n];
+        p.d[m * p.n + n] = v;
+      }
     }
   }
 }
@@ -424,7 +427,7 @@ Layout backward_layout(const cnd_linear& p, const int32_t mask[3]) {
 
 void launch_double(const DoubleProduct& p, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>((p.m + kTile - 1) / kTile),
-                  static_cast<unsigned>((p.n + kTile - 1) / kTile));
+                  static_cast<unsigned>(std::min<int64_t>((p.n + kTile - 1) / kTile, 65535)));
   double_product_kernel<<<grid, 256, 0, stream>>>(p);
   count_launch();
 }
