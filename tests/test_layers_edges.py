@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 
 import pytest
 import torch
@@ -307,3 +308,32 @@ def test_linear_float64_of_many_features():
     out = torch_convnd.linear(rows, up)
     dx, dw = torch.autograd.grad(out, (rows, up), torch.eye(2, device="cuda", dtype=torch.float64))
     assert torch.equal(dx, up) and torch.equal(dw, rows)
+
+
+# ---- calls from several threads ----------------------------------------------------------
+
+
+@gpu
+def test_layer_norm_widths_in_parallel_threads():
+    """Calls of one kernel that want different amounts of shared memory do not disturb one
+    another."""
+    cases = [(randn((64, width), torch.float32, width), []) for width in (2056, 4096)]
+    for x, expected in cases:
+        expected.append(torch_convnd.layer_norm(x))
+    failures = []
+
+    def work(x, expected):
+        try:
+            for _ in range(3000):
+                y = torch_convnd.layer_norm(x)
+            if not torch.equal(y, expected[0]):
+                failures.append("values")
+        except RuntimeError as error:
+            failures.append(str(error))
+
+    threads = [threading.Thread(target=work, args=case) for case in cases for _ in range(3)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failures, failures[:2]

@@ -1199,7 +1199,14 @@ int tile_blocks(const NormShape& s, bool backward) {
   return tile_blocks_of(s.chunks <= 32 ? 1 : 2, s.shift, backward);
 }
 
-// The ring of a block: its share of 200 KB, at most 16 stages. Tiles of short rows are 8 KB.
+// The ring of a block: its share of 200 KB, at most 16 stages but four at least. Tiles of short
+// rows are 8 KB.
+constexpr int kRingTotal = 200 * 1024;
+// The most that any call of a tile kernel (two blocks an SM and more) and of a ring kernel (four
+// stages of two rows) takes. A kernel's limit is set to this in every call, not to what the call
+// takes: another thread's call may come between setting the limit and the launch.
+constexpr int kTileShared = kRingTotal / 2, kRingShared = 4 * 2 * kMostChunks * 16;
+static_assert(kRingShared >= kRingTotal);
 Ring make_ring(const NormShape& s, int dtype, int64_t width, bool backward) {
   Ring r{};
   if (s.ring) {
@@ -1212,7 +1219,7 @@ Ring make_ring(const NormShape& s, int dtype, int64_t width, bool backward) {
     r.stage_bytes = (row * r.tile + 31) / 16 * 16;
   }
   if (backward) r.stage_bytes *= 2;
-  const uint32_t share = 200 * 1024 / (s.ring ? ring_blocks(s) : tile_blocks(s, backward));
+  const uint32_t share = kRingTotal / (s.ring ? ring_blocks(s) : tile_blocks(s, backward));
   r.stages = static_cast<int>(std::min<uint32_t>(16, std::max<uint32_t>(4, share / r.stage_bytes)));
   r.error = device_error_word();
   r.timeout_ns = wait_timeout_ns();
@@ -1262,8 +1269,7 @@ struct LaunchTile {
                                                : norm_forward_tile_kernel<T, V, NV, G, false>);
       const uint32_t bytes = std::max<uint32_t>(ring.stage_bytes * ring.stages,
                                                 static_cast<uint32_t>(a.width) * 2 * sizeof(float));
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(bytes));
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileShared);
       kernel<<<blocks, kTileThreads, bytes, stream>>>(a, ring);
     }
   }
@@ -1282,8 +1288,7 @@ struct LaunchRing {
                                 : (kBackward ? norm_backward_ring_kernel<T, V, NV, G, false>
                                              : norm_forward_ring_kernel<T, V, NV, G, false>);
     const uint32_t bytes = ring.stage_bytes * ring.stages;
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         static_cast<int>(bytes));
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingShared);
     kernel<<<blocks, G, bytes, stream>>>(a, ring);
   }
 };
