@@ -521,7 +521,7 @@ struct Ring {
   uint64_t timeout_ns;
 };
 
-constexpr uint32_t kSiteRing = 0x701;
+constexpr uint32_t kSiteRing = 0x701, kSiteRingDrain = 0x702;
 
 template <bool kBackward, bool kShift>
 struct RowRing {
@@ -585,11 +585,16 @@ struct RowRing {
     if (++fill == ring.stages) fill = 0;
   }
 
-  // Waits for the current stage. After a wait that expired no other one waits or asks.
+  // Waits for the current stage. After a wait that expired no other one waits or asks, and the
+  // copies on their way are drained: here (kHere), as the tile kernels do it, or behind the
+  // last row. Which one only decides what registers the compiler finds for the loop: 65536 x
+  // 512 bf16 by the tile 31 us here and 43 behind it, 16384 x 4096 row by row 58 and 54.
+  template <bool kHere>
   __device__ __forceinline__ const uint8_t* wait() {
     if (!dead && !dev::mbar_wait(&full[stage], phase, dev::ErrorWord{ring.error}, kSiteRing,
                                  ring.timeout_ns)) {
       dead = true;
+      if (kHere) drain();
     }
     return data + stage * ring.stage_bytes;
   }
@@ -598,6 +603,18 @@ struct RowRing {
     if (++stage == ring.stages) {
       stage = 0;
       phase ^= 1u;
+    }
+  }
+
+  // After a wait that expired: thread 0 gives the copies that it asked for a bounded time to land
+  // before the block may exit. Of a barrier's two phases the one in progress ends when its copy has
+  // landed, the other has ended; both are waited for, as the walk does not keep which is which.
+  __device__ __forceinline__ void drain() {
+    if (!dead || threadIdx.x != 0) return;
+#pragma unroll 1
+    for (uint32_t i = 0; i < 2u * ring.stages; ++i) {
+      dev::mbar_wait(&full[i / 2], i & 1u, dev::ErrorWord{ring.error}, kSiteRingDrain,
+                     ring.timeout_ns / 16 + 1);
     }
   }
 };
@@ -630,7 +647,7 @@ __global__ void __launch_bounds__(G, ring_blocks_of(G, kShift))
     load_span_params<T>(a.bias, a.param_f32, s, 0.0f, b[k]);
   }
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T* data = reinterpret_cast<const T*>(ring.wait());
+    const T* data = reinterpret_cast<const T*>(ring.template wait<false>());
     Two x[NV][V / 2];
     float sum[1] = {0.0f};
 #pragma unroll
@@ -672,6 +689,7 @@ __global__ void __launch_bounds__(G, ring_blocks_of(G, kShift))
     }
     ring.advance();
   }
+  ring.drain();
 }
 
 template <typename T, int V, int NV, int G, bool kShift>
@@ -722,7 +740,7 @@ __global__ void __launch_bounds__(G, ring_blocks_of(G, kShift))
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       if (row0 + r * step < a.rows) {
-        at[r] = ring.wait();
+        at[r] = ring.template wait<false>();
         ring.advance();
         Two pairs[2] = {same(0.0f), same(0.0f)};
 #pragma unroll
@@ -769,6 +787,7 @@ __global__ void __launch_bounds__(G, ring_blocks_of(G, kShift))
       }
     }
   }
+  ring.drain();
   if (!a.want_params) return;
   float* partial = static_cast<float*>(a.partials) + static_cast<int64_t>(blockIdx.x) * 2 * width;
 #pragma unroll
@@ -812,7 +831,7 @@ __global__ void __launch_bounds__(kTileThreads, tile_blocks_of(NV, kShift, false
   }
   for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * tile; row0 < a.rows;
        row0 += static_cast<int64_t>(gridDim.x) * tile) {
-    const T* data = reinterpret_cast<const T*>(ring.wait());
+    const T* data = reinterpret_cast<const T*>(ring.template wait<true>());
 #pragma unroll 2
     for (int i0 = 0; i0 < tile; i0 += kGroups) {
       const int64_t row = row0 + i0 + group;
@@ -899,7 +918,7 @@ __global__ void __launch_bounds__(kTileThreads, tile_blocks_of(NV, kShift, true)
   const int64_t step = static_cast<int64_t>(gridDim.x) * tile;
   for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * tile; row0 < a.rows; row0 += step) {
     fetch(row0 + step, slot ^ 1);
-    const uint8_t* at = ring.wait();
+    const uint8_t* at = ring.template wait<true>();
     const T* xs = reinterpret_cast<const T*>(at);
     const T* ds = reinterpret_cast<const T*>(at + ring_args.stage_bytes / 2);
 #pragma unroll 2
