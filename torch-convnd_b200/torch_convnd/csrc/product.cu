@@ -321,11 +321,15 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
         }
       }
     }
-    if (!ok && issued > 0 && rank == 0) {
-      // give loads in flight a bounded time to land before the block may exit
-      const int previous = stage == 0 ? a.stages - 1 : stage - 1;
-      wait_warp<kPair>(&full[previous], stage == 0 ? phase ^ 1u : phase, err, kSiteDrain,
-                       a.timeout_ns / 8 + 1);
+    // The last loads of each stage land before the block may exit, or have had a bounded time to:
+    // MMAs that gave up have not waited for them. (A pair's loads all signal the leader.)
+    for (int left = rank == 0 ? min(issued, static_cast<uint32_t>(a.stages)) : 0; left > 0; --left) {
+      if (stage == 0) {
+        stage = a.stages;
+        phase ^= 1u;
+      }
+      --stage;
+      wait_warp<kPair>(&full[stage], phase, err, kSiteDrain, a.timeout_ns / 8 + 1);
     }
   } else if (warp == 1) {
     // ---- MMAs: the leader CTA's warp, converged; elect.sync issues ----
@@ -496,7 +500,13 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
         free_set(cross_empty, release_cross, cross);
         cross ^= 1;
       } else {
-        ok = ok && wait_warp<kPair>(&acc_full[set], set_phase, err, kSiteEpilogue, a.timeout_ns);
+        if (ok && !wait_warp<kPair>(&acc_full[set], set_phase, err, kSiteEpilogue, a.timeout_ns)) {
+          ok = false;
+          if (asked) {  // the residual tile on its way has a bounded time to land
+            dev::mbar_wait_warp(&residual_full[group], residual_phase, err, kSiteDrain,
+                                a.timeout_ns / 8 + 1);
+          }
+        }
         dev::tc_fence_after();
       }
 
@@ -657,10 +667,6 @@ __global__ void __launch_bounds__(block_threads(kGroups), 1)
           set_phase ^= 1u;
         }
       }
-    }
-    if (asked) {  // a wait ran out: the tile on its way has a bounded time to land
-      dev::mbar_wait_warp(&residual_full[group], residual_phase, err, kSiteDrain,
-                          a.timeout_ns / 8 + 1);
     }
     if (leader) dev::bulk_wait_group<0>();
   }
