@@ -843,8 +843,10 @@ struct Along {
   }
 };
 
+// Three blocks an SM: at the 94 registers of two, 8 x 1022 columns of 4097 float32 steps took 187 us,
+// at 78 133.
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 8 ? 2 : 3)
     steps_forward_kernel(const __grid_constant__ RecurrenceArgs a, bool aligned) {
   using A = typename Wide<T>::type;
   __shared__ Map<A> maps[kWarps];
