@@ -225,7 +225,8 @@ CND_API int cnd_set_default_fp32_mode(int32_t mode);
  * whose producer never issues a load, so the MMA thread's wait expires after
  * `timeout_ms`; the kernel then returns normally with the device error word set.
  * Returns CND_ERR_TIMEOUT when that path works (no fault, no hang), another status
- * otherwise. Allocates and frees its own small buffers. */
+ * otherwise. A negative `timeout_ms` waits as long and returns CND_OK with the error word still
+ * set, for the next cnd_device_status to report. Allocates and frees its own small buffers. */
 CND_API int cnd_debug_stall_test(int32_t timeout_ms, void* stream);
 
 /* Benchmark support. While enabled, every pass the library launches is bracketed by a

@@ -337,3 +337,31 @@ def test_layer_norm_widths_in_parallel_threads():
     for thread in threads:
         thread.join()
     assert not failures, failures[:2]
+
+
+# ---- waits that expired elsewhere --------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape,dim", [((1, 20000, 256), 1), ((2, 60000), 1)])
+def test_recurrence_after_another_kernels_expired_wait(shape, dim, dtype):
+    """An error that nobody has read yet does not cut the recurrence's own waits short."""
+    x, g, _ = recurrence_inputs(shape, dim, dtype, initial=False)
+    dy = randn(shape, dtype, 5)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (x, g)]
+        y, last = torch_convnd.gated_recurrence(*leaves, dim=dim)
+        return [y, last, *torch.autograd.grad(y, leaves, dy)]
+
+    torch_convnd.device_status()
+    expected = step()
+    library = _native.core()
+    assert library.cnd_debug_stall_test(-20, None) == 0, library.cnd_last_error()
+    for _ in range(5):
+        for got, ref in zip(step(), expected):
+            assert torch.equal(got, ref)
+    with pytest.raises(RuntimeError, match="bounded wait expired"):
+        torch_convnd.device_status()
+    torch_convnd.device_status()

@@ -1245,8 +1245,8 @@ int cnd_device_status(void* stream_handle) {
   if (value != 0) {
     cudaMemset(word, 0, sizeof(value));
     return fail(CND_ERR_TIMEOUT,
-                "a bounded wait expired inside a convolution kernel (site 0x%x); results of "
-                "that launch are invalid",
+                "a bounded wait expired inside a kernel (site 0x%x); the results of that launch, one "
+                "of those since the last check, are invalid",
                 value);
   }
   return CND_OK;
@@ -1320,9 +1320,9 @@ int cnd_debug_stall_test(int32_t timeout_ms, void* stream_handle) {
     cudaFree(buffer);
     return fail(CND_ERR_UNSUPPORTED, "cnd_debug_stall_test: planning failed");
   }
-  int rc = launch_fprop(pass, plan, stream,
-                        static_cast<uint64_t>(timeout_ms > 0 ? timeout_ms : 50) * 1000000ull, 1);
-  if (rc == CND_OK) rc = cnd_device_status(stream);
+  const int64_t limit = timeout_ms < 0 ? -static_cast<int64_t>(timeout_ms) : timeout_ms > 0 ? timeout_ms : 50;
+  int rc = launch_fprop(pass, plan, stream, static_cast<uint64_t>(limit) * 1000000ull, 1);
+  if (rc == CND_OK && timeout_ms >= 0) rc = cnd_device_status(stream);
   cudaStreamSynchronize(stream);
   cudaFree(buffer);
   return rc;

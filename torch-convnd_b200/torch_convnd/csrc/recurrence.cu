@@ -27,7 +27,7 @@
 // of the group before published. The association is fixed, so repeated calls give the
 // same bits. The exchange area starts as all ones, a NaN that no arithmetic produces, and a
 // map (a state) is stored at once, so a reader polls the value itself: no flag, no fence, one
-// trip to L2. Waits are bounded and end at once when any wait has expired.
+// trip to L2. Waits are bounded and end at once when any wait of the launch has expired.
 //
 // The forward keeps the state before each block of 64 steps (256 in step layout), from which
 // the backward recomputes the others in float32: it reads x, g and dy only, and its states
@@ -78,10 +78,10 @@ struct RecurrenceArgs {
   int lanes, per_block;  // step layout: lanes of a column, columns of a block
   int balanced;  // steps a thread takes when one chunk holds them all, 0: the most it can
   // exchange between chunks (shared != 0): maps [chunks][padded], states [groups][padded],
-  // one ticket counter; all bits set at the start
+  // a ticket counter and a word that an expired wait clears; all bits set at the start
   int shared;
   void *maps, *bases;
-  unsigned int *ticket, *error;
+  unsigned int *ticket, *waiting, *error;
   uint64_t timeout_ns;
 };
 
@@ -137,7 +137,8 @@ __device__ __forceinline__ void store_exchange(Bits* p, Bits v) {
 }
 
 // Reads *p again until it has been written. Gives up (error word set) after the timeout, or
-// as soon as another wait has.
+// as soon as another wait of this launch has. (Not by the error word, which may hold what some
+// other kernel's wait left there.)
 template <typename Bits>
 __device__ __forceinline__ Bits settle(const Bits* p, Bits v, const RecurrenceArgs& a,
                                        unsigned int site) {
@@ -147,11 +148,12 @@ __device__ __forceinline__ Bits settle(const Bits* p, Bits v, const RecurrenceAr
     v = load_exchange(p);
     if (v != ~Bits{0}) return v;
     if (spin % 64 == 0) {
-      if (*static_cast<volatile unsigned int*>(a.error) != 0) return v;
-      if (dev::global_timer_ns() - start > a.timeout_ns) {
+      const bool late = dev::global_timer_ns() - start > a.timeout_ns;
+      if (late) {
+        *static_cast<volatile unsigned int*>(a.waiting) = 0;
         atomicCAS(a.error, 0u, site);
-        return v;
       }
+      if (late || *static_cast<volatile unsigned int*>(a.waiting) == 0) return v;
     }
   }
 }
@@ -1034,7 +1036,7 @@ struct RecurrencePlan {
   int lanes, per_block;  // step layout
   int balanced;
   bool shared;
-  size_t maps = 0, bases = 0, ticket = 0, total = 0;
+  size_t maps = 0, bases = 0, ticket = 0, waiting = 0, total = 0;
 };
 
 RecurrencePlan plan_recurrence(int dtype, int64_t outer, int64_t steps, int64_t inner,
@@ -1082,6 +1084,7 @@ RecurrencePlan plan_recurrence(int dtype, int64_t outer, int64_t steps, int64_t 
       return at;
     };
     p.ticket = take(sizeof(unsigned int));
+    p.waiting = take(sizeof(unsigned int));
     p.maps = take(static_cast<size_t>(p.chunks * padded) * 2 * wide);
     p.bases = take(static_cast<size_t>(groups * padded) * wide);
   }
@@ -1109,6 +1112,7 @@ int bind_exchange(const char* who, const RecurrencePlan& p, void* workspace, siz
   a->maps = base + p.maps;
   a->bases = base + p.bases;
   a->ticket = reinterpret_cast<unsigned int*>(base + p.ticket);
+  a->waiting = reinterpret_cast<unsigned int*>(base + p.waiting);
   a->error = device_error_word();
   a->timeout_ns = wait_timeout_ns();
   if (a->error == nullptr) return fail(CND_ERR_CUDA, "device error word unavailable");
