@@ -365,3 +365,27 @@ def test_recurrence_after_another_kernels_expired_wait(shape, dim, dtype):
     with pytest.raises(RuntimeError, match="bounded wait expired"):
         torch_convnd.device_status()
     torch_convnd.device_status()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_recurrence_nan_of_all_ones_is_sent_between_chunks(dtype):
+    """NaNs whose bits are those of an exchange slot not written yet, in x and in the gate."""
+    bits = torch.int32 if dtype == torch.float32 else torch.int64
+    for shape, dim in (((1, 4000, 40), 1), ((2, 30000), 1)):
+        x, g, _ = recurrence_inputs(shape, dim, dtype, initial=False)
+        clean = torch_convnd.gated_recurrence(x, g, dim=dim)[0].movedim(dim, 0)
+        x.view(bits).movedim(dim, 0)[1000].flatten()[:1] = -1
+        g.view(bits).movedim(dim, 0)[2000].flatten()[-1:] = -1
+        y, last = torch_convnd.gated_recurrence(x, g, dim=dim)
+        y = y.movedim(dim, 0).flatten(1)
+        assert torch.equal(y[:1000, 0], clean.flatten(1)[:1000, 0]) and torch.isnan(y[1000:, 0]).all()
+        assert torch.equal(y[:2000, -1], clean.flatten(1)[:2000, -1]) and torch.isnan(y[2000:, -1]).all()
+        leaves = [t.detach().requires_grad_() for t in (x, g)]
+        out = torch_convnd.gated_recurrence(*leaves, dim=dim)[0]
+        dx, dgate = torch.autograd.grad(out, leaves, torch.ones_like(out))
+        # the flow goes through the gates behind a step only
+        flow = dx.movedim(dim, 0).flatten(1)
+        assert torch.isfinite(flow[:, 0]).all() and torch.isnan(flow[:2001, -1]).all()
+        assert torch.isfinite(flow[2001:, -1]).all()
+    torch_convnd.device_status()

@@ -25,7 +25,7 @@
 // so whoever a block waits for is already running; each chunk composes the maps of the
 // chunks before it in its group of kGroup, in order, with the state that the last chunk
 // of the group before published. The association is fixed, so repeated calls give the
-// same bits. The exchange area starts as all ones, a NaN that no arithmetic produces, and a
+// same bits. The exchange area starts as all ones, a NaN that is never sent, and a
 // map (a state) is stored at once, so a reader polls the value itself: no flag, no fence, one
 // trip to L2. Waits are bounded and end at once when any wait of the launch has expired.
 //
@@ -127,8 +127,11 @@ __device__ __forceinline__ Bits load_exchange(const Bits* p) {
   return v;
 }
 
+// (All ones would read as not written yet. float32 arithmetic never gives that NaN, float64
+// arithmetic may hand on a NaN operand's bits: it leaves as another NaN.)
 template <typename Bits>
 __device__ __forceinline__ void store_exchange(Bits* p, Bits v) {
+  if (v == ~Bits{0}) v >>= 1;
   if constexpr (sizeof(Bits) == 4) {
     asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
   } else {
