@@ -389,3 +389,36 @@ def test_recurrence_nan_of_all_ones_is_sent_between_chunks(dtype):
         assert torch.isfinite(flow[:, 0]).all() and torch.isnan(flow[:2001, -1]).all()
         assert torch.isfinite(flow[2001:, -1]).all()
     torch_convnd.device_status()
+
+
+# ---- other ways of differentiating and tracing --------------------------------------------
+
+CALLS = {
+    "layer_norm": lambda t: torch_convnd.layer_norm(t),
+    "layer_norm, weight": lambda t: torch_convnd.layer_norm(t.detach() * 0, t[0]),
+    "linear": lambda t: torch_convnd.linear(t, t.detach()),
+    "linear, residual": lambda t: torch_convnd.linear(t.detach(), t.detach()[:, :], residual=t @ t.t()),
+    "gated_recurrence": lambda t: torch_convnd.gated_recurrence(t, t.detach(), dim=0)[0],
+    "gated_recurrence, initial": lambda t: torch_convnd.gated_recurrence(
+        t.detach(), t.detach(), t[0], dim=0)[0],
+}
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_forward_mode_is_refused(name):
+    """A tangent would be lost in silence; the refusal comes before the device is looked at."""
+    x = torch.ones(4, 8)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(CALLS[name], (x,), (torch.ones_like(x),))
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            CALLS[name](dual)
+
+
+@gpu
+def test_forward_mode_is_refused_on_the_device():
+    x = torch.ones((4, 8), device="cuda")
+    for call in CALLS.values():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(call, (x,), (torch.ones_like(x),))

@@ -144,12 +144,17 @@ struct Edges {
   bool operator()(bool present) { return present && ctx->needs_input_grad(next++); }
 };
 
-bool wants_grad(std::initializer_list<const at::Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return false;
+// Whether a backward may follow. A tangent (forward-mode differentiation) would be lost below the
+// autograd key without a word, so it is refused.
+bool wants_grad(const char* op, std::initializer_list<const at::Tensor*> tensors) {
+  bool wanted = false;
   for (const at::Tensor* t : tensors) {
-    if (t != nullptr && t->defined() && t->requires_grad()) return true;
+    if (t == nullptr || !t->defined()) continue;
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "torch_convnd::", op,
+                                " does not support forward-mode differentiation");
+    wanted = wanted || t->requires_grad();
   }
-  return false;
+  return wanted && at::GradMode::is_enabled();
 }
 
 const at::Tensor* pointer(const OptTensor& t) { return given(t) ? &*t : nullptr; }
@@ -313,7 +318,7 @@ class LayerNormFunction : public torch::autograd::Function<LayerNormFunction> {
 
 at::Tensor layer_norm_autograd(const at::Tensor& input, const OptTensor& weight,
                                const OptTensor& bias, double eps) {
-  if (wants_grad({&input, pointer(weight), pointer(bias)})) {
+  if (wants_grad("layer_norm", {&input, pointer(weight), pointer(bias)})) {
     return LayerNormFunction::apply(input, weight, bias, eps);
   }
   static const auto op = find_op<decltype(layer_norm_cuda)>("torch_convnd::layer_norm");
@@ -505,7 +510,7 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
 at::Tensor linear_autograd(const at::Tensor& input, const at::Tensor& weight,
                            const OptTensor& bias, const OptTensor& residual,
                            c10::string_view activation) {
-  if (wants_grad({&input, &weight, pointer(bias), pointer(residual)})) {
+  if (wants_grad("linear", {&input, &weight, pointer(bias), pointer(residual)})) {
     return LinearFunction::apply(input, weight, bias, residual, activation);
   }
   static const auto op = find_op<decltype(linear_cuda)>("torch_convnd::linear");
@@ -745,7 +750,7 @@ std::tuple<at::Tensor, at::Tensor> gated_recurrence_autograd(const at::Tensor& i
                                                              const at::Tensor& gate,
                                                              const OptTensor& initial,
                                                              int64_t dim) {
-  if (wants_grad({&input, &gate, pointer(initial)})) {
+  if (wants_grad("gated_recurrence", {&input, &gate, pointer(initial)})) {
     auto outputs = RecurrenceFunction::apply(input, gate, initial, dim);
     return {outputs[0], outputs[1]};
   }
