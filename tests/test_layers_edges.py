@@ -422,3 +422,34 @@ def test_forward_mode_is_refused_on_the_device():
     for call in CALLS.values():
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.func.jvp(call, (x,), (torch.ones_like(x),))
+
+
+def graphs_over(lengths, call):
+    """Graphs that torch.compile makes of `call` over several lengths of a dynamic axis."""
+    from torch._dynamo.testing import CompileCounter
+
+    torch._dynamo.reset()
+    counter = CompileCounter()
+    compiled = torch.compile(call, backend=counter, dynamic=True, fullgraph=True)
+    for length in lengths:
+        compiled(torch.empty((3, length, 8), device="meta", requires_grad=True))
+    torch._dynamo.reset()
+    return counter.frame_count
+
+
+@pytest.mark.parametrize("dim", [1, 2])
+def test_recurrence_compiles_once_for_all_lengths(dim):
+    def call(x):
+        t = x if dim == 1 else x.transpose(1, 2).contiguous()
+        return torch_convnd.gated_recurrence(t, t, dim=dim)[0]
+
+    assert graphs_over((65, 130, 300, 777, 1200), call) == 1
+
+
+def test_recurrence_fake_counts_kept_states_like_the_library():
+    from torch_convnd._layers import _kept_states
+
+    count = _native.core().cnd_gated_recurrence_blocks
+    for steps in (0, 1, 2, 63, 64, 65, 128, 249, 250, 251, 256, 257, 506, 1000, 1 << 20):
+        for inner in (0, 1, 2, 33):
+            assert _kept_states(steps, inner) == count(2, 3, steps, inner), (steps, inner)

@@ -169,20 +169,22 @@ def _fake_recurrence(input, gate, initial, dim):
     return _dense_like(input), _state_like(input, dim)
 
 
-def _fake_recurrence_train(input, gate, initial, dim):
-    from ._native import core
+def _kept_states(steps, inner):
+    """cnd_gated_recurrence_blocks(), in arithmetic that sizes known only as symbols go through."""
+    if steps == 0:
+        return 0
+    return (steps + 6) // 256 + 1 if inner == 1 and steps > 1 else (steps - 1) // 64 + 1
 
+
+def _fake_recurrence_train(input, gate, initial, dim):
     last = _state_like(input, dim)
     dense = _dense_like(input)
     steps, own = dense.shape[dim], dense.stride(dim)
-    outer = 1
-    for size, stride in zip(dense.shape, dense.stride()):
-        if steps > 1 and size > 1 and stride > own:
-            outer *= size
-    columns = last.numel()
-    code = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2, torch.float64: 3}[input.dtype]
-    blocks = core().cnd_gated_recurrence_blocks(code, outer, steps, columns // max(1, outer))
-    return dense, last, input.new_empty((blocks, columns), dtype=_wide(input))
+    inner = 1
+    for d, (size, stride) in enumerate(zip(dense.shape, dense.stride())):
+        if d != dim % input.ndim and not (steps > 1 and size > 1 and stride > own):
+            inner *= size
+    return dense, last, input.new_empty((_kept_states(steps, inner), last.numel()), dtype=_wide(input))
 
 
 def _fake_recurrence_backward(grad_output, grad_last, input, gate, states, dim, output_mask):
