@@ -5,7 +5,8 @@
  * Conventions are those of convnd_b200.h: device pointers and sizes only, a caller-provided
  * workspace, a cudaStream_t as void* (NULL = legacy default stream), CND_OK or a negative
  * status with the message in cnd_last_error(). Every call only enqueues work on `stream`.
- * Every output is written in full. None of these operators has a counterpart in the
+ * Every output is written in full. Buffers are aligned to their elements, a workspace to 16 bytes
+ * (what is not is refused). None of these operators has a counterpart in the
  * reference.
  */
 #ifndef CONVND_B200_LAYERS_H

@@ -453,3 +453,50 @@ def test_recurrence_fake_counts_kept_states_like_the_library():
     for steps in (0, 1, 2, 63, 64, 65, 128, 249, 250, 251, 256, 257, 506, 1000, 1 << 20):
         for inner in (0, 1, 2, 33):
             assert _kept_states(steps, inner) == count(2, 3, steps, inner), (steps, inner)
+
+
+# ---- C ABI: addresses that no element can have ---------------------------------------------
+
+
+def abi_cases():
+    """(call of test_layers_capi, keyword, address, status): every buffer of every entry point,
+    off its elements by half of one, and every workspace off 16 bytes."""
+    import test_layers_capi as abi
+
+    half, wide = abi.A + 1, abi.A + 2
+    for name in ("x", "w", "b", "y"):
+        yield abi.norm_forward, name, half, -1
+    yield abi.norm_forward, "stats", wide, -1
+    for name in ("dy", "x", "w", "dx", "dw", "db"):
+        yield abi.norm_backward, name, half, -1
+    yield abi.norm_backward, "stats", wide, -1
+    for name in ("x", "w", "b", "residual", "y", "pre"):
+        yield abi.linear_forward, name, half, -1
+    for name in ("dy", "pre", "x", "w", "dx", "dw", "db"):
+        yield abi.linear_backward, name, half, -1
+    for name in ("x", "gate", "y"):
+        yield abi.recurrence_forward, name, half, -1
+    for name in ("initial", "last", "states"):
+        yield abi.recurrence_forward, name, wide, -1
+    for name in ("dy", "x", "gate", "dx", "dgate"):
+        yield abi.recurrence_backward, name, half, -1
+    for name in ("dlast", "states", "dinitial"):
+        yield abi.recurrence_backward, name, wide, -1
+    for run in (abi.norm_backward, abi.linear_backward, abi.recurrence_forward, abi.recurrence_backward):
+        yield run, "workspace", abi.A + 8, -4
+
+
+@pytest.mark.parametrize("run,name,address,status", [
+    pytest.param(*case, id=f"{case[0].__name__}-{case[1]}") for case in abi_cases()])
+def test_c_abi_refuses_misaligned_buffers(run, name, address, status):
+    got, message = run(**{name: address})
+    assert got == status and "aligned" in message
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_c_abi_refuses_a_misaligned_linear_workspace(dtype):
+    import test_layers_capi as abi
+
+    odd = {"dtype": dtype, "in_features": 63, "x_stride": 63}  # operands are prepared there
+    got, message = abi.linear_forward(odd, workspace=abi.A + 8)
+    assert got == -4 and "aligned" in message

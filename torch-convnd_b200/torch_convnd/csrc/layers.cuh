@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 #include <type_traits>
 
 #include "convnd_b200_layers.h"
@@ -179,6 +180,19 @@ inline int64_t product(int64_t a, int64_t b) {
 }
 
 inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Whether buffers (some may be NULL) start on multiples of `size` bytes, their elements' or, for a
+// workspace, 16. An address in between would be a fault on the device.
+inline bool aligned_to(size_t size, std::initializer_list<const void*> buffers) {
+  for (const void* p : buffers) {
+    if (reinterpret_cast<uintptr_t>(p) % size != 0) return false;
+  }
+  return true;
+}
+inline int wide_size(int dtype) { return dtype == CND_F64 ? 8 : 4; }  // of statistics and states
+inline int misaligned(const char* who) {
+  return fail(CND_ERR_INVALID, "%s: a buffer is not aligned to its elements", who);
+}
 
 // Status of the launches made so far on this thread.
 inline int launch_status(const char* what) {

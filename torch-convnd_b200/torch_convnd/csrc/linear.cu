@@ -458,6 +458,9 @@ int check_workspace(const char* who, const void* workspace, size_t bytes, size_t
     return fail(CND_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who,
                 workspace == nullptr ? size_t{0} : bytes, need);
   }
+  if (need > 0 && !aligned16(workspace)) {
+    return fail(CND_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", who);
+  }
   return CND_OK;
 }
 
@@ -484,6 +487,9 @@ int cnd_linear_forward(const cnd_linear* problem, const void* x, const void* wei
   if (problem->rows == 0) return CND_OK;
   if (x == nullptr || weight == nullptr || y == nullptr) {
     return fail(CND_ERR_INVALID, "cnd_linear_forward: x, weight and y must not be NULL");
+  }
+  if (!aligned_to(element_size(problem->dtype), {x, weight, bias, residual, y, pre})) {
+    return misaligned("cnd_linear_forward");
   }
   const cnd_linear& q = *problem;
   const int64_t rows = q.rows, in = q.in_features, out = q.out_features;
@@ -572,6 +578,9 @@ int cnd_linear_backward(const cnd_linear* problem, const void* dy, const void* p
                     (want_x && (dx == nullptr || weight == nullptr)) ||
                     (want_w && x == nullptr)))) {
     return fail(CND_ERR_INVALID, "cnd_linear_backward: a required buffer is NULL");
+  }
+  if (!aligned_to(element_size(q.dtype), {dy, pre, x, weight, dx, dweight, dbias})) {
+    return misaligned("cnd_linear_backward");
   }
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   if (rows == 0) {

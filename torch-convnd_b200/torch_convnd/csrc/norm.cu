@@ -1375,6 +1375,10 @@ int cnd_layer_norm_forward(int32_t dtype, int32_t param_dtype, int64_t rows, int
   if (x == nullptr || y == nullptr) {
     return fail(CND_ERR_INVALID, "cnd_layer_norm_forward: x and y must not be NULL");
   }
+  if (!aligned_to(element_size(dtype), {x, y}) ||
+      !aligned_to(element_size(param_dtype), {weight, bias}) || !aligned_to(wide_size(dtype), {stats})) {
+    return misaligned("cnd_layer_norm_forward");
+  }
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   NormArgs a{};
   a.x = x;
@@ -1461,6 +1465,11 @@ int cnd_layer_norm_backward(int32_t dtype, int32_t param_dtype, int64_t rows, in
                     (output_mask[0] && dx == nullptr)))) {
     return fail(CND_ERR_INVALID, "cnd_layer_norm_backward: a required buffer is NULL");
   }
+  if (!aligned_to(element_size(dtype), {dy, x, dx}) ||
+      !aligned_to(element_size(param_dtype), {weight, dweight, dbias}) ||
+      !aligned_to(wide_size(dtype), {stats})) {
+    return misaligned("cnd_layer_norm_backward");
+  }
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   if (rows == 0) {
     const size_t bytes = static_cast<size_t>(width) * element_size(param_dtype);
@@ -1472,6 +1481,9 @@ int cnd_layer_norm_backward(int32_t dtype, int32_t param_dtype, int64_t rows, in
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
     return fail(CND_ERR_WORKSPACE, "cnd_layer_norm_backward: workspace of %zu bytes, %zu needed",
                 workspace == nullptr ? size_t{0} : workspace_bytes, need);
+  }
+  if (need > 0 && !aligned16(workspace)) {
+    return fail(CND_ERR_WORKSPACE, "cnd_layer_norm_backward: workspace must be 16-byte aligned");
   }
   NormArgs a{};
   a.x = x;

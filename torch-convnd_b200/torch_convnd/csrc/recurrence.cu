@@ -1111,6 +1111,9 @@ int bind_exchange(const char* who, const RecurrencePlan& p, void* workspace, siz
     return fail(CND_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who,
                 workspace == nullptr ? size_t{0} : bytes, p.total);
   }
+  if (!aligned16(workspace)) {
+    return fail(CND_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", who);
+  }
   char* base = static_cast<char*>(workspace);
   a->maps = base + p.maps;
   a->bases = base + p.bases;
@@ -1132,13 +1135,6 @@ bool pairs_aligned(int dtype, int64_t inner, std::initializer_list<const void*> 
   if (inner % 2 != 0) return false;
   for (const void* p : pointers) {
     if (reinterpret_cast<uintptr_t>(p) % (2 * element_size(dtype)) != 0) return false;
-  }
-  return true;
-}
-
-bool runs_aligned(std::initializer_list<const void*> pointers) {
-  for (const void* p : pointers) {
-    if (!aligned16(p)) return false;
   }
   return true;
 }
@@ -1213,6 +1209,10 @@ int cnd_gated_recurrence_forward(int32_t dtype, int64_t outer, int64_t steps, in
   if (last == nullptr || (steps > 0 && (x == nullptr || gate == nullptr || y == nullptr))) {
     return fail(CND_ERR_INVALID, "cnd_gated_recurrence_forward: a required buffer is NULL");
   }
+  if (!aligned_to(element_size(dtype), {x, gate, y}) ||
+      !aligned_to(wide_size(dtype), {initial, last, states})) {
+    return misaligned("cnd_gated_recurrence_forward");
+  }
   RecurrenceArgs a{};
   a.x = x;
   a.gate = gate;
@@ -1228,7 +1228,7 @@ int cnd_gated_recurrence_forward(int32_t dtype, int64_t outer, int64_t steps, in
   rc = bind_exchange("cnd_gated_recurrence_forward", p, workspace, workspace_bytes, &a, stream);
   if (rc != CND_OK) return rc;
   const unsigned grid = recurrence_grid(p);
-  const bool vectors = runs_aligned({x, gate, y});
+  const bool vectors = aligned_to(16, {x, gate, y});
   const bool small = columns * std::max<int64_t>(steps, 1) * element_size(dtype) <= UINT32_MAX;
   with_dtype(dtype, [&](auto zero) {
     using T = decltype(zero);
@@ -1268,6 +1268,10 @@ int cnd_gated_recurrence_backward(int32_t dtype, int64_t outer, int64_t steps, i
                      (output_mask[0] && dx == nullptr) || (output_mask[1] && dgate == nullptr)))) {
     return fail(CND_ERR_INVALID, "cnd_gated_recurrence_backward: a required buffer is NULL");
   }
+  if (!aligned_to(element_size(dtype), {dy, x, gate, dx, dgate}) ||
+      !aligned_to(wide_size(dtype), {dlast, states, dinitial})) {
+    return misaligned("cnd_gated_recurrence_backward");
+  }
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   RecurrenceArgs a{};
   a.x = x;
@@ -1286,7 +1290,7 @@ int cnd_gated_recurrence_backward(int32_t dtype, int64_t outer, int64_t steps, i
   rc = bind_exchange("cnd_gated_recurrence_backward", p, workspace, workspace_bytes, &a, stream);
   if (rc != CND_OK) return rc;
   const unsigned grid = recurrence_grid(p);
-  const bool vectors = runs_aligned({x, gate, dy, dx, dgate});
+  const bool vectors = aligned_to(16, {x, gate, dy, dx, dgate});
   const bool small = columns * std::max<int64_t>(steps, 1) * element_size(dtype) <= UINT32_MAX;
   with_dtype(dtype, [&](auto zero) {
     using T = decltype(zero);
