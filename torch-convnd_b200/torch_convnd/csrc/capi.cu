@@ -35,6 +35,8 @@ namespace {
 
 std::atomic<int64_t> g_launches{0};
 
+}  // namespace
+
 uint64_t wait_timeout_ns() {
   static uint64_t value = 0;
   static std::once_flag once;
@@ -48,8 +50,6 @@ uint64_t wait_timeout_ns() {
   });
   return value;
 }
-
-}  // namespace
 
 void count_launch(int n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 

@@ -25,6 +25,9 @@ constexpr int kTileRows = 128;     // MMA M
 unsigned int* device_error_word();
 void count_launch(int n = 1);
 
+// Limit of every wait inside a kernel (CND_WAIT_TIMEOUT_MS, 2 s).
+uint64_t wait_timeout_ns();
+
 // Geometry of one implicit-GEMM pass, in the "box" decomposition used by the tcgen05
 // kernels: the last three spatial axes are tiled by a dense box of output positions
 // (b[0] x b[1] x b[2], innermost last) that one TMA load fetches for each tap; every

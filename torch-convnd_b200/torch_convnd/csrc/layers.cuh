@@ -201,11 +201,10 @@ inline int launch_status(const char* what) {
   return CND_OK;
 }
 
-// SMs of the current device.
+// SMs of the current device, which launches go by; and of a B200, which plans and workspace sizes
+// go by: they are the same on a machine without a GPU.
 int sm_count();
-
-// Limit of every wait inside a kernel (CND_WAIT_TIMEOUT_MS, 2 s).
-uint64_t wait_timeout_ns();
+constexpr int kSms = 148;
 
 }  // namespace layers
 }  // namespace cnd

@@ -304,7 +304,7 @@ size_t up1024(size_t v) { return (v + 1023) / 1024 * 1024; }
 // Row ranges of prepare_kernel's grid: about eight blocks an SM, 32 rows or more each.
 int prepare_ranges(int64_t rows, int64_t width) {
   const int64_t across = (width + kPrepareColumns - 1) / kPrepareColumns;
-  const int64_t ranges = std::min<int64_t>((rows + 31) / 32, (148 * 8 + across - 1) / across);
+  const int64_t ranges = std::min<int64_t>((rows + 31) / 32, (kSms * 8 + across - 1) / across);
   return static_cast<int>(std::max<int64_t>(1, ranges));
 }
 

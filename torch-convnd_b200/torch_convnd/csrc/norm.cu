@@ -17,7 +17,6 @@
 // bulk copies cannot take stay in registers. Rows wider than 28 KB and float64 are walked
 // in chunks and read again for each pass.
 #include <algorithm>
-#include <cstdlib>
 
 #include "layers.cuh"
 #include "pair.cuh"
@@ -31,18 +30,9 @@ int sm_count() {
       cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
       count <= 0) {
     cudaGetLastError();
-    return 148;
+    return kSms;
   }
   return count;
-}
-
-uint64_t wait_timeout_ns() {
-  static const uint64_t value = [] {
-    const char* env = std::getenv("CND_WAIT_TIMEOUT_MS");
-    const long long parsed = env != nullptr ? std::atoll(env) : 0;
-    return (parsed > 0 ? static_cast<uint64_t>(parsed) : uint64_t{2000}) * 1000000u;
-  }();
-  return value;
 }
 
 namespace {
@@ -1162,15 +1152,15 @@ int norm_backward_blocks(const NormShape& s, int64_t rows, int64_t width) {
     // column kernel: row ranges of at least 64 rows
     const int64_t most = std::max<int64_t>(1, rows / 64);
     const int64_t across = (width + 127) / 128;
-    return static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, 8 * 148 / across)));
+    return static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, 8 * kSms / across)));
   }
   if (s.ring) {
     // a multiple of 8 where blocks take several rows: one shift a block
-    return static_cast<int>(std::min<int64_t>(rows, 148 * ring_blocks(s) / 8 * 8));
+    return static_cast<int>(std::min<int64_t>(rows, kSms * ring_blocks(s) / 8 * 8));
   }
   const int per_block = norm_rows_per_block(s);
   const int64_t need = (rows + per_block - 1) / per_block;
-  return static_cast<int>(std::min<int64_t>(need, 4 * 148));
+  return static_cast<int>(std::min<int64_t>(need, 4 * kSms));
 }
 
 // Vectors a thread, threads a row, rows in flight.

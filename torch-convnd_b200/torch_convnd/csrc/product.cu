@@ -26,9 +26,6 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <atomic>
-#include <cstdlib>
-#include <cstring>
 
 #include "activation.cuh"
 #include "layers.cuh"
@@ -831,7 +828,7 @@ ProductPlan plan_product(int64_t m, int64_t n, int64_t k, int parts) {
       {1, 2, 256, 8.5, 0.32, 5.5}, {1, 1, 128, 5.0, 0.27, 3.0}, {1, 1, 64, 4.3, 0.25, 1.9},
       {3, 2, 128, 8.0, 0.52, 4.0}, {3, 1, 128, 5.0, 0.62, 3.0}, {3, 1, 64, 4.3, 0.47, 2.0},
   };
-  const int64_t sms = 148, blocks = (k + block_depth(parts) - 1) / block_depth(parts);
+  const int64_t sms = kSms, blocks = (k + block_depth(parts) - 1) / block_depth(parts);
   ProductPlan best{1, 64, 1, 1};
   double best_cost = 0;
   for (const Cut& c : kCuts) {

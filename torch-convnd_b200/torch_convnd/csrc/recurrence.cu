@@ -33,8 +33,6 @@
 // the backward recomputes the others in float32: it reads x, g and dy only, and its states
 // carry no rounding to the tensors' type.
 #include <algorithm>
-#include <cstdlib>
-
 #include <type_traits>
 
 #include "layers.cuh"

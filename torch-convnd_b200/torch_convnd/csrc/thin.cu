@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }  // namespace
 
 int thin_blocks(int64_t rows) {
-  return static_cast<int>(std::min<int64_t>((rows + kRows - 1) / kRows, 148));
+  return static_cast<int>(std::min<int64_t>((rows + kRows - 1) / kRows, kSms));
 }
 
 int launch_thin_backward(const ThinBackward& p, cudaStream_t stream) {
