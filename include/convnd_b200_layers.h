@@ -52,7 +52,8 @@ CND_API int cnd_layer_norm_backward(int32_t dtype, int32_t param_dtype, int64_t 
  * terms each and the six products above 2^-24 are summed (float32 accuracy; a non-finite
  * operand gives a non-finite result, but an infinity may come out as NaN); float64 runs on
  * the CUDA cores. cnd_linear_forward writes z to `pre` (same shape and type as y) when it is
- * not NULL; the backward of an activation needs it. x, weight, dy, pre and dx are 16-byte
+ * not NULL; the backward of an activation needs it. Both z and the dz below are rounded to
+ * `dtype` there. x, weight, dy, pre and dx are 16-byte
  * aligned (float64: their natural alignment):
  *   dz = dy * act'(z), dx = dz W, dW = dz^T x, dbias = column sums of dz
  * (the residual's gradient is dy itself). `pre` may be NULL for CND_ACT_NONE. The
@@ -84,7 +85,8 @@ CND_API int cnd_linear_backward(const cnd_linear* problem, const void* dy, const
  *   f_t = sigmoid(gate_t), h_t = f_t * h_{t-1} + (1 - f_t) * x_t, y_t = h_t,
  * with h_{-1} = initial ([outer][inner] float32, float64 for CND_F64; NULL = zeros) and
  * last = h_{steps-1} of the same type and shape. States are held in float32 (float64). A
- * gate of -inf restarts a column (h_t = x_t), +inf holds it (h_t = h_{t-1}, x_t finite).
+ * gate of -inf restarts a column (h_t = x_t, h_{t-1} finite), +inf holds it (h_t = h_{t-1}, x_t
+ * finite); what is not finite stays, as 0 * inf is NaN.
  * `states` (NULL when no backward follows) receives the states before each block of steps,
  * [cnd_gated_recurrence_blocks()][outer][inner]; the backward recomputes the others.
  * Backward, with dy ([outer][steps][inner], NULL = zeros) and dlast ([outer][inner], NULL =

@@ -49,7 +49,7 @@ def layer_norm(
     Statistics and sums are float32 (float64 for a float64 input). ``weight`` and ``bias``
     are vectors of the last dimension's size, of the input's dtype or float32. The result is
     contiguous; an input whose rows have unit stride and one common distance is read in
-    place. ``eps`` must not be negative. First derivatives only.
+    place. ``eps`` must not be negative. First derivatives only, in reverse mode.
     """
     if not is_loaded():
         load_native()
@@ -69,7 +69,10 @@ def linear(
     ``input`` is ``[..., in_features]``, ``weight`` ``[out_features, in_features]``,
     ``residual`` has the output's shape; all share one dtype (autocast casts them).
     ``activation`` is None, ``'gelu'`` (exact) or ``'silu'``. Products accumulate in
-    float32; float32 operands keep float32 accuracy. First derivatives only.
+    float32; float32 operands keep float32 accuracy. For the backward of an activation, the
+    value before it and its gradient are kept in the tensors' dtype: in 16 bits, gradients are
+    about half again as far from exact as with both in float32, for half the traffic. First
+    derivatives only, in reverse mode.
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"Invalid activation {activation!r}; expected None, 'gelu' or 'silu'")
@@ -92,7 +95,8 @@ def gated_recurrence(
     shape without ``dim``, float32, or float64 for a float64 input). ``initial`` is the state
     before the first step, of the last state's shape and dtype (default zeros), so a sequence
     can be continued call by call, one step at a time or many. A gate of ``-inf`` restarts its
-    column, ``+inf`` holds it. First derivatives only.
+    column, ``+inf`` holds it (of finite states and inputs). First derivatives only, in reverse
+    mode.
     """
     if not is_loaded():
         load_native()

@@ -13,12 +13,11 @@ namespace layers {
 // where Q(a) = erfcx(a / sqrt 2) / 2 is smooth and falls from 0.5 to 0.066 on [0, 6]. Q is the
 // polynomial of degree 9 in a - 3 with the least relative error there, 9.0e-5 (fitted to
 // double-precision erfc by iteratively reweighted least squares at Chebyshev points). Beyond
-// 6, Phi(-a) is below 1e-9, and a Q(a) and a phi(a) are taken with the a of 6: GELU and its slope
-// there, below 1e-8 and 4e-8, are some percent (GELU 1 to 3) and more off. Used where the result
-// is rounded to 16 bits (2^-11 and more):
-// half an instruction a value and step and one exponential, shared with phi. A
-// reciprocal beside the exponential costs 3 % more (1M x 64 -> 256 GELU 319 us against 310,
-// where no activation took 192).
+// 6, Phi(-a) is below 1e-9, and a Q(a) and a phi(a) are taken with the a of 6: GELU there, below
+// 6e-9, is 1 to 3 % off, and its slope, below 4e-8, too small by up to 6 / a. Used where the result
+// is rounded to 16 bits (2^-11 and more): half an instruction a value and step and one
+// exponential, shared with phi. A reciprocal beside the exponential costs 3 % more (1M x 64 ->
+// 256 GELU 319 us against 310, where no activation took 192).
 __device__ __forceinline__ Two normal_tail(Two v, Two* size, Two* gauss) {
   float lo, hi;
   unpack(v, &lo, &hi);

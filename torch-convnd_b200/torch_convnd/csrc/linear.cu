@@ -9,6 +9,11 @@
 // and sums its columns (dbias). Operands that TMA can read as they lie are not copied. The
 // backward of thin 16-bit layers with an activation is one kernel (thin.cu). float64 runs on
 // the CUDA cores.
+//
+// In 16-bit layers z and dz are rounded to the operands' type: dz has to be for the products
+// (two terms of it would double them), z to be kept at half the traffic (float32 would move 1.07
+// GB more for 1M x 64 -> 256, 164 us). Against float64 the gradients are 1.46 times as far off as
+// with both in float32, 1.41 times with dz alone rounded; dbias sums dz before its rounding.
 #include <algorithm>
 
 #include "activation.cuh"

@@ -8,14 +8,15 @@
 // A row is held in registers or shared memory between its two sums (the squares are of centred
 // values, so a large mean costs no digits), so every element is read once: both passes are
 // bound by memory traffic, 2 and 3 elements per position. bf16 forward / backward: 1M x 64 in
-// 57 / 95 us (4.7 / 4.2 TB/s), 16384 x 4096 in 53 / 83 us (5.1 / 4.9), of 6.55 TB/s copied.
+// 58 / 92 us (4.6 / 4.4 TB/s), 16384 x 4096 in 52 / 85 us (5.2 / 4.7), of 6.55 TB/s copied.
 // A row belongs to G lanes of a warp or to a block of G threads; a block walks rows with a
 // grid stride, each thread always holding the same columns, so the weight's gradient
 // accumulates in registers, is combined once per block and leaves as one partial row per
 // block, summed in order by a second launch. Rows that are back to back come through a ring
 // of bulk copies, whole rows of more than 64 vectors and tiles of shorter ones; rows that
 // bulk copies cannot take stay in registers. Rows wider than 28 KB and float64 are walked
-// in chunks and read again for each pass.
+// in chunks, element by element, and read again for each pass: 8192 x 8192 float32 134 / 299 us,
+// 4.0 and 2.7 TB/s of what one reading would move.
 #include <algorithm>
 
 #include "layers.cuh"
@@ -1140,8 +1141,8 @@ int norm_rows_per_block(const NormShape& s) {
 
 // Short rows back to back, in vectors, come by the tile; others (rows apart from one another,
 // single elements) are held in registers as they are loaded. bf16, forward / backward, registers
-// against tiles: 1M x 64 76 / 109 us and 57 / 104, 65536 x 512 64 / 99 and 44 / 70,
-// 65536 x 64 11.5 / 26 and 9.5 / 24; the same from 1 to 1024 rows.
+// against tiles: 1M x 64 76 / 109 us and 56 / 98, 65536 x 512 64 / 99 and 31 / 64,
+// 65536 x 64 11.5 / 26 and 8 / 19; the same from 1 to 1024 rows.
 bool norm_tiles(const NormShape& s, int64_t width, int64_t x_stride, int64_t dy_stride) {
   return !s.loops && !s.ring && s.vector > 1 && x_stride == width && dy_stride == width;
 }

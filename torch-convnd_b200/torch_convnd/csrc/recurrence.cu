@@ -9,10 +9,10 @@
 // to a map, a block composes its threads' maps in shared memory to find the state each of
 // them starts from, and the thread then walks its steps from that state: x, g and dy are
 // read once and stay in registers between the two walks. The traffic is 3 elements a step
-// forward, 5 backward. float32, 8 x 33 x 129600: 100 / 181 us, 4.1 / 3.8 TB/s. What is
+// forward, 5 backward. float32, 8 x 33 x 129600: 98 / 180 us, 4.2 / 3.8 TB/s. What is
 // between that and the 6.55 TB/s of a copy is latency: a block loads, composes, waits and
 // stores one after the other, and 128 registers leave room for two blocks on an SM. Most of
-// it is seen where 16-bit columns share the time axis (65536 x 512 bf16, 87 / 180 us).
+// it is seen where 16-bit columns share the time axis (65536 x 512 bf16, 87 / 176 us).
 //
 // Column layout (inner > 1): the lanes of a warp hold two columns each, in packed float32
 // pairs, the warps of a block follow one another in time. Step layout (inner = 1, steps
